@@ -453,6 +453,153 @@ tbh_status tbh_attention(tbh_device *dev, const tbh_attention_shape *shape, cons
 tbh_status tbh_attention_device(tbh_device *dev, const tbh_attention_shape *shape, const float *q,
                                 const float *k, const float *v, const float *mask, float *out, void *stream);
 
+/* ---- serving many requests from one paged cache ------------------------ */
+/* The decode step above keeps the cache of one sequence.  These calls serve a
+ * batch: requests of any lengths share one key/value cache cut into blocks of
+ * block_size tokens (the reference's KVCache is paged too, 16 tokens a page,
+ * but holds one sequence: KVCache.swift:61-120).  One step of a batch is
+ *   tbh_paged_plan_device       lengths -> blocks, slots, positions (once)
+ *   tbh_paged_append_device     a layer's new keys and values -> the cache
+ *   tbh_paged_attention_device  the layer's attention over the cache
+ *   tbh_sample_device           logits -> tokens
+ * All of them take device pointers, are enqueued on `stream` and return after
+ * the launch; lengths, tables and slots are read on the device, so a captured
+ * step replays with new ones.  Device-side values out of range are never
+ * followed: a block id outside the cache holds nothing, a slot outside it is
+ * not written, lengths are clamped to what the table and the rows can hold.
+ *
+ * The cache of a layer is two arrays (keys, values), each
+ * [num_blocks][num_kv_heads][block_size][head_dim] of `type`, 16-byte aligned.
+ * Request b is row b of block_table [max_requests][max_blocks]; its position p
+ * lies in block block_table[b][p / block_size] at row p % block_size, and the
+ * slot of that place is block * block_size + p % block_size. */
+enum { TBH_F32 = 0, TBH_BF16 = 1 };   /* element types of the cache and of rows */
+
+typedef struct tbh_paged_layout {
+    int32_t num_blocks;      /* blocks in each array; num_blocks * block_size < 2^31 */
+    int32_t block_size;      /* tokens per block: a power of two, 1 .. 1024 */
+    int32_t num_kv_heads;
+    int32_t head_dim;        /* 1 .. 256 */
+    int32_t type;            /* TBH_F32 or TBH_BF16 */
+    int32_t max_requests;    /* rows of the block table */
+    int32_t max_blocks;      /* entries per row */
+} tbh_paged_layout;
+
+/* Plans a step.  new_lens[max_requests]: tokens each request adds (0: idle
+ * this step; negative: the request is released).  context_lens: tokens each
+ * holds so far, in the first ceil(context / block_size) blocks of its row.
+ * free_blocks[num_blocks] is a stack of free block ids, free_count[1] its
+ * height.  In order:
+ *   - released rows push their blocks (row by row, in table order);
+ *   - row b with n = new_lens[b] > 0 needs ceil((context + n) / block_size) -
+ *     ceil(context / block_size) blocks and is granted its tokens if context +
+ *     n fits the table row and the needs of rows 0 .. b (of those that fit
+ *     theirs) do not exceed the stack, or it needs none: no row overtakes one
+ *     that waits for blocks;
+ *   - granted rows pop their blocks off the stack (row by row) into the table.
+ * Outputs: query_start[max_requests + 1], running sums of max(new_lens, 0);
+ * granted[max_requests], n or 0; context_out, free_count_out: the lengths and
+ * the height after the step; slots[max_tokens], positions[max_tokens] of token
+ * query_start[b] + i, position context[b] + i, and -1 for rows not granted and
+ * for entries behind the last token (tokens past max_tokens get none).
+ * context_out and free_count_out may be context_lens and free_count; else a
+ * plan can be dropped: entries of the table and of the stack that the old
+ * lengths and height refer to are not changed.  Only the block_size, num_blocks,
+ * max_requests and max_blocks of the layout are read. */
+tbh_status tbh_paged_plan_device(tbh_device *dev, const tbh_paged_layout *layout, const int32_t *new_lens,
+                                 const int32_t *context_lens, int32_t *block_table, int32_t *free_blocks,
+                                 const int32_t *free_count, int64_t max_tokens, int32_t *query_start,
+                                 int32_t *granted, int32_t *context_out, int32_t *free_count_out,
+                                 int32_t *slots, int32_t *positions, void *stream);
+
+/* Rows of a projection on their way to the attention and the cache. */
+typedef struct tbh_paged_rows {
+    int64_t tokens;
+    int32_t x_type;          /* of q, k and v */
+    int32_t num_heads;       /* of q */
+    const void *q;           /* [tokens][num_heads * head_dim], or NULL */
+    const void *k;           /* [tokens][num_kv_heads * head_dim] */
+    const void *v;           /* as k */
+    int64_t q_stride;        /* elements from one row to the next */
+    int64_t k_stride;
+    int64_t v_stride;
+    void *q_out;             /* [tokens][num_heads * head_dim]; may be q itself (same type and stride) */
+    int64_t q_out_stride;
+    int32_t q_out_type;
+    float rope_base;         /* 0: no rotation */
+    const int32_t *slots;    /* [tokens]; distinct, or negative: the row is not stored */
+    const int32_t *positions;/* [tokens]; read with rope_base > 0, negative as 0 */
+} tbh_paged_rows;
+
+/* Stores the rows' keys and values at their slots, rounded once to the
+ * cache's type, and, with rope_base > 0, rotates keys and queries first:
+ * interleaved pairs (2i, 2i + 1) by the angle position * rope_base^(-2i /
+ * head_dim), as ModelRunner.applyRoPE (ModelRunner.swift:470-494).  The angle
+ * is that of real arithmetic (the reference, and the decode step here, round
+ * it to fp32, which at position 10^5 is off by up to 4e-3).  q NULL: no
+ * queries.  An odd head_dim is not rotated (TBH_E_INVALID). */
+tbh_status tbh_paged_append_device(tbh_device *dev, const tbh_paged_layout *layout, const tbh_paged_rows *rows,
+                                   void *k_cache, void *v_cache, void *stream);
+
+/* A batch of queries over the cache. */
+typedef struct tbh_paged_queries {
+    int64_t tokens;              /* rows of q and out */
+    int32_t type;                /* of q and out */
+    int32_t num_heads;
+    const void *q;               /* [tokens][num_heads * head_dim] */
+    void *out;                   /* as q, not overlapping it */
+    int64_t q_stride;
+    int64_t out_stride;
+    const int32_t *query_start;  /* [max_requests + 1], not descending */
+    const int32_t *context_lens; /* [max_requests], with the step's own tokens */
+    float scale;                 /* of the scores; 0: 1 / sqrt(head_dim) */
+    int32_t max_query_len;       /* at least the longest query_start[b + 1] - query_start[b], */
+    int32_t max_context_len;     /* and the longest context: they choose launch shapes only; 0: unknown */
+} tbh_paged_queries;
+
+/* Attention of each request's newest tokens over its cache: row i of request
+ * b's n rows has position context_lens[b] - n + i and attends to every
+ * position up to its own, out = sum softmax(scale q . k) v per head, query
+ * head h reading key/value head h / (num_heads / num_kv_heads).  Prompt
+ * chunks and single tokens mix in one call.  A row with nothing to attend to
+ * (negative position, no block) gives zeros; rows behind query_start's last
+ * entry are left as they are.  Whatever lies in the cache behind a request's
+ * length is not used (it may be NaN).  Scores, softmax and sums are fp32; fp32
+ * q keeps fp32's precision over a bf16 cache as well, bf16 q over a bf16 cache
+ * has its probabilities rounded to bf16 for the second product.
+ * num_heads must be a multiple of num_kv_heads.  Calls that split a long
+ * context over blocks keep partial results in the workspace of (device,
+ * stream), as tbh_matmul_device does, with its rule for captured graphs. */
+tbh_status tbh_paged_attention_device(tbh_device *dev, const tbh_paged_layout *layout,
+                                      const tbh_paged_queries *queries, const void *k_cache, const void *v_cache,
+                                      const int32_t *block_table, void *stream);
+
+/* ---- sampling ---------------------------------------------------------- */
+/* Sampler (Sampler.swift) with the random numbers given by the caller: one
+ * token per row of `logits` [rows][ld] (ld >= vocab).  With w_i =
+ * exp((logit_i - max) / temperature):
+ *   top_k  > 0 keeps the top_k largest logits (equal ones: lowest index first);
+ *   top_p  < 1 keeps of those, largest first, the shortest prefix whose w sum
+ *          to at least top_p of their sum (at least one);
+ *   min_p  > 0 keeps of those the ones with w_i >= min_p;
+ * tokens[r] is the first kept j, in index order, with sum of w over kept i <= j
+ * above u[r] times the sum of all kept; probs[r] (if not NULL) is its share of
+ * that sum.  temperature <= 0 (or NaN) takes the largest logit, the first of
+ * equal ones, with probability 1.  NaN and -inf are never taken (+inf shares
+ * all of the weight); a row of nothing else gives token -1, probability 0.
+ * u is clamped to [0, 1).  temperature, top_k, top_p, min_p: [rows] each, or
+ * NULL for 1, 0, 1, 0 everywhere; NaN top_p or min_p filter nothing, and the
+ * largest logit always stays.  Weights are summed as whole multiples of 2^-43 of
+ * the largest (64-bit integers), so results do not depend on the order of sums;
+ * what weighs less than half of that is never taken.
+ * vocab up to 2^20 (TBH_E_UNSUPPORTED above). */
+tbh_status tbh_sample(tbh_device *dev, const float *logits, int64_t rows, int64_t vocab, const float *temperature,
+                      const int32_t *top_k, const float *top_p, const float *min_p, const float *u,
+                      int32_t *tokens, float *probs);
+tbh_status tbh_sample_device(tbh_device *dev, const float *logits, int64_t ld, int64_t rows, int64_t vocab,
+                             const float *temperature, const int32_t *top_k, const float *top_p,
+                             const float *min_p, const float *u, int32_t *tokens, float *probs, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

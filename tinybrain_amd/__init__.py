@@ -16,10 +16,12 @@ from .quantized import (Layout, PreconditionFailure, QuantizationMode,  # noqa: 
 from .backend import DeviceWeight, HIPBackend, HIPBackendError  # noqa: F401
 from .decoder import Decoder, DecoderConfig  # noqa: F401
 from .linear import LinearLayerWeights  # noqa: F401
+from .paged import PagedKVCache, PagedPlan  # noqa: F401
 from .tbf import TBFFile  # noqa: F401
 
 __all__ = [
     "HIPBackend", "HIPBackendError", "DeviceWeight", "QuantizedTensor", "LinearLayerWeights", "Decoder", "DecoderConfig", "TBFFile",
+    "PagedKVCache", "PagedPlan",
     "QuantizationMode", "QuantizationPrecision", "Layout", "PreconditionFailure",
     "quantize", "quantize_int4_flat", "packInt4", "unpackInt4",
 ]

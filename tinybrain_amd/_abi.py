@@ -21,6 +21,9 @@ PATH_NAMES = {0: "int8_row", 1: "int4_kgroup", 2: "int4_ngroup", 3: "generic"}
 # device options (tbh_device_set_option)
 OPT_SGEMV_MIN_ROWS, OPT_NOALLOC_SCRATCH_BYTES, OPT_MFMA_MIN_ROWS, OPT_HOST_ENTRY, OPT_HOST_WAIT = 1, 2, 3, 4, 5
 
+# element types of the paged cache and of rows
+F32, BF16 = 0, 1
+
 # every symbol the header declares
 EXPORTS = [
     "tbh_abi_version", "tbh_last_error", "tbh_status_string",
@@ -36,6 +39,8 @@ EXPORTS = [
     "tbh_softmax", "tbh_softmax_device", "tbh_rmsnorm", "tbh_rmsnorm_device",
     "tbh_silu", "tbh_silu_device", "tbh_gelu", "tbh_gelu_device",
     "tbh_attention", "tbh_attention_device",
+    "tbh_paged_plan_device", "tbh_paged_append_device", "tbh_paged_attention_device",
+    "tbh_sample", "tbh_sample_device",
 ]
 
 
@@ -47,6 +52,48 @@ class AttentionShape(ctypes.Structure):
         ("head_dim", ctypes.c_int32),
         ("num_heads", ctypes.c_int32),
         ("num_kv_heads", ctypes.c_int32),
+    ]
+
+
+class PagedLayout(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("num_blocks", "block_size", "num_kv_heads", "head_dim", "type",
+                                              "max_requests", "max_blocks")]
+
+
+class PagedRows(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("x_type", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64),
+        ("k_stride", ctypes.c_int64),
+        ("v_stride", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p),
+        ("q_out_stride", ctypes.c_int64),
+        ("q_out_type", ctypes.c_int32),
+        ("rope_base", ctypes.c_float),
+        ("slots", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+    ]
+
+
+class PagedQueries(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("type", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64),
+        ("query_start", ctypes.c_void_p),
+        ("context_lens", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("max_query_len", ctypes.c_int32),
+        ("max_context_len", ctypes.c_int32),
     ]
 
 
@@ -190,6 +237,15 @@ def lib() -> ctypes.CDLL:
     sp = ctypes.POINTER(AttentionShape)
     L.tbh_attention.argtypes = [vp, sp, vp, vp, vp, vp, vp]
     L.tbh_attention_device.argtypes = [vp, sp, vp, vp, vp, vp, vp, vp]
+    lp = ctypes.POINTER(PagedLayout)
+    L.tbh_paged_plan_device.argtypes = [vp, lp] + [vp] * 5 + [i64] + [vp] * 7
+    L.tbh_paged_append_device.argtypes = [vp, lp, ctypes.POINTER(PagedRows), vp, vp, vp]
+    L.tbh_paged_attention_device.argtypes = [vp, lp, ctypes.POINTER(PagedQueries), vp, vp, vp, vp]
+    L.tbh_sample.argtypes = [vp, vp, i64, i64] + [vp] * 7
+    L.tbh_sample_device.argtypes = [vp, vp, i64, i64, i64] + [vp] * 8
+    for name in ("tbh_paged_plan_device", "tbh_paged_append_device", "tbh_paged_attention_device",
+                 "tbh_sample", "tbh_sample_device"):
+        getattr(L, name).restype = i32
     for name in ("tbh_tbf_open", "tbh_tbf_close", "tbh_tbf_get_config", "tbh_tbf_tensor",
                  "tbh_tbf_find", "tbh_tbf_qtensor", "tbh_tbf_floats", "tbh_tbf_load_decoder"):
         getattr(L, name).restype = i32

@@ -36,6 +36,7 @@ from typing import Dict, Optional, Sequence
 import numpy as np
 
 from . import _abi
+from .paged import PagedPlan
 from .quantized import PreconditionFailure, QuantizedTensor
 
 
@@ -409,6 +410,204 @@ class HIPBackend:
                                               v.data_ptr(), None if m is None else m.data_ptr(),
                                               out.data_ptr(), self._stream(q, stream)))
         return out
+
+    # -- serving many requests from one paged cache (see paged.py) --------------
+    def paged_plan_device(self, newLens, contextLens, blockTable, freeBlocks, freeCount, blockSize: int,
+                          maxTokens: int, contextOut=None, freeCountOut=None, stream=None) -> PagedPlan:
+        """tbh_paged_plan_device: which blocks, slots and positions a step's
+        new tokens take.  int32 cuda tensors: newLens and contextLens
+        [requests], blockTable [requests, blocks], freeBlocks [blocks of the
+        cache], freeCount [1].  blockTable and freeBlocks are updated in
+        place; lengths and height come back in the plan, or go to contextOut
+        and freeCountOut (contextLens and freeCount themselves: in place)."""
+        import torch
+
+        for t in (newLens, contextLens, blockTable, freeBlocks, freeCount):
+            self._int_tensor(t)
+        b = newLens.numel()
+        if contextLens.numel() != b or blockTable.dim() != 2 or blockTable.shape[0] != b or freeCount.numel() != 1:
+            raise PreconditionFailure("plan: lengths and block table must have one row per request")
+        if maxTokens < 0:
+            raise PreconditionFailure("plan: maxTokens must not be negative")
+        sizes = [b + 1, b, maxTokens, maxTokens, b, 1]
+        start, granted, slots, positions, ctx, count = self._made(
+            torch.empty(sum(sizes), dtype=torch.int32, device=newLens.device), stream).split(sizes)
+        if contextOut is not None:
+            ctx = self._int_tensor(contextOut)
+        if freeCountOut is not None:
+            count = self._int_tensor(freeCountOut)
+        if ctx.numel() != b or count.numel() != 1:
+            raise PreconditionFailure("plan: contextOut [requests] and freeCountOut [1]")
+        layout = _abi.PagedLayout(freeBlocks.numel(), blockSize, 0, 0, 0, b, blockTable.shape[1])
+        _check(self._lib.tbh_paged_plan_device(
+            self._dev, ctypes.byref(layout), newLens.data_ptr(), contextLens.data_ptr(), blockTable.data_ptr(),
+            freeBlocks.data_ptr(), freeCount.data_ptr(), maxTokens, start.data_ptr(), granted.data_ptr(),
+            ctx.data_ptr(), count.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+            self._stream(newLens, stream)))
+        return PagedPlan(start, granted, slots, positions, ctx, count)
+
+    def paged_append_device(self, keys, values, slots, k, v, q=None, positions=None, ropeBase: float = 0.0,
+                            qOut=None, stream=None):
+        """tbh_paged_append_device: rows k, v [tokens, kvHeads * headDim] to
+        their slots of the cache arrays keys, values [blocks, kvHeads,
+        blockSize, headDim]; with ropeBase > 0 keys and queries q [tokens,
+        heads * headDim] are rotated by their positions.  Rows may be slices
+        of a wider matrix (only the last dimension must be contiguous).
+        Returns the queries: qOut, which may be q itself or of the other type,
+        else a new tensor of q's type; None without q."""
+        import torch
+
+        layout = self._paged_layout(keys, values)
+        xt = self._paged_type(k)
+        hd, nkv = layout.head_dim, layout.num_kv_heads
+        for t, n in ((k, nkv), (v, nkv)) + (((q, 0),) if q is not None else ()):
+            self._row_tensor(t)
+            if t.dtype != k.dtype or t.shape[0] != k.shape[0]:
+                raise PreconditionFailure("append: q, k and v must have one type and number of rows")
+            if t.shape[1] % hd or (n and t.shape[1] != n * hd):
+                raise PreconditionFailure("append: rows do not match the cache's heads")
+        self._int_tensor(slots)
+        if slots.numel() != k.shape[0]:
+            raise PreconditionFailure("append: slots must have one entry per row")
+        if positions is not None and self._int_tensor(positions).numel() != k.shape[0]:
+            raise PreconditionFailure("append: positions must have one entry per row")
+        if ropeBase and positions is None:
+            raise PreconditionFailure("append: positions are needed to rotate")
+        if q is not None:
+            if qOut is None:
+                qOut = self._made(torch.empty(q.shape, dtype=q.dtype, device=q.device), stream)
+            elif tuple(self._row_tensor(qOut).shape) != tuple(q.shape):
+                raise PreconditionFailure("append: qOut must be shaped like q")
+        rows = _abi.PagedRows(
+            k.shape[0], xt, 0 if q is None else q.shape[1] // hd, None if q is None else q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), 0 if q is None else q.stride(0), k.stride(0), v.stride(0),
+            None if q is None else qOut.data_ptr(), 0 if q is None else qOut.stride(0),
+            xt if q is None else self._paged_type(qOut), float(ropeBase), slots.data_ptr(),
+            None if positions is None else positions.data_ptr())
+        _check(self._lib.tbh_paged_append_device(self._dev, ctypes.byref(layout), ctypes.byref(rows),
+                                                 keys.data_ptr(), values.data_ptr(), self._stream(k, stream)))
+        return qOut if q is not None else None
+
+    def paged_attention_device(self, q, keys, values, blockTable, queryStart, contextLens, numHeads: int,
+                               scale: float = 0.0, maxQueryLen: int = 0, maxContextLen: int = 0, out=None,
+                               stream=None):
+        """tbh_paged_attention_device: q [tokens, numHeads * headDim] (float32
+        or bfloat16), request b's rows queryStart[b] .. queryStart[b + 1], its
+        newest positions of contextLens[b], over the cache; returns a tensor
+        like q (rows behind the last request are left as they were in out).
+        maxQueryLen and maxContextLen, if known, choose launch shapes only."""
+        import torch
+
+        layout = self._paged_layout(keys, values)
+        self._row_tensor(q)
+        for t in (blockTable, queryStart, contextLens):
+            self._int_tensor(t)
+        b = contextLens.numel()
+        if q.shape[1] != numHeads * layout.head_dim or numHeads <= 0 or numHeads % layout.num_kv_heads:
+            raise PreconditionFailure("attention: query shape does not match the heads")
+        if blockTable.dim() != 2 or blockTable.shape[0] != b or queryStart.numel() != b + 1:
+            raise PreconditionFailure("attention: block table and query starts must have one row per request")
+        layout.max_requests, layout.max_blocks = b, blockTable.shape[1]
+        if out is None:
+            out = self._made(torch.empty(q.shape, dtype=q.dtype, device=q.device), stream)
+        elif tuple(self._row_tensor(out).shape) != tuple(q.shape) or out.dtype != q.dtype:
+            raise PreconditionFailure("attention: out must be like the queries")
+        args = _abi.PagedQueries(q.shape[0], self._paged_type(q), numHeads, q.data_ptr(), out.data_ptr(),
+                                 q.stride(0), out.stride(0), queryStart.data_ptr(), contextLens.data_ptr(),
+                                 float(scale), int(maxQueryLen), int(maxContextLen))
+        _check(self._lib.tbh_paged_attention_device(self._dev, ctypes.byref(layout), ctypes.byref(args),
+                                                    keys.data_ptr(), values.data_ptr(), blockTable.data_ptr(),
+                                                    self._stream(q, stream)))
+        return out
+
+    def _here(self, t) -> bool:
+        """Whether a tensor is on this backend's GPU."""
+        return t.is_cuda and t.get_device() == self.device
+
+    def _int_tensor(self, t):
+        import torch
+
+        if t.dtype != torch.int32 or not t.is_contiguous() or not self._here(t):
+            raise PreconditionFailure("expected a contiguous int32 tensor on this device")
+        return t
+
+    def _row_tensor(self, t):
+        if t.dim() != 2 or not self._here(t) or (t.shape[1] > 1 and t.stride(1) != 1):
+            raise PreconditionFailure("expected rows on this device, contiguous along the last dimension")
+        return t
+
+    @staticmethod
+    def _made(t, stream):
+        """A result allocated on torch's current stream and written on `stream`."""
+        if stream is not None:
+            t.record_stream(stream)
+        return t
+
+    @staticmethod
+    def _paged_type(t) -> int:
+        import torch
+
+        if t.dtype == torch.float32:
+            return _abi.F32
+        if t.dtype == torch.bfloat16:
+            return _abi.BF16
+        raise PreconditionFailure("expected float32 or bfloat16")
+
+    def _paged_layout(self, keys, values) -> _abi.PagedLayout:
+        if keys.dim() != 4 or keys.shape != values.shape or keys.dtype != values.dtype:
+            raise PreconditionFailure("the cache is two equal arrays [blocks, kvHeads, blockSize, headDim]")
+        if not (self._here(keys) and self._here(values) and keys.is_contiguous() and values.is_contiguous()):
+            raise PreconditionFailure("the cache must be contiguous tensors on this device")
+        n, nkv, bs, hd = keys.shape
+        return _abi.PagedLayout(n, bs, nkv, hd, self._paged_type(keys), 0, 0)
+
+    # -- Sampler (Sampler.swift) with the caller's random numbers ----------------
+    def sample(self, logits: np.ndarray, u, temperature=1.0, topK=0, topP=1.0, minP=0.0):
+        """tbh_sample on host arrays: logits [rows, vocab] or [vocab], u and
+        the settings one number or one per row.  Returns (tokens int32, probs
+        float32), shaped like the rows."""
+        x = np.ascontiguousarray(logits, np.float32)
+        if x.ndim not in (1, 2):
+            raise PreconditionFailure("sample: logits must be [vocab] or [rows, vocab]")
+        rows, vocab = (1, x.shape[0]) if x.ndim == 1 else x.shape
+
+        def per_row(value, dtype):
+            a = np.asarray(value, dtype)
+            if a.ndim > 1 or (a.ndim == 1 and a.shape[0] != rows):
+                raise PreconditionFailure("sample: settings must be one number or one per row")
+            return np.ascontiguousarray(np.broadcast_to(a, (rows,)))
+
+        args = [per_row(temperature, np.float32), per_row(topK, np.int32), per_row(topP, np.float32),
+                per_row(minP, np.float32), per_row(u, np.float32)]
+        tokens, probs = np.empty(rows, np.int32), np.empty(rows, np.float32)
+        _check(self._lib.tbh_sample(self._dev, x.ctypes.data, rows, vocab, *[a.ctypes.data for a in args],
+                                    tokens.ctypes.data, probs.ctypes.data))
+        return (tokens[0], probs[0]) if x.ndim == 1 else (tokens, probs)
+
+    def sample_device(self, logits, u, temperature=None, topK=None, topP=None, minP=None, tokens=None, probs=None,
+                      stream=None):
+        """tbh_sample_device on torch tensors: logits float32 [rows, vocab]
+        (rows may be strided), u float32 [rows], settings None or [rows]
+        (float32; topK int32).  Returns (tokens int32, probs float32)."""
+        import torch
+
+        if logits.dim() != 2 or logits.dtype != torch.float32 or not self._here(logits) or \
+                (logits.shape[1] > 1 and logits.stride(1) != 1):
+            raise PreconditionFailure("sample: logits must be float32 device rows [rows, vocab]")
+        rows, vocab = logits.shape
+        for t, dtype in ((u, torch.float32), (temperature, torch.float32), (topK, torch.int32), (topP, torch.float32),
+                         (minP, torch.float32), (tokens, torch.int32), (probs, torch.float32)):
+            if t is not None and (t.dtype != dtype or t.numel() != rows or not t.is_contiguous() or not self._here(t)):
+                raise PreconditionFailure("sample: u and settings must be contiguous device tensors, one entry per row")
+        if tokens is None:
+            tokens = self._made(torch.empty(rows, dtype=torch.int32, device=logits.device), stream)
+        if probs is None:
+            probs = self._made(torch.empty(rows, dtype=torch.float32, device=logits.device), stream)
+        _check(self._lib.tbh_sample_device(
+            self._dev, logits.data_ptr(), logits.stride(0), rows, vocab,
+            *[None if t is None else t.data_ptr() for t in (temperature, topK, topP, minP)], u.data_ptr(),
+            tokens.data_ptr(), probs.data_ptr(), self._stream(logits, stream)))
+        return tokens, probs
 
     def close(self) -> None:
         with self._lock:
