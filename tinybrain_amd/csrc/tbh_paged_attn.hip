@@ -102,8 +102,565 @@ __global__ __launch_bounds__(256) void paged_rows(const PagedArgs a) {
             ((XT *)a.out)[t * a.out_stride + (int64_t)h * a.hd + lane + 64 * i] = (XT)(seen ? o[i] / l : 0.0f);
 }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// A request's rows as the kernels below take them: row r of a key/value head
+// is token r / rep, query head r % rep of its group.
+struct Request {
+    int32_t first, n;      // its rows of q that exist
+    int32_t rows;          // n * rep
+    int32_t held;          // positions in the cache
+    int32_t base;          // position of its first row, negative where rows exceed positions
+};
+
+__device__ __forceinline__ Request request(const PagedArgs &a, int32_t b) {
+    Request r;
+    const int64_t first = a.start[b], end = a.start[b + 1];
+    r.held = (int32_t)min((int64_t)max(a.ctx[b], 0), (int64_t)a.most << a.shift);
+    r.first = (int32_t)first;
+    const bool ok = first >= 0 && first < a.tokens && end > first;
+    r.n = ok ? (int32_t)(min(end, a.tokens) - first) : 0;
+    r.base = ok ? (int32_t)(r.held - (end - first)) : 0;
+    r.rows = r.n * a.rep;
+    return r;
+}
+
+// How a range of `len` positions is cut for at most `splits` blocks: parts of
+// `chunk` positions, a multiple of 128 and at least the caller's.
+struct Cut {
+    int32_t parts, chunk;
+};
+__device__ __forceinline__ Cut cut(int32_t len, int32_t splits, int32_t least) {
+    const int32_t even = (len + splits - 1) / splits;
+    const int32_t chunk = max(least, (even + 127) / 128 * 128);
+    return {max(1, (len + chunk - 1) / chunk), chunk};
+}
+
+struct SplitArgs {
+    PagedArgs a;
+    int32_t splits, least; // see cut
+    int32_t slots;         // rows of a unit in the partials, at most 16
+    int32_t long_rows;     // requests of more rows are another launch's (paged_tile)
+    bool scan;             // units are groups of 16 rows of any request, else requests
+    bool qvec;             // q rows are 16-byte aligned
+    float2 *ml;            // partials [unit][split][slots]: (max, sum)
+    float *po;             // and sums of p v, [unit][split][slots][head_dim]
+};
+
+// 16 rows of one key/value head.
+struct Group {
+    Request q;
+    int32_t b, kvh, row0, rows;    // rows: of this group
+    int32_t len;                   // positions its last row sees
+};
+
+// Finds group `index` of the requests' groups of ROWS rows, heads fastest.
+template <int ROWS>
+__device__ __forceinline__ bool find_group(const PagedArgs &a, int64_t index, int32_t more_than, Group &g) {
+    const int lane = threadIdx.x & 63;
+    g.kvh = (int)(index % a.nkv);
+    int32_t left = (int32_t)(index / a.nkv);
+    for (int32_t b0 = 0; b0 < a.requests; b0 += 64) {
+        Request r{};
+        if (b0 + lane < a.requests) r = request(a, b0 + lane);
+        const int32_t mine = r.rows > more_than ? (r.rows + ROWS - 1) / ROWS : 0;
+        int32_t in = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int32_t o = __shfl_up(in, d);
+            if (lane >= d) in += o;
+        }
+        const int32_t total = __builtin_amdgcn_readlane(in, 63);
+        if (left < total) {
+            const int l = __builtin_ctzll(__ballot(in > left));
+            g.b = b0 + l;
+            // the last rows first: they see the most positions
+            g.row0 = (__builtin_amdgcn_readlane(in, l) - 1 - left) * ROWS;
+            g.q.first = __builtin_amdgcn_readlane(r.first, l);
+            g.q.n = __builtin_amdgcn_readlane(r.n, l);
+            g.q.rows = __builtin_amdgcn_readlane(r.rows, l);
+            g.q.held = __builtin_amdgcn_readlane(r.held, l);
+            g.q.base = __builtin_amdgcn_readlane(r.base, l);
+            return true;
+        }
+        left -= total;
+    }
+    return false;
+}
+
+template <int ROWS>
+__device__ __forceinline__ void set_rows(const PagedArgs &a, Group &g, int32_t row0) {
+    g.row0 = row0;
+    g.rows = min(ROWS, g.q.rows - row0);
+    g.len = min(g.q.held, max(0, g.q.base + (row0 + g.rows - 1) / a.rep + 1));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Largest value over the four lanes that hold one row (lane % 16).
+__device__ __forceinline__ float row4_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float row4_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// x as a sum of NP bf16 values: exact for NP = 3 (8 + 8 + 8 bits), rounded for 1.
+template <int NP>
+__device__ __forceinline__ void pieces(float x, __bf16 (&p)[NP]) {
+    p[0] = (__bf16)x;
+    if constexpr (NP == 3) {
+        const float r = x - (float)p[0];
+        const bool finite = fabsf((float)p[0]) < INFINITY;   // inf and NaN are held by the first piece
+        p[1] = (__bf16)(finite ? r : 0.0f);
+        p[2] = (__bf16)(finite ? r - (float)p[1] : 0.0f);
+    }
+}
+
+// Eight elements of row n of q from dimension d on (0 behind the head).
+template <class XT>
+__device__ __forceinline__ void load_q8(const PagedArgs &a, int64_t t, int head, int d, bool vec, float (&x)[8]) {
+    const XT *p = (const XT *)a.q + t * a.q_stride + (int64_t)head * a.hd + d;
+    if (vec) {
+        unpack(*(const Vec8<XT> *)p, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (float)p[i];
+    }
+}
+
+template <int N>
+struct __attribute__((aligned(4))) Words {
+    uint32_t w[N];
+};
+
+// The two products of 32 positions (two tiles of 16, each inside a block) with
+// 16 rows, operands straight from the cache.  Scores are formed transposed,
+// keys x queries, so that lane (g = lane / 16, n = lane % 16) holds positions 4g
+// + i of each tile for row n: the layout in which the second product, values
+// transposed x probabilities, takes its right operand, if its reduction index
+// 8g + c (bf16) or g (fp32) is read as position 4g + c % 4 of tile c / 4, or 4g +
+// i in the i-th instruction.  VD = HD / 16 consecutive dimensions of a value
+// row per lane: lane (g, n) ends with outputs 4 VD g .. 4 VD (g + 1) of row n.
+template <class XT, class CT, int HD>
+struct Step;
+
+template <class XT, int HD>
+struct Step<XT, __bf16, HD> {
+    static constexpr int NP = sizeof(XT) == 4 ? 3 : 1;   // bf16 pieces of q and p
+    static constexpr int NJ = HD / 32, VD = HD / 16, VW = VD / 2;
+    bf16x8 q[NP][NJ];
+    bf16x8 k[2][NJ];
+    Words<VW> v[2][4];
+
+    __device__ __forceinline__ void load_q(const PagedArgs &a, int64_t t, int head, int g, bool vec) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            float x[8];
+            load_q8<XT>(a, t, head, 32 * j + 8 * g, vec, x);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                __bf16 p[NP];
+                pieces<NP>(x[c], p);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) q[i][j][c] = p[i];
+            }
+        }
+    }
+    __device__ __forceinline__ void load(int t, const __bf16 *kp, const __bf16 *vp, int g, int n) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) k[t][j] = *(const bf16x8 *)(kp + n * HD + 32 * j + 8 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[t][i] = *(const Words<VW> *)(vp + (4 * g + i) * HD + VD * n);
+    }
+    __device__ __forceinline__ void drop_value(int t, int i) {
+#pragma unroll
+        for (int w = 0; w < VW; ++w) v[t][i].w[w] = 0;
+    }
+    __device__ __forceinline__ bool odd_values() const {   // inf or NaN among this lane's values
+        bool r = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int w = 0; w < VW; ++w)
+                    r |= (v[t][i].w[w] & 0x7F80u) == 0x7F80u || (v[t][i].w[w] & 0x7F800000u) == 0x7F800000u;
+        return r;
+    }
+    __device__ __forceinline__ f32x4 scores(int t) const {
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = NP - 1; i >= 0; --i)              // the smallest pieces first
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[t][j], q[i][j], s, 0, 0, 0);
+        return s;
+    }
+    __device__ __forceinline__ void values(const f32x4 (&p)[2], f32x4 (&o)[VD]) const {
+        bf16x8 pp[NP];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            __bf16 x[NP];
+            pieces<NP>(p[c / 4][c % 4], x);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) pp[i][c] = x[i];
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {              // dimension 2w + h of eight positions
+                uint32_t e[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    e[c] = __builtin_amdgcn_perm(v[c / 2][2 * (c % 2) + 1].w[w], v[c / 2][2 * (c % 2)].w[w],
+                                                 h ? 0x07060302u : 0x05040100u);
+                const bf16x8 vv = __builtin_bit_cast(bf16x8, uint4{e[0], e[1], e[2], e[3]});
+#pragma unroll
+                for (int i = NP - 1; i >= 0; --i)
+                    o[2 * w + h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pp[i], o[2 * w + h], 0, 0, 0);
+            }
+    }
+};
+
+template <class XT, int HD>
+struct Step<XT, float, HD> {
+    static constexpr int NJ = HD / 16, VD = HD / 16;
+    float q[NJ][4];
+    f32x4 k[2][NJ];
+    Words<VD> v[2][4];
+
+    __device__ __forceinline__ void load_q(const PagedArgs &a, int64_t t, int head, int g, bool) {
+        const XT *p = (const XT *)a.q + t * a.q_stride + (int64_t)head * a.hd + 4 * g;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) q[j][c] = (float)p[16 * j + c];
+    }
+    __device__ __forceinline__ void load(int t, const float *kp, const float *vp, int g, int n) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) k[t][j] = *(const f32x4 *)(kp + n * HD + 16 * j + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[t][i] = *(const Words<VD> *)(vp + (4 * g + i) * HD + VD * n);
+    }
+    __device__ __forceinline__ void drop_value(int t, int i) {
+#pragma unroll
+        for (int w = 0; w < VD; ++w) v[t][i].w[w] = 0;
+    }
+    __device__ __forceinline__ bool odd_values() const {
+        bool r = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int w = 0; w < VD; ++w) r |= (v[t][i].w[w] & 0x7F800000u) == 0x7F800000u;
+        return r;
+    }
+    __device__ __forceinline__ f32x4 scores(int t) const {
+        f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};   // two chains: half the rounding of one
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                s[c & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][j][c], q[j][c], s[c & 1], 0, 0, 0);
+        return s[0] + s[1];
+    }
+    __device__ __forceinline__ void values(const f32x4 (&p)[2], f32x4 (&o)[VD]) const {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int d = 0; d < VD; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, v[t][i].w[d]), p[t][i], o[d],
+                                                                0, 0, 0);
+    }
+};
+
+// o += p v over 32 positions without the matrix instruction, for steps where
+// some rows do not see a position whose value is inf or NaN: its probability 0
+// times that value would be NaN.
+template <class CT, int HD>
+__device__ __forceinline__ void values_apart(const f32x4 (&p)[2], const CT *const (&vp)[2], int32_t p0, int32_t end,
+                                             int32_t last, const bool (&there)[2], int lane, f32x4 (&o)[HD / 16]) {
+    constexpr int VD = HD / 16;
+    const int g = lane >> 4, n = lane & 15;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll 1
+            for (int h = 0; h < 4; ++h) {
+                const float x = __shfl(p[t][i], 16 * h + n);
+                const int32_t pos = p0 + 16 * t + 4 * h + i;
+                if (!there[t] || pos >= end || pos > last) continue;
+                const CT *row = vp[t] + (4 * h + i) * HD + 4 * VD * g;
+#pragma unroll
+                for (int e = 0; e < 4 * VD; ++e) o[e % VD][e / VD] += x * (float)row[e];
+            }
+}
+
+// Few rows per request (single tokens of grouped heads, short chunks): 16 rows
+// and one part of the positions a block, its four waves taking steps of 32
+// positions in turn and meeting in LDS at the end.  Bound by reading the cache.
+template <class XT, class CT, int HD>
+__global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
+    constexpr int VD = HD / 16, LD = HD + 4;
+    __shared__ __attribute__((aligned(16))) float so[4][16][LD];
+    __shared__ float2 sml[4][16];
+    const PagedArgs &a = sa.a;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int g = lane >> 4, n = lane & 15;
+    const int split = (int)(blockIdx.x % sa.splits);
+    const int64_t unit = blockIdx.x / sa.splits;
+    Group gr;
+    bool alone = false;            // more rows than a unit has places for: no parts
+    if (sa.scan) {
+        if (!find_group<16>(a, unit, 0, gr)) return;
+    } else {
+        gr.kvh = (int)(unit % a.nkv);
+        gr.b = (int32_t)(unit / a.nkv);
+        gr.q = request(a, gr.b);
+        gr.row0 = 0;
+        if (gr.q.rows == 0 || gr.q.rows > sa.long_rows) return;
+        alone = gr.q.rows > sa.slots;
+    }
+    const int32_t end_row = sa.scan ? gr.row0 + 1 : gr.q.rows;
+    const int32_t *table = a.table + (int64_t)gr.b * a.most;
+    const float c2 = a.scale * 1.44269504f;   // scores in powers of two
+    const int64_t head_rows = (int64_t)HD << a.shift;
+    const CT *kb = (const CT *)a.kc + gr.kvh * head_rows, *vb = (const CT *)a.vc + gr.kvh * head_rows;
+
+    for (int32_t row0 = gr.row0; row0 < end_row; row0 += 16) {
+        set_rows<16>(a, gr, row0);
+        const Cut ct = alone ? Cut{1, max(gr.len, 1)} : cut(gr.len, sa.splits, sa.least);
+        if (split >= ct.parts) return;
+        const int32_t c0 = split * ct.chunk, c1 = min(gr.len, c0 + ct.chunk);
+        const int32_t r = row0 + min(n, gr.rows - 1);
+        const int32_t token = r / a.rep;
+        const int32_t last = min(gr.q.base + token, gr.q.held - 1);   // this row's position
+        const int32_t first_last = min(gr.q.base + row0 / a.rep, gr.q.held - 1);   // the first row's
+        Step<XT, CT, HD> st;
+        st.load_q(a, gr.q.first + token, gr.kvh * a.rep + r % a.rep, g, sa.qvec);
+
+        float m = -INFINITY, l = 0.0f;   // l: this lane's positions only
+        bool seen = false;
+        f32x4 o[VD];
+#pragma unroll
+        for (int d = 0; d < VD; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int32_t p0 = c0 + 32 * w; p0 < c1; p0 += 128) {
+            bool there[2];               // the tile has a block (uniform)
+            const CT *vp[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int32_t p = p0 + 16 * t;
+                const int32_t id = p < c1 ? __builtin_amdgcn_readfirstlane(table[p >> a.shift]) : -1;
+                there[t] = (uint32_t)id < (uint32_t)a.num_blocks;
+                const int64_t at =
+                    (int64_t)(there[t] ? id : 0) * a.nkv * head_rows + (int64_t)(p & ((1 << a.shift) - 1)) * HD;
+                vp[t] = vb + at;
+                st.load(t, kb + at, vp[t], g, n);
+            }
+            f32x4 s[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) s[t] = st.scores(t);
+            float nm = m;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                seen |= there[t] && p0 + 16 * t <= last;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool on = there[t] && p0 + 16 * t + 4 * g + i <= last;
+                    s[t][i] = on ? s[t][i] * c2 : -INFINITY;
+                    nm = fmaxf(nm, s[t][i]);
+                }
+            }
+            if (!there[0] || !there[1] || p0 + 32 > c1) {   // what lies there may be NaN: 0 * NaN
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!there[t] || p0 + 16 * t + 4 * g + i >= c1) st.drop_value(t, i);
+            }
+            nm = row4_max(nm);
+            const float ref = nm == -INFINITY ? 0.0f : nm;
+            const float corr = exp2_fast(m - ref);
+            m = nm;
+            l *= corr;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[t][i] = exp2_fast(s[t][i] - ref);
+                    l += s[t][i];
+                }
+#pragma unroll
+            for (int d = 0; d < VD; ++d) o[d] *= corr;
+            if (p0 + 31 > first_last && __any(st.odd_values()))
+                values_apart<CT, HD>(s, vp, p0, c1, last, there, lane, o);
+            else
+                st.values(s, o);
+        }
+        l = row4_sum(l);
+        if (m == -INFINITY) l = seen ? 1.0f : 0.0f;   // positions seen, each of score -inf; none at all
+
+        // the four waves' parts
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < VD; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) so[w][n][4 * VD * g + VD * i + d] = o[d][i];
+        if (g == 0) sml[w][n] = float2{m, l};
+        __syncthreads();
+        for (int e = tid; e < gr.rows * HD; e += 256) {
+            const int rr = e / HD, d = e % HD;
+            float mm = -INFINITY, ll = 0.0f, v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mm = fmaxf(mm, sml[i][rr].x);
+            float none = 0.0f;           // a wave has seen positions
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 ml = sml[i][rr];
+                const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - mm);
+                none = fmaxf(none, ml.y);
+                ll += f * ml.y;
+                v += f * so[i][rr][d];
+            }
+            if (mm == -INFINITY) ll = none;
+            if (ct.parts == 1) {
+                const int32_t tt = (row0 + rr) / a.rep;
+                const int head = gr.kvh * a.rep + (row0 + rr) % a.rep;
+                // nothing seen: 0; only scores of -inf: 0 / 0
+                const float res = mm == -INFINITY ? (ll > 0.0f ? NAN : 0.0f) : v / ll;
+                ((XT *)a.out)[(int64_t)(gr.q.first + tt) * a.out_stride + (int64_t)head * HD + d] = (XT)res;
+            } else {
+                const int64_t at = (unit * sa.splits + split) * sa.slots + rr;
+                if (d == 0) sa.ml[at] = float2{mm, ll};
+                sa.po[at * HD + d] = v;
+            }
+        }
+    }
+}
+
+// Joins paged_split's parts: a block per unit and row, HD / 4 threads across the
+// head, the parts dealt over the rest.
+template <class XT, int HD>
+__global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa) {
+    constexpr int T = HD / 4, G = 256 / T;
+    __shared__ f32x4 red[G][T];
+    __shared__ float sl[G];
+    const PagedArgs &a = sa.a;
+    const int tid = threadIdx.x, d4 = tid % T, sg = tid / T;
+    const int rr = (int)(blockIdx.x % sa.slots);
+    const int64_t unit = blockIdx.x / sa.slots;
+    Group gr;
+    if (sa.scan) {
+        if (!find_group<16>(a, unit, 0, gr)) return;
+    } else {
+        gr.kvh = (int)(unit % a.nkv);
+        gr.b = (int32_t)(unit / a.nkv);
+        gr.q = request(a, gr.b);
+        gr.row0 = 0;
+        if (gr.q.rows == 0 || gr.q.rows > sa.long_rows || gr.q.rows > sa.slots) return;
+    }
+    set_rows<16>(a, gr, gr.row0);
+    const Cut ct = cut(gr.len, sa.splits, sa.least);
+    if (ct.parts == 1 || rr >= gr.rows) return;
+    const float2 *ml = sa.ml + unit * sa.splits * sa.slots + rr;
+    const float *po = sa.po + (unit * sa.splits * sa.slots + rr) * HD + 4 * d4;
+    float mm = -INFINITY, any = 0.0f;
+    for (int s = 0; s < ct.parts; ++s) {
+        const float2 x = ml[(int64_t)s * sa.slots];
+        mm = fmaxf(mm, x.x);
+        any = fmaxf(any, x.y);
+    }
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.0f;
+    if (sg < G)
+        for (int s = sg; s < ct.parts; s += G) {
+            const float2 x = ml[(int64_t)s * sa.slots];
+            const float f = x.x == -INFINITY ? 0.0f : exp2_fast(x.x - mm);
+            l += f * x.y;
+            o += f * *(const f32x4 *)(po + (int64_t)s * sa.slots * HD);
+        }
+    if (sg < G) {
+        red[sg][d4] = o;
+        if (d4 == 0) sl[sg] = l;
+    }
+    __syncthreads();
+    if (sg != 0) return;
+    f32x4 v = red[0][d4];
+    float ll = sl[0];
+    for (int i = 1; i < G; ++i) {
+        v += red[i][d4];
+        ll += sl[i];
+    }
+    const int32_t row = gr.row0 + rr;
+    XT *out = (XT *)a.out + (int64_t)(gr.q.first + row / a.rep) * a.out_stride +
+              (int64_t)(gr.kvh * a.rep + row % a.rep) * HD + 4 * d4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = (XT)(mm == -INFINITY ? (any > 0.0f ? NAN : 0.0f) : v[i] / ll);
+}
+
+// Positions a part of paged_split has at least, for `units` units: enough blocks
+// to fill the chip, parts no longer than 1024 (a batch's longest request would
+// else end long after the others) and no shorter than 128 (a step per wave).
+int32_t split_least(int64_t units, int64_t context, int64_t cus) {
+    const int64_t parts = std::max<int64_t>(1, 4 * cus / std::max<int64_t>(units, 1));
+    const int64_t even = (context + parts - 1) / parts;
+    return (int32_t)std::min<int64_t>(1024, std::max<int64_t>(128, (even + 127) / 128 * 128));
+}
+
+constexpr int64_t kMaxSplits = 64;
+
+template <class XT, class CT, int HD>
+hipError_t launch_split(tbh_device *dev, const PagedArgs &a, int64_t query, int64_t context, bool tiles,
+                        hipStream_t s) {
+    SplitArgs sa{};
+    sa.a = a;
+    sa.qvec = aligned(a.q, 16) && (a.q_stride * (int64_t)sizeof(XT)) % 16 == 0;
+    sa.scan = !tiles && query * a.rep > 16;
+    const int64_t units = (sa.scan ? a.tokens * a.rep / 16 + std::min<int64_t>(a.requests, a.tokens) : a.requests) *
+                          a.nkv;
+    sa.long_rows = tiles ? 16 : INT32_MAX;
+    sa.slots = (int32_t)std::min<int64_t>(16, query * a.rep);
+    sa.least = split_least(units, context, std::max(1, dev->cu_count));
+    sa.splits = (int32_t)std::min<int64_t>((context + sa.least - 1) / sa.least, kMaxSplits);
+    if (sa.splits > 1) {
+        const int64_t rows = units * sa.splits * sa.slots;
+        const size_t head = (size_t)rows * sizeof(float2);   // rows of head_dim floats follow, 16-byte aligned
+        const size_t pad = (head + 255) / 256 * 256;
+        char *ws = (char *)stream_workspace(dev, s, pad + (size_t)rows * HD * sizeof(float));
+        if (ws) {
+            sa.ml = (float2 *)ws;
+            sa.po = (float *)(ws + pad);
+        } else {
+            sa.splits = 1;   // no workspace (graph capture before any eager call): whole contexts
+        }
+    }
+    if (units * std::max(sa.splits, sa.slots) > INT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((paged_split<XT, CT, HD>), dim3((unsigned)(units * sa.splits)), dim3(256), 0, s, sa);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || sa.splits == 1) return e;
+    hipLaunchKernelGGL((paged_split_merge<XT, HD>), dim3((unsigned)(units * sa.slots)), dim3(256), 0, s, sa);
+    return hipGetLastError();
+}
+
 template <class XT, class CT>
-hipError_t launch_paged(const PagedArgs &a, hipStream_t s) {
+hipError_t launch_paged(tbh_device *dev, const PagedArgs &a, int64_t query, int64_t context, hipStream_t s) {
+    // the matrix kernels take a tile of 16 positions from one block
+    if (a.shift >= 4 && a.num_blocks > 0 && a.most > 0) {
+        switch (a.hd) {
+        case 32: return launch_split<XT, CT, 32>(dev, a, query, context, false, s);
+        case 64: return launch_split<XT, CT, 64>(dev, a, query, context, false, s);
+        case 96: return launch_split<XT, CT, 96>(dev, a, query, context, false, s);
+        case 128: return launch_split<XT, CT, 128>(dev, a, query, context, false, s);
+        default: break;
+        }
+    }
     hipLaunchKernelGGL((paged_rows<XT, CT>), dim3((unsigned)((a.tokens * a.nh + 3) / 4)), dim3(256), 0, s, a);
     return hipGetLastError();
 }
@@ -162,12 +719,15 @@ tbh_status tbh_paged_attention_device(tbh_device *dev, const tbh_paged_layout *l
     a.rep = q.num_heads / layout->num_kv_heads;
     a.scale = q.scale != 0.0f ? q.scale : 1.0f / std::sqrt((float)layout->head_dim);
     const hipStream_t s = (hipStream_t)stream;
+    const int64_t query = q.max_query_len ? std::min<int64_t>(q.max_query_len, q.tokens) : q.tokens;
+    const int64_t table = (int64_t)layout->max_blocks * layout->block_size;
+    const int64_t context = q.max_context_len ? std::min<int64_t>(q.max_context_len, table) : table;
     hipError_t e;
     switch ((q.type == TBH_BF16) * 2 + (layout->type == TBH_BF16)) {
-    case 0: e = launch_paged<float, float>(a, s); break;
-    case 1: e = launch_paged<float, __bf16>(a, s); break;
-    case 2: e = launch_paged<__bf16, float>(a, s); break;
-    default: e = launch_paged<__bf16, __bf16>(a, s); break;
+    case 0: e = launch_paged<float, float>(dev, a, query, context, s); break;
+    case 1: e = launch_paged<float, __bf16>(dev, a, query, context, s); break;
+    case 2: e = launch_paged<__bf16, float>(dev, a, query, context, s); break;
+    default: e = launch_paged<__bf16, __bf16>(dev, a, query, context, s); break;
     }
     return e == hipSuccess ? TBH_OK : hip_error(e, "paged attention launch");
 }
