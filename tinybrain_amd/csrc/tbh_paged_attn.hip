@@ -45,6 +45,13 @@ __device__ __forceinline__ int64_t place(const PagedArgs &a, int32_t b, int32_t 
     return ((((int64_t)id * a.nkv + kvh) << a.shift) + (pos & ((1 << a.shift) - 1))) * a.hd;
 }
 
+// Orders a wave's LDS writes before later LDS reads by its other lanes.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // Any head dimension, type and alignment: one wave per (token, query head),
 // 64 positions a pass, a position per lane for the scores and an output
 // dimension per lane for the values.
@@ -62,9 +69,7 @@ __global__ __launch_bounds__(256) void paged_rows(const PagedArgs a) {
     const int64_t behind = (int64_t)a.start[b + 1] - 1 - t;   // rows of the request after this one
     const int32_t last = (int32_t)min(held - 1, held - 1 - behind);   // this row's position
     for (int d = lane; d < a.hd; d += 64) qs[w][d] = elem<XT>(a.q, t * a.q_stride + (int64_t)h * a.hd + d);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    wave_lds_fence();
 
     float m = -INFINITY, l = 0.0f, o[kMaxHeadDim / 64] = {};
     bool seen = false;
@@ -139,6 +144,7 @@ __device__ __forceinline__ Cut cut(int32_t len, int32_t splits, int32_t least) {
 
 struct SplitArgs {
     PagedArgs a;
+    int32_t units;         // (16 rows, key/value head) pairs
     int32_t splits, least; // see cut
     int32_t slots;         // rows of a unit in the partials, at most 16
     int32_t long_rows;     // requests of more rows are another launch's (paged_tile)
@@ -157,10 +163,10 @@ struct Group {
 
 // Finds group `index` of the requests' groups of ROWS rows, heads fastest.
 template <int ROWS>
-__device__ __forceinline__ bool find_group(const PagedArgs &a, int64_t index, int32_t more_than, Group &g) {
+__device__ __forceinline__ bool find_group(const PagedArgs &a, uint32_t index, int32_t more_than, Group &g) {
     const int lane = threadIdx.x & 63;
-    g.kvh = (int)(index % a.nkv);
-    int32_t left = (int32_t)(index / a.nkv);
+    g.kvh = (int)(index % (uint32_t)a.nkv);
+    int32_t left = (int32_t)(index / (uint32_t)a.nkv);
     for (int32_t b0 = 0; b0 < a.requests; b0 += 64) {
         Request r{};
         if (b0 + lane < a.requests) r = request(a, b0 + lane);
@@ -270,26 +276,30 @@ struct Step<XT, __bf16, HD> {
             }
         }
     }
-    __device__ __forceinline__ void load(int t, const __bf16 *kp, const __bf16 *vp, int g, int n) {
+    __device__ __forceinline__ void load_keys(int t, const __bf16 *p, int g, int n) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) k[t][j] = *(const bf16x8 *)(kp + n * HD + 32 * j + 8 * g);
+        for (int j = 0; j < NJ; ++j) k[t][j] = *(const bf16x8 *)(p + n * HD + 32 * j + 8 * g);
+    }
+    __device__ __forceinline__ void load_values(int t, const __bf16 *p, int g, int n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[t][i] = *(const Words<VW> *)(vp + (4 * g + i) * HD + VD * n);
+        for (int i = 0; i < 4; ++i) v[t][i] = *(const Words<VW> *)(p + (4 * g + i) * HD + VD * n);
     }
     __device__ __forceinline__ void drop_value(int t, int i) {
 #pragma unroll
         for (int w = 0; w < VW; ++w) v[t][i].w[w] = 0;
     }
     __device__ __forceinline__ bool odd_values() const {   // inf or NaN among this lane's values
-        bool r = false;
+        uint32_t lo = 0, hi = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int w = 0; w < VW; ++w)
-                    r |= (v[t][i].w[w] & 0x7F80u) == 0x7F80u || (v[t][i].w[w] & 0x7F800000u) == 0x7F800000u;
-        return r;
+                for (int w = 0; w < VW; ++w) {
+                    lo = max(lo, v[t][i].w[w] & 0x7F80u);
+                    hi = max(hi, v[t][i].w[w] & 0x7F800000u);
+                }
+        return lo == 0x7F80u || hi == 0x7F800000u;
     }
     __device__ __forceinline__ f32x4 scores(int t) const {
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
@@ -339,25 +349,27 @@ struct Step<XT, float, HD> {
 #pragma unroll
             for (int c = 0; c < 4; ++c) q[j][c] = (float)p[16 * j + c];
     }
-    __device__ __forceinline__ void load(int t, const float *kp, const float *vp, int g, int n) {
+    __device__ __forceinline__ void load_keys(int t, const float *p, int g, int n) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) k[t][j] = *(const f32x4 *)(kp + n * HD + 16 * j + 4 * g);
+        for (int j = 0; j < NJ; ++j) k[t][j] = *(const f32x4 *)(p + n * HD + 16 * j + 4 * g);
+    }
+    __device__ __forceinline__ void load_values(int t, const float *p, int g, int n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[t][i] = *(const Words<VD> *)(vp + (4 * g + i) * HD + VD * n);
+        for (int i = 0; i < 4; ++i) v[t][i] = *(const Words<VD> *)(p + (4 * g + i) * HD + VD * n);
     }
     __device__ __forceinline__ void drop_value(int t, int i) {
 #pragma unroll
         for (int w = 0; w < VD; ++w) v[t][i].w[w] = 0;
     }
     __device__ __forceinline__ bool odd_values() const {
-        bool r = false;
+        uint32_t e = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int w = 0; w < VD; ++w) r |= (v[t][i].w[w] & 0x7F800000u) == 0x7F800000u;
-        return r;
+                for (int w = 0; w < VD; ++w) e = max(e, v[t][i].w[w] & 0x7F800000u);
+        return e == 0x7F800000u;
     }
     __device__ __forceinline__ f32x4 scores(int t) const {
         f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};   // two chains: half the rounding of one
@@ -382,25 +394,26 @@ struct Step<XT, float, HD> {
 
 // o += p v over 32 positions without the matrix instruction, for steps where
 // some rows do not see a position whose value is inf or NaN: its probability 0
-// times that value would be NaN.
+// times that value would be NaN.  ps: this wave's LDS, [position][row].
 template <class CT, int HD>
-__device__ __forceinline__ void values_apart(const f32x4 (&p)[2], const CT *const (&vp)[2], int32_t p0, int32_t end,
-                                             int32_t last, const bool (&there)[2], int lane, f32x4 (&o)[HD / 16]) {
+__device__ __forceinline__ void values_apart(const f32x4 (&p)[2], float *ps, const CT *v0, const CT *v1, int32_t p0,
+                                             int32_t end, int32_t last, int there, int lane, f32x4 (&o)[HD / 16]) {
     constexpr int VD = HD / 16;
     const int g = lane >> 4, n = lane & 15;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) ps[(16 * t + 4 * g + i) * 16 + n] = p[t][i];
+    wave_lds_fence();
 #pragma unroll 1
-            for (int h = 0; h < 4; ++h) {
-                const float x = __shfl(p[t][i], 16 * h + n);
-                const int32_t pos = p0 + 16 * t + 4 * h + i;
-                if (!there[t] || pos >= end || pos > last) continue;
-                const CT *row = vp[t] + (4 * h + i) * HD + 4 * VD * g;
+    for (int j = 0; j < 32 && p0 + j < end; ++j) {
+        if (!(there >> (j >> 4) & 1) || p0 + j > last) continue;
+        const float x = ps[j * 16 + n];
+        const CT *row = (j < 16 ? v0 : v1) + (j & 15) * HD + 4 * VD * g;
 #pragma unroll
-                for (int e = 0; e < 4 * VD; ++e) o[e % VD][e / VD] += x * (float)row[e];
-            }
+        for (int e = 0; e < 4 * VD; ++e) o[e % VD][e / VD] += x * (float)row[e];
+    }
+    wave_lds_fence();
 }
 
 // Few rows per request (single tokens of grouped heads, short chunks): 16 rows
@@ -414,15 +427,17 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
     const PagedArgs &a = sa.a;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, n = lane & 15;
-    const int split = (int)(blockIdx.x % sa.splits);
-    const int64_t unit = blockIdx.x / sa.splits;
+    // The units run fastest: consecutive blocks go to different XCDs, and with the
+    // parts fastest one XCD would get every request's first part and another only
+    // those of the longest (64 requests of 100 .. 8192 positions: 216 us for 107).
+    const uint32_t unit = blockIdx.x % (uint32_t)sa.units, split = blockIdx.x / (uint32_t)sa.units;
     Group gr;
     bool alone = false;            // more rows than a unit has places for: no parts
     if (sa.scan) {
         if (!find_group<16>(a, unit, 0, gr)) return;
     } else {
-        gr.kvh = (int)(unit % a.nkv);
-        gr.b = (int32_t)(unit / a.nkv);
+        gr.kvh = (int)(unit % (uint32_t)a.nkv);
+        gr.b = (int32_t)(unit / (uint32_t)a.nkv);
         gr.q = request(a, gr.b);
         gr.row0 = 0;
         if (gr.q.rows == 0 || gr.q.rows > sa.long_rows) return;
@@ -431,59 +446,79 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
     const int32_t end_row = sa.scan ? gr.row0 + 1 : gr.q.rows;
     const int32_t *table = a.table + (int64_t)gr.b * a.most;
     const float c2 = a.scale * 1.44269504f;   // scores in powers of two
-    const int64_t head_rows = (int64_t)HD << a.shift;
-    const CT *kb = (const CT *)a.kc + gr.kvh * head_rows, *vb = (const CT *)a.vc + gr.kvh * head_rows;
+    const int32_t head_rows = HD << a.shift, in_block = (1 << a.shift) - 1;
+    const int64_t block_rows = (int64_t)head_rows * a.nkv;
+    const CT *kb = (const CT *)a.kc + (int64_t)gr.kvh * head_rows, *vb = (const CT *)a.vc + (int64_t)gr.kvh * head_rows;
 
     for (int32_t row0 = gr.row0; row0 < end_row; row0 += 16) {
         set_rows<16>(a, gr, row0);
         const Cut ct = alone ? Cut{1, max(gr.len, 1)} : cut(gr.len, sa.splits, sa.least);
-        if (split >= ct.parts) return;
+        if ((int32_t)split >= ct.parts) return;
         const int32_t c0 = split * ct.chunk, c1 = min(gr.len, c0 + ct.chunk);
         const int32_t r = row0 + min(n, gr.rows - 1);
         const int32_t token = r / a.rep;
         const int32_t last = min(gr.q.base + token, gr.q.held - 1);   // this row's position
         const int32_t first_last = min(gr.q.base + row0 / a.rep, gr.q.held - 1);   // the first row's
         Step<XT, CT, HD> st;
+
+        // The blocks of a step's two tiles are looked up two steps ahead, its
+        // keys loaded once the step before has used its own, values likewise.
+        struct Pair {
+            int32_t id[2];
+        };
+        auto look = [&](int32_t p0) {
+            Pair r;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int32_t p = p0 + 16 * t;
+                r.id[t] = p < c1 ? table[p >> a.shift] : -1;
+            }
+            return r;
+        };
+        auto there = [&](const Pair &x, int t) { return (uint32_t)x.id[t] < (uint32_t)a.num_blocks; };
+        auto at = [&](const Pair &x, int t, int32_t p0) {   // a tile without a block: any block's rows, not used
+            return (int64_t)(there(x, t) ? x.id[t] : 0) * block_rows + ((p0 + 16 * t) & in_block) * HD;
+        };
+        int32_t p0 = c0 + 32 * w;
+        Pair cur = look(p0), nxt = look(p0 + 128);
         st.load_q(a, gr.q.first + token, gr.kvh * a.rep + r % a.rep, g, sa.qvec);
+        if (p0 < c1) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) st.load_keys(t, kb + at(cur, t, p0), g, n);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) st.load_values(t, vb + at(cur, t, p0), g, n);
+        }
 
         float m = -INFINITY, l = 0.0f;   // l: this lane's positions only
         bool seen = false;
         f32x4 o[VD];
 #pragma unroll
         for (int d = 0; d < VD; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int32_t p0 = c0 + 32 * w; p0 < c1; p0 += 128) {
-            bool there[2];               // the tile has a block (uniform)
-            const CT *vp[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int32_t p = p0 + 16 * t;
-                const int32_t id = p < c1 ? __builtin_amdgcn_readfirstlane(table[p >> a.shift]) : -1;
-                there[t] = (uint32_t)id < (uint32_t)a.num_blocks;
-                const int64_t at =
-                    (int64_t)(there[t] ? id : 0) * a.nkv * head_rows + (int64_t)(p & ((1 << a.shift) - 1)) * HD;
-                vp[t] = vb + at;
-                st.load(t, kb + at, vp[t], g, n);
-            }
+        for (; p0 < c1; p0 += 128) {
+            const Pair far = look(p0 + 256);
+            const bool th[2] = {there(cur, 0), there(cur, 1)};
             f32x4 s[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) s[t] = st.scores(t);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) st.load_keys(t, kb + at(nxt, t, p0 + 128), g, n);   // behind the part: block 0
             float nm = m;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                seen |= there[t] && p0 + 16 * t <= last;
+                seen |= th[t] && p0 + 16 * t <= last;
+                const int32_t lim = th[t] ? last - (p0 + 16 * t + 4 * g) : -1;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const bool on = there[t] && p0 + 16 * t + 4 * g + i <= last;
-                    s[t][i] = on ? s[t][i] * c2 : -INFINITY;
+                    s[t][i] = i <= lim ? s[t][i] * c2 : -INFINITY;
                     nm = fmaxf(nm, s[t][i]);
                 }
             }
-            if (!there[0] || !there[1] || p0 + 32 > c1) {   // what lies there may be NaN: 0 * NaN
+            if (!th[0] || !th[1] || p0 + 32 > c1) {   // what lies there may be NaN: 0 * NaN
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (!there[t] || p0 + 16 * t + 4 * g + i >= c1) st.drop_value(t, i);
+                        if (!th[t] || p0 + 16 * t + 4 * g + i >= c1) st.drop_value(t, i);
             }
             nm = row4_max(nm);
             const float ref = nm == -INFINITY ? 0.0f : nm;
@@ -497,12 +532,19 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
                     s[t][i] = exp2_fast(s[t][i] - ref);
                     l += s[t][i];
                 }
+            if (__any(corr != 1.0f)) {
 #pragma unroll
-            for (int d = 0; d < VD; ++d) o[d] *= corr;
+                for (int d = 0; d < VD; ++d) o[d] *= corr;
+            }
             if (p0 + 31 > first_last && __any(st.odd_values()))
-                values_apart<CT, HD>(s, vp, p0, c1, last, there, lane, o);
+                values_apart<CT, HD>(s, &so[w][0][0], vb + at(cur, 0, p0), vb + at(cur, 1, p0), p0, c1, last,
+                                     th[0] | th[1] << 1, lane, o);
             else
                 st.values(s, o);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) st.load_values(t, vb + at(nxt, t, p0 + 128), g, n);
+            cur = nxt;
+            nxt = far;
         }
         l = row4_sum(l);
         if (m == -INFINITY) l = seen ? 1.0f : 0.0f;   // positions seen, each of score -inf; none at all
@@ -537,7 +579,7 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
                 const float res = mm == -INFINITY ? (ll > 0.0f ? NAN : 0.0f) : v / ll;
                 ((XT *)a.out)[(int64_t)(gr.q.first + tt) * a.out_stride + (int64_t)head * HD + d] = (XT)res;
             } else {
-                const int64_t at = (unit * sa.splits + split) * sa.slots + rr;
+                const int64_t at = ((int64_t)unit * sa.splits + split) * sa.slots + rr;
                 if (d == 0) sa.ml[at] = float2{mm, ll};
                 sa.po[at * HD + d] = v;
             }
@@ -546,63 +588,54 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
 }
 
 // Joins paged_split's parts: a block per unit and row, HD / 4 threads across the
-// head, the parts dealt over the rest.
+// head, the parts dealt over the rest.  Every wave holds the parts' factors, one
+// per lane.
 template <class XT, int HD>
 __global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa) {
     constexpr int T = HD / 4, G = 256 / T;
     __shared__ f32x4 red[G][T];
-    __shared__ float sl[G];
     const PagedArgs &a = sa.a;
-    const int tid = threadIdx.x, d4 = tid % T, sg = tid / T;
-    const int rr = (int)(blockIdx.x % sa.slots);
-    const int64_t unit = blockIdx.x / sa.slots;
+    const int tid = threadIdx.x, lane = tid & 63, d4 = tid % T, sg = tid / T;
+    const uint32_t rr = blockIdx.x % (uint32_t)sa.slots, unit = blockIdx.x / (uint32_t)sa.slots;
+    const int64_t at0 = (int64_t)unit * sa.splits * sa.slots + rr;
+    const float2 mine = sa.ml[at0 + (int64_t)min(lane, sa.splits - 1) * sa.slots];   // before the request is known
     Group gr;
     if (sa.scan) {
         if (!find_group<16>(a, unit, 0, gr)) return;
     } else {
-        gr.kvh = (int)(unit % a.nkv);
-        gr.b = (int32_t)(unit / a.nkv);
+        gr.kvh = (int)(unit % (uint32_t)a.nkv);
+        gr.b = (int32_t)(unit / (uint32_t)a.nkv);
         gr.q = request(a, gr.b);
         gr.row0 = 0;
         if (gr.q.rows == 0 || gr.q.rows > sa.long_rows || gr.q.rows > sa.slots) return;
     }
     set_rows<16>(a, gr, gr.row0);
     const Cut ct = cut(gr.len, sa.splits, sa.least);
-    if (ct.parts == 1 || rr >= gr.rows) return;
-    const float2 *ml = sa.ml + unit * sa.splits * sa.slots + rr;
-    const float *po = sa.po + (unit * sa.splits * sa.slots + rr) * HD + 4 * d4;
-    float mm = -INFINITY, any = 0.0f;
-    for (int s = 0; s < ct.parts; ++s) {
-        const float2 x = ml[(int64_t)s * sa.slots];
-        mm = fmaxf(mm, x.x);
-        any = fmaxf(any, x.y);
-    }
+    if (ct.parts == 1 || (int32_t)rr >= gr.rows) return;
+    const float *po = sa.po + at0 * HD + 4 * d4;
+    const bool part = lane < ct.parts;
+    const float mm = wave::max(part ? mine.x : -INFINITY);
+    const float f = part && mine.x != -INFINITY ? exp2_fast(mine.x - mm) : 0.0f;
+    const float l = wave::sum(part && f != 0.0f ? f * mine.y : 0.0f);
+    const bool any = __any(part && mine.y > 0.0f);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.0f;
-    if (sg < G)
-        for (int s = sg; s < ct.parts; s += G) {
-            const float2 x = ml[(int64_t)s * sa.slots];
-            const float f = x.x == -INFINITY ? 0.0f : exp2_fast(x.x - mm);
-            l += f * x.y;
-            o += f * *(const f32x4 *)(po + (int64_t)s * sa.slots * HD);
-        }
-    if (sg < G) {
-        red[sg][d4] = o;
-        if (d4 == 0) sl[sg] = l;
+#pragma unroll 4
+    for (int s0 = 0; s0 < ct.parts; s0 += G) {
+        const int s = s0 + sg;
+        const float fs = __shfl(f, min(s, 63));
+        if (s < ct.parts && sg < G) o += fs * *(const f32x4 *)(po + (int64_t)s * sa.slots * HD);
     }
+    if (sg < G) red[sg][d4] = o;
     __syncthreads();
     if (sg != 0) return;
     f32x4 v = red[0][d4];
-    float ll = sl[0];
-    for (int i = 1; i < G; ++i) {
-        v += red[i][d4];
-        ll += sl[i];
-    }
+#pragma unroll
+    for (int i = 1; i < G; ++i) v += red[i][d4];
     const int32_t row = gr.row0 + rr;
     XT *out = (XT *)a.out + (int64_t)(gr.q.first + row / a.rep) * a.out_stride +
               (int64_t)(gr.kvh * a.rep + row % a.rep) * HD + 4 * d4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = (XT)(mm == -INFINITY ? (any > 0.0f ? NAN : 0.0f) : v[i] / ll);
+    for (int i = 0; i < 4; ++i) out[i] = (XT)(mm == -INFINITY ? (any ? NAN : 0.0f) : v[i] / l);
 }
 
 // Positions a part of paged_split has at least, for `units` units: enough blocks
@@ -642,6 +675,7 @@ hipError_t launch_split(tbh_device *dev, const PagedArgs &a, int64_t query, int6
         }
     }
     if (units * std::max(sa.splits, sa.slots) > INT32_MAX) return hipErrorInvalidValue;
+    sa.units = (int32_t)units;
     hipLaunchKernelGGL((paged_split<XT, CT, HD>), dim3((unsigned)(units * sa.splits)), dim3(256), 0, s, sa);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || sa.splits == 1) return e;
