@@ -25,6 +25,7 @@
 // outputs, one 16-byte store.
 #pragma once
 
+#include "tbh_dma.h"
 #include "tbh_internal.h"
 
 #include <algorithm>
@@ -39,7 +40,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
+using dma::dma16;
+using dma::i32x4;
+using dma::lds_addr;
+using dma::make_rsrc;
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -91,26 +95,7 @@ struct Args {
     int32_t row_base, row_end;
 };
 
-__device__ __forceinline__ i32x4 make_rsrc(const void *p, int bytes) {
-    const uint64_t a = (uint64_t)p;
-    const int n = max(bytes, 0);
-    // base (48 bits, stride 0: raw buffer), size, 32-bit data format
-    return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
-                 __builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xFFFFu)),
-                 __builtin_amdgcn_readfirstlane(n), 0x00020000};
-}
-
-// 16 (or 4) bytes per active lane from buffer offset `off` + `soff` to LDS
-// byte lds + 16 (4) * lane; offsets past the buffer's size write zeros.  No
-// register receives the load; completion is waited for by dma_wait.  (One
-// wait state between the write of M0 and the load that reads it.  M0 is a
-// reserved register, which the compiler neither allocates nor takes as a
-// clobber; the built kernels use it in these statements only.)
-__device__ __forceinline__ void dma16(uint32_t lds, i32x4 r, uint32_t off, uint32_t soff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(r),
-                 "s"(soff) : "memory");
-}
-// The same from the lanes of `mask` alone, 16 or 4 bytes a lane (called with
+// dma16 from the lanes of `mask` alone, 16 or 4 bytes a lane (called with
 // every lane active, as EXEC is left, and without a branch that would end the
 // basic block the surrounding instructions are scheduled in).
 template <int BYTES>
@@ -130,10 +115,6 @@ __device__ __forceinline__ void dma_lanes(uint32_t lds, i32x4 r, uint32_t off, u
 template <int LEFT>
 __device__ __forceinline__ void dma_wait() {
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(LEFT) : "memory");
-}
-
-__device__ __forceinline__ uint32_t lds_addr(const void *p) {
-    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)p;
 }
 
 __device__ __forceinline__ uint32_t pack_hi16(float lo_elem, float hi_elem) {

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "tbh_dma.h"
 #include "tbh_paged.h"
 #include "tbh_wave.h"
 
@@ -683,10 +684,369 @@ hipError_t launch_split(tbh_device *dev, const PagedArgs &a, int64_t query, int6
     return hipGetLastError();
 }
 
+struct TileArgs {
+    PagedArgs a;
+    int32_t units;         // (kTileRows rows, key/value head) pairs
+    int32_t splits, least; // see cut
+    bool qvec;             // q rows are 16-byte aligned
+    float2 *ml;            // partials [unit][split][kTileRows]: (max, sum)
+    float *po;             // and sums of p v, [unit][split][kTileRows][head_dim]
+};
+
+// Rows of a tile: two column groups of 16 per wave for bf16 rows; fp32 rows, whose
+// three pieces triple the matrix work per LDS read and the registers of q, one.
+template <class XT>
+constexpr int kTileRows = sizeof(XT) == 2 ? 128 : 64;
+
+// Many rows per request over a bf16 cache. A block takes kTileRows rows of one
+// key/value head and one part of the positions: four waves of 16 or 32 rows,
+// tiles of 64 positions in two LDS buffers, each wave copying 16 positions of the
+// next tile straight to LDS while this one is multiplied, one barrier a tile.
+// The copies go through a buffer resource per 16 positions that ends with them,
+// so positions behind the part or without a block read as zeros.  The products
+// are those of Step: scores transposed, so that the probabilities need no
+// shuffle; keys are read from LDS as stored, values through the transposing LDS
+// read (four positions of one dimension per lane).  LDS rows are swizzled, 16-byte
+// pieces of keys by the row, 32-byte pieces of values likewise, so that both
+// reads touch every bank once; the copies permute their global addresses for it.
+template <class XT, int HD>
+__global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
+    constexpr int NP = sizeof(XT) == 4 ? 3 : 1, ROWS = kTileRows<XT>, CG = ROWS / 64;
+    constexpr int NJ = HD / 32, ND = HD / 16;
+    constexpr int CR = HD / 8, NL = CR / 4;                // 16-byte pieces per row, copies per wave and tile
+    constexpr int KD = 16 / CR, VD2 = 8 / ND;              // rows per 256 bytes of LDS, as 16- and 32-byte pieces count
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    __shared__ __attribute__((aligned(256))) uint16_t kl[2][64 * HD], vl[2][64 * HD];
+    __shared__ float ps[4][16 * 16 * CG];
+    const PagedArgs &a = ta.a;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int g = lane >> 4, n = lane & 15;
+    const uint32_t unit = blockIdx.x % (uint32_t)ta.units, split = blockIdx.x / (uint32_t)ta.units;
+    Group gr;
+    if (!find_group<ROWS>(a, unit, 16, gr)) return;
+    set_rows<ROWS>(a, gr, gr.row0);
+    const Cut ct = cut(gr.len, ta.splits, ta.least);
+    if ((int32_t)split >= ct.parts) return;
+    const int32_t c0 = split * ct.chunk, c1 = min(gr.len, c0 + ct.chunk);
+    const int32_t *table = a.table + (int64_t)gr.b * a.most;
+    const float c2 = fabsf(a.scale) * 1.44269504f;   // a negative scale turns q's sign
+    const int32_t head_rows = HD << a.shift, in_block = (1 << a.shift) - 1;
+    const int64_t block_rows = (int64_t)head_rows * a.nkv;
+    const __bf16 *kb = (const __bf16 *)a.kc + (int64_t)gr.kvh * head_rows;
+    const __bf16 *vb = (const __bf16 *)a.vc + (int64_t)gr.kvh * head_rows;
+
+    // Wave w copies positions 16 w .. of a tile, NL pieces of 1 KiB of keys and of values.
+    uint32_t koff[NL], voff[NL];
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+        const int r = (64 * j + lane) / CR, c = (64 * j + lane) % CR;
+        koff[j] = 16 * (r * CR + (c ^ (r / KD & (CR - 1))));
+        voff[j] = 16 * (r * CR + ((((c >> 1) ^ (r / VD2 & (ND - 1))) << 1) | (c & 1)));
+    }
+    const uint32_t kdst = dma::lds_addr(&kl[0][16 * w * HD]), vdst = dma::lds_addr(&vl[0][16 * w * HD]);
+    auto copy = [&](int buf, int32_t p0) {
+        const int32_t p = p0 + 16 * w;
+        const int32_t id = p < c1 ? table[p >> a.shift] : -1;
+        const bool ok = (uint32_t)id < (uint32_t)a.num_blocks;
+        const int64_t at = (int64_t)(ok ? id : 0) * block_rows + (p & in_block) * HD;
+        const int bytes = ok ? min(16, c1 - p) * HD * 2 : 0;
+        const dma::i32x4 kr = dma::make_rsrc(kb + at, bytes), vr = dma::make_rsrc(vb + at, bytes);
+        const uint32_t kd = __builtin_amdgcn_readfirstlane(kdst + buf * 128 * HD);
+        const uint32_t vd = __builtin_amdgcn_readfirstlane(vdst + buf * 128 * HD);
+#pragma unroll
+        for (int j = 0; j < NL; ++j) dma::dma16(kd + 1024 * j, kr, koff[j], 0);
+#pragma unroll
+        for (int j = 0; j < NL; ++j) dma::dma16(vd + 1024 * j, vr, voff[j], 0);
+    };
+    copy(0, c0);
+
+    // this wave's rows and their positions
+    const int32_t wrow = gr.row0 + 16 * CG * w, wrows = min(16 * CG, gr.row0 + gr.rows - wrow);   // may be none
+    int32_t row[CG], last[CG];
+    bf16x8 q[CG][NP][NJ];
+#pragma unroll
+    for (int c = 0; c < CG; ++c) {
+        row[c] = min(wrow + 16 * c + n, gr.row0 + gr.rows - 1);
+        const int32_t token = row[c] / a.rep;
+        last[c] = min(gr.q.base + token, gr.q.held - 1);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            float x[8];
+            load_q8<XT>(a, gr.q.first + token, gr.kvh * a.rep + row[c] % a.rep, 32 * j + 8 * g, ta.qvec, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                __bf16 p[NP];
+                pieces<NP>(a.scale < 0.0f ? -x[e] : x[e], p);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) q[c][i][j][e] = p[i];
+            }
+        }
+    }
+    // positions of the wave's first and last row
+    const int32_t low = min(gr.q.base + wrow / a.rep, gr.q.held - 1);
+    const int32_t high = wrows > 0 ? min(gr.q.base + (wrow + wrows - 1) / a.rep, gr.q.held - 1) : -1;
+
+    // m: largest raw score; mr: it in powers of two, rounded, the reference of l
+    // and o; l: this lane's positions only
+    float m[CG], mr[CG], l[CG];
+    bool seen[CG];
+    f32x4 o[CG][ND];
+#pragma unroll
+    for (int c = 0; c < CG; ++c) {
+        m[c] = -INFINITY;
+        mr[c] = l[c] = 0.0f;
+        seen[c] = false;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // eight positions of dimension 16 d + n (see Step), from a buffer of values
+    auto value = [&](int buf, int d, int u) {
+        s16x4 h[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int r = 32 * u + 16 * t + 4 * g + n / 4;
+            const int vs = ((d ^ (r / VD2 & (ND - 1))) << 1) | (n >> 1 & 1);
+            h[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4 *)&vl[buf][r * HD + 8 * vs + 4 * (n & 1)]);
+        }
+        return s16x8{h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
+    };
+    int buf = 0;
+    for (int32_t p0 = c0; p0 < c1; p0 += 64, buf ^= 1) {
+        // this tile has landed, and every wave is done with the other buffer
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (p0 + 64 < c1) copy(buf ^ 1, p0 + 64);
+        if (p0 > high) continue;
+        f32x4 s[CG][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            bf16x8 k[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                k[j] = *(const bf16x8 *)&kl[buf][(16 * t + n) * HD + 8 * ((4 * j + g) ^ (n / KD & (CR - 1)))];
+#pragma unroll
+            for (int c = 0; c < CG; ++c) {
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = NP - 1; i >= 0; --i)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+                        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[j], q[c][i][j], x, 0, 0, 0);
+                s[c][t] = x;
+            }
+        }
+        int hole = 0;                        // sub-tiles without a block
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            if (p0 + 16 * t < c1) hole |= ((uint32_t)table[(p0 + 16 * t) >> a.shift] >= (uint32_t)a.num_blocks) << t;
+        const bool border = p0 + 63 > low;   // some row does not see all of the tile
+        if (hole || border) {
+#pragma unroll
+            for (int c = 0; c < CG; ++c)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int32_t lim = hole >> t & 1 ? -1 : last[c] - (p0 + 16 * t + 4 * g);
+                    seen[c] |= !(hole >> t & 1) && p0 + 16 * t <= last[c];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[c][t][i] = i <= lim ? s[c][t][i] : -INFINITY;
+                }
+        } else {
+#pragma unroll
+            for (int c = 0; c < CG; ++c) seen[c] = true;
+        }
+        bf16x8 pp[CG][NP][2];
+#pragma unroll
+        for (int c = 0; c < CG; ++c) {
+            float nm = m[c];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) nm = fmaxf(nm, s[c][t][i]);
+            nm = row4_max(nm);
+            const float ref = nm == -INFINITY ? 0.0f : nm * c2;
+            if (__any(nm > m[c])) {
+                const float corr = m[c] == -INFINITY ? 0.0f : exp2_fast(mr[c] - ref);
+                l[c] *= corr;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[c][d] *= corr;
+            }
+            m[c] = nm;
+            mr[c] = ref;
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[c][t][i] = exp2_fast(fmaf(s[c][t][i], c2, -ref));
+                    sum[i & 1] += s[c][t][i];
+                    __bf16 x[NP];
+                    pieces<NP>(s[c][t][i], x);
+#pragma unroll
+                    for (int k = 0; k < NP; ++k) pp[c][k][t / 2][4 * (t & 1) + i] = x[k];
+                }
+            l[c] += sum[0] + sum[1];
+        }
+        bool odd = false;                    // inf or NaN among the values, which rows that do not see it must not
+        if (border) {                        // multiply by 0
+            uint32_t e = 0;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const s16x8 v = value(buf, d, u);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) e = max(e, (uint32_t)(v[i] & 0x7F80));
+                }
+            odd = __any(e == 0x7F80u);
+        }
+        if (odd) {
+            // positions one by one, as paged_split's values_apart
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int c = 0; c < CG; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ps[w][(4 * g + i) * 16 * CG + 16 * c + n] = s[c][t][i];
+                wave_lds_fence();
+#pragma unroll 1
+                for (int e = 0; e < 16; ++e) {
+                    const int r = 16 * t + e;
+#pragma unroll
+                    for (int c = 0; c < CG; ++c) {
+                        if ((hole >> t & 1) || p0 + r > last[c]) continue;
+                        const float x = ps[w][e * 16 * CG + 16 * c + n];
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) {
+                            const int vs = ((d ^ (r / VD2 & (ND - 1))) << 1) | g >> 1;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                o[c][d][i] += x * __builtin_bit_cast(
+                                                      float, (uint32_t)vl[buf][r * HD + 8 * vs + 4 * (g & 1) + i] << 16);
+                        }
+                    }
+                }
+                wave_lds_fence();
+            }
+            continue;
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const bf16x8 v = __builtin_bit_cast(bf16x8, value(buf, d, u));
+#pragma unroll
+                for (int c = 0; c < CG; ++c)
+#pragma unroll
+                    for (int k = NP - 1; k >= 0; --k)
+                        o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pp[c][k][u], o[c][d], 0, 0, 0);
+            }
+    }
+#pragma unroll
+    for (int c = 0; c < CG; ++c) {
+        const float ll = row4_sum(l[c]);
+        if (wrow + 16 * c + n >= gr.row0 + gr.rows) continue;
+        if (ct.parts == 1) {
+            const bool none = m[c] == -INFINITY;      // nothing seen: 0; only scores of -inf: 0 / 0
+            XT *out = (XT *)a.out + (int64_t)(gr.q.first + row[c] / a.rep) * a.out_stride +
+                      (int64_t)(gr.kvh * a.rep + row[c] % a.rep) * HD + 4 * g;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    out[16 * d + i] = (XT)(none ? (seen[c] ? NAN : 0.0f) : o[c][d][i] / ll);
+        } else {
+            const int64_t r = ((int64_t)unit * ta.splits + split) * ROWS + row[c] - gr.row0;
+            if (g == 0)
+                ta.ml[r] = m[c] == -INFINITY ? float2{-INFINITY, seen[c] ? 1.0f : 0.0f} : float2{mr[c], ll};
+#pragma unroll
+            for (int d = 0; d < ND; ++d) *(f32x4 *)(ta.po + r * HD + 16 * d + 4 * g) = o[c][d];
+        }
+    }
+}
+
+// Joins paged_tile's parts: HD / 4 threads a row.
+template <class XT, int HD>
+__global__ __launch_bounds__(256) void paged_tile_merge(const TileArgs ta) {
+    constexpr int T = HD / 4, R = 256 / T;
+    const PagedArgs &a = ta.a;
+    const uint32_t unit = blockIdx.x / (kTileRows<XT> / R);
+    const int rr = (int)(blockIdx.x % (kTileRows<XT> / R)) * R + threadIdx.x / T, d4 = threadIdx.x % T;
+    Group gr;
+    if (!find_group<kTileRows<XT>>(a, unit, 16, gr)) return;
+    set_rows<kTileRows<XT>>(a, gr, gr.row0);
+    const Cut ct = cut(gr.len, ta.splits, ta.least);
+    if (ct.parts == 1 || rr >= gr.rows) return;
+    const int64_t at0 = (int64_t)unit * ta.splits * kTileRows<XT> + rr;
+    float mm = -INFINITY, any = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < ct.parts; ++s) {
+        const float2 x = ta.ml[at0 + (int64_t)s * kTileRows<XT>];
+        mm = fmaxf(mm, x.x);
+        any = fmaxf(any, x.y);
+    }
+    float l = 0.0f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < ct.parts; ++s) {
+        const int64_t r = at0 + (int64_t)s * kTileRows<XT>;
+        const float2 x = ta.ml[r];
+        const float f = x.x == -INFINITY ? 0.0f : exp2_fast(x.x - mm);
+        if (x.x != -INFINITY) l += f * x.y;
+        o += f * *(const f32x4 *)(ta.po + r * HD + 4 * d4);
+    }
+    const int32_t row = gr.row0 + rr;
+    XT *out = (XT *)a.out + (int64_t)(gr.q.first + row / a.rep) * a.out_stride +
+              (int64_t)(gr.kvh * a.rep + row % a.rep) * HD + 4 * d4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = (XT)(mm == -INFINITY ? (any > 0.0f ? NAN : 0.0f) : o[i] / l);
+}
+
+// Positions a part of paged_tile has at least: parts fill the chip's two blocks
+// per CU twice over, of at least 512 positions.
+template <class XT, int HD>
+hipError_t launch_tile(tbh_device *dev, const PagedArgs &a, int64_t context, hipStream_t s) {
+    TileArgs ta{};
+    ta.a = a;
+    ta.qvec = aligned(a.q, 16) && (a.q_stride * (int64_t)sizeof(XT)) % 16 == 0;
+    const int64_t rows = a.tokens * a.rep;
+    const int64_t units = (rows / kTileRows<XT> + std::min<int64_t>(a.requests, rows / 17 + 1)) * a.nkv;
+    const int64_t parts = std::max<int64_t>(1, 4 * (int64_t)std::max(1, dev->cu_count) / units);
+    ta.least = (int32_t)std::max<int64_t>(512, ((context + parts - 1) / parts + 127) / 128 * 128);
+    ta.splits = (int32_t)std::min<int64_t>((context + ta.least - 1) / ta.least, kMaxSplits);
+    if (ta.splits > 1) {
+        const int64_t n = units * ta.splits * kTileRows<XT>;
+        const size_t head = (size_t)n * sizeof(float2);
+        char *ws = (char *)stream_workspace(dev, s, head + (size_t)n * HD * sizeof(float));
+        if (ws) {
+            ta.ml = (float2 *)ws;
+            ta.po = (float *)(ws + head);
+        } else {
+            ta.splits = 1;   // no workspace (graph capture before any eager call): whole contexts
+        }
+    }
+    if (units * std::max<int64_t>(ta.splits, kTileRows<XT> * HD / 1024) > INT32_MAX) return hipErrorInvalidValue;
+    ta.units = (int32_t)units;
+    hipLaunchKernelGGL((paged_tile<XT, HD>), dim3((unsigned)(units * ta.splits)), dim3(256), 0, s, ta);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || ta.splits == 1) return e;
+    hipLaunchKernelGGL((paged_tile_merge<XT, HD>), dim3((unsigned)(units * (kTileRows<XT> * HD / 1024))), dim3(256), 0, s,
+                       ta);
+    return hipGetLastError();
+}
+
 template <class XT, class CT>
 hipError_t launch_paged(tbh_device *dev, const PagedArgs &a, int64_t query, int64_t context, hipStream_t s) {
     // the matrix kernels take a tile of 16 positions from one block
     if (a.shift >= 4 && a.num_blocks > 0 && a.most > 0) {
+        if constexpr (sizeof(CT) == 2) {
+            if (query * a.rep > 16 && (a.hd == 64 || a.hd == 128)) {
+                const hipError_t e = a.hd == 64 ? launch_tile<XT, 64>(dev, a, context, s) : launch_tile<XT, 128>(dev, a, context, s);
+                if (e != hipSuccess) return e;
+                return a.hd == 64 ? launch_split<XT, CT, 64>(dev, a, query, context, true, s)
+                                  : launch_split<XT, CT, 128>(dev, a, query, context, true, s);
+            }
+        }
         switch (a.hd) {
         case 32: return launch_split<XT, CT, 32>(dev, a, query, context, false, s);
         case 64: return launch_split<XT, CT, 64>(dev, a, query, context, false, s);
