@@ -205,14 +205,31 @@ __device__ __forceinline__ void set_rows(const PagedArgs &a, Group &g, int32_t r
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Largest value over the four lanes that hold one row (lane % 16).
+// Largest value, sum over the four lanes that hold one row (lane % 16).  A
+// half swap of v with itself leaves one partner's value in its first result and
+// the other's in its second, in both partners.
+struct Both {
+    float x, y;
+};
+__device__ __forceinline__ Both half_swap16(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t x = r[0], y = r[1];
+    return {__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)};
+}
+__device__ __forceinline__ Both half_swap32(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t x = r[0], y = r[1];
+    return {__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)};
+}
 __device__ __forceinline__ float row4_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    const Both a = half_swap16(v), b = half_swap32(fmaxf(a.x, a.y));
+    return fmaxf(b.x, b.y);
 }
 __device__ __forceinline__ float row4_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    const Both a = half_swap16(v), b = half_swap32(a.x + a.y);
+    return b.x + b.y;
 }
 
 // x as a sum of NP bf16 values: exact for NP = 3 (8 + 8 + 8 bits), rounded for 1.
@@ -462,26 +479,27 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
         const int32_t first_last = min(gr.q.base + row0 / a.rep, gr.q.held - 1);   // the first row's
         Step<XT, CT, HD> st;
 
-        // The blocks of a step's two tiles are looked up two steps ahead, its
-        // keys loaded once the step before has used its own, values likewise.
+        // A step's keys are loaded once the step before has used its own, values
+        // likewise.  The blocks of 32 steps (two tiles each) are looked up at once,
+        // one per lane.
+        auto window = [&](int32_t p) {
+            const int32_t x = p + 128 * (lane >> 1) + 16 * (lane & 1);
+            return x < c1 ? table[x >> a.shift] : -1;
+        };
         struct Pair {
             int32_t id[2];
         };
-        auto look = [&](int32_t p0) {
-            Pair r;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int32_t p = p0 + 16 * t;
-                r.id[t] = p < c1 ? table[p >> a.shift] : -1;
-            }
-            return r;
+        int32_t p0 = c0 + 32 * w;
+        int32_t ids = window(p0);
+        auto pair = [&](int32_t p) {           // of the step at p, in the window
+            const int i = (p - c0) >> 7 & 31;
+            return Pair{{__builtin_amdgcn_readlane(ids, 2 * i), __builtin_amdgcn_readlane(ids, 2 * i + 1)}};
         };
         auto there = [&](const Pair &x, int t) { return (uint32_t)x.id[t] < (uint32_t)a.num_blocks; };
         auto at = [&](const Pair &x, int t, int32_t p0) {   // a tile without a block: any block's rows, not used
             return (int64_t)(there(x, t) ? x.id[t] : 0) * block_rows + ((p0 + 16 * t) & in_block) * HD;
         };
-        int32_t p0 = c0 + 32 * w;
-        Pair cur = look(p0), nxt = look(p0 + 128);
+        Pair cur = pair(p0);
         st.load_q(a, gr.q.first + token, gr.kvh * a.rep + r % a.rep, g, sa.qvec);
         if (p0 < c1) {
 #pragma unroll
@@ -496,7 +514,8 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
 #pragma unroll
         for (int d = 0; d < VD; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (; p0 < c1; p0 += 128) {
-            const Pair far = look(p0 + 256);
+            if (((p0 - c0) >> 7 & 31) == 31) ids = window(p0 + 128);
+            const Pair nxt = pair(p0 + 128);
             const bool th[2] = {there(cur, 0), there(cur, 1)};
             f32x4 s[2];
 #pragma unroll
@@ -545,7 +564,6 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) st.load_values(t, vb + at(nxt, t, p0 + 128), g, n);
             cur = nxt;
-            nxt = far;
         }
         l = row4_sum(l);
         if (m == -INFINITY) l = seen ? 1.0f : 0.0f;   // positions seen, each of score -inf; none at all
@@ -745,10 +763,18 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
         voff[j] = 16 * (r * CR + ((((c >> 1) ^ (r / VD2 & (ND - 1))) << 1) | (c & 1)));
     }
     const uint32_t kdst = dma::lds_addr(&kl[0][16 * w * HD]), vdst = dma::lds_addr(&vl[0][16 * w * HD]);
-    auto copy = [&](int buf, int32_t p0) {
+    // The blocks of 64 sub-tiles of 16 positions, one per lane: those of this
+    // tile's window and of the next.  (A look-up per tile would stall the wave
+    // for its latency, behind the copies in flight: 204 us for 110 with windows at
+    // 2048 tokens over 4096, 32 heads of 128 on 8.)
+    auto window = [&](int32_t p) {
+        return p + 16 * lane < c1 ? table[(p + 16 * lane) >> a.shift] : -1;
+    };
+    int32_t ids = window(c0), ids_next = window(c0 + 1024);
+    auto copy = [&](int buf, int32_t p0, int32_t from) {   // from: the window's ids
         const int32_t p = p0 + 16 * w;
-        const int32_t id = p < c1 ? table[p >> a.shift] : -1;
-        const bool ok = (uint32_t)id < (uint32_t)a.num_blocks;
+        const int32_t id = __builtin_amdgcn_readlane(from, (p - c0) >> 4 & 63);
+        const bool ok = p < c1 && (uint32_t)id < (uint32_t)a.num_blocks;
         const int64_t at = (int64_t)(ok ? id : 0) * block_rows + (p & in_block) * HD;
         const int bytes = ok ? min(16, c1 - p) * HD * 2 : 0;
         const dma::i32x4 kr = dma::make_rsrc(kb + at, bytes), vr = dma::make_rsrc(vb + at, bytes);
@@ -759,7 +785,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
 #pragma unroll
         for (int j = 0; j < NL; ++j) dma::dma16(vd + 1024 * j, vr, voff[j], 0);
     };
-    copy(0, c0);
+    copy(0, c0, ids);
+    uint64_t blocks = __ballot((uint32_t)ids < (uint32_t)a.num_blocks);   // sub-tiles of the window that have one
 
     // this wave's rows and their positions
     const int32_t wrow = gr.row0 + 16 * CG * w, wrows = min(16 * CG, gr.row0 + gr.rows - wrow);   // may be none
@@ -816,7 +843,13 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
     for (int32_t p0 = c0; p0 < c1; p0 += 64, buf ^= 1) {
         // this tile has landed, and every wave is done with the other buffer
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (p0 + 64 < c1) copy(buf ^ 1, p0 + 64);
+        const int32_t at = (p0 - c0) >> 4 & 63;       // of the window
+        if (at == 0 && p0 != c0) {
+            ids = ids_next;
+            ids_next = window(p0 + 1024);
+            blocks = __ballot((uint32_t)ids < (uint32_t)a.num_blocks);
+        }
+        if (p0 + 64 < c1) copy(buf ^ 1, p0 + 64, at == 60 ? ids_next : ids);
         if (p0 > high) continue;
         f32x4 s[CG][4];
 #pragma unroll
@@ -836,10 +869,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
                 s[c][t] = x;
             }
         }
-        int hole = 0;                        // sub-tiles without a block
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-            if (p0 + 16 * t < c1) hole |= ((uint32_t)table[(p0 + 16 * t) >> a.shift] >= (uint32_t)a.num_blocks) << t;
+        // sub-tiles without a block (those behind the part are no row's to see)
+        const int hole = (int)(~blocks >> at) & 15 & (p0 + 64 <= c1 ? 15 : (1 << ((c1 - p0 + 15) >> 4)) - 1);
         const bool border = p0 + 63 > low;   // some row does not see all of the tile
         if (hole || border) {
 #pragma unroll
@@ -923,6 +954,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
                             for (int i = 0; i < 4; ++i)
                                 o[c][d][i] += x * __builtin_bit_cast(
                                                       float, (uint32_t)vl[buf][r * HD + 8 * vs + 4 * (g & 1) + i] << 16);
+                            __builtin_amdgcn_sched_barrier(0);   // few values at a time: registers
                         }
                     }
                 }
