@@ -53,59 +53,81 @@ __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
-// Any head dimension, type and alignment: one wave per (token, query head),
-// 64 positions a pass, a position per lane for the scores and an output
-// dimension per lane for the values.
-template <class XT, class CT>
-__global__ __launch_bounds__(256) void paged_rows(const PagedArgs a) {
-    __shared__ float qs[4][kMaxHeadDim];
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + w;
-    if (row >= a.tokens * a.nh) return;
-    const int64_t t = row / a.nh;
-    const int h = (int)(row % a.nh), kvh = h / a.rep;
-    const int32_t b = request_of(a, (int32_t)t);
-    if (b >= a.requests) return;                 // behind the last request's rows
-    const int64_t held = min((int64_t)max(a.ctx[b], 0), (int64_t)a.most << a.shift);
-    const int64_t behind = (int64_t)a.start[b + 1] - 1 - t;   // rows of the request after this one
-    const int32_t last = (int32_t)min(held - 1, held - 1 - behind);   // this row's position
-    for (int d = lane; d < a.hd; d += 64) qs[w][d] = elem<XT>(a.q, t * a.q_stride + (int64_t)h * a.hd + d);
-    wave_lds_fence();
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-    float m = -INFINITY, l = 0.0f, o[kMaxHeadDim / 64] = {};
-    bool seen = false;
-    for (int32_t p0 = 0; p0 <= last; p0 += 64) {
-        const int32_t pos = p0 + lane;
-        const int64_t at = pos <= last ? place(a, b, pos, kvh) : -1;
+// One row's part of the softmax over positions [c0, end), by one wave: 64
+// positions a pass, a position per lane for the scores and an output dimension
+// per lane (lane, lane + 64, ...) for the values.  m: largest score in powers of
+// two, l and o: sums relative to it.  qs: the wave's LDS, head_dim floats.
+struct RowPart {
+    float m, l, o[kMaxHeadDim / 64];
+    bool seen;             // a position of the range is in a block
+};
+
+template <class XT, class CT>
+__device__ __forceinline__ RowPart row_part(const PagedArgs &a, int32_t b, int64_t t, int head, int32_t c0, int32_t end,
+                                            float *qs) {
+    const int lane = threadIdx.x & 63, kvh = head / a.rep;
+    const float c2 = a.scale * 1.44269504f;
+    wave_lds_fence();
+    for (int d = lane; d < a.hd; d += 64) qs[d] = elem<XT>(a.q, t * a.q_stride + (int64_t)head * a.hd + d);
+    wave_lds_fence();
+    RowPart r{-INFINITY, 0.0f, {}, false};
+    for (int32_t p0 = c0; p0 < end; p0 += 64) {
+        const int64_t at = p0 + lane < end ? place(a, b, p0 + lane, kvh) : -1;
         const uint64_t valid = __ballot(at >= 0);
         if (!valid) continue;
-        seen = true;
+        r.seen = true;
         float s = -INFINITY;
         if (at >= 0) {
             float dot = 0.0f;
-            for (int d = 0; d < a.hd; ++d) dot += qs[w][d] * elem<CT>(a.kc, at + d);
-            s = dot * a.scale;
+            for (int d = 0; d < a.hd; ++d) dot += qs[d] * elem<CT>(a.kc, at + d);
+            s = dot * c2;
         }
-        const float nm = fmaxf(m, wave::max(s));
+        const float nm = fmaxf(r.m, wave::max(s));
         const float ref = nm == -INFINITY ? 0.0f : nm;
-        const float corr = expf(m - ref), p = at >= 0 ? expf(s - ref) : 0.0f;
-        l = l * corr + wave::sum(p);
+        const float corr = exp2_fast(r.m - ref), p = at >= 0 ? exp2_fast(s - ref) : 0.0f;
+        r.l = r.l * corr + wave::sum(p);
 #pragma unroll
-        for (int i = 0; i < kMaxHeadDim / 64; ++i) o[i] *= corr;
+        for (int i = 0; i < kMaxHeadDim / 64; ++i) r.o[i] *= corr;
         for (uint64_t v = valid; v; v &= v - 1) {
             const int j = __builtin_ctzll(v);
             const float pj = wave::lane_value(p, j);
             const int64_t vj = __shfl(at, j);
 #pragma unroll
             for (int i = 0; i < kMaxHeadDim / 64; ++i)
-                if (lane + 64 * i < a.hd) o[i] += pj * elem<CT>(a.vc, vj + lane + 64 * i);
+                if (lane + 64 * i < a.hd) r.o[i] += pj * elem<CT>(a.vc, vj + lane + 64 * i);
         }
-        m = nm;
+        r.m = nm;
     }
+    return r;
+}
+
+// The row's result from all of its positions.
+template <class XT>
+__device__ __forceinline__ void store_row(const PagedArgs &a, int64_t t, int head, const RowPart &r) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < kMaxHeadDim / 64; ++i)
         if (lane + 64 * i < a.hd)
-            ((XT *)a.out)[t * a.out_stride + (int64_t)h * a.hd + lane + 64 * i] = (XT)(seen ? o[i] / l : 0.0f);
+            ((XT *)a.out)[t * a.out_stride + (int64_t)head * a.hd + lane + 64 * i] = (XT)(r.seen ? r.o[i] / r.l : 0.0f);
+}
+
+// Any head dimension, block size and alignment: one wave per (token, query head).
+template <class XT, class CT>
+__global__ __launch_bounds__(256) void paged_rows(const PagedArgs a) {
+    __shared__ float qs[4][kMaxHeadDim];
+    const int w = threadIdx.x >> 6;
+    const int64_t row = (int64_t)blockIdx.x * 4 + w;
+    if (row >= a.tokens * a.nh) return;
+    const int64_t t = row / a.nh;
+    const int h = (int)(row % a.nh);
+    const int32_t b = request_of(a, (int32_t)t);
+    if (b >= a.requests) return;                 // behind the last request's rows
+    const int64_t held = min((int64_t)max(a.ctx[b], 0), (int64_t)a.most << a.shift);
+    const int64_t behind = (int64_t)a.start[b + 1] - 1 - t;   // rows of the request after this one
+    const int32_t last = (int32_t)min(held - 1, held - 1 - behind);   // this row's position
+    store_row<XT>(a, t, h, row_part<XT, CT>(a, b, t, h, 0, last + 1, qs[w]));
 }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -162,9 +184,13 @@ struct Group {
     int32_t len;                   // positions its last row sees
 };
 
-// Finds group `index` of the requests' groups of ROWS rows, heads fastest.
+// Finds group `index` of the requests' groups of ROWS rows, heads fastest, a
+// request's last rows first: they see the most positions.  pair_up: the second
+// half of a request's groups follows from its first rows on, so that blocks that
+// run side by side, half the launch apart, see as many positions as the others.
 template <int ROWS>
-__device__ __forceinline__ bool find_group(const PagedArgs &a, uint32_t index, int32_t more_than, Group &g) {
+__device__ __forceinline__ bool find_group(const PagedArgs &a, uint32_t index, int32_t more_than, bool pair_up,
+                                           Group &g) {
     const int lane = threadIdx.x & 63;
     g.kvh = (int)(index % (uint32_t)a.nkv);
     int32_t left = (int32_t)(index / (uint32_t)a.nkv);
@@ -182,8 +208,9 @@ __device__ __forceinline__ bool find_group(const PagedArgs &a, uint32_t index, i
         if (left < total) {
             const int l = __builtin_ctzll(__ballot(in > left));
             g.b = b0 + l;
-            // the last rows first: they see the most positions
-            g.row0 = (__builtin_amdgcn_readlane(in, l) - 1 - left) * ROWS;
+            const int32_t n = __builtin_amdgcn_readlane(mine, l), k = left - (__builtin_amdgcn_readlane(in, l) - n);
+            const int32_t half = (n + 1) / 2;
+            g.row0 = (pair_up && k >= half ? k - half : n - 1 - k) * ROWS;
             g.q.first = __builtin_amdgcn_readlane(r.first, l);
             g.q.n = __builtin_amdgcn_readlane(r.n, l);
             g.q.rows = __builtin_amdgcn_readlane(r.rows, l);
@@ -202,8 +229,6 @@ __device__ __forceinline__ void set_rows(const PagedArgs &a, Group &g, int32_t r
     g.rows = min(ROWS, g.q.rows - row0);
     g.len = min(g.q.held, max(0, g.q.base + (row0 + g.rows - 1) / a.rep + 1));
 }
-
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Largest value, sum over the four lanes that hold one row (lane % 16).  A
 // half swap of v with itself leaves one partner's value in its first result and
@@ -253,6 +278,17 @@ __device__ __forceinline__ void load_q8(const PagedArgs &a, int64_t t, int head,
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = (float)p[i];
+    }
+}
+
+// The same of a probability: finite, or NaN, which every piece then is.
+template <int NP>
+__device__ __forceinline__ void pieces_of_p(float x, __bf16 (&p)[NP]) {
+    p[0] = (__bf16)x;
+    if constexpr (NP == 3) {
+        const float r = x - (float)p[0];
+        p[1] = (__bf16)r;
+        p[2] = (__bf16)(r - (float)p[1]);
     }
 }
 
@@ -306,19 +342,6 @@ struct Step<XT, __bf16, HD> {
 #pragma unroll
         for (int w = 0; w < VW; ++w) v[t][i].w[w] = 0;
     }
-    __device__ __forceinline__ bool odd_values() const {   // inf or NaN among this lane's values
-        uint32_t lo = 0, hi = 0;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int w = 0; w < VW; ++w) {
-                    lo = max(lo, v[t][i].w[w] & 0x7F80u);
-                    hi = max(hi, v[t][i].w[w] & 0x7F800000u);
-                }
-        return lo == 0x7F80u || hi == 0x7F800000u;
-    }
     __device__ __forceinline__ f32x4 scores(int t) const {
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -332,7 +355,7 @@ struct Step<XT, __bf16, HD> {
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             __bf16 x[NP];
-            pieces<NP>(p[c / 4][c % 4], x);
+            pieces_of_p<NP>(p[c / 4][c % 4], x);
 #pragma unroll
             for (int i = 0; i < NP; ++i) pp[i][c] = x[i];
         }
@@ -379,16 +402,6 @@ struct Step<XT, float, HD> {
 #pragma unroll
         for (int w = 0; w < VD; ++w) v[t][i].w[w] = 0;
     }
-    __device__ __forceinline__ bool odd_values() const {
-        uint32_t e = 0;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int w = 0; w < VD; ++w) e = max(e, v[t][i].w[w] & 0x7F800000u);
-        return e == 0x7F800000u;
-    }
     __device__ __forceinline__ f32x4 scores(int t) const {
         f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};   // two chains: half the rounding of one
 #pragma unroll
@@ -410,30 +423,6 @@ struct Step<XT, float, HD> {
     }
 };
 
-// o += p v over 32 positions without the matrix instruction, for steps where
-// some rows do not see a position whose value is inf or NaN: its probability 0
-// times that value would be NaN.  ps: this wave's LDS, [position][row].
-template <class CT, int HD>
-__device__ __forceinline__ void values_apart(const f32x4 (&p)[2], float *ps, const CT *v0, const CT *v1, int32_t p0,
-                                             int32_t end, int32_t last, int there, int lane, f32x4 (&o)[HD / 16]) {
-    constexpr int VD = HD / 16;
-    const int g = lane >> 4, n = lane & 15;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ps[(16 * t + 4 * g + i) * 16 + n] = p[t][i];
-    wave_lds_fence();
-#pragma unroll 1
-    for (int j = 0; j < 32 && p0 + j < end; ++j) {
-        if (!(there >> (j >> 4) & 1) || p0 + j > last) continue;
-        const float x = ps[j * 16 + n];
-        const CT *row = (j < 16 ? v0 : v1) + (j & 15) * HD + 4 * VD * g;
-#pragma unroll
-        for (int e = 0; e < 4 * VD; ++e) o[e % VD][e / VD] += x * (float)row[e];
-    }
-    wave_lds_fence();
-}
-
 // Few rows per request (single tokens of grouped heads, short chunks): 16 rows
 // and one part of the positions a block, its four waves taking steps of 32
 // positions in turn and meeting in LDS at the end.  Bound by reading the cache.
@@ -442,6 +431,7 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
     constexpr int VD = HD / 16, LD = HD + 4;
     __shared__ __attribute__((aligned(16))) float so[4][16][LD];
     __shared__ float2 sml[4][16];
+    __shared__ int odd;
     const PagedArgs &a = sa.a;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, n = lane & 15;
@@ -452,7 +442,7 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
     Group gr;
     bool alone = false;            // more rows than a unit has places for: no parts
     if (sa.scan) {
-        if (!find_group<16>(a, unit, 0, gr)) return;
+        if (!find_group<16>(a, unit, 0, false, gr)) return;
     } else {
         gr.kvh = (int)(unit % (uint32_t)a.nkv);
         gr.b = (int32_t)(unit / (uint32_t)a.nkv);
@@ -509,7 +499,7 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
         }
 
         float m = -INFINITY, l = 0.0f;   // l: this lane's positions only
-        bool seen = false;
+        int32_t first = INT32_MAX;       // this wave's first position in a block
         f32x4 o[VD];
 #pragma unroll
         for (int d = 0; d < VD; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -525,7 +515,7 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
             float nm = m;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                seen |= th[t] && p0 + 16 * t <= last;
+                if (th[t]) first = min(first, p0 + 16 * t);
                 const int32_t lim = th[t] ? last - (p0 + 16 * t + 4 * g) : -1;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -556,20 +546,17 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
 #pragma unroll
                 for (int d = 0; d < VD; ++d) o[d] *= corr;
             }
-            if (p0 + 31 > first_last && __any(st.odd_values()))
-                values_apart<CT, HD>(s, &so[w][0][0], vb + at(cur, 0, p0), vb + at(cur, 1, p0), p0, c1, last,
-                                     th[0] | th[1] << 1, lane, o);
-            else
-                st.values(s, o);
+            st.values(s, o);
 #pragma unroll
             for (int t = 0; t < 2; ++t) st.load_values(t, vb + at(nxt, t, p0 + 128), g, n);
             cur = nxt;
         }
         l = row4_sum(l);
-        if (m == -INFINITY) l = seen ? 1.0f : 0.0f;   // positions seen, each of score -inf; none at all
+        if (m == -INFINITY) l = first <= last ? 1.0f : 0.0f;   // positions seen, each of score -inf; none at all
 
         // the four waves' parts
         __syncthreads();
+        if (tid == 0) odd = 0;
 #pragma unroll
         for (int d = 0; d < VD; ++d)
 #pragma unroll
@@ -591,6 +578,7 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
                 v += f * so[i][rr][d];
             }
             if (mm == -INFINITY) ll = none;
+            if (!(fabsf(v) < INFINITY)) odd = 1;
             if (ct.parts == 1) {
                 const int32_t tt = (row0 + rr) / a.rep;
                 const int head = gr.kvh * a.rep + (row0 + rr) % a.rep;
@@ -601,6 +589,24 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
                 const int64_t at = ((int64_t)unit * sa.splits + split) * sa.slots + rr;
                 if (d == 0) sa.ml[at] = float2{mm, ll};
                 sa.po[at * HD + d] = v;
+            }
+        }
+        if (first_last + 1 >= c1) continue;      // every row sees all of the part (uniform)
+        // An inf or NaN among the values that some rows do not see became NaN in
+        // theirs, 0 times it: those parts once more, a row at a time.
+        __syncthreads();
+        if (!odd) continue;
+        for (int rr = w; rr < gr.rows; rr += 4) {
+            const int32_t tt = (row0 + rr) / a.rep;
+            const int head = gr.kvh * a.rep + (row0 + rr) % a.rep;
+            const int32_t end = min(c1, gr.q.base + tt + 1);
+            const RowPart x = row_part<XT, CT>(a, gr.b, gr.q.first + tt, head, c0, end, &so[w][0][0]);
+            if (ct.parts == 1) {
+                store_row<XT>(a, gr.q.first + tt, head, x);
+            } else {
+                const int64_t at = ((int64_t)unit * sa.splits + split) * sa.slots + rr;
+                if (lane == 0) sa.ml[at] = x.m == -INFINITY ? float2{x.m, x.seen ? 1.0f : 0.0f} : float2{x.m, x.l};
+                for (int i = 0; 64 * i + lane < HD; ++i) sa.po[at * HD + 64 * i + lane] = x.o[i];
             }
         }
     }
@@ -620,7 +626,7 @@ __global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa) {
     const float2 mine = sa.ml[at0 + (int64_t)min(lane, sa.splits - 1) * sa.slots];   // before the request is known
     Group gr;
     if (sa.scan) {
-        if (!find_group<16>(a, unit, 0, gr)) return;
+        if (!find_group<16>(a, unit, 0, false, gr)) return;
     } else {
         gr.kvh = (int)(unit % (uint32_t)a.nkv);
         gr.b = (int32_t)(unit / (uint32_t)a.nkv);
@@ -706,6 +712,7 @@ struct TileArgs {
     PagedArgs a;
     int32_t units;         // (kTileRows rows, key/value head) pairs
     int32_t splits, least; // see cut
+    bool pair_up;          // see find_group
     bool qvec;             // q rows are 16-byte aligned
     float2 *ml;            // partials [unit][split][kTileRows]: (max, sum)
     float *po;             // and sums of p v, [unit][split][kTileRows][head_dim]
@@ -736,13 +743,13 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
     __shared__ __attribute__((aligned(256))) uint16_t kl[2][64 * HD], vl[2][64 * HD];
-    __shared__ float ps[4][16 * 16 * CG];
+    __shared__ float qs[4][HD];
     const PagedArgs &a = ta.a;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, n = lane & 15;
     const uint32_t unit = blockIdx.x % (uint32_t)ta.units, split = blockIdx.x / (uint32_t)ta.units;
     Group gr;
-    if (!find_group<ROWS>(a, unit, 16, gr)) return;
+    if (!find_group<ROWS>(a, unit, 16, ta.pair_up, gr)) return;
     set_rows<ROWS>(a, gr, gr.row0);
     const Cut ct = cut(gr.len, ta.splits, ta.least);
     if ((int32_t)split >= ct.parts) return;
@@ -765,8 +772,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
     const uint32_t kdst = dma::lds_addr(&kl[0][16 * w * HD]), vdst = dma::lds_addr(&vl[0][16 * w * HD]);
     // The blocks of 64 sub-tiles of 16 positions, one per lane: those of this
     // tile's window and of the next.  (A look-up per tile would stall the wave
-    // for its latency, behind the copies in flight: 204 us for 110 with windows at
-    // 2048 tokens over 4096, 32 heads of 128 on 8.)
+    // for its latency, behind the copies in flight.)
     auto window = [&](int32_t p) {
         return p + 16 * lane < c1 ? table[(p + 16 * lane) >> a.shift] : -1;
     };
@@ -814,19 +820,24 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
     const int32_t low = min(gr.q.base + wrow / a.rep, gr.q.held - 1);
     const int32_t high = wrows > 0 ? min(gr.q.base + (wrow + wrows - 1) / a.rep, gr.q.held - 1) : -1;
 
-    // m: largest raw score; mr: it in powers of two, rounded, the reference of l
-    // and o; l: this lane's positions only
-    float m[CG], mr[CG], l[CG];
-    bool seen[CG];
-    f32x4 o[CG][ND];
+    // mr: what the exponents of l and o are relative to, in powers of two: a
+    // score at most kLag below the row's largest (moving it with every new
+    // maximum cost a tenth of the kernel's vector instructions); -inf: no score
+    // above -inf yet.  l: sums of p as the second product has them, by a row of ones
+    constexpr float kLag = 8.0f;
+    float mr[CG];
+    int32_t first = INT32_MAX;                // first position in a block
+    f32x4 l[CG], o[CG][ND];
 #pragma unroll
     for (int c = 0; c < CG; ++c) {
-        m[c] = -INFINITY;
-        mr[c] = l[c] = 0.0f;
-        seen[c] = false;
+        mr[c] = -INFINITY;
+        l[c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    bf16x8 ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.0f;
     // eight positions of dimension 16 d + n (see Step), from a buffer of values
     auto value = [&](int buf, int d, int u) {
         s16x4 h[2];
@@ -869,8 +880,9 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
                 s[c][t] = x;
             }
         }
-        // sub-tiles without a block (those behind the part are no row's to see)
-        const int hole = (int)(~blocks >> at) & 15 & (p0 + 64 <= c1 ? 15 : (1 << ((c1 - p0 + 15) >> 4)) - 1);
+        // sub-tiles of the part, those without a block
+        const int part = p0 + 64 <= c1 ? 15 : (1 << ((c1 - p0 + 15) >> 4)) - 1, hole = (int)(~blocks >> at) & part;
+        if (first == INT32_MAX && hole != part) first = p0 + 16 * __builtin_ctz(part & ~hole);
         const bool border = p0 + 63 > low;   // some row does not see all of the tile
         if (hole || border) {
 #pragma unroll
@@ -878,89 +890,43 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     const int32_t lim = hole >> t & 1 ? -1 : last[c] - (p0 + 16 * t + 4 * g);
-                    seen[c] |= !(hole >> t & 1) && p0 + 16 * t <= last[c];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[c][t][i] = i <= lim ? s[c][t][i] : -INFINITY;
                 }
-        } else {
-#pragma unroll
-            for (int c = 0; c < CG; ++c) seen[c] = true;
         }
         bf16x8 pp[CG][NP][2];
 #pragma unroll
         for (int c = 0; c < CG; ++c) {
-            float nm = m[c];
+            float nm = s[c][0][0];
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) nm = fmaxf(nm, s[c][t][i]);
-            nm = row4_max(nm);
-            const float ref = nm == -INFINITY ? 0.0f : nm * c2;
-            if (__any(nm > m[c])) {
-                const float corr = m[c] == -INFINITY ? 0.0f : exp2_fast(mr[c] - ref);
+            nm = row4_max(nm) * c2;
+            const bool move = nm > mr[c] + kLag;
+            if (__any(move)) {
+                const float to = move ? nm : mr[c], corr = move ? exp2_fast(mr[c] - to) : 1.0f;
+                mr[c] = to;
                 l[c] *= corr;
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[c][d] *= corr;
             }
-            m[c] = nm;
-            mr[c] = ref;
-            float sum[2] = {0.0f, 0.0f};
+            const float ref = mr[c] == -INFINITY ? 0.0f : mr[c];
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     s[c][t][i] = exp2_fast(fmaf(s[c][t][i], c2, -ref));
-                    sum[i & 1] += s[c][t][i];
                     __bf16 x[NP];
-                    pieces<NP>(s[c][t][i], x);
+                    pieces_of_p<NP>(s[c][t][i], x);
 #pragma unroll
                     for (int k = 0; k < NP; ++k) pp[c][k][t / 2][4 * (t & 1) + i] = x[k];
                 }
-            l[c] += sum[0] + sum[1];
-        }
-        bool odd = false;                    // inf or NaN among the values, which rows that do not see it must not
-        if (border) {                        // multiply by 0
-            uint32_t e = 0;
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const s16x8 v = value(buf, d, u);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) e = max(e, (uint32_t)(v[i] & 0x7F80));
-                }
-            odd = __any(e == 0x7F80u);
-        }
-        if (odd) {
-            // positions one by one, as paged_split's values_apart
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                for (int c = 0; c < CG; ++c)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) ps[w][(4 * g + i) * 16 * CG + 16 * c + n] = s[c][t][i];
-                wave_lds_fence();
-#pragma unroll 1
-                for (int e = 0; e < 16; ++e) {
-                    const int r = 16 * t + e;
-#pragma unroll
-                    for (int c = 0; c < CG; ++c) {
-                        if ((hole >> t & 1) || p0 + r > last[c]) continue;
-                        const float x = ps[w][e * 16 * CG + 16 * c + n];
-#pragma unroll
-                        for (int d = 0; d < ND; ++d) {
-                            const int vs = ((d ^ (r / VD2 & (ND - 1))) << 1) | g >> 1;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                o[c][d][i] += x * __builtin_bit_cast(
-                                                      float, (uint32_t)vl[buf][r * HD + 8 * vs + 4 * (g & 1) + i] << 16);
-                            __builtin_amdgcn_sched_barrier(0);   // few values at a time: registers
-                        }
-                    }
-                }
-                wave_lds_fence();
-            }
-            continue;
+                for (int k = NP - 1; k >= 0; --k)
+                    l[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pp[c][k][u], l[c], 0, 0, 0);
         }
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -974,25 +940,45 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
                         o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pp[c][k][u], o[c][d], 0, 0, 0);
             }
     }
+    bool odd = false;                             // inf or NaN in a row
 #pragma unroll
     for (int c = 0; c < CG; ++c) {
-        const float ll = row4_sum(l[c]);
         if (wrow + 16 * c + n >= gr.row0 + gr.rows) continue;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) odd |= !(fabsf(o[c][d][i]) < INFINITY);
+        const bool none = mr[c] == -INFINITY, seen = first <= last[c];
         if (ct.parts == 1) {
-            const bool none = m[c] == -INFINITY;      // nothing seen: 0; only scores of -inf: 0 / 0
+            // nothing seen: 0; only scores of -inf: 0 / 0
             XT *out = (XT *)a.out + (int64_t)(gr.q.first + row[c] / a.rep) * a.out_stride +
                       (int64_t)(gr.kvh * a.rep + row[c] % a.rep) * HD + 4 * g;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    out[16 * d + i] = (XT)(none ? (seen[c] ? NAN : 0.0f) : o[c][d][i] / ll);
+                    out[16 * d + i] = (XT)(none ? (seen ? NAN : 0.0f) : o[c][d][i] / l[c][0]);
         } else {
             const int64_t r = ((int64_t)unit * ta.splits + split) * ROWS + row[c] - gr.row0;
-            if (g == 0)
-                ta.ml[r] = m[c] == -INFINITY ? float2{-INFINITY, seen[c] ? 1.0f : 0.0f} : float2{mr[c], ll};
+            if (g == 0) ta.ml[r] = none ? float2{-INFINITY, seen ? 1.0f : 0.0f} : float2{mr[c], l[c][0]};
 #pragma unroll
             for (int d = 0; d < ND; ++d) *(f32x4 *)(ta.po + r * HD + 16 * d + 4 * g) = o[c][d];
+        }
+    }
+    if (low + 1 >= c1 || !__any(odd)) return;
+    // as in paged_split: the wave's rows one at a time, where one may have met an
+    // inf or NaN that it does not see
+    for (int rr = 0; rr < wrows; ++rr) {
+        const int32_t tt = (wrow + rr) / a.rep;
+        const int head = gr.kvh * a.rep + (wrow + rr) % a.rep;
+        const RowPart x =
+            row_part<XT, __bf16>(a, gr.b, gr.q.first + tt, head, c0, min(c1, gr.q.base + tt + 1), qs[w]);
+        if (ct.parts == 1) {
+            store_row<XT>(a, gr.q.first + tt, head, x);
+        } else {
+            const int64_t r = ((int64_t)unit * ta.splits + split) * ROWS + wrow + rr - gr.row0;
+            if (lane == 0) ta.ml[r] = x.m == -INFINITY ? float2{x.m, x.seen ? 1.0f : 0.0f} : float2{x.m, x.l};
+            for (int i = 0; 64 * i + lane < HD; ++i) ta.po[r * HD + 64 * i + lane] = x.o[i];
         }
     }
 }
@@ -1005,7 +991,7 @@ __global__ __launch_bounds__(256) void paged_tile_merge(const TileArgs ta) {
     const uint32_t unit = blockIdx.x / (kTileRows<XT> / R);
     const int rr = (int)(blockIdx.x % (kTileRows<XT> / R)) * R + threadIdx.x / T, d4 = threadIdx.x % T;
     Group gr;
-    if (!find_group<kTileRows<XT>>(a, unit, 16, gr)) return;
+    if (!find_group<kTileRows<XT>>(a, unit, 16, ta.pair_up, gr)) return;
     set_rows<kTileRows<XT>>(a, gr, gr.row0);
     const Cut ct = cut(gr.len, ta.splits, ta.least);
     if (ct.parts == 1 || rr >= gr.rows) return;
@@ -1059,6 +1045,8 @@ hipError_t launch_tile(tbh_device *dev, const PagedArgs &a, int64_t context, hip
     }
     if (units * std::max<int64_t>(ta.splits, kTileRows<XT> * HD / 1024) > INT32_MAX) return hipErrorInvalidValue;
     ta.units = (int32_t)units;
+    // two blocks share a CU: all run at once, or the longest have to come first
+    ta.pair_up = rows / kTileRows<XT> * a.nkv <= 2 * (int64_t)std::max(1, dev->cu_count);
     hipLaunchKernelGGL((paged_tile<XT, HD>), dim3((unsigned)(units * ta.splits)), dim3(256), 0, s, ta);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || ta.splits == 1) return e;
