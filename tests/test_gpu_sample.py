@@ -31,7 +31,7 @@ def _check(backend, x, u, t=1.0, k=0, p=1.0, m=0.0):
 
 SETTINGS = [dict(), dict(t=0.7), dict(t=0.0), dict(k=1), dict(k=5), dict(k=40), dict(k=700), dict(k=1 << 30),
             dict(p=0.9), dict(p=0.5, t=1.5), dict(p=0.999), dict(p=0.0), dict(p=-1.0), dict(m=0.05), dict(m=1.0),
-            dict(t=0.8, k=50, p=0.95, m=0.02), dict(k=3000, p=0.3), dict(t=100.0, k=200, p=0.7), dict(t=1e-3),
+            dict(t=0.8, k=50, p=0.95, m=0.02), dict(k=3000, p=0.3), dict(t=100.0, k=200, p=0.7), dict(t=1e-3), dict(t=1e-30, k=30, p=0.9),
             dict(t=-1.0), dict(t=float("nan")), dict(p=float("nan"), k=-3, m=float("nan")), dict(t=float("inf"), p=0.6)]
 
 

@@ -3,14 +3,21 @@
 //
 // Every filter keeps a prefix of the row in the order (logit descending, index
 // ascending), so the kept set is one pair (key, index): the last kept element.
-// A row's prefix is found without a sort: histograms of element counts (top-k)
-// or weights (top-p) over ever narrower ranges of keys, then, once the border
-// lies among at most kCand elements, each of them counts the others before it.
+// A row's prefix is found without a sort.  A histogram of the distance to the
+// largest logit, of element counts (top-k) or weights (top-p), names the bin the
+// border lies in.  If at most kCand elements lie in it and above it, they finish
+// the row among themselves in LDS: each counts those before it.  Else those of
+// the bin alone place the border, and the whole row is summed once more.  Bins of
+// more elements (equal logits, high temperatures) are narrowed by key first.
 //
-// Weights exp((l - max) / T) are formed in double precision and summed as
-// 64-bit integers of 2^-43: sums are exact and do not depend on their order,
-// and a token on the border of the cumulative sum is off by at most the weights'
-// own rounding.
+// Weights exp((l - max) / T) are summed as 64-bit integers of 2^-43: sums are
+// exact and do not depend on their order, and a token on the border of the
+// cumulative sum is off by at most the weights' own rounding.  A weight is formed
+// in double precision from a table of 2^(j / 64) and a polynomial of degree 5 on
+// +-1/128 (its error, (ln 2 / 128)^6 / 720, is below 2^-54).
+//
+// One block of 1024 threads takes a row; rows of up to 32 Ki logits stay in its
+// registers, longer ones are read again for each pass.
 #include <algorithm>
 #include <cstring>
 #include <new>
@@ -53,6 +60,7 @@ struct Shared {
         uint64_t wsum[kBins];
         uint64_t seg[kSegs];
     };
+    double pow2[64];                            // 2^(j / 64)
     uint32_t ckey[kCand], cidx[kCand];
     uint64_t cw[kCand];
     uint64_t red[kWaves];
@@ -68,20 +76,55 @@ __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
     return v;
 }
 
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_sum32(uint32_t v) {
+    v = dpp_add<wave::kXor1>(v);
+    v = dpp_add<wave::kXor2>(v);
+    v = dpp_add<wave::kHalfMirror>(v);
+    v = dpp_add<wave::kRowMirror>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 0) + (uint32_t)__builtin_amdgcn_readlane((int)v, 16) +
+           (uint32_t)__builtin_amdgcn_readlane((int)v, 32) + (uint32_t)__builtin_amdgcn_readlane((int)v, 48);
+}
+// Wave sum of values below 2^50, as two sums of 25 bits (64 of them fit 32).
+__device__ __forceinline__ uint64_t wave_sum50(uint64_t v) {
+    return ((uint64_t)wave_sum32((uint32_t)(v >> 25)) << 25) + wave_sum32((uint32_t)v & 0x1FFFFFFu);
+}
+
 struct Row {
     const float *x;
     int32_t vocab;
-    double m, inv_t;        // largest logit, 1 / temperature (1 where m is inf: all others weigh nothing)
-    uint32_t top;           // its key
+    double m, c;            // largest logit; log2(e) / temperature
+    const double *pow2;
+    uint32_t top;           // m's key
     // kept so far: key above `key`, or equal and index at most idx
     uint32_t key;
     uint32_t idx;
 
     __device__ __forceinline__ bool kept(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= idx); }
-    __device__ __forceinline__ double share(float l) const {   // exp((l - max) / T)
-        return (double)l == m ? 1.0 : exp(((double)l - m) * inv_t);
+    // log2 of a weight, at least -64; -64 for NaN and -inf
+    __device__ __forceinline__ double log_weight(float l) const {
+        if (m == INFINITY) return l == INFINITY ? 0.0 : -64.0;
+        const double t = ((double)l - m) * c;
+        return t > -64.0 ? t : -64.0;           // NaN too
     }
-    __device__ __forceinline__ uint64_t weight(float l) const { return (uint64_t)(share(l) * kOne + 0.5); }
+    __device__ __forceinline__ uint64_t weight_of(double t) const {   // round(2^(43 + t)), -64 <= t <= 0
+        constexpr double kShift = 6755399441055744.0;                 // 1.5 2^52: rounds to whole numbers
+        const double kd = fma(t, 64.0, kShift);
+        const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, kd);
+        const double r = fma(kd - kShift, -1.0 / 64.0, t);
+        double p = 1.3333558146428443e-3;                             // ln(2)^n / n!
+        p = fma(p, r, 9.618129107628477e-3);
+        p = fma(p, r, 5.550410866482158e-2);
+        p = fma(p, r, 2.402265069591007e-1);
+        p = fma(p, r, 6.931471805599453e-1);
+        p = fma(p, r, 1.0);
+        const double w = __builtin_amdgcn_ldexp(p * pow2[k & 63], (k >> 6) + 43);
+        return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // 2^52: to whole numbers
+    }
+    __device__ __forceinline__ uint64_t weight(float l) const { return weight_of(log_weight(l)); }
 };
 
 // Block sum of v in every thread.
@@ -207,7 +250,57 @@ __device__ void narrow(Row &row, uint64_t target, Shared &sh) {
     __syncthreads();
 }
 
+// The row's elements, four neighbours per thread and pass: pass p covers 4096 of
+// them, wave w's part of it piece 16 p + w of 256.  REG: up to 8 passes, held in
+// registers.
+template <bool REG, bool VEC>
+struct Elems {
+    float4 v[REG ? 8 : 1];
+    const float *x;
+    int32_t vocab;
+
+    static __device__ __forceinline__ float4 at(const float *x, int32_t i, int32_t vocab) {
+        if (VEC && i + 4 <= vocab) return *(const float4 *)(x + i);
+        float e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[k] = i + k < vocab ? x[i + k] : -INFINITY;
+        return float4{e[0], e[1], e[2], e[3]};
+    }
+    __device__ __forceinline__ void load(const float *x_, int32_t vocab_) {
+        x = x_;
+        vocab = vocab_;
+        if constexpr (REG) {
+#pragma unroll
+            for (int p = 0; p < 8; ++p) v[p] = at(x, 4096 * p + 4 * (int)threadIdx.x, vocab);
+        }
+    }
+    // f(piece, index of the first, four elements); elements behind the row are -inf
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        const int tid = threadIdx.x, wave = tid >> 6;
+        if constexpr (REG) {
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+                if (4096 * p < vocab) f(16 * p + wave, 4096 * p + 4 * tid, v[p]);
+                __builtin_amdgcn_sched_barrier(0);   // one pass at a time: registers
+            }
+        } else {
+            const int32_t n = (vocab + 4095) / 4096;
+            float4 a = at(x, 4 * tid, vocab);
+            for (int32_t p = 0; p < n; ++p) {
+                const float4 b = p + 1 < n ? at(x, 4096 * (p + 1) + 4 * tid, vocab) : a;   // the next, meanwhile
+                f(16 * p + wave, 4096 * p + 4 * tid, a);
+                a = b;
+            }
+        }
+    }
+};
+
+// Bin of a weight by its logarithm: 1/64 nats wide, from 2^-46 down the last.
+__device__ __forceinline__ int bin_of(double t) { return min(kBins - 1, (int)(t * -44.3614195558365)); }
+
 // One block per row.
+template <bool REG, bool VEC>
 __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
     __shared__ Shared sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -215,13 +308,34 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
     Row row;
     row.x = a.logits + r * a.ld;
     row.vocab = a.vocab;
+    row.pow2 = sh.pow2;
+    Elems<REG, VEC> el;
+    el.load(row.x, a.vocab);
+    if (tid < 64) sh.pow2[tid] = exp2(tid * (1.0 / 64.0));
+    for (int b = tid; b < kBins; b += kThreads) {
+        sh.cnt[b] = 0;
+        sh.wsum[b] = 0;
+    }
+    if (tid == 0) sh.n = 0;
+    const float t = a.temperature ? a.temperature[r] : 1.0f;
+    const int32_t k = a.top_k ? a.top_k[r] : 0;
+    const float p = a.top_p ? a.top_p[r] : 1.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
+    float u = a.u[r];
 
     // largest logit, first of equal ones
-    uint64_t best = 0;
-    for (int32_t i = tid; i < a.vocab; i += kThreads) {
-        const uint64_t v = (uint64_t)key_of(row.x[i]) << 32 | (uint32_t)~i;
-        best = best > v ? best : v;
-    }
+    uint32_t bk = 0, bi = 0;
+    el.each([&](int, int32_t i, const float4 &v) {
+        const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t key = key_of(e[j]);
+            if (key > bk) {                      // indices rise: the first of equal ones stays
+                bk = key;
+                bi = i + j;
+            }
+        }
+    });
+    uint64_t best = (uint64_t)bk << 32 | (uint32_t)~bi;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
         const uint64_t o = __shfl_xor(best, d);
@@ -233,7 +347,6 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
     __syncthreads();
     row.top = (uint32_t)(best >> 32);
     const uint32_t arg = ~(uint32_t)best;
-    const float t = a.temperature ? a.temperature[r] : 1.0f;
     if (row.top <= kNone || !(t > 0.0f)) {
         if (tid == 0) {
             const bool none = row.top <= kNone;
@@ -242,58 +355,227 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
         }
         return;
     }
-    row.m = (double)row.x[arg];
-    row.inv_t = row.m == INFINITY ? 1.0 : 1.0 / (double)t;
+    row.m = (double)(row.top & 0x80000000u ? __builtin_bit_cast(float, row.top & 0x7FFFFFFFu)
+                                           : __builtin_bit_cast(float, ~row.top));
+    row.c = 1.4426950408889634 / (double)t;
     row.key = kNone + 1;      // everything above -inf ...
     row.idx = 0xFFFFFFFFu;
+    u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+    // a weight below min_p is one whose logarithm is below min_p's
+    const double cut = mp > 0.0f ? log2((double)mp) : -INFINITY;
+    auto passes = [&](double lw, uint32_t key) { return key == row.top || !(lw < cut); };
 
-    const int32_t k = a.top_k ? a.top_k[r] : 0;
-    if (k > 0 && k < a.vocab) {
-        uint64_t n = 0;       // elements above -inf
-        for (int32_t i = tid; i < a.vocab; i += kThreads) n += key_of(row.x[i]) > kNone;
-        n = block_sum64(n, sh);
-        if ((uint64_t)k < n) narrow<false>(row, (uint64_t)k, sh);
-    }
-    const float p = a.top_p ? a.top_p[r] : 1.0f;
-    if (p < 1.0f) {
-        uint64_t s = 0;
-        for (int32_t i = tid; i < a.vocab; i += kThreads) {
-            const float l = row.x[i];
-            if (row.kept(key_of(l), i)) s += row.weight(l);
+    // The border's bin, of the first `target` elements or of that much weight.
+    struct Border {
+        uint64_t above;       // what lies in the bins before it
+        uint32_t bin, pop, upto;   // its elements; those up to and with it
+    };
+    auto find = [&](bool by_weight, uint64_t target) {
+        __syncthreads();
+        const uint32_t c0 = sh.cnt[2 * tid], c1 = sh.cnt[2 * tid + 1];
+        const uint64_t v0 = by_weight ? sh.wsum[2 * tid] : c0, v1 = by_weight ? sh.wsum[2 * tid + 1] : c1;
+        uint64_t in = v0 + v1;
+        uint32_t cin = c0 + c1;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint64_t o = __shfl_up(in, d);
+            const uint32_t co = __shfl_up(cin, d);
+            if (lane >= d) {
+                in += o;
+                cin += co;
+            }
         }
-        const double want = ceil((double)p * (double)block_sum64(s, sh));
-        narrow<true>(row, want >= 1.0 ? (uint64_t)want : 1, sh);
-    }
-    // a weight below min_p is one of a logit below max + T log(min_p)
-    const float mp = a.min_p ? a.min_p[r] : 0.0f;
-    const double cut = mp > 0.0f ? log((double)mp) : -INFINITY;
+        if (lane == 63) {
+            sh.red[wave] = in;
+            sh.redc[wave] = cin;
+        }
+        if (tid == 0) sh.bin = kBins;
+        __syncthreads();
+        uint64_t b0 = in - v0 - v1;
+        uint32_t n0 = cin - c0 - c1;
+        for (int i = 0; i < wave; ++i) {
+            b0 += sh.red[i];
+            n0 += sh.redc[i];
+        }
+        const uint64_t b1 = b0 + v0, b2 = b1 + v1;
+        if (b0 < target && b1 >= target) {
+            sh.bin = 2 * tid;
+            sh.above_w = b0;
+            sh.pop = c0;
+            sh.above_c = n0 + c0;
+        } else if (b1 < target && b2 >= target) {
+            sh.bin = 2 * tid + 1;
+            sh.above_w = b1;
+            sh.pop = c1;
+            sh.above_c = n0 + c0 + c1;
+        }
+        __syncthreads();
+        return Border{sh.above_w, sh.bin, sh.pop, sh.above_c};
+    };
+    // The elements of bins `from` .. `to` as candidates (at most kCand).
+    auto gather = [&](uint32_t from, uint32_t to) {
+        el.each([&](int, int32_t i, const float4 &v) {
+            const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (!(e[j] > -INFINITY)) continue;
+                const double lw = row.log_weight(e[j]);
+                const uint32_t b = bin_of(lw);
+                if (b < from || b > to) continue;
+                const uint32_t at = atomicAdd(&sh.n, 1u);
+                sh.ckey[at] = key_of(e[j]);
+                sh.cidx[at] = i + j;
+                sh.cw[at] = row.weight_of(lw);
+            }
+        });
+        __syncthreads();
+    };
+    // The row's token from all elements it may be, n candidates; all: the weight
+    // that top_p is of (0: the first k's).
+    auto finish = [&](uint32_t n, uint64_t all) {
+        const bool mine = tid < (int)n;
+        const uint32_t key = mine ? sh.ckey[tid] : 0, ix = mine ? sh.cidx[tid] : 0;
+        const uint64_t w = mine ? sh.cw[tid] : 0;
+        uint32_t rank = 0;
+        uint64_t before = 0;
+        if (64 * wave < (int)n)
+            for (uint32_t j = 0; j < n; ++j) {
+                const uint32_t kj = sh.ckey[j];
+                if (kj > key || (kj == key && sh.cidx[j] < ix)) {
+                    ++rank;
+                    before += sh.cw[j];
+                }
+            }
+        bool keep = mine && (k <= 0 || rank < (uint32_t)k);
+        if (p < 1.0f) {
+            const double want = ceil((double)p * (double)(all ? all : block_sum64(keep ? w : 0, sh)));
+            keep &= before < (want >= 1.0 ? (uint64_t)want : 1);
+        }
+        if (mp > 0.0f && keep) {
+            const float l = key & 0x80000000u ? __builtin_bit_cast(float, key & 0x7FFFFFFFu)
+                                              : __builtin_bit_cast(float, ~key);
+            keep = passes(row.log_weight(l), key);
+        }
+        const uint64_t total = block_sum64(keep ? w : 0, sh);
+        if (mine) sh.cw[tid] = keep ? w : 0;
+        __syncthreads();
+        const uint64_t at = (uint64_t)((double)u * (double)total);
+        uint64_t run = 0;
+        if (64 * wave < (int)n)
+            for (uint32_t j = 0; j < n; ++j)
+                if (sh.cidx[j] < ix) run += sh.cw[j];
+        if (keep && run <= at && at < run + w) {
+            a.tokens[r] = (int32_t)ix;
+            if (a.probs) a.probs[r] = (float)(exp2(row.log_weight(row.x[ix])) * (kOne / (double)total));
+        }
+    };
 
-    auto weight = [&](int32_t i) -> uint64_t {
-        const float l = row.x[i];
-        if (!row.kept(key_of(l), i) || ((double)l != row.m && ((double)l - row.m) * row.inv_t < cut)) return 0;
-        return row.weight(l);
+    bool counted = false;                         // the histogram holds counts
+    if (k > 0 && k < a.vocab) {
+        el.each([&](int, int32_t, const float4 &v) {
+            const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (e[j] > -INFINITY) {
+                    const int b = bin_of(row.log_weight(e[j]));
+                    if (b < kBins - 1) atomicAdd(&sh.cnt[b], 1u);   // what weighs nothing need not be counted
+                }
+        });
+        counted = true;
+        const Border bd = find(false, (uint64_t)k);
+        if (bd.bin < (uint32_t)kBins) {           // else fewer than k elements weigh something: all are kept
+            if (bd.upto <= kCand) {
+                gather(0, bd.bin);
+                finish(bd.upto, 0);
+                return;
+            }
+            narrow<false>(row, (uint64_t)k, sh);
+        }
+    }
+    if (p < 1.0f) {
+        const bool whole = row.key == kNone + 1 && row.idx == 0xFFFFFFFFu;
+        uint64_t s = 0;
+        if (whole) {
+            if (counted) {
+                __syncthreads();
+                for (int b = tid; b < kBins; b += kThreads) sh.cnt[b] = 0;
+                __syncthreads();
+            }
+            el.each([&](int, int32_t, const float4 &v) {
+                const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const double lw = row.log_weight(e[j]);
+                    const int b = bin_of(lw);
+                    if (b < kBins - 1) {
+                        const uint64_t w = row.weight_of(lw);
+                        s += w;
+                        atomicAdd(&sh.cnt[b], 1u);
+                        atomicAdd((unsigned long long *)&sh.wsum[b], (unsigned long long)w);
+                    }
+                }
+            });
+        } else {
+            el.each([&](int, int32_t i, const float4 &v) {
+                const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (row.kept(key_of(e[j]), i + j)) s += row.weight(e[j]);
+            });
+        }
+        const uint64_t all = block_sum64(s, sh);
+        const double want = ceil((double)p * (double)all);
+        const uint64_t target = want >= 1.0 ? (uint64_t)want : 1;
+        bool done = false;
+        if (whole) {
+            const Border bd = find(true, target);
+            if (bd.upto <= kCand) {
+                gather(0, bd.bin);
+                finish(bd.upto, all);
+                return;
+            }
+            if (bd.pop <= kCand) {
+                gather(bd.bin, bd.bin);
+                for (uint32_t c = tid; c < bd.pop; c += kThreads) {
+                    const uint32_t key = sh.ckey[c], ix = sh.cidx[c];
+                    uint64_t before = bd.above;
+                    for (uint32_t j = 0; j < bd.pop; ++j)
+                        if (sh.ckey[j] > key || (sh.ckey[j] == key && sh.cidx[j] < ix)) before += sh.cw[j];
+                    if (before < target && before + sh.cw[c] >= target) {
+                        sh.key = key;
+                        sh.idx = ix;
+                    }
+                }
+                __syncthreads();
+                row.key = sh.key;
+                row.idx = sh.idx;
+                done = true;
+            }
+        }
+        if (!done) narrow<true>(row, target, sh);
+    }
+
+    auto weight = [&](float l, int32_t i) -> uint64_t {
+        const uint32_t key = key_of(l);
+        const double lw = row.log_weight(l);
+        return row.kept(key, i) && passes(lw, key) ? row.weight_of(lw) : 0;
     };
     // sums of pieces of 256 elements, in index order
     const int32_t segs = (a.vocab + kSeg - 1) / kSeg;
-    uint64_t all = 0;
-    for (int32_t g = wave; g < segs; g += kWaves) {
-        uint64_t s = 0;
-        for (int j = 0; j < kSeg / 64; ++j) {
-            const int32_t i = g * kSeg + j * 64 + lane;
-            if (i < a.vocab) s += weight(i);
-        }
-        s = wave_sum64(s);
-        if (lane == 0) sh.seg[g] = s;
-        all += s;
-    }
-    if (lane == 0) sh.red[wave] = all;
+    __syncthreads();                              // the histogram's memory holds them
+    uint64_t sum = 0;
+    el.each([&](int piece, int32_t i, const float4 &v) {
+        const uint64_t s = weight(v.x, i) + weight(v.y, i + 1) + weight(v.z, i + 2) + weight(v.w, i + 3);
+        const uint64_t total = wave_sum50(s);
+        if (lane == 0 && piece < segs) sh.seg[piece] = total;
+        sum += total;
+    });
+    if (lane == 0) sh.red[wave] = sum;
     __syncthreads();
     uint64_t total = 0;
     for (int i = 0; i < kWaves; ++i) total += sh.red[i];
     if (wave != 0) return;
-    float u = a.u[r];
-    u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
-    uint64_t at = (uint64_t)((double)u * (double)total);      // below the total
+    const uint64_t at = (uint64_t)((double)u * (double)total);      // below the total
     // the piece, then the element whose running sum passes `at`
     int32_t piece = -1;
     uint64_t run = 0;
@@ -317,7 +599,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
     int32_t token = -1;
     for (int j = 0; j < kSeg / 64 && token < 0 && piece >= 0; ++j) {
         const int32_t i = piece * kSeg + j * 64 + lane;
-        uint64_t in = i < a.vocab ? weight(i) : 0;
+        uint64_t in = i < a.vocab ? weight(row.x[i], i) : 0;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const uint64_t o = __shfl_up(in, d);
@@ -329,7 +611,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
     }
     if (lane == 0) {
         a.tokens[r] = token;
-        if (a.probs) a.probs[r] = token < 0 ? 0.0f : (float)(row.share(row.x[token]) * (kOne / (double)total));
+        if (a.probs)
+            a.probs[r] = token < 0 ? 0.0f : (float)(exp2(row.log_weight(row.x[token])) * (kOne / (double)total));
     }
 }
 
@@ -346,7 +629,12 @@ tbh_status check_sample(const char *what, tbh_device *dev, const float *logits, 
 }
 
 hipError_t launch_sample(const SampleArgs &a, int64_t rows, hipStream_t s) {
-    hipLaunchKernelGGL(sample_rows, dim3((unsigned)rows), dim3(kThreads), 0, s, a);
+    const dim3 grid((unsigned)rows), block(kThreads);
+    const bool vec = ((uintptr_t)a.logits & 15) == 0 && (a.ld % 4 == 0 || rows == 1), reg = a.vocab <= 8 * 4096;
+    if (reg && vec) hipLaunchKernelGGL((sample_rows<true, true>), grid, block, 0, s, a);
+    else if (reg) hipLaunchKernelGGL((sample_rows<true, false>), grid, block, 0, s, a);
+    else if (vec) hipLaunchKernelGGL((sample_rows<false, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((sample_rows<false, false>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 
