@@ -53,21 +53,29 @@ __device__ __forceinline__ uint32_t key_of(float l) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 constexpr uint32_t kNone = 0x007FFFFFu;         // key of -inf
+__device__ __forceinline__ float logit_of(uint32_t key) {
+    return key & 0x80000000u ? __builtin_bit_cast(float, key & 0x7FFFFFFFu) : __builtin_bit_cast(float, ~key);
+}
 
 struct Shared {
-    uint32_t cnt[kBins];
+    union {
+        uint32_t cnt[kBins];
+        uint32_t ranks[kThreads];               // partial ranks of candidates
+    };
     union {
         uint64_t wsum[kBins];
         uint64_t seg[kSegs];
     };
+    uint64_t sums[kThreads];                    // and partial sums
     double pow2[64];                            // 2^(j / 64)
-    uint32_t ckey[kCand], cidx[kCand];
+    uint32_t ckey[kCand];
+    int32_t cidx[kCand];
     uint64_t cw[kCand];
     uint64_t red[kWaves];
     uint32_t redc[kWaves];
     uint64_t above_w;
-    uint32_t above_c, bin, pop, n, key, idx;
-    int32_t token;
+    uint32_t above_c, bin, pop, n, key;
+    int32_t idx;
 };
 
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
@@ -96,19 +104,23 @@ __device__ __forceinline__ uint64_t wave_sum50(uint64_t v) {
 struct Row {
     const float *x;
     int32_t vocab;
-    double m, c;            // largest logit; log2(e) / temperature
+    float cap;              // largest logit; of a row with inf: the largest finite float, standing for inf
+    float bins;             // 64 / temperature
+    double c;               // log2(e) / temperature
     const double *pow2;
-    uint32_t top;           // m's key
-    // kept so far: key above `key`, or equal and index at most idx
-    uint32_t key;
-    uint32_t idx;
+    uint32_t top;           // the largest logit's key
+    // kept so far: logits above `least`, or equal and of index at most idx
+    float least;
+    int32_t idx;
 
-    __device__ __forceinline__ bool kept(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= idx); }
-    // log2 of a weight, at least -64; -64 for NaN and -inf
+    __device__ __forceinline__ bool kept(float l, int32_t i) const { return l > least || (l == least && i <= idx); }
+    // log2 of the weight of a kept logit, at least -64
     __device__ __forceinline__ double log_weight(float l) const {
-        if (m == INFINITY) return l == INFINITY ? 0.0 : -64.0;
-        const double t = ((double)l - m) * c;
-        return t > -64.0 ? t : -64.0;           // NaN too
+        return fmax(((double)fminf(l, cap) - (double)cap) * c, -64.0);
+    }
+    // Distance to the largest logit in 1/64 of a power of e: from 2^-46 down the last bin.
+    __device__ __forceinline__ uint32_t bin(float l) const {
+        return (uint32_t)min(kBins - 1, (int)((cap - fminf(l, cap)) * bins));
     }
     __device__ __forceinline__ uint64_t weight_of(double t) const {   // round(2^(43 + t)), -64 <= t <= 0
         constexpr double kShift = 6755399441055744.0;                 // 1.5 2^52: rounds to whole numbers
@@ -125,6 +137,16 @@ struct Row {
         return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // 2^52: to whole numbers
     }
     __device__ __forceinline__ uint64_t weight(float l) const { return weight_of(log_weight(l)); }
+    // Four at once.  The compiler would move each into the branch that uses it, where
+    // its chain of dependent operations waits alone; the empty statement keeps them
+    // side by side (a row of 32000 logits without filters: 29 us, 22 with it).
+    __device__ __forceinline__ void weights4(const float (&e)[4], double (&lw)[4], uint64_t (&w)[4]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lw[j] = log_weight(e[j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = weight_of(lw[j]);
+        asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
+    }
 };
 
 // Block sum of v in every thread.
@@ -139,12 +161,12 @@ __device__ __forceinline__ uint64_t block_sum64(uint64_t v, Shared &sh) {
     return t;
 }
 
-// Cuts row.key / row.idx down to the shortest prefix whose count (BYW false) or
+// Cuts row.least / row.idx down to the shortest prefix whose count (BYW false) or
 // weight reaches `target` (at least 1, and the kept elements reach it).
 template <bool BYW>
 __device__ void narrow(Row &row, uint64_t target, Shared &sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    uint32_t hi = row.top, lo = row.key;
+    uint32_t hi = row.top, lo = key_of(row.least);
     uint64_t above = 0;                          // count or weight of the keys above hi
     for (;;) {
         const uint32_t span = hi - lo;
@@ -157,7 +179,7 @@ __device__ void narrow(Row &row, uint64_t target, Shared &sh) {
         for (int32_t i = tid; i < row.vocab; i += kThreads) {
             const float l = row.x[i];
             const uint32_t k = key_of(l);
-            if (k <= hi && k >= lo && row.kept(k, i)) {
+            if (k <= hi && k >= lo && row.kept(l, i)) {
                 const uint32_t b = (hi - k) >> shift;
                 atomicAdd(&sh.cnt[b], 1u);
                 if (BYW) atomicAdd((unsigned long long *)&sh.wsum[b], (unsigned long long)row.weight(l));
@@ -200,7 +222,7 @@ __device__ void narrow(Row &row, uint64_t target, Shared &sh) {
             for (int32_t i = tid; i < row.vocab; i += kThreads) {
                 const float l = row.x[i];
                 const uint32_t k = key_of(l);
-                if (k <= hi && k >= lo && row.kept(k, i)) {
+                if (k <= hi && k >= lo && row.kept(l, i)) {
                     const uint32_t at = atomicAdd(&sh.n, 1u);
                     sh.ckey[at] = k;
                     sh.cidx[at] = i;
@@ -209,7 +231,8 @@ __device__ void narrow(Row &row, uint64_t target, Shared &sh) {
             }
             __syncthreads();
             for (uint32_t c = tid; c < pop; c += kThreads) {
-                const uint32_t k = sh.ckey[c], ix = sh.cidx[c];
+                const uint32_t k = sh.ckey[c];
+                const int32_t ix = sh.cidx[c];
                 uint64_t s = above;
                 for (uint32_t j = 0; j < pop; ++j)
                     if (sh.ckey[j] > k || (sh.ckey[j] == k && sh.cidx[j] < ix)) s += sh.cw[j];
@@ -219,19 +242,19 @@ __device__ void narrow(Row &row, uint64_t target, Shared &sh) {
                 }
             }
             __syncthreads();
-            row.key = sh.key;
+            row.least = logit_of(sh.key);
             row.idx = sh.idx;
             __syncthreads();
             return;
         }
     }
     // many equal logits: the border is the R-th of them in index order
-    const float l = hi & 0x80000000u ? __builtin_bit_cast(float, hi & 0x7FFFFFFFu) : __builtin_bit_cast(float, ~hi);
+    const float l = logit_of(hi);
     const uint64_t w = BYW ? row.weight(l) : 1;
     uint64_t left = (target - above + w - 1) / w;
     for (int32_t i0 = 0; i0 < row.vocab; i0 += kThreads) {
         const int32_t i = i0 + tid;
-        const bool on = i < row.vocab && key_of(row.x[i]) == hi && row.kept(hi, i);
+        const bool on = i < row.vocab && row.x[i] == l && row.kept(l, i);
         const uint64_t m = __ballot(on);
         if (lane == 0) sh.redc[wave] = __popcll(m);
         __syncthreads();
@@ -245,7 +268,7 @@ __device__ void narrow(Row &row, uint64_t target, Shared &sh) {
         if (total >= left) break;
         left -= total;
     }
-    row.key = hi;
+    row.least = l;
     row.idx = sh.idx;
     __syncthreads();
 }
@@ -295,9 +318,6 @@ struct Elems {
         }
     }
 };
-
-// Bin of a weight by its logarithm: 1/64 nats wide, from 2^-46 down the last.
-__device__ __forceinline__ int bin_of(double t) { return min(kBins - 1, (int)(t * -44.3614195558365)); }
 
 // One block per row.
 template <bool REG, bool VEC>
@@ -355,15 +375,16 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
         }
         return;
     }
-    row.m = (double)(row.top & 0x80000000u ? __builtin_bit_cast(float, row.top & 0x7FFFFFFFu)
-                                           : __builtin_bit_cast(float, ~row.top));
+    const float largest = logit_of(row.top);
+    const bool inf = largest == INFINITY;
+    row.cap = inf ? 3.40282347e38f : largest;
+    row.bins = 64.0f / t;
     row.c = 1.4426950408889634 / (double)t;
-    row.key = kNone + 1;      // everything above -inf ...
-    row.idx = 0xFFFFFFFFu;
+    row.least = inf ? row.cap : -INFINITY;    // everything above -inf, or the infinities alone ...
+    row.idx = -1;
     u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
-    // a weight below min_p is one whose logarithm is below min_p's
-    const double cut = mp > 0.0f ? log2((double)mp) : -INFINITY;
-    auto passes = [&](double lw, uint32_t key) { return key == row.top || !(lw < cut); };
+    // the least logarithm of a weight that min_p keeps (the largest, 0, always)
+    const double cut = mp > 0.0f ? fmin(log2((double)mp), 0.0) : -INFINITY;
 
     // The border's bin, of the first `target` elements or of that much weight.
     struct Border {
@@ -412,74 +433,90 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
         __syncthreads();
         return Border{sh.above_w, sh.bin, sh.pop, sh.above_c};
     };
-    // The elements of bins `from` .. `to` as candidates (at most kCand).
+    // The kept elements of bins `from` .. `to` as candidates (at most kCand).
     auto gather = [&](uint32_t from, uint32_t to) {
         el.each([&](int, int32_t i, const float4 &v) {
             const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (!(e[j] > -INFINITY)) continue;
-                const double lw = row.log_weight(e[j]);
-                const uint32_t b = bin_of(lw);
-                if (b < from || b > to) continue;
+                const uint32_t b = row.bin(e[j]);
+                if (b < from || b > to || !row.kept(e[j], i + j)) continue;
                 const uint32_t at = atomicAdd(&sh.n, 1u);
                 sh.ckey[at] = key_of(e[j]);
                 sh.cidx[at] = i + j;
-                sh.cw[at] = row.weight_of(lw);
             }
         });
         __syncthreads();
+        if (tid < (int)sh.n) sh.cw[tid] = row.weight(logit_of(sh.ckey[tid]));
+        __syncthreads();
     };
+    // Over n candidates: how many of those for which first(j, c) holds, and their
+    // weight, for candidate c = this thread's column; the threads of a column
+    // share the others, and column c's first thread (tid c) returns the sums.
+    struct Count {
+        uint32_t n;
+        uint64_t w;
+    };
+    auto tally = [&](uint32_t n, auto first) {
+        const uint32_t cols = n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512, rows = kThreads / cols;
+        const uint32_t c = tid & (cols - 1), s0 = tid / cols;
+        const uint32_t key = c < n ? sh.ckey[c] : 0;
+        const int32_t ix = c < n ? sh.cidx[c] : 0;
+        Count t{0, 0};
+#pragma unroll 4
+        for (uint32_t j = s0; j < n; j += rows)
+            if (first(sh.ckey[j], sh.cidx[j], key, ix)) {
+                ++t.n;
+                t.w += sh.cw[j];
+            }
+        __syncthreads();
+        sh.ranks[tid] = t.n;
+        sh.sums[tid] = t.w;
+        __syncthreads();
+        if (tid < (int)cols) {
+#pragma unroll 4
+            for (uint32_t q = 1; q < rows; ++q) {
+                t.n += sh.ranks[q * cols + tid];
+                t.w += sh.sums[q * cols + tid];
+            }
+        }
+        return t;
+    };
+    auto in_order = [](uint32_t kj, int32_t ij, uint32_t key, int32_t ix) { return kj > key || (kj == key && ij < ix); };
     // The row's token from all elements it may be, n candidates; all: the weight
     // that top_p is of (0: the first k's).
     auto finish = [&](uint32_t n, uint64_t all) {
         const bool mine = tid < (int)n;
-        const uint32_t key = mine ? sh.ckey[tid] : 0, ix = mine ? sh.cidx[tid] : 0;
         const uint64_t w = mine ? sh.cw[tid] : 0;
-        uint32_t rank = 0;
-        uint64_t before = 0;
-        if (64 * wave < (int)n)
-            for (uint32_t j = 0; j < n; ++j) {
-                const uint32_t kj = sh.ckey[j];
-                if (kj > key || (kj == key && sh.cidx[j] < ix)) {
-                    ++rank;
-                    before += sh.cw[j];
-                }
-            }
-        bool keep = mine && (k <= 0 || rank < (uint32_t)k);
+        const Count before = tally(n, in_order);
+        bool keep = mine && (k <= 0 || before.n < (uint32_t)k);
         if (p < 1.0f) {
             const double want = ceil((double)p * (double)(all ? all : block_sum64(keep ? w : 0, sh)));
-            keep &= before < (want >= 1.0 ? (uint64_t)want : 1);
+            keep &= before.w < (want >= 1.0 ? (uint64_t)want : 1);
         }
-        if (mp > 0.0f && keep) {
-            const float l = key & 0x80000000u ? __builtin_bit_cast(float, key & 0x7FFFFFFFu)
-                                              : __builtin_bit_cast(float, ~key);
-            keep = passes(row.log_weight(l), key);
-        }
+        if (mp > 0.0f && keep) keep = row.log_weight(logit_of(sh.ckey[tid])) >= cut;
         const uint64_t total = block_sum64(keep ? w : 0, sh);
         if (mine) sh.cw[tid] = keep ? w : 0;
         __syncthreads();
         const uint64_t at = (uint64_t)((double)u * (double)total);
-        uint64_t run = 0;
-        if (64 * wave < (int)n)
-            for (uint32_t j = 0; j < n; ++j)
-                if (sh.cidx[j] < ix) run += sh.cw[j];
+        const uint64_t run = tally(n, [](uint32_t, int32_t ij, uint32_t, int32_t ix) { return ij < ix; }).w;
         if (keep && run <= at && at < run + w) {
-            a.tokens[r] = (int32_t)ix;
-            if (a.probs) a.probs[r] = (float)(exp2(row.log_weight(row.x[ix])) * (kOne / (double)total));
+            a.tokens[r] = sh.cidx[tid];
+            if (a.probs) a.probs[r] = (float)(exp2(row.log_weight(logit_of(sh.ckey[tid]))) * (kOne / (double)total));
         }
     };
 
-    bool counted = false;                         // the histogram holds counts
+    uint32_t edge = kBins, edge_pop = 0;          // the bin in which top_p's border lies, still to be placed
+    uint64_t edge_above = 0, edge_target = 0;
+    bool counted = false, whole = true;           // the histogram holds counts; nothing is cut off yet
     if (k > 0 && k < a.vocab) {
-        el.each([&](int, int32_t, const float4 &v) {
+        el.each([&](int, int32_t i, const float4 &v) {
             const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (e[j] > -INFINITY) {
-                    const int b = bin_of(row.log_weight(e[j]));
-                    if (b < kBins - 1) atomicAdd(&sh.cnt[b], 1u);   // what weighs nothing need not be counted
-                }
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t b = row.bin(e[j]);
+                if (b < kBins - 1 && row.kept(e[j], i + j)) atomicAdd(&sh.cnt[b], 1u);   // the last weighs nothing
+            }
         });
         counted = true;
         const Border bd = find(false, (uint64_t)k);
@@ -490,86 +527,111 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
                 return;
             }
             narrow<false>(row, (uint64_t)k, sh);
+            whole = false;
         }
     }
     if (p < 1.0f) {
-        const bool whole = row.key == kNone + 1 && row.idx == 0xFFFFFFFFu;
         uint64_t s = 0;
-        if (whole) {
-            if (counted) {
-                __syncthreads();
-                for (int b = tid; b < kBins; b += kThreads) sh.cnt[b] = 0;
-                __syncthreads();
+        if (counted) {
+            __syncthreads();
+            for (int b = tid; b < kBins; b += kThreads) {
+                sh.cnt[b] = 0;
+                sh.wsum[b] = 0;
             }
-            el.each([&](int, int32_t, const float4 &v) {
-                const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const double lw = row.log_weight(e[j]);
-                    const int b = bin_of(lw);
-                    if (b < kBins - 1) {
-                        const uint64_t w = row.weight_of(lw);
-                        s += w;
-                        atomicAdd(&sh.cnt[b], 1u);
-                        atomicAdd((unsigned long long *)&sh.wsum[b], (unsigned long long)w);
-                    }
-                }
-            });
-        } else {
-            el.each([&](int, int32_t i, const float4 &v) {
-                const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (row.kept(key_of(e[j]), i + j)) s += row.weight(e[j]);
-            });
+            if (tid == 0) sh.n = 0;
+            __syncthreads();
         }
+        el.each([&](int, int32_t i, const float4 &v) {
+            const float e[4] = {v.x, v.y, v.z, v.w};
+            double lw[4];
+            uint64_t w[4];
+            row.weights4(e, lw, w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t b = row.bin(e[j]);
+                if (b < kBins - 1 && row.kept(e[j], i + j)) {
+                    s += w[j];
+                    atomicAdd(&sh.cnt[b], 1u);
+                    atomicAdd((unsigned long long *)&sh.wsum[b], (unsigned long long)w[j]);
+                }
+            }
+        });
         const uint64_t all = block_sum64(s, sh);
         const double want = ceil((double)p * (double)all);
         const uint64_t target = want >= 1.0 ? (uint64_t)want : 1;
-        bool done = false;
-        if (whole) {
-            const Border bd = find(true, target);
-            if (bd.upto <= kCand) {
-                gather(0, bd.bin);
-                finish(bd.upto, all);
-                return;
-            }
-            if (bd.pop <= kCand) {
-                gather(bd.bin, bd.bin);
-                for (uint32_t c = tid; c < bd.pop; c += kThreads) {
-                    const uint32_t key = sh.ckey[c], ix = sh.cidx[c];
-                    uint64_t before = bd.above;
-                    for (uint32_t j = 0; j < bd.pop; ++j)
-                        if (sh.ckey[j] > key || (sh.ckey[j] == key && sh.cidx[j] < ix)) before += sh.cw[j];
-                    if (before < target && before + sh.cw[c] >= target) {
-                        sh.key = key;
-                        sh.idx = ix;
-                    }
-                }
-                __syncthreads();
-                row.key = sh.key;
-                row.idx = sh.idx;
-                done = true;
-            }
+        const Border bd = find(true, target);
+        if (whole && bd.upto <= kCand) {
+            gather(0, bd.bin);
+            finish(bd.upto, all);
+            return;
         }
-        if (!done) narrow<true>(row, target, sh);
+        if (bd.pop <= kCand) {
+            edge = bd.bin;
+            edge_pop = bd.pop;
+            edge_above = bd.above;
+            edge_target = target;
+        } else {
+            narrow<true>(row, target, sh);
+        }
     }
 
     auto weight = [&](float l, int32_t i) -> uint64_t {
-        const uint32_t key = key_of(l);
         const double lw = row.log_weight(l);
-        return row.kept(key, i) && passes(lw, key) ? row.weight_of(lw) : 0;
+        return row.kept(l, i) && lw >= cut ? row.weight_of(lw) : 0;
     };
-    // sums of pieces of 256 elements, in index order
+    // sums of pieces of 256 elements, in index order; those of the border's bin
+    // are set aside and added once it is placed among them
     const int32_t segs = (a.vocab + kSeg - 1) / kSeg;
     __syncthreads();                              // the histogram's memory holds them
     uint64_t sum = 0;
     el.each([&](int piece, int32_t i, const float4 &v) {
-        const uint64_t s = weight(v.x, i) + weight(v.y, i + 1) + weight(v.z, i + 2) + weight(v.w, i + 3);
-        const uint64_t total = wave_sum50(s);
+        const float e[4] = {v.x, v.y, v.z, v.w};
+        bool on[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            on[j] = row.kept(e[j], i + j);
+            if (edge < (uint32_t)kBins) {
+                const uint32_t b = row.bin(e[j]);
+                if (on[j] && b == edge) {
+                    const uint32_t at = atomicAdd(&sh.n, 1u);
+                    sh.ckey[at] = key_of(e[j]);
+                    sh.cidx[at] = i + j;
+                }
+                on[j] &= b < edge;
+            }
+        }
+        uint64_t total = 0;
+        if (__any(on[0] || on[1] || on[2] || on[3])) {
+            double lw[4];
+            uint64_t w[4], s = 0;
+            row.weights4(e, lw, w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s += on[j] && lw[j] >= cut ? w[j] : 0;
+            total = wave_sum50(s);
+        }
         if (lane == 0 && piece < segs) sh.seg[piece] = total;
         sum += total;
     });
+    if (edge < (uint32_t)kBins) {
+        __syncthreads();
+        if (tid < (int)edge_pop) sh.cw[tid] = row.weight(logit_of(sh.ckey[tid]));
+        __syncthreads();
+        const uint64_t before = edge_above + tally(edge_pop, in_order).w;
+        const bool mine = tid < (int)edge_pop && before < edge_target;
+        const uint64_t w = mine ? sh.cw[tid] : 0;
+        if (mine) {
+            if (row.log_weight(logit_of(sh.ckey[tid])) >= cut)
+                atomicAdd((unsigned long long *)&sh.seg[sh.cidx[tid] / kSeg], (unsigned long long)w);
+            if (before + w >= edge_target) {      // the last one kept
+                sh.key = sh.ckey[tid];
+                sh.idx = sh.cidx[tid];
+            }
+        }
+        sum += wave_sum64(mine && row.log_weight(logit_of(sh.ckey[tid])) >= cut ? w : 0);
+        __syncthreads();
+        row.least = logit_of(sh.key);
+        row.idx = sh.idx;
+    }
     if (lane == 0) sh.red[wave] = sum;
     __syncthreads();
     uint64_t total = 0;
