@@ -253,3 +253,17 @@ def test_sample_refusals():
     g = _abi.lib().tbh_sample
     assert g(None, PTR, 1, 4, None, None, None, None, PTR, PTR, PTR) == _abi.E_INVALID
     assert g(DEV, PTR, 1, big, None, None, None, None, PTR, PTR, PTR) == _abi.E_UNSUPPORTED
+
+
+def test_packed_structs_are_the_declared_ones():
+    # the wrapper packs the C structs' bytes itself
+    from tinybrain_amd import HIPBackend
+
+    for packer, struct in ((HIPBackend._layout, _abi.PagedLayout), (HIPBackend._rows, _abi.PagedRows),
+                           (HIPBackend._queries, _abi.PagedQueries)):
+        values = list(range(1, len(struct._fields_) + 1))
+        want = struct(*values)
+        got = struct.from_buffer_copy(packer.pack(*values))
+        assert packer.size == ctypes.sizeof(struct)
+        for name, _ in struct._fields_:
+            assert getattr(got, name) == getattr(want, name), name

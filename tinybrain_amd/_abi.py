@@ -237,10 +237,10 @@ def lib() -> ctypes.CDLL:
     sp = ctypes.POINTER(AttentionShape)
     L.tbh_attention.argtypes = [vp, sp, vp, vp, vp, vp, vp]
     L.tbh_attention_device.argtypes = [vp, sp, vp, vp, vp, vp, vp, vp]
-    lp = ctypes.POINTER(PagedLayout)
-    L.tbh_paged_plan_device.argtypes = [vp, lp] + [vp] * 5 + [i64] + [vp] * 7
-    L.tbh_paged_append_device.argtypes = [vp, lp, ctypes.POINTER(PagedRows), vp, vp, vp]
-    L.tbh_paged_attention_device.argtypes = [vp, lp, ctypes.POINTER(PagedQueries), vp, vp, vp, vp]
+    # the structs as plain pointers: packed bytes, or byref of the classes above
+    L.tbh_paged_plan_device.argtypes = [vp] * 7 + [i64] + [vp] * 7
+    L.tbh_paged_append_device.argtypes = [vp] * 6
+    L.tbh_paged_attention_device.argtypes = [vp] * 7
     L.tbh_sample.argtypes = [vp, vp, i64, i64] + [vp] * 7
     L.tbh_sample_device.argtypes = [vp, vp, i64, i64, i64] + [vp] * 8
     for name in ("tbh_paged_plan_device", "tbh_paged_append_device", "tbh_paged_attention_device",

@@ -28,6 +28,7 @@ All compute runs in libtinybrain_hip.so; nothing here computes a product.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 import uuid
 import weakref
@@ -412,6 +413,14 @@ class HIPBackend:
         return out
 
     # -- serving many requests from one paged cache (see paged.py) --------------
+    # A decode step makes these calls once per layer, and its kernels take a few
+    # microseconds: the structs are packed in one go and the stream's handle read
+    # directly (us per call of the plan, append and attention of a small step, with
+    # ctypes.Structure and stream objects: 14.5, 16.6, 16.6; so: 10.6, 11.5, 12.2).
+    _layout = struct.Struct("@7i")                       # tbh_paged_layout
+    _rows = struct.Struct("@q2i3P3qPqif2P")              # tbh_paged_rows
+    _queries = struct.Struct("@q2i2P2q2Pf2i4x")          # tbh_paged_queries
+
     def paged_plan_device(self, newLens, contextLens, blockTable, freeBlocks, freeCount, blockSize: int,
                           maxTokens: int, contextOut=None, freeCountOut=None, stream=None) -> PagedPlan:
         """tbh_paged_plan_device: which blocks, slots and positions a step's
@@ -422,28 +431,30 @@ class HIPBackend:
         and freeCountOut (contextLens and freeCount themselves: in place)."""
         import torch
 
-        for t in (newLens, contextLens, blockTable, freeBlocks, freeCount):
-            self._int_tensor(t)
+        self._ints(torch.int32, newLens, contextLens, blockTable, freeBlocks, freeCount)
         b = newLens.numel()
         if contextLens.numel() != b or blockTable.dim() != 2 or blockTable.shape[0] != b or freeCount.numel() != 1:
             raise PreconditionFailure("plan: lengths and block table must have one row per request")
         if maxTokens < 0:
             raise PreconditionFailure("plan: maxTokens must not be negative")
-        sizes = [b + 1, b, maxTokens, maxTokens, b, 1]
-        start, granted, slots, positions, ctx, count = self._made(
-            torch.empty(sum(sizes), dtype=torch.int32, device=newLens.device), stream).split(sizes)
+        out = torch.empty(3 * b + 2 + 2 * maxTokens, dtype=torch.int32, device=newLens.device)
+        self._made(out, stream)
+        start, granted, slots, positions, ctx, count = torch.split_with_sizes(
+            out, (b + 1, b, maxTokens, maxTokens, b, 1))
         if contextOut is not None:
-            ctx = self._int_tensor(contextOut)
+            self._ints(torch.int32, contextOut)
+            ctx = contextOut
         if freeCountOut is not None:
-            count = self._int_tensor(freeCountOut)
+            self._ints(torch.int32, freeCountOut)
+            count = freeCountOut
         if ctx.numel() != b or count.numel() != 1:
             raise PreconditionFailure("plan: contextOut [requests] and freeCountOut [1]")
-        layout = _abi.PagedLayout(freeBlocks.numel(), blockSize, 0, 0, 0, b, blockTable.shape[1])
+        at = out.data_ptr()
         _check(self._lib.tbh_paged_plan_device(
-            self._dev, ctypes.byref(layout), newLens.data_ptr(), contextLens.data_ptr(), blockTable.data_ptr(),
-            freeBlocks.data_ptr(), freeCount.data_ptr(), maxTokens, start.data_ptr(), granted.data_ptr(),
-            ctx.data_ptr(), count.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-            self._stream(newLens, stream)))
+            self._dev, self._layout.pack(freeBlocks.numel(), blockSize, 0, 0, 0, b, blockTable.shape[1]),
+            newLens.data_ptr(), contextLens.data_ptr(), blockTable.data_ptr(), freeBlocks.data_ptr(),
+            freeCount.data_ptr(), maxTokens, at, at + 4 * (b + 1), ctx.data_ptr(), count.data_ptr(),
+            at + 4 * (2 * b + 1), at + 4 * (2 * b + 1 + maxTokens), self._raw_stream(stream)))
         return PagedPlan(start, granted, slots, positions, ctx, count)
 
     def paged_append_device(self, keys, values, slots, k, v, q=None, positions=None, ropeBase: float = 0.0,
@@ -457,35 +468,42 @@ class HIPBackend:
         else a new tensor of q's type; None without q."""
         import torch
 
-        layout = self._paged_layout(keys, values)
-        xt = self._paged_type(k)
-        hd, nkv = layout.head_dim, layout.num_kv_heads
-        for t, n in ((k, nkv), (v, nkv)) + (((q, 0),) if q is not None else ()):
-            self._row_tensor(t)
-            if t.dtype != k.dtype or t.shape[0] != k.shape[0]:
-                raise PreconditionFailure("append: q, k and v must have one type and number of rows")
-            if t.shape[1] % hd or (n and t.shape[1] != n * hd):
-                raise PreconditionFailure("append: rows do not match the cache's heads")
-        self._int_tensor(slots)
-        if slots.numel() != k.shape[0]:
+        n, nkv, bs, hd, ct = self._kv_arrays(keys, values)
+        tokens, width = self._row_shape(k)
+        if width != nkv * hd or self._row_shape(v) != (tokens, width):
+            raise PreconditionFailure("append: k and v must be rows [tokens, kvHeads * headDim]")
+        if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+            raise PreconditionFailure("append: q, k and v must have one type")
+        self._ints(torch.int32, slots)
+        if slots.numel() != tokens:
             raise PreconditionFailure("append: slots must have one entry per row")
-        if positions is not None and self._int_tensor(positions).numel() != k.shape[0]:
-            raise PreconditionFailure("append: positions must have one entry per row")
-        if ropeBase and positions is None:
+        at = 0
+        if positions is not None:
+            self._ints(torch.int32, positions)
+            at = positions.data_ptr()
+            if positions.numel() != tokens:
+                raise PreconditionFailure("append: positions must have one entry per row")
+        elif ropeBase:
             raise PreconditionFailure("append: positions are needed to rotate")
+        xt = self._paged_type(k)
+        heads, qp, qs, op, os, ot = 0, 0, 0, 0, 0, xt
         if q is not None:
+            rows, width = self._row_shape(q)
+            if rows != tokens or width % hd:
+                raise PreconditionFailure("append: q must be rows [tokens, heads * headDim]")
             if qOut is None:
-                qOut = self._made(torch.empty(q.shape, dtype=q.dtype, device=q.device), stream)
-            elif tuple(self._row_tensor(qOut).shape) != tuple(q.shape):
-                raise PreconditionFailure("append: qOut must be shaped like q")
-        rows = _abi.PagedRows(
-            k.shape[0], xt, 0 if q is None else q.shape[1] // hd, None if q is None else q.data_ptr(), k.data_ptr(),
-            v.data_ptr(), 0 if q is None else q.stride(0), k.stride(0), v.stride(0),
-            None if q is None else qOut.data_ptr(), 0 if q is None else qOut.stride(0),
-            xt if q is None else self._paged_type(qOut), float(ropeBase), slots.data_ptr(),
-            None if positions is None else positions.data_ptr())
-        _check(self._lib.tbh_paged_append_device(self._dev, ctypes.byref(layout), ctypes.byref(rows),
-                                                 keys.data_ptr(), values.data_ptr(), self._stream(k, stream)))
+                qOut = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                self._made(qOut, stream)
+            else:
+                if self._row_shape(qOut) != (rows, width):
+                    raise PreconditionFailure("append: qOut must be shaped like q")
+                ot = self._paged_type(qOut)
+            heads, qp, qs, op, os = width // hd, q.data_ptr(), q.stride(0), qOut.data_ptr(), qOut.stride(0)
+        _check(self._lib.tbh_paged_append_device(
+            self._dev, self._layout.pack(n, bs, nkv, hd, ct, 0, 0),
+            self._rows.pack(tokens, xt, heads, qp, k.data_ptr(), v.data_ptr(), qs, k.stride(0), v.stride(0), op, os,
+                            ot, ropeBase, slots.data_ptr(), at),
+            keys.data_ptr(), values.data_ptr(), self._raw_stream(stream)))
         return qOut if q is not None else None
 
     def paged_attention_device(self, q, keys, values, blockTable, queryStart, contextLens, numHeads: int,
@@ -498,50 +516,50 @@ class HIPBackend:
         maxQueryLen and maxContextLen, if known, choose launch shapes only."""
         import torch
 
-        layout = self._paged_layout(keys, values)
-        self._row_tensor(q)
-        for t in (blockTable, queryStart, contextLens):
-            self._int_tensor(t)
+        n, nkv, bs, hd, ct = self._kv_arrays(keys, values)
+        tokens, width = shape = self._row_shape(q)
+        self._ints(torch.int32, blockTable, queryStart, contextLens)
         b = contextLens.numel()
-        if q.shape[1] != numHeads * layout.head_dim or numHeads <= 0 or numHeads % layout.num_kv_heads:
+        if width != numHeads * hd or numHeads <= 0 or numHeads % nkv:
             raise PreconditionFailure("attention: query shape does not match the heads")
         if blockTable.dim() != 2 or blockTable.shape[0] != b or queryStart.numel() != b + 1:
             raise PreconditionFailure("attention: block table and query starts must have one row per request")
-        layout.max_requests, layout.max_blocks = b, blockTable.shape[1]
+        xt = self._paged_type(q)
         if out is None:
-            out = self._made(torch.empty(q.shape, dtype=q.dtype, device=q.device), stream)
-        elif tuple(self._row_tensor(out).shape) != tuple(q.shape) or out.dtype != q.dtype:
+            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+            self._made(out, stream)
+        elif self._row_shape(out) != shape or out.dtype != q.dtype:
             raise PreconditionFailure("attention: out must be like the queries")
-        args = _abi.PagedQueries(q.shape[0], self._paged_type(q), numHeads, q.data_ptr(), out.data_ptr(),
-                                 q.stride(0), out.stride(0), queryStart.data_ptr(), contextLens.data_ptr(),
-                                 float(scale), int(maxQueryLen), int(maxContextLen))
-        _check(self._lib.tbh_paged_attention_device(self._dev, ctypes.byref(layout), ctypes.byref(args),
-                                                    keys.data_ptr(), values.data_ptr(), blockTable.data_ptr(),
-                                                    self._stream(q, stream)))
+        _check(self._lib.tbh_paged_attention_device(
+            self._dev, self._layout.pack(n, bs, nkv, hd, ct, b, blockTable.shape[1]),
+            self._queries.pack(tokens, xt, numHeads, q.data_ptr(), out.data_ptr(), q.stride(0), out.stride(0),
+                               queryStart.data_ptr(), contextLens.data_ptr(), scale, maxQueryLen, maxContextLen),
+            keys.data_ptr(), values.data_ptr(), blockTable.data_ptr(), self._raw_stream(stream)))
         return out
 
-    def _here(self, t) -> bool:
-        """Whether a tensor is on this backend's GPU."""
-        return t.is_cuda and t.get_device() == self.device
-
-    def _int_tensor(self, t):
+    def _raw_stream(self, stream) -> int:
+        if stream is not None:
+            return stream.cuda_stream
         import torch
 
-        if t.dtype != torch.int32 or not t.is_contiguous() or not self._here(t):
-            raise PreconditionFailure("expected a contiguous int32 tensor on this device")
-        return t
+        return torch._C._cuda_getCurrentRawStream(self.device)
 
-    def _row_tensor(self, t):
-        if t.dim() != 2 or not self._here(t) or (t.shape[1] > 1 and t.stride(1) != 1):
+    def _ints(self, dtype, *tensors) -> None:
+        for t in tensors:
+            if t.dtype != dtype or not t.is_contiguous() or t.get_device() != self.device:
+                raise PreconditionFailure("expected a contiguous int32 tensor on this device")
+
+    def _row_shape(self, t):
+        shape = tuple(t.shape)
+        if len(shape) != 2 or t.get_device() != self.device or (shape[1] > 1 and t.stride(1) != 1):
             raise PreconditionFailure("expected rows on this device, contiguous along the last dimension")
-        return t
+        return shape
 
     @staticmethod
-    def _made(t, stream):
+    def _made(t, stream) -> None:
         """A result allocated on torch's current stream and written on `stream`."""
         if stream is not None:
             t.record_stream(stream)
-        return t
 
     @staticmethod
     def _paged_type(t) -> int:
@@ -553,13 +571,16 @@ class HIPBackend:
             return _abi.BF16
         raise PreconditionFailure("expected float32 or bfloat16")
 
-    def _paged_layout(self, keys, values) -> _abi.PagedLayout:
-        if keys.dim() != 4 or keys.shape != values.shape or keys.dtype != values.dtype:
+    def _kv_arrays(self, keys, values):
+        """blocks, kvHeads, blockSize, headDim, type of the cache arrays."""
+        shape = tuple(keys.shape)
+        if len(shape) != 4 or shape != tuple(values.shape) or keys.dtype != values.dtype:
             raise PreconditionFailure("the cache is two equal arrays [blocks, kvHeads, blockSize, headDim]")
-        if not (self._here(keys) and self._here(values) and keys.is_contiguous() and values.is_contiguous()):
+        if not (keys.is_contiguous() and values.is_contiguous() and keys.get_device() == self.device
+                and values.get_device() == self.device):
             raise PreconditionFailure("the cache must be contiguous tensors on this device")
-        n, nkv, bs, hd = keys.shape
-        return _abi.PagedLayout(n, bs, nkv, hd, self._paged_type(keys), 0, 0)
+        n, nkv, bs, hd = shape
+        return n, nkv, bs, hd, self._paged_type(keys)
 
     # -- Sampler (Sampler.swift) with the caller's random numbers ----------------
     def sample(self, logits: np.ndarray, u, temperature=1.0, topK=0, topP=1.0, minP=0.0):
@@ -591,22 +612,25 @@ class HIPBackend:
         (float32; topK int32).  Returns (tokens int32, probs float32)."""
         import torch
 
-        if logits.dim() != 2 or logits.dtype != torch.float32 or not self._here(logits) or \
-                (logits.shape[1] > 1 and logits.stride(1) != 1):
-            raise PreconditionFailure("sample: logits must be float32 device rows [rows, vocab]")
-        rows, vocab = logits.shape
+        if logits.dtype != torch.float32:
+            raise PreconditionFailure("sample: logits must be float32")
+        rows, vocab = self._row_shape(logits)
         for t, dtype in ((u, torch.float32), (temperature, torch.float32), (topK, torch.int32), (topP, torch.float32),
                          (minP, torch.float32), (tokens, torch.int32), (probs, torch.float32)):
-            if t is not None and (t.dtype != dtype or t.numel() != rows or not t.is_contiguous() or not self._here(t)):
+            if t is not None and (t.dtype != dtype or t.numel() != rows or not t.is_contiguous()
+                                  or t.get_device() != self.device):
                 raise PreconditionFailure("sample: u and settings must be contiguous device tensors, one entry per row")
         if tokens is None:
-            tokens = self._made(torch.empty(rows, dtype=torch.int32, device=logits.device), stream)
+            tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+            self._made(tokens, stream)
         if probs is None:
-            probs = self._made(torch.empty(rows, dtype=torch.float32, device=logits.device), stream)
+            probs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+            self._made(probs, stream)
         _check(self._lib.tbh_sample_device(
             self._dev, logits.data_ptr(), logits.stride(0), rows, vocab,
-            *[None if t is None else t.data_ptr() for t in (temperature, topK, topP, minP)], u.data_ptr(),
-            tokens.data_ptr(), probs.data_ptr(), self._stream(logits, stream)))
+            temperature.data_ptr() if temperature is not None else None, topK.data_ptr() if topK is not None else None,
+            topP.data_ptr() if topP is not None else None, minP.data_ptr() if minP is not None else None, u.data_ptr(),
+            tokens.data_ptr(), probs.data_ptr(), self._raw_stream(stream)))
         return tokens, probs
 
     def close(self) -> None:

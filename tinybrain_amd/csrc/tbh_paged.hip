@@ -19,60 +19,86 @@ struct PlanArgs {
 };
 
 constexpr int kPlanThreads = 1024;
+// Tokens that plan_rows places itself (with at most 1024 requests): a launch of
+// plan_tokens costs as much as four of its passes.  us of the plan of 64 requests
+// and tokens: 14.4 in two launches, 7.8 in one.
+constexpr int64_t kSoloTokens = 4096;
 
-// Inclusive sum over a wave, lane by lane.
-__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int64_t o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
+// Inclusive sum over a wave, lane by lane, of values whose sum fits 32 bits.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t shifted(uint32_t v) {   // 0 where no lane is that far down
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += shifted<0x111, 0xF>(v);    // row_shr 1, 2, 4, 8 within the 16-lane rows
+    v += shifted<0x112, 0xF>(v);
+    v += shifted<0x114, 0xF>(v);
+    v += shifted<0x118, 0xF>(v);
+    v += shifted<0x142, 0xA>(v);    // the last lane of rows 0 and 2 to rows 1 and 3,
+    return v + shifted<0x143, 0xC>(v);   // of row 1 to rows 2 and 3
 }
 
-// Exclusive sum over the block's threads; total: over all of them.  red: one
-// entry per wave.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *red, int64_t &total) {
+// Exclusive sum over the block's threads of values in 0 .. 2^31 - 1; total: over
+// all of them.  red: one entry per wave.
+__device__ __forceinline__ int64_t block_scan(int32_t v, int64_t *red, int64_t &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t in = wave_scan(v, lane);
+    // in halves of 16 bits, whose sums fit 32
+    const int64_t in = ((int64_t)wave_scan((uint32_t)v >> 16) << 16) + wave_scan((uint32_t)v & 0xFFFFu);
     __syncthreads();
     if (lane == 63) red[wave] = in;
     __syncthreads();
-    int64_t before = 0;
-    total = 0;
+    // lane i of every wave: the sum of the waves up to i
+    int64_t w = lane < kPlanThreads / 64 ? red[lane] : 0;
 #pragma unroll
-    for (int i = 0; i < kPlanThreads / 64; ++i) {
-        const int64_t r = red[i];
-        before += i < wave ? r : 0;
-        total += r;
+    for (int d = 1; d < kPlanThreads / 64; d *= 2) {
+        const int64_t o = __shfl_up(w, d);
+        if (lane >= d) w += o;
     }
-    return before + in - v;
+    total = __shfl(w, kPlanThreads / 64 - 1);
+    const int64_t before = __shfl(w, max(wave - 1, 0));
+    return (wave ? before : 0) + in - v;
 }
 
 __device__ __forceinline__ int32_t blocks_of(int64_t tokens, int shift) {
     return (int32_t)((tokens + (1 << shift) - 1) >> shift);
 }
 
-// Rows of the plan: one block, a row per thread and tile of 1024 rows, its
-// sums by block scans with a carry.  A wave copies its own rows' lists of
-// blocks, one row after another, 64 entries at a time.
-__global__ __launch_bounds__(kPlanThreads) void plan_rows(const PlanArgs a) {
+// First index whose value exceeds e, of n ascending values, the last of which does.
+__device__ __forceinline__ int32_t first_above(const int32_t *v, int32_t n, int32_t e) {
+    int32_t lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int32_t mid = (lo + hi) >> 1;
+        if (v[mid] > e) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+// Rows of the plan: one block, a row per thread and tile of 1024 rows, its sums by
+// block scans with a carry.  Bound by its chain of dependent steps: lengths, scan,
+// blocks off the stack.  New blocks, and the tokens of a small step (solo), are
+// dealt over all threads, each finding its row in the tile's sums.
+__global__ __launch_bounds__(kPlanThreads) void plan_rows(const PlanArgs a, bool solo) {
     __shared__ int64_t red[kPlanThreads / 64];
+    __shared__ int32_t upto[kPlanThreads], have_[kPlanThreads];   // blocks asked for by the tile's rows up to this
+    __shared__ int32_t end_[kPlanThreads], base_[kPlanThreads];   // tokens likewise; context, or -1: not granted
+    __shared__ int32_t took;
     const int tid = threadIdx.x, lane = tid & 63;
     const int64_t capacity = (int64_t)a.most << a.shift;
     int64_t height = min(max(a.free_count[0], 0), a.num_blocks);
+    if (tid == 0) took = 0;
 
-    // released rows push their blocks
+    // released rows push their blocks, a wave its own rows', one after another
     for (int32_t r0 = 0; r0 < a.rows; r0 += kPlanThreads) {
         const int32_t r = r0 + tid;
-        const int64_t held =
+        const int32_t held =
             r < a.rows && a.new_lens[r] < 0 ? blocks_of(min((int64_t)max(a.ctx[r], 0), capacity), a.shift) : 0;
         if (!__syncthreads_or(held > 0)) continue;
         int64_t total;
         const int64_t at = height + block_scan(held, red, total);
         for (uint64_t m = __ballot(held > 0); m; m &= m - 1) {
             const int l = __builtin_ctzll(m);
-            const int32_t n = __builtin_amdgcn_readlane((int)held, l);
+            const int32_t n = __builtin_amdgcn_readlane(held, l);
             const int64_t to = __shfl(at, l);
             const int32_t *from = a.table + (int64_t)(r0 + (tid & ~63) + l) * a.most;
             for (int32_t j = lane; j < n; j += 64)
@@ -82,15 +108,15 @@ __global__ __launch_bounds__(kPlanThreads) void plan_rows(const PlanArgs a) {
     }
     __syncthreads();   // the pushed ids are read below
 
-    int64_t tokens = 0, asked = 0, taken = 0;
+    int64_t tokens = 0, asked = 0;
     for (int32_t r0 = 0; r0 < a.rows; r0 += kPlanThreads) {
-        const int32_t r = r0 + tid;
+        const int32_t r = r0 + tid, tile = min(kPlanThreads, a.rows - r0);
         const bool row = r < a.rows;
         const int32_t n = row ? a.new_lens[r] : 0, c = row ? max(a.ctx[r], 0) : 0;
-        const int64_t more = max(n, 0);
-        const bool fits = more > 0 && c + more <= capacity;
+        const int32_t more = max(n, 0);
+        const bool fits = more > 0 && (int64_t)c + more <= capacity;
         const int32_t have = blocks_of(c, a.shift);
-        const int64_t need = fits ? blocks_of(c + more, a.shift) - have : 0;
+        const int32_t need = fits ? blocks_of((int64_t)c + more, a.shift) - have : 0;
         int64_t tile_tokens, tile_need;
         const int64_t first = tokens + block_scan(more, red, tile_tokens);
         const int64_t before = asked + block_scan(need, red, tile_need);
@@ -100,23 +126,49 @@ __global__ __launch_bounds__(kPlanThreads) void plan_rows(const PlanArgs a) {
             a.granted[r] = ok ? n : 0;
             a.ctx_out[r] = n < 0 ? 0 : ok ? c + n : c;
         }
-        for (uint64_t m = __ballot(ok && need > 0); m; m &= m - 1) {
-            const int l = __builtin_ctzll(m);
-            const int32_t k = __builtin_amdgcn_readlane((int)need, l);
-            const int64_t top = height - 1 - __shfl(before, l);
-            int32_t *to = a.table + (int64_t)(r0 + (tid & ~63) + l) * a.most + __builtin_amdgcn_readlane(have, l);
-            for (int32_t j = lane; j < k; j += 64) to[j] = a.free_blocks[top - j];
+        upto[tid] = (int32_t)(before + need - asked);
+        have_[tid] = have;
+        end_[tid] = (int32_t)min(first + more, (int64_t)INT32_MAX);
+        base_[tid] = ok ? c : -1;
+        // rows that are given blocks come before those that are not: the highest
+        // of a wave's has the most
+        const uint64_t given = __ballot(ok && need > 0);
+        if (given && lane == 63 - __builtin_clzll(given)) atomicMax(&took, (int32_t)(before + need));
+        __syncthreads();
+        const int32_t fresh = (int32_t)max(took - asked, (int64_t)0);   // this tile's
+        for (int32_t e = tid; e < fresh; e += kPlanThreads) {
+            const int32_t i = first_above(upto, tile, e);
+            const int32_t j = e - (i ? upto[i - 1] : 0);
+            a.table[(int64_t)(r0 + i) * a.most + have_[i] + j] = a.free_blocks[height - 1 - asked - e];
         }
+        if (solo) {                               // one tile
+            for (int32_t t = tid; t < a.max_tokens; t += kPlanThreads) {
+                int32_t slot = -1, pos = -1;
+                if (t < tile_tokens) {
+                    const int32_t i = first_above(end_, tile, t), base = base_[i];
+                    if (base >= 0) {
+                        pos = base + t - (i ? end_[i - 1] : 0);
+                        const int32_t j = (pos >> a.shift) - have_[i];
+                        const int32_t id = j < 0 ? a.table[(int64_t)i * a.most + (pos >> a.shift)]
+                                                 : a.free_blocks[height - 1 - (i ? upto[i - 1] : 0) - j];
+                        if ((uint32_t)id < (uint32_t)a.num_blocks)
+                            slot = (id << a.shift) + (pos & ((1 << a.shift) - 1));
+                    }
+                }
+                a.slots[t] = slot;
+                a.positions[t] = pos;
+            }
+        }
+        __syncthreads();                          // the next tile writes the sums anew
         tokens += tile_tokens;
         asked += tile_need;
-        int64_t tile_taken;
-        block_scan(ok ? need : 0, red, tile_taken);
-        taken += tile_taken;
     }
     if (tid == 0) {
         a.start[a.rows] = (int32_t)min(tokens, (int64_t)INT32_MAX);
-        a.free_out[0] = (int32_t)(height - taken);
+        a.free_out[0] = (int32_t)height - took;
     }
+    if (solo && a.rows == 0)
+        for (int32_t t = tid; t < a.max_tokens; t += kPlanThreads) a.slots[t] = a.positions[t] = -1;
 }
 
 // Last row whose start is at most t (the rows before it may be empty).
@@ -302,9 +354,10 @@ tbh_status tbh_paged_plan_device(tbh_device *dev, const tbh_paged_layout *layout
     a.shift = log2_of(layout->block_size);
     a.max_tokens = max_tokens;
     const hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(plan_rows, dim3(1), dim3(kPlanThreads), 0, s, a);
+    const bool solo = B <= kPlanThreads && max_tokens <= kSoloTokens;
+    hipLaunchKernelGGL(plan_rows, dim3(1), dim3(kPlanThreads), 0, s, a, solo);
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess && max_tokens > 0) {
+    if (e == hipSuccess && max_tokens > 0 && !solo) {
         hipLaunchKernelGGL(plan_tokens, dim3((unsigned)((max_tokens + 255) / 256)), dim3(256), 0, s, a);
         e = hipGetLastError();
     }
