@@ -718,10 +718,33 @@ struct TileArgs {
     float *po;             // and sums of p v, [unit][split][kTileRows][head_dim]
 };
 
-// Rows of a tile: two column groups of 16 per wave for bf16 rows; fp32 rows, whose
-// three pieces triple the matrix work per LDS read and the registers of q, one.
-template <class XT>
-constexpr int kTileRows = sizeof(XT) == 2 ? 128 : 64;
+// Rows of a tile: two column groups of 16 per wave for bf16 rows over a bf16 cache;
+// one where the matrix work per LDS read is more (three pieces of fp32 rows, the
+// fp32 matrix instruction).
+template <class XT, class CT>
+constexpr int kTileRows = sizeof(XT) + sizeof(CT) == 4 ? 128 : 64;
+
+// As in paged_split: the wave's rows one at a time, where one may have met an inf
+// or NaN that it does not see.
+template <class XT, class CT, int HD>
+__device__ __forceinline__ void rows_apart(const TileArgs &ta, const Group &gr, uint32_t unit, uint32_t split,
+                                           int32_t parts, int32_t c0, int32_t c1, int32_t wrow, int32_t wrows,
+                                           float *qs) {
+    const PagedArgs &a = ta.a;
+    const int lane = threadIdx.x & 63;
+    for (int rr = 0; rr < wrows; ++rr) {
+        const int32_t tt = (wrow + rr) / a.rep;
+        const int head = gr.kvh * a.rep + (wrow + rr) % a.rep;
+        const RowPart x = row_part<XT, CT>(a, gr.b, gr.q.first + tt, head, c0, min(c1, gr.q.base + tt + 1), qs);
+        if (parts == 1) {
+            store_row<XT>(a, gr.q.first + tt, head, x);
+        } else {
+            const int64_t r = ((int64_t)unit * ta.splits + split) * kTileRows<XT, CT> + wrow + rr - gr.row0;
+            if (lane == 0) ta.ml[r] = x.m == -INFINITY ? float2{x.m, x.seen ? 1.0f : 0.0f} : float2{x.m, x.l};
+            for (int i = 0; 64 * i + lane < HD; ++i) ta.po[r * HD + 64 * i + lane] = x.o[i];
+        }
+    }
+}
 
 // Many rows per request over a bf16 cache. A block takes kTileRows rows of one
 // key/value head and one part of the positions: four waves of 16 or 32 rows,
@@ -736,7 +759,7 @@ constexpr int kTileRows = sizeof(XT) == 2 ? 128 : 64;
 // reads touch every bank once; the copies permute their global addresses for it.
 template <class XT, int HD>
 __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
-    constexpr int NP = sizeof(XT) == 4 ? 3 : 1, ROWS = kTileRows<XT>, CG = ROWS / 64;
+    constexpr int NP = sizeof(XT) == 4 ? 3 : 1, ROWS = kTileRows<XT, __bf16>, CG = ROWS / 64;
     constexpr int NJ = HD / 32, ND = HD / 16;
     constexpr int CR = HD / 8, NL = CR / 4;                // 16-byte pieces per row, copies per wave and tile
     constexpr int KD = 16 / CR, VD2 = 8 / ND;              // rows per 256 bytes of LDS, as 16- and 32-byte pieces count
@@ -966,40 +989,214 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
         }
     }
     if (low + 1 >= c1 || !__any(odd)) return;
-    // as in paged_split: the wave's rows one at a time, where one may have met an
-    // inf or NaN that it does not see
-    for (int rr = 0; rr < wrows; ++rr) {
-        const int32_t tt = (wrow + rr) / a.rep;
-        const int head = gr.kvh * a.rep + (wrow + rr) % a.rep;
-        const RowPart x =
-            row_part<XT, __bf16>(a, gr.b, gr.q.first + tt, head, c0, min(c1, gr.q.base + tt + 1), qs[w]);
-        if (ct.parts == 1) {
-            store_row<XT>(a, gr.q.first + tt, head, x);
-        } else {
-            const int64_t r = ((int64_t)unit * ta.splits + split) * ROWS + wrow + rr - gr.row0;
-            if (lane == 0) ta.ml[r] = x.m == -INFINITY ? float2{x.m, x.seen ? 1.0f : 0.0f} : float2{x.m, x.l};
-            for (int i = 0; 64 * i + lane < HD; ++i) ta.po[r * HD + 64 * i + lane] = x.o[i];
-        }
+    rows_apart<XT, __bf16, HD>(ta, gr, unit, split, ct.parts, c0, c1, wrow, wrows, qs[w]);
+}
+
+// Many rows per request over an fp32 cache, as paged_tile but on the fp32 matrix
+// instruction (256 flop per clock and CU, which bounds it): four waves of 16
+// rows, tiles of 32 positions, a wave copying eight of them.  The products are
+// those of Step: values need no transposing read, as the instruction's reduction
+// takes one position per lane.  Outputs are dealt four consecutive dimensions of
+// every 64 to a lane, so that 16 lanes read 256 bytes of a value row at once;
+// keys' 16-byte pieces are swizzled by the row.  A tile's values are summed before
+// they join the running sums: an eighth of the roundings.
+template <class XT, int HD>
+__global__ __launch_bounds__(256, 2) void paged_tile_f32(const TileArgs ta) {
+    constexpr int ROWS = kTileRows<XT, float>, POS = 32;
+    constexpr int NJ = HD / 16, NH = HD / 64;
+    constexpr int CR = HD / 4, NL = 8 * CR / 64;           // 16-byte pieces per row, copies per wave and tile
+    __shared__ __attribute__((aligned(256))) float kl[2][POS * HD], vl[2][POS * HD];
+    __shared__ float qs[4][HD];
+    const PagedArgs &a = ta.a;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int g = lane >> 4, n = lane & 15;
+    const uint32_t unit = blockIdx.x % (uint32_t)ta.units, split = blockIdx.x / (uint32_t)ta.units;
+    Group gr;
+    if (!find_group<ROWS>(a, unit, 16, ta.pair_up, gr)) return;
+    set_rows<ROWS>(a, gr, gr.row0);
+    const Cut ct = cut(gr.len, ta.splits, ta.least);
+    if ((int32_t)split >= ct.parts) return;
+    const int32_t c0 = split * ct.chunk, c1 = min(gr.len, c0 + ct.chunk);
+    const int32_t *table = a.table + (int64_t)gr.b * a.most;
+    const float c2 = fabsf(a.scale) * 1.44269504f;         // a negative scale turns q's sign
+    const int32_t head_rows = HD << a.shift, in_block = (1 << a.shift) - 1;
+    const int64_t block_rows = (int64_t)head_rows * a.nkv;
+    const float *kb = (const float *)a.kc + (int64_t)gr.kvh * head_rows;
+    const float *vb = (const float *)a.vc + (int64_t)gr.kvh * head_rows;
+
+    // wave w copies positions 8 w .. of a tile
+    uint32_t koff[NL], voff[NL];
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+        const int r = (64 * j + lane) / CR, c = (64 * j + lane) % CR;
+        koff[j] = 16 * (r * CR + (c ^ (8 * (w & 1) + r)));   // the row's place among 16
+        voff[j] = 16 * (64 * j + lane);
     }
+    const uint32_t kdst = dma::lds_addr(&kl[0][8 * w * HD]), vdst = dma::lds_addr(&vl[0][8 * w * HD]);
+    auto window = [&](int32_t p) {                         // as in paged_tile
+        return p + 16 * lane < c1 ? table[(p + 16 * lane) >> a.shift] : -1;
+    };
+    int32_t ids = window(c0), ids_next = window(c0 + 1024);
+    auto copy = [&](int buf, int32_t p0, int32_t from) {
+        const int32_t p = p0 + 8 * w;
+        const int32_t id = __builtin_amdgcn_readlane(from, (p - c0) >> 4 & 63);
+        const bool ok = p < c1 && (uint32_t)id < (uint32_t)a.num_blocks;
+        const int64_t at = (int64_t)(ok ? id : 0) * block_rows + (p & in_block) * HD;
+        const int bytes = ok ? min(8, c1 - p) * HD * 4 : 0;
+        const dma::i32x4 kr = dma::make_rsrc(kb + at, bytes), vr = dma::make_rsrc(vb + at, bytes);
+        const uint32_t kd = __builtin_amdgcn_readfirstlane(kdst + buf * POS * HD * 4);
+        const uint32_t vd = __builtin_amdgcn_readfirstlane(vdst + buf * POS * HD * 4);
+#pragma unroll
+        for (int j = 0; j < NL; ++j) dma::dma16(kd + 1024 * j, kr, koff[j], 0);
+#pragma unroll
+        for (int j = 0; j < NL; ++j) dma::dma16(vd + 1024 * j, vr, voff[j], 0);
+    };
+    copy(0, c0, ids);
+    uint64_t blocks = __ballot((uint32_t)ids < (uint32_t)a.num_blocks);
+
+    const int32_t wrow = gr.row0 + 16 * w, wrows = min(16, gr.row0 + gr.rows - wrow);   // may be none
+    const int32_t row = min(wrow + n, gr.row0 + gr.rows - 1), token = row / a.rep;
+    const int32_t last = min(gr.q.base + token, gr.q.held - 1);
+    float q[NJ][4];
+    {
+        const XT *x = (const XT *)a.q + (gr.q.first + token) * a.q_stride +
+                      (int64_t)(gr.kvh * a.rep + row % a.rep) * HD + 4 * g;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) q[j][c] = a.scale < 0.0f ? -(float)x[16 * j + c] : (float)x[16 * j + c];
+    }
+    const int32_t low = min(gr.q.base + wrow / a.rep, gr.q.held - 1);
+    const int32_t high = wrows > 0 ? min(gr.q.base + (wrow + wrows - 1) / a.rep, gr.q.held - 1) : -1;
+
+    constexpr float kLag = 8.0f;                           // as in paged_tile
+    float mr = -INFINITY, l = 0.0f;                        // l: this lane's positions only
+    int32_t first = INT32_MAX;
+    f32x4 o[4 * NH];
+#pragma unroll
+    for (int d = 0; d < 4 * NH; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int buf = 0;
+    for (int32_t p0 = c0; p0 < c1; p0 += POS, buf ^= 1) {
+        // this tile has landed, and every wave is done with the other buffer
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const int32_t at = (p0 - c0) >> 4 & 63;            // of the window
+        if (at == 0 && p0 != c0) {
+            ids = ids_next;
+            ids_next = window(p0 + 1024);
+            blocks = __ballot((uint32_t)ids < (uint32_t)a.num_blocks);
+        }
+        if (p0 + POS < c1) copy(buf ^ 1, p0 + POS, at == 62 ? ids_next : ids);
+        if (p0 > high) continue;
+        f32x4 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};   // two chains: half the rounding of one
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const f32x4 k = *(const f32x4 *)&kl[buf][(16 * t + n) * HD + 4 * ((4 * j + g) ^ n)];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    x[c & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c], q[j][c], x[c & 1], 0, 0, 0);
+            }
+            s[t] = x[0] + x[1];
+        }
+        // sub-tiles of the part, those without a block
+        const int part = p0 + 16 < c1 ? 3 : 1, hole = (int)(~blocks >> at) & part;
+        if (first == INT32_MAX && hole != part) first = p0 + 16 * __builtin_ctz(part & ~hole);
+        if (hole || p0 + POS - 1 > low) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int32_t lim = hole >> t & 1 ? -1 : last - (p0 + 16 * t + 4 * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][i] = i <= lim ? s[t][i] : -INFINITY;
+            }
+        }
+        float nm = s[0][0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nm = fmaxf(nm, s[t][i]);
+        nm = row4_max(nm) * c2;
+        const bool move = nm > mr + kLag;
+        if (__any(move)) {
+            const float to = move ? nm : mr, corr = move ? exp2_fast(mr - to) : 1.0f;
+            mr = to;
+            l *= corr;
+#pragma unroll
+            for (int d = 0; d < 4 * NH; ++d) o[d] *= corr;
+        }
+        const float ref = mr == -INFINITY ? 0.0f : mr;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][i] = exp2_fast(fmaf(s[t][i], c2, -ref));
+        l += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
+        f32x4 pv[4 * NH];
+#pragma unroll
+        for (int d = 0; d < 4 * NH; ++d) pv[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    const f32x4 v = *(const f32x4 *)&vl[buf][(16 * t + 4 * g + i) * HD + 64 * h + 4 * n];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        pv[4 * h + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[c], s[t][i], pv[4 * h + c], 0, 0, 0);
+                }
+#pragma unroll
+        for (int d = 0; d < 4 * NH; ++d) o[d] += pv[d];
+    }
+    l = row4_sum(l);
+
+    // lane (g, n): outputs 64 h + 16 g + 4 i + c of row n
+    bool odd = false;                                      // inf or NaN in a row
+    if (wrow + n < gr.row0 + gr.rows) {
+#pragma unroll
+        for (int d = 0; d < 4 * NH; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) odd |= !(fabsf(o[d][i]) < INFINITY);
+        const bool none = mr == -INFINITY, seen = first <= last;
+        const int64_t r = ((int64_t)unit * ta.splits + split) * ROWS + row - gr.row0;
+        XT *out = (XT *)a.out + (int64_t)(gr.q.first + token) * a.out_stride +
+                  (int64_t)(gr.kvh * a.rep + row % a.rep) * HD + 16 * g;
+        if (ct.parts > 1 && g == 0) ta.ml[r] = none ? float2{-INFINITY, seen ? 1.0f : 0.0f} : float2{mr, l};
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 v = {o[4 * h][i], o[4 * h + 1][i], o[4 * h + 2][i], o[4 * h + 3][i]};
+                if (ct.parts == 1) {
+                    // nothing seen: 0; only scores of -inf: 0 / 0
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) out[64 * h + 4 * i + c] = (XT)(none ? (seen ? NAN : 0.0f) : v[c] / l);
+                } else {
+                    *(f32x4 *)(ta.po + r * HD + 64 * h + 16 * g + 4 * i) = v;
+                }
+            }
+    }
+    if (low + 1 >= c1 || !__any(odd)) return;
+    rows_apart<XT, float, HD>(ta, gr, unit, split, ct.parts, c0, c1, wrow, wrows, qs[w]);
 }
 
 // Joins paged_tile's parts: HD / 4 threads a row.
-template <class XT, int HD>
+template <class XT, class CT, int HD>
 __global__ __launch_bounds__(256) void paged_tile_merge(const TileArgs ta) {
     constexpr int T = HD / 4, R = 256 / T;
     const PagedArgs &a = ta.a;
-    const uint32_t unit = blockIdx.x / (kTileRows<XT> / R);
-    const int rr = (int)(blockIdx.x % (kTileRows<XT> / R)) * R + threadIdx.x / T, d4 = threadIdx.x % T;
+    const uint32_t unit = blockIdx.x / (kTileRows<XT, CT> / R);
+    const int rr = (int)(blockIdx.x % (kTileRows<XT, CT> / R)) * R + threadIdx.x / T, d4 = threadIdx.x % T;
     Group gr;
-    if (!find_group<kTileRows<XT>>(a, unit, 16, ta.pair_up, gr)) return;
-    set_rows<kTileRows<XT>>(a, gr, gr.row0);
+    if (!find_group<kTileRows<XT, CT>>(a, unit, 16, ta.pair_up, gr)) return;
+    set_rows<kTileRows<XT, CT>>(a, gr, gr.row0);
     const Cut ct = cut(gr.len, ta.splits, ta.least);
     if (ct.parts == 1 || rr >= gr.rows) return;
-    const int64_t at0 = (int64_t)unit * ta.splits * kTileRows<XT> + rr;
+    const int64_t at0 = (int64_t)unit * ta.splits * kTileRows<XT, CT> + rr;
     float mm = -INFINITY, any = 0.0f;
 #pragma unroll 4
     for (int s = 0; s < ct.parts; ++s) {
-        const float2 x = ta.ml[at0 + (int64_t)s * kTileRows<XT>];
+        const float2 x = ta.ml[at0 + (int64_t)s * kTileRows<XT, CT>];
         mm = fmaxf(mm, x.x);
         any = fmaxf(any, x.y);
     }
@@ -1007,7 +1204,7 @@ __global__ __launch_bounds__(256) void paged_tile_merge(const TileArgs ta) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int s = 0; s < ct.parts; ++s) {
-        const int64_t r = at0 + (int64_t)s * kTileRows<XT>;
+        const int64_t r = at0 + (int64_t)s * kTileRows<XT, CT>;
         const float2 x = ta.ml[r];
         const float f = x.x == -INFINITY ? 0.0f : exp2_fast(x.x - mm);
         if (x.x != -INFINITY) l += f * x.y;
@@ -1022,18 +1219,18 @@ __global__ __launch_bounds__(256) void paged_tile_merge(const TileArgs ta) {
 
 // Positions a part of paged_tile has at least: parts fill the chip's two blocks
 // per CU twice over, of at least 512 positions.
-template <class XT, int HD>
+template <class XT, class CT, int HD>
 hipError_t launch_tile(tbh_device *dev, const PagedArgs &a, int64_t context, hipStream_t s) {
     TileArgs ta{};
     ta.a = a;
     ta.qvec = aligned(a.q, 16) && (a.q_stride * (int64_t)sizeof(XT)) % 16 == 0;
     const int64_t rows = a.tokens * a.rep;
-    const int64_t units = (rows / kTileRows<XT> + std::min<int64_t>(a.requests, rows / 17 + 1)) * a.nkv;
+    const int64_t units = (rows / kTileRows<XT, CT> + std::min<int64_t>(a.requests, rows / 17 + 1)) * a.nkv;
     const int64_t parts = std::max<int64_t>(1, 4 * (int64_t)std::max(1, dev->cu_count) / units);
     ta.least = (int32_t)std::max<int64_t>(512, ((context + parts - 1) / parts + 127) / 128 * 128);
     ta.splits = (int32_t)std::min<int64_t>((context + ta.least - 1) / ta.least, kMaxSplits);
     if (ta.splits > 1) {
-        const int64_t n = units * ta.splits * kTileRows<XT>;
+        const int64_t n = units * ta.splits * kTileRows<XT, CT>;
         const size_t head = (size_t)n * sizeof(float2);
         char *ws = (char *)stream_workspace(dev, s, head + (size_t)n * HD * sizeof(float));
         if (ws) {
@@ -1043,14 +1240,16 @@ hipError_t launch_tile(tbh_device *dev, const PagedArgs &a, int64_t context, hip
             ta.splits = 1;   // no workspace (graph capture before any eager call): whole contexts
         }
     }
-    if (units * std::max<int64_t>(ta.splits, kTileRows<XT> * HD / 1024) > INT32_MAX) return hipErrorInvalidValue;
+    if (units * std::max<int64_t>(ta.splits, kTileRows<XT, CT> * HD / 1024) > INT32_MAX) return hipErrorInvalidValue;
     ta.units = (int32_t)units;
     // two blocks share a CU: all run at once, or the longest have to come first
-    ta.pair_up = rows / kTileRows<XT> * a.nkv <= 2 * (int64_t)std::max(1, dev->cu_count);
-    hipLaunchKernelGGL((paged_tile<XT, HD>), dim3((unsigned)(units * ta.splits)), dim3(256), 0, s, ta);
+    ta.pair_up = rows / kTileRows<XT, CT> * a.nkv <= 2 * (int64_t)std::max(1, dev->cu_count);
+    const dim3 grid((unsigned)(units * ta.splits));
+    if constexpr (sizeof(CT) == 2) hipLaunchKernelGGL((paged_tile<XT, HD>), grid, dim3(256), 0, s, ta);
+    else hipLaunchKernelGGL((paged_tile_f32<XT, HD>), grid, dim3(256), 0, s, ta);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || ta.splits == 1) return e;
-    hipLaunchKernelGGL((paged_tile_merge<XT, HD>), dim3((unsigned)(units * (kTileRows<XT> * HD / 1024))), dim3(256), 0, s,
+    hipLaunchKernelGGL((paged_tile_merge<XT, CT, HD>), dim3((unsigned)(units * (kTileRows<XT, CT> * HD / 1024))), dim3(256), 0, s,
                        ta);
     return hipGetLastError();
 }
@@ -1059,13 +1258,12 @@ template <class XT, class CT>
 hipError_t launch_paged(tbh_device *dev, const PagedArgs &a, int64_t query, int64_t context, hipStream_t s) {
     // the matrix kernels take a tile of 16 positions from one block
     if (a.shift >= 4 && a.num_blocks > 0 && a.most > 0) {
-        if constexpr (sizeof(CT) == 2) {
-            if (query * a.rep > 16 && (a.hd == 64 || a.hd == 128)) {
-                const hipError_t e = a.hd == 64 ? launch_tile<XT, 64>(dev, a, context, s) : launch_tile<XT, 128>(dev, a, context, s);
-                if (e != hipSuccess) return e;
-                return a.hd == 64 ? launch_split<XT, CT, 64>(dev, a, query, context, true, s)
-                                  : launch_split<XT, CT, 128>(dev, a, query, context, true, s);
-            }
+        if (query * a.rep > 16 && (a.hd == 64 || a.hd == 128)) {
+            const hipError_t e = a.hd == 64 ? launch_tile<XT, CT, 64>(dev, a, context, s)
+                                            : launch_tile<XT, CT, 128>(dev, a, context, s);
+            if (e != hipSuccess) return e;
+            return a.hd == 64 ? launch_split<XT, CT, 64>(dev, a, query, context, true, s)
+                              : launch_split<XT, CT, 128>(dev, a, query, context, true, s);
         }
         switch (a.hd) {
         case 32: return launch_split<XT, CT, 32>(dev, a, query, context, false, s);
