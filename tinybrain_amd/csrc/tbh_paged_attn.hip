@@ -426,19 +426,26 @@ struct Step<XT, float, HD> {
 // Few rows per request (single tokens of grouped heads, short chunks): 16 rows
 // and one part of the positions a block, its four waves taking steps of 32
 // positions in turn and meeting in LDS at the end.  Bound by reading the cache.
+template <int HD>
+struct SplitLds {
+    float so[4][16][HD + 4];
+    float2 sml[4][16];
+    int odd;
+};
+
 template <class XT, class CT, int HD>
-__global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
-    constexpr int VD = HD / 16, LD = HD + 4;
-    __shared__ __attribute__((aligned(16))) float so[4][16][LD];
-    __shared__ float2 sml[4][16];
-    __shared__ int odd;
+__device__ __forceinline__ void split_block(const SplitArgs &sa, uint32_t block, SplitLds<HD> &lds) {
+    constexpr int VD = HD / 16;
+    auto &so = lds.so;
+    auto &sml = lds.sml;
+    int &odd = lds.odd;
     const PagedArgs &a = sa.a;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, n = lane & 15;
     // The units run fastest: consecutive blocks go to different XCDs, and with the
     // parts fastest one XCD would get every request's first part and another only
     // those of the longest (64 requests of 100 .. 8192 positions: 216 us for 107).
-    const uint32_t unit = blockIdx.x % (uint32_t)sa.units, split = blockIdx.x / (uint32_t)sa.units;
+    const uint32_t unit = block % (uint32_t)sa.units, split = block / (uint32_t)sa.units;
     Group gr;
     bool alone = false;            // more rows than a unit has places for: no parts
     if (sa.scan) {
@@ -612,16 +619,22 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
     }
 }
 
+template <class XT, class CT, int HD>
+__global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
+    __shared__ __attribute__((aligned(16))) SplitLds<HD> lds;
+    split_block<XT, CT, HD>(sa, blockIdx.x, lds);
+}
+
 // Joins paged_split's parts: a block per unit and row, HD / 4 threads across the
 // head, the parts dealt over the rest.  Every wave holds the parts' factors, one
 // per lane.
 template <class XT, int HD>
-__global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa) {
+__device__ __forceinline__ void split_merge(const SplitArgs &sa, uint32_t block, f32x4 *lds) {
     constexpr int T = HD / 4, G = 256 / T;
-    __shared__ f32x4 red[G][T];
+    f32x4 (*red)[T] = (f32x4 (*)[T])lds;
     const PagedArgs &a = sa.a;
     const int tid = threadIdx.x, lane = tid & 63, d4 = tid % T, sg = tid / T;
-    const uint32_t rr = blockIdx.x % (uint32_t)sa.slots, unit = blockIdx.x / (uint32_t)sa.slots;
+    const uint32_t rr = block % (uint32_t)sa.slots, unit = block / (uint32_t)sa.slots;
     const int64_t at0 = (int64_t)unit * sa.splits * sa.slots + rr;
     const float2 mine = sa.ml[at0 + (int64_t)min(lane, sa.splits - 1) * sa.slots];   // before the request is known
     Group gr;
@@ -663,6 +676,14 @@ __global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa) {
     for (int i = 0; i < 4; ++i) out[i] = (XT)(mm == -INFINITY ? (any ? NAN : 0.0f) : v[i] / l);
 }
 
+template <class XT, int HD>
+__global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa) {
+    __shared__ f32x4 red[256];
+    split_merge<XT, HD>(sa, blockIdx.x, red);
+}
+
+constexpr int64_t kMaxSplits = 64;   // a lane each in split_merge
+
 // Positions a part of paged_split has at least, for `units` units: enough blocks
 // to fill the chip, parts no longer than 1024 (a batch's longest request would
 // else end long after the others) and no shorter than 128 (a step per wave).
@@ -672,40 +693,23 @@ int32_t split_least(int64_t units, int64_t context, int64_t cus) {
     return (int32_t)std::min<int64_t>(1024, std::max<int64_t>(128, (even + 127) / 128 * 128));
 }
 
-constexpr int64_t kMaxSplits = 64;
+// Partials of `rows` rows: (max, sum) pairs, then rows of head_dim floats.
+size_t partial_head(int64_t rows) { return ((size_t)rows * sizeof(float2) + 255) / 256 * 256; }
+size_t partial_bytes(int64_t rows, int hd) { return partial_head(rows) + ((size_t)rows * hd * sizeof(float) + 255) / 256 * 256; }
 
-template <class XT, class CT, int HD>
-hipError_t launch_split(tbh_device *dev, const PagedArgs &a, int64_t query, int64_t context, bool tiles,
-                        hipStream_t s) {
+SplitArgs plan_split(const PagedArgs &a, int64_t query, int64_t context, bool tiles, size_t elem, int64_t cus) {
     SplitArgs sa{};
     sa.a = a;
-    sa.qvec = aligned(a.q, 16) && (a.q_stride * (int64_t)sizeof(XT)) % 16 == 0;
+    sa.qvec = aligned(a.q, 16) && (a.q_stride * (int64_t)elem) % 16 == 0;
     sa.scan = !tiles && query * a.rep > 16;
     const int64_t units = (sa.scan ? a.tokens * a.rep / 16 + std::min<int64_t>(a.requests, a.tokens) : a.requests) *
-                          a.nkv;
+                          (int64_t)a.nkv;
+    sa.units = (int32_t)std::min<int64_t>(units, INT32_MAX);
     sa.long_rows = tiles ? 16 : INT32_MAX;
     sa.slots = (int32_t)std::min<int64_t>(16, query * a.rep);
-    sa.least = split_least(units, context, std::max(1, dev->cu_count));
-    sa.splits = (int32_t)std::min<int64_t>((context + sa.least - 1) / sa.least, kMaxSplits);
-    if (sa.splits > 1) {
-        const int64_t rows = units * sa.splits * sa.slots;
-        const size_t head = (size_t)rows * sizeof(float2);   // rows of head_dim floats follow, 16-byte aligned
-        const size_t pad = (head + 255) / 256 * 256;
-        char *ws = (char *)stream_workspace(dev, s, pad + (size_t)rows * HD * sizeof(float));
-        if (ws) {
-            sa.ml = (float2 *)ws;
-            sa.po = (float *)(ws + pad);
-        } else {
-            sa.splits = 1;   // no workspace (graph capture before any eager call): whole contexts
-        }
-    }
-    if (units * std::max(sa.splits, sa.slots) > INT32_MAX) return hipErrorInvalidValue;
-    sa.units = (int32_t)units;
-    hipLaunchKernelGGL((paged_split<XT, CT, HD>), dim3((unsigned)(units * sa.splits)), dim3(256), 0, s, sa);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || sa.splits == 1) return e;
-    hipLaunchKernelGGL((paged_split_merge<XT, HD>), dim3((unsigned)(units * sa.slots)), dim3(256), 0, s, sa);
-    return hipGetLastError();
+    sa.least = split_least(units, context, cus);
+    sa.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>((context + sa.least - 1) / sa.least, kMaxSplits));
+    return sa;
 }
 
 struct TileArgs {
@@ -714,6 +718,7 @@ struct TileArgs {
     int32_t splits, least; // see cut
     bool pair_up;          // see find_group
     bool qvec;             // q rows are 16-byte aligned
+    uint32_t blocks, merge_blocks;   // of the launch that takes split_block's work too
     float2 *ml;            // partials [unit][split][kTileRows]: (max, sum)
     float *po;             // and sums of p v, [unit][split][kTileRows][head_dim]
 };
@@ -757,20 +762,26 @@ __device__ __forceinline__ void rows_apart(const TileArgs &ta, const Group &gr, 
 // read (four positions of one dimension per lane).  LDS rows are swizzled, 16-byte
 // pieces of keys by the row, 32-byte pieces of values likewise, so that both
 // reads touch every bank once; the copies permute their global addresses for it.
+template <int HD>
+struct TileLds {
+    __attribute__((aligned(256))) unsigned char k[2][64 * HD * 2], v[2][64 * HD * 2];   // 32 positions of fp32
+    float qs[4][HD];
+};
+
 template <class XT, int HD>
-__global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
+__device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, TileLds<HD> &lds, __bf16) {
     constexpr int NP = sizeof(XT) == 4 ? 3 : 1, ROWS = kTileRows<XT, __bf16>, CG = ROWS / 64;
     constexpr int NJ = HD / 32, ND = HD / 16;
     constexpr int CR = HD / 8, NL = CR / 4;                // 16-byte pieces per row, copies per wave and tile
     constexpr int KD = 16 / CR, VD2 = 8 / ND;              // rows per 256 bytes of LDS, as 16- and 32-byte pieces count
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
-    __shared__ __attribute__((aligned(256))) uint16_t kl[2][64 * HD], vl[2][64 * HD];
-    __shared__ float qs[4][HD];
+    uint16_t (*kl)[64 * HD] = (uint16_t (*)[64 * HD])lds.k, (*vl)[64 * HD] = (uint16_t (*)[64 * HD])lds.v;
+    auto &qs = lds.qs;
     const PagedArgs &a = ta.a;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, n = lane & 15;
-    const uint32_t unit = blockIdx.x % (uint32_t)ta.units, split = blockIdx.x / (uint32_t)ta.units;
+    const uint32_t unit = block % (uint32_t)ta.units, split = block / (uint32_t)ta.units;
     Group gr;
     if (!find_group<ROWS>(a, unit, 16, ta.pair_up, gr)) return;
     set_rows<ROWS>(a, gr, gr.row0);
@@ -1001,16 +1012,16 @@ __global__ __launch_bounds__(256, 2) void paged_tile(const TileArgs ta) {
 // keys' 16-byte pieces are swizzled by the row.  A tile's values are summed before
 // they join the running sums: an eighth of the roundings.
 template <class XT, int HD>
-__global__ __launch_bounds__(256, 2) void paged_tile_f32(const TileArgs ta) {
+__device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, TileLds<HD> &lds, float) {
     constexpr int ROWS = kTileRows<XT, float>, POS = 32;
     constexpr int NJ = HD / 16, NH = HD / 64;
     constexpr int CR = HD / 4, NL = 8 * CR / 64;           // 16-byte pieces per row, copies per wave and tile
-    __shared__ __attribute__((aligned(256))) float kl[2][POS * HD], vl[2][POS * HD];
-    __shared__ float qs[4][HD];
+    float (*kl)[POS * HD] = (float (*)[POS * HD])lds.k, (*vl)[POS * HD] = (float (*)[POS * HD])lds.v;
+    auto &qs = lds.qs;
     const PagedArgs &a = ta.a;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, n = lane & 15;
-    const uint32_t unit = blockIdx.x % (uint32_t)ta.units, split = blockIdx.x / (uint32_t)ta.units;
+    const uint32_t unit = block % (uint32_t)ta.units, split = block / (uint32_t)ta.units;
     Group gr;
     if (!find_group<ROWS>(a, unit, 16, ta.pair_up, gr)) return;
     set_rows<ROWS>(a, gr, gr.row0);
@@ -1182,11 +1193,11 @@ __global__ __launch_bounds__(256, 2) void paged_tile_f32(const TileArgs ta) {
 
 // Joins paged_tile's parts: HD / 4 threads a row.
 template <class XT, class CT, int HD>
-__global__ __launch_bounds__(256) void paged_tile_merge(const TileArgs ta) {
+__device__ __forceinline__ void tile_merge(const TileArgs &ta, uint32_t block) {
     constexpr int T = HD / 4, R = 256 / T;
     const PagedArgs &a = ta.a;
-    const uint32_t unit = blockIdx.x / (kTileRows<XT, CT> / R);
-    const int rr = (int)(blockIdx.x % (kTileRows<XT, CT> / R)) * R + threadIdx.x / T, d4 = threadIdx.x % T;
+    const uint32_t unit = block / (kTileRows<XT, CT> / R);
+    const int rr = (int)(block % (kTileRows<XT, CT> / R)) * R + threadIdx.x / T, d4 = threadIdx.x % T;
     Group gr;
     if (!find_group<kTileRows<XT, CT>>(a, unit, 16, ta.pair_up, gr)) return;
     set_rows<kTileRows<XT, CT>>(a, gr, gr.row0);
@@ -1217,40 +1228,91 @@ __global__ __launch_bounds__(256) void paged_tile_merge(const TileArgs ta) {
     for (int i = 0; i < 4; ++i) out[i] = (XT)(mm == -INFINITY ? (any > 0.0f ? NAN : 0.0f) : o[i] / l);
 }
 
-// Positions a part of paged_tile has at least: parts fill the chip's two blocks
-// per CU twice over, of at least 512 positions.
+// One launch for a batch of chunks and single tokens: the tiles' blocks, then those
+// of the requests with few rows, which fill in beside them (31 tokens and a
+// 333-token chunk over fp32: 38 us in two launches, BOTH so); likewise their merges.
 template <class XT, class CT, int HD>
-hipError_t launch_tile(tbh_device *dev, const PagedArgs &a, int64_t context, hipStream_t s) {
+__global__ __launch_bounds__(256, 2) void paged_both(const TileArgs ta, const SplitArgs sa) {
+    __shared__ __attribute__((aligned(256))) union {
+        TileLds<HD> tile;
+        SplitLds<HD> split;
+    } lds;
+    if (blockIdx.x < ta.blocks) tile_block<XT, HD>(ta, blockIdx.x, lds.tile, CT{});
+    else split_block<XT, CT, HD>(sa, blockIdx.x - ta.blocks, lds.split);
+}
+
+template <class XT, class CT, int HD>
+__global__ __launch_bounds__(256) void paged_both_merge(const TileArgs ta, const SplitArgs sa) {
+    __shared__ f32x4 red[256];
+    if (blockIdx.x < ta.merge_blocks) tile_merge<XT, CT, HD>(ta, blockIdx.x);
+    else split_merge<XT, HD>(sa, blockIdx.x - ta.merge_blocks, red);
+}
+
+// Parts of paged_both's tiles: enough to fill two blocks per CU twice over, of at
+// least 512 positions.  (2048 rows over 4096, which fill the chip with whole
+// contexts: 168 us, 203 in two parts, 244 in four: partials of fp32 rows cost
+// more than the evener blocks gain.)
+TileArgs plan_tile(const PagedArgs &a, int64_t context, int64_t tile_rows, size_t elem, int64_t cus) {
     TileArgs ta{};
     ta.a = a;
-    ta.qvec = aligned(a.q, 16) && (a.q_stride * (int64_t)sizeof(XT)) % 16 == 0;
+    ta.qvec = aligned(a.q, 16) && (a.q_stride * (int64_t)elem) % 16 == 0;
     const int64_t rows = a.tokens * a.rep;
-    const int64_t units = (rows / kTileRows<XT, CT> + std::min<int64_t>(a.requests, rows / 17 + 1)) * a.nkv;
-    const int64_t parts = std::max<int64_t>(1, 4 * (int64_t)std::max(1, dev->cu_count) / units);
-    ta.least = (int32_t)std::max<int64_t>(512, ((context + parts - 1) / parts + 127) / 128 * 128);
-    ta.splits = (int32_t)std::min<int64_t>((context + ta.least - 1) / ta.least, kMaxSplits);
-    if (ta.splits > 1) {
-        const int64_t n = units * ta.splits * kTileRows<XT, CT>;
-        const size_t head = (size_t)n * sizeof(float2);
-        char *ws = (char *)stream_workspace(dev, s, head + (size_t)n * HD * sizeof(float));
+    const int64_t units = (rows / tile_rows + std::min<int64_t>(a.requests, rows / 17 + 1)) * (int64_t)a.nkv;
+    ta.units = (int32_t)std::min<int64_t>(units, INT32_MAX);
+    const int64_t full = std::max<int64_t>(1, rows / tile_rows * a.nkv);   // without the requests' last, partial tiles
+    const int64_t parts = 10 * full >= 9 * 2 * cus ? 1 : std::max<int64_t>(1, 4 * cus / full);
+    ta.least = 256;
+    ta.splits = (int32_t)std::max<int64_t>(1, std::min({parts, (context + ta.least - 1) / ta.least, kMaxSplits}));
+    // two blocks share a CU: all run at once, or the longest have to come first
+    ta.pair_up = rows / tile_rows * a.nkv <= 2 * cus;
+    return ta;
+}
+
+template <class XT, class CT, int HD>
+hipError_t launch_matrix(tbh_device *dev, const PagedArgs &a, int64_t query, int64_t context, hipStream_t s) {
+    constexpr int R = kTileRows<XT, CT>;
+    const int64_t cus = std::max(1, dev->cu_count);
+    const bool tiles = (HD == 64 || HD == 128) && query * a.rep > 16;
+    SplitArgs sa = plan_split(a, query, context, tiles, sizeof(XT), cus);
+    TileArgs ta{};
+    if (tiles) ta = plan_tile(a, context, R, sizeof(XT), cus);
+    const int64_t tile_rows = tiles && ta.splits > 1 ? (int64_t)ta.units * ta.splits * R : 0;
+    const int64_t split_rows = sa.splits > 1 ? (int64_t)sa.units * sa.splits * sa.slots : 0;
+    if (tile_rows + split_rows > 0) {
+        const size_t tb = tile_rows ? partial_bytes(tile_rows, HD) : 0, sb = split_rows ? partial_bytes(split_rows, HD) : 0;
+        char *ws = (char *)stream_workspace(dev, s, tb + sb);
         if (ws) {
             ta.ml = (float2 *)ws;
-            ta.po = (float *)(ws + head);
+            ta.po = (float *)(ws + partial_head(tile_rows));
+            sa.ml = (float2 *)(ws + tb);
+            sa.po = (float *)(ws + tb + partial_head(split_rows));
         } else {
-            ta.splits = 1;   // no workspace (graph capture before any eager call): whole contexts
+            ta.splits = sa.splits = 1;   // no workspace (graph capture before any eager call): whole contexts
         }
     }
-    if (units * std::max<int64_t>(ta.splits, kTileRows<XT, CT> * HD / 1024) > INT32_MAX) return hipErrorInvalidValue;
-    ta.units = (int32_t)units;
-    // two blocks share a CU: all run at once, or the longest have to come first
-    ta.pair_up = rows / kTileRows<XT, CT> * a.nkv <= 2 * (int64_t)std::max(1, dev->cu_count);
-    const dim3 grid((unsigned)(units * ta.splits));
-    if constexpr (sizeof(CT) == 2) hipLaunchKernelGGL((paged_tile<XT, HD>), grid, dim3(256), 0, s, ta);
-    else hipLaunchKernelGGL((paged_tile_f32<XT, HD>), grid, dim3(256), 0, s, ta);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || ta.splits == 1) return e;
-    hipLaunchKernelGGL((paged_tile_merge<XT, CT, HD>), dim3((unsigned)(units * (kTileRows<XT, CT> * HD / 1024))), dim3(256), 0, s,
-                       ta);
+    const int64_t tile_blocks = tiles ? (int64_t)ta.units * ta.splits : 0, split_blocks = (int64_t)sa.units * sa.splits;
+    const int64_t tile_merges = tiles && ta.splits > 1 ? (int64_t)ta.units * (R * HD / 1024) : 0;
+    const int64_t split_merges = sa.splits > 1 ? (int64_t)sa.units * sa.slots : 0;
+    if (std::max(tile_blocks + split_blocks, tile_merges + split_merges) > INT32_MAX || sa.units == INT32_MAX ||
+        ta.units == INT32_MAX)
+        return hipErrorInvalidValue;
+    ta.blocks = (uint32_t)tile_blocks;
+    ta.merge_blocks = (uint32_t)tile_merges;
+    if constexpr (HD == 64 || HD == 128) {
+        if (tiles) {
+            hipLaunchKernelGGL((paged_both<XT, CT, HD>), dim3((unsigned)(tile_blocks + split_blocks)), dim3(256), 0, s, ta,
+                               sa);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess || tile_merges + split_merges == 0) return e;
+            hipLaunchKernelGGL((paged_both_merge<XT, CT, HD>), dim3((unsigned)(tile_merges + split_merges)), dim3(256), 0,
+                               s, ta, sa);
+            return hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL((paged_split<XT, CT, HD>), dim3((unsigned)split_blocks), dim3(256), 0, s, sa);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || split_merges == 0) return e;
+    hipLaunchKernelGGL((paged_split_merge<XT, HD>), dim3((unsigned)split_merges), dim3(256), 0, s, sa);
     return hipGetLastError();
 }
 
@@ -1258,18 +1320,11 @@ template <class XT, class CT>
 hipError_t launch_paged(tbh_device *dev, const PagedArgs &a, int64_t query, int64_t context, hipStream_t s) {
     // the matrix kernels take a tile of 16 positions from one block
     if (a.shift >= 4 && a.num_blocks > 0 && a.most > 0) {
-        if (query * a.rep > 16 && (a.hd == 64 || a.hd == 128)) {
-            const hipError_t e = a.hd == 64 ? launch_tile<XT, CT, 64>(dev, a, context, s)
-                                            : launch_tile<XT, CT, 128>(dev, a, context, s);
-            if (e != hipSuccess) return e;
-            return a.hd == 64 ? launch_split<XT, CT, 64>(dev, a, query, context, true, s)
-                              : launch_split<XT, CT, 128>(dev, a, query, context, true, s);
-        }
         switch (a.hd) {
-        case 32: return launch_split<XT, CT, 32>(dev, a, query, context, false, s);
-        case 64: return launch_split<XT, CT, 64>(dev, a, query, context, false, s);
-        case 96: return launch_split<XT, CT, 96>(dev, a, query, context, false, s);
-        case 128: return launch_split<XT, CT, 128>(dev, a, query, context, false, s);
+        case 32: return launch_matrix<XT, CT, 32>(dev, a, query, context, s);
+        case 64: return launch_matrix<XT, CT, 64>(dev, a, query, context, s);
+        case 96: return launch_matrix<XT, CT, 96>(dev, a, query, context, s);
+        case 128: return launch_matrix<XT, CT, 128>(dev, a, query, context, s);
         default: break;
         }
     }
