@@ -1230,7 +1230,7 @@ __device__ __forceinline__ void tile_merge(const TileArgs &ta, uint32_t block) {
 
 // One launch for a batch of chunks and single tokens: the tiles' blocks, then those
 // of the requests with few rows, which fill in beside them (31 tokens and a
-// 333-token chunk over fp32: 38 us in two launches, BOTH so); likewise their merges.
+// 333-token chunk over fp32: 48 us in two launches and two merges, 35 so); likewise their merges.
 template <class XT, class CT, int HD>
 __global__ __launch_bounds__(256, 2) void paged_both(const TileArgs ta, const SplitArgs sa) {
     __shared__ __attribute__((aligned(256))) union {

@@ -78,27 +78,52 @@ struct Shared {
     int32_t idx;
 };
 
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    return v;
-}
-
+// Sums, scans and extremes of a wave through DPP (a chain of __shfl steps goes
+// through LDS: 0.4 us each here).
 template <int CTRL>
-__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
-    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
 }
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
+
 __device__ __forceinline__ uint32_t wave_sum32(uint32_t v) {
-    v = dpp_add<wave::kXor1>(v);
-    v = dpp_add<wave::kXor2>(v);
-    v = dpp_add<wave::kHalfMirror>(v);
-    v = dpp_add<wave::kRowMirror>(v);
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 0) + (uint32_t)__builtin_amdgcn_readlane((int)v, 16) +
-           (uint32_t)__builtin_amdgcn_readlane((int)v, 32) + (uint32_t)__builtin_amdgcn_readlane((int)v, 48);
+    v += dpp<wave::kXor1>(v);
+    v += dpp<wave::kXor2>(v);
+    v += dpp<wave::kHalfMirror>(v);
+    v += dpp<wave::kRowMirror>(v);
+    return lane_of(v, 0) + lane_of(v, 16) + lane_of(v, 32) + lane_of(v, 48);
 }
-// Wave sum of values below 2^50, as two sums of 25 bits (64 of them fit 32).
+__device__ __forceinline__ uint32_t wave_max32(uint32_t v) {
+    v = max(v, dpp<wave::kXor1>(v));
+    v = max(v, dpp<wave::kXor2>(v));
+    v = max(v, dpp<wave::kHalfMirror>(v));
+    v = max(v, dpp<wave::kRowMirror>(v));
+    return max(max(lane_of(v, 0), lane_of(v, 16)), max(lane_of(v, 32), lane_of(v, 48)));
+}
+// of values below 2^50: two sums of 25 bits (64 of them fit 32); of any: of 22
 __device__ __forceinline__ uint64_t wave_sum50(uint64_t v) {
     return ((uint64_t)wave_sum32((uint32_t)(v >> 25)) << 25) + wave_sum32((uint32_t)v & 0x1FFFFFFu);
+}
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
+    return ((uint64_t)wave_sum32((uint32_t)(v >> 44)) << 44) + ((uint64_t)wave_sum32((uint32_t)(v >> 22) & 0x3FFFFFu) << 22) +
+           wave_sum32((uint32_t)v & 0x3FFFFFu);
+}
+// Inclusive sums, lane by lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t shifted(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_scan32(uint32_t v) {
+    v += shifted<0x111, 0xF>(v);    // row_shr 1, 2, 4, 8 within the 16-lane rows
+    v += shifted<0x112, 0xF>(v);
+    v += shifted<0x114, 0xF>(v);
+    v += shifted<0x118, 0xF>(v);
+    v += shifted<0x142, 0xA>(v);    // the last lane of rows 0 and 2 to rows 1 and 3,
+    return v + shifted<0x143, 0xC>(v);   // of row 1 to rows 2 and 3
+}
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
+    return ((uint64_t)wave_scan32((uint32_t)(v >> 44)) << 44) + ((uint64_t)wave_scan32((uint32_t)(v >> 22) & 0x3FFFFFu) << 22) +
+           wave_scan32((uint32_t)v & 0x3FFFFFu);
 }
 
 struct Row {
@@ -188,12 +213,7 @@ __device__ void narrow(Row &row, uint64_t target, Shared &sh) {
         __syncthreads();
         // bins 2 tid and 2 tid + 1: the first whose running sum reaches the target
         uint64_t v0 = BYW ? sh.wsum[2 * tid] : sh.cnt[2 * tid], v1 = BYW ? sh.wsum[2 * tid + 1] : sh.cnt[2 * tid + 1];
-        uint64_t in = v0 + v1;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint64_t o = __shfl_up(in, d);
-            if (lane >= d) in += o;
-        }
+        const uint64_t in = wave_scan64(v0 + v1);
         if (lane == 63) sh.red[wave] = in;
         __syncthreads();
         uint64_t before = above;
@@ -355,14 +375,11 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
             }
         }
     });
-    uint64_t best = (uint64_t)bk << 32 | (uint32_t)~bi;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint64_t o = __shfl_xor(best, d);
-        best = best > o ? best : o;
-    }
+    const uint32_t wk = wave_max32(bk), wi = wave_max32(bk == wk ? ~bi : 0);
+    uint64_t best = (uint64_t)wk << 32 | wi;
     if (lane == 0) sh.red[wave] = best;
     __syncthreads();
+#pragma unroll
     for (int i = 0; i < kWaves; ++i) best = best > sh.red[i] ? best : sh.red[i];
     __syncthreads();
     row.top = (uint32_t)(best >> 32);
@@ -395,17 +412,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
         __syncthreads();
         const uint32_t c0 = sh.cnt[2 * tid], c1 = sh.cnt[2 * tid + 1];
         const uint64_t v0 = by_weight ? sh.wsum[2 * tid] : c0, v1 = by_weight ? sh.wsum[2 * tid + 1] : c1;
-        uint64_t in = v0 + v1;
-        uint32_t cin = c0 + c1;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint64_t o = __shfl_up(in, d);
-            const uint32_t co = __shfl_up(cin, d);
-            if (lane >= d) {
-                in += o;
-                cin += co;
-            }
-        }
+        const uint64_t in = wave_scan64(v0 + v1);
+        const uint32_t cin = wave_scan32(c0 + c1);
         if (lane == 63) {
             sh.red[wave] = in;
             sh.redc[wave] = cin;
@@ -414,9 +422,10 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
         __syncthreads();
         uint64_t b0 = in - v0 - v1;
         uint32_t n0 = cin - c0 - c1;
-        for (int i = 0; i < wave; ++i) {
-            b0 += sh.red[i];
-            n0 += sh.redc[i];
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            b0 += i < wave ? sh.red[i] : 0;
+            n0 += i < wave ? sh.redc[i] : 0;
         }
         const uint64_t b1 = b0 + v0, b2 = b1 + v1;
         if (b0 < target && b1 >= target) {
@@ -642,12 +651,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
     int32_t piece = -1;
     uint64_t run = 0;
     for (int32_t g0 = 0; piece < 0; g0 += 64) {
-        uint64_t in = g0 + lane < segs ? sh.seg[g0 + lane] : 0;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint64_t o = __shfl_up(in, d);
-            if (lane >= d) in += o;
-        }
+        const uint64_t in = wave_scan64(g0 + lane < segs ? sh.seg[g0 + lane] : 0);
         const uint64_t over = __ballot(run + in > at);
         if (over) {
             const int f = __builtin_ctzll(over);
@@ -659,17 +663,20 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
         }
     }
     int32_t token = -1;
-    for (int j = 0; j < kSeg / 64 && token < 0 && piece >= 0; ++j) {
-        const int32_t i = piece * kSeg + j * 64 + lane;
-        uint64_t in = i < a.vocab ? weight(row.x[i], i) : 0;
+    if (piece >= 0) {
+        uint64_t w[kSeg / 64];
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint64_t o = __shfl_up(in, d);
-            if (lane >= d) in += o;
+        for (int j = 0; j < kSeg / 64; ++j) {
+            const int32_t i = piece * kSeg + j * 64 + lane;
+            w[j] = i < a.vocab ? weight(row.x[i], i) : 0;
         }
-        const uint64_t over = __ballot(run + in > at);
-        if (over) token = piece * kSeg + j * 64 + __builtin_ctzll(over);
-        else run += __shfl(in, 63);
+#pragma unroll
+        for (int j = 0; j < kSeg / 64; ++j) {
+            const uint64_t in = wave_scan64(w[j]);
+            const uint64_t over = __ballot(run + in > at);
+            if (over && token < 0) token = piece * kSeg + j * 64 + __builtin_ctzll(over);
+            run += __shfl(in, 63);
+        }
     }
     if (lane == 0) {
         a.tokens[r] = token;
