@@ -16,8 +16,7 @@
 // in double precision from a table of 2^(j / 64) and a polynomial of degree 5 on
 // +-1/128 (its error, (ln 2 / 128)^6 / 720, is below 2^-54).
 //
-// One block of 1024 threads takes a row; rows of up to 32 Ki logits stay in its
-// registers, longer ones are read again for each pass.
+// One block of 1024 threads takes a row, in two to four passes over it.
 #include <algorithm>
 #include <cstring>
 #include <new>
@@ -294,53 +293,38 @@ __device__ void narrow(Row &row, uint64_t target, Shared &sh) {
 }
 
 // The row's elements, four neighbours per thread and pass: pass p covers 4096 of
-// them, wave w's part of it piece 16 p + w of 256.  REG: up to 8 passes, held in
-// registers.
-template <bool REG, bool VEC>
+// them, wave w's part of it piece 16 p + w of 256.  Every use reads them again, a
+// row stays in its XCD's cache: held in registers, eight passes unrolled, a row
+// of 32000 took 20.5 us for 18.7 (no filters) and one of 1000 9.5 for 6.7, as the
+// code grew eightfold.
+template <bool VEC>
 struct Elems {
-    float4 v[REG ? 8 : 1];
     const float *x;
     int32_t vocab;
 
-    static __device__ __forceinline__ float4 at(const float *x, int32_t i, int32_t vocab) {
+    __device__ __forceinline__ float4 at(int32_t i) const {
         if (VEC && i + 4 <= vocab) return *(const float4 *)(x + i);
         float e[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) e[k] = i + k < vocab ? x[i + k] : -INFINITY;
         return float4{e[0], e[1], e[2], e[3]};
     }
-    __device__ __forceinline__ void load(const float *x_, int32_t vocab_) {
-        x = x_;
-        vocab = vocab_;
-        if constexpr (REG) {
-#pragma unroll
-            for (int p = 0; p < 8; ++p) v[p] = at(x, 4096 * p + 4 * (int)threadIdx.x, vocab);
-        }
-    }
     // f(piece, index of the first, four elements); elements behind the row are -inf
     template <class F>
     __device__ __forceinline__ void each(F f) const {
         const int tid = threadIdx.x, wave = tid >> 6;
-        if constexpr (REG) {
-#pragma unroll
-            for (int p = 0; p < 8; ++p) {
-                if (4096 * p < vocab) f(16 * p + wave, 4096 * p + 4 * tid, v[p]);
-                __builtin_amdgcn_sched_barrier(0);   // one pass at a time: registers
-            }
-        } else {
-            const int32_t n = (vocab + 4095) / 4096;
-            float4 a = at(x, 4 * tid, vocab);
-            for (int32_t p = 0; p < n; ++p) {
-                const float4 b = p + 1 < n ? at(x, 4096 * (p + 1) + 4 * tid, vocab) : a;   // the next, meanwhile
-                f(16 * p + wave, 4096 * p + 4 * tid, a);
-                a = b;
-            }
+        const int32_t n = (vocab + 4095) / 4096;
+        float4 a = at(4 * tid);
+        for (int32_t p = 0; p < n; ++p) {
+            const float4 b = p + 1 < n ? at(4096 * (p + 1) + 4 * tid) : a;   // the next, meanwhile
+            f(16 * p + wave, 4096 * p + 4 * tid, a);
+            a = b;
         }
     }
 };
 
 // One block per row.
-template <bool REG, bool VEC>
+template <bool VEC>
 __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
     __shared__ Shared sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -349,8 +333,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
     row.x = a.logits + r * a.ld;
     row.vocab = a.vocab;
     row.pow2 = sh.pow2;
-    Elems<REG, VEC> el;
-    el.load(row.x, a.vocab);
+    const Elems<VEC> el{row.x, a.vocab};
     if (tid < 64) sh.pow2[tid] = exp2(tid * (1.0 / 64.0));
     for (int b = tid; b < kBins; b += kThreads) {
         sh.cnt[b] = 0;
@@ -699,11 +682,9 @@ tbh_status check_sample(const char *what, tbh_device *dev, const float *logits, 
 
 hipError_t launch_sample(const SampleArgs &a, int64_t rows, hipStream_t s) {
     const dim3 grid((unsigned)rows), block(kThreads);
-    const bool vec = ((uintptr_t)a.logits & 15) == 0 && (a.ld % 4 == 0 || rows == 1), reg = a.vocab <= 8 * 4096;
-    if (reg && vec) hipLaunchKernelGGL((sample_rows<true, true>), grid, block, 0, s, a);
-    else if (reg) hipLaunchKernelGGL((sample_rows<true, false>), grid, block, 0, s, a);
-    else if (vec) hipLaunchKernelGGL((sample_rows<false, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((sample_rows<false, false>), grid, block, 0, s, a);
+    const bool vec = ((uintptr_t)a.logits & 15) == 0 && (a.ld % 4 == 0 || rows == 1);
+    if (vec) hipLaunchKernelGGL((sample_rows<true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((sample_rows<false>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 
