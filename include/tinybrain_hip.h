@@ -550,7 +550,7 @@ typedef struct tbh_paged_queries {
     void *out;                   /* as q, not overlapping it */
     int64_t q_stride;
     int64_t out_stride;
-    const int32_t *query_start;  /* [max_requests + 1], not descending */
+    const int32_t *query_start;  /* [max_requests + 1], not negative, not descending */
     const int32_t *context_lens; /* [max_requests], with the step's own tokens */
     float scale;                 /* of the scores; 0: 1 / sqrt(head_dim) */
     int32_t max_query_len;       /* at least the longest query_start[b + 1] - query_start[b], */
@@ -562,8 +562,8 @@ typedef struct tbh_paged_queries {
  * position up to its own, out = sum softmax(scale q . k) v per head, query
  * head h reading key/value head h / (num_heads / num_kv_heads).  Prompt
  * chunks and single tokens mix in one call.  A row with nothing to attend to
- * (negative position, no block) gives zeros; rows behind query_start's last
- * entry are left as they are.  Whatever lies in the cache behind a request's
+ * (negative position, no block) gives zeros; rows before query_start's first
+ * entry or behind its last are left as they are.  Whatever lies in the cache behind a request's
  * length is not used (it may be NaN).  Scores, softmax and sums are fp32; fp32
  * q keeps fp32's precision over a bf16 cache as well, bf16 q over a bf16 cache
  * has its probabilities rounded to bf16 for the second product.

@@ -309,6 +309,18 @@ def test_attention_rows_with_nothing_to_see(torch, backend, x, cache, hd):
     assert np.isfinite(out[:5]).all()                   # the other requests are not touched by it
 
 
+@pytest.mark.parametrize("hd", [64, 128, 6])
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_attention_rows_before_the_first_request(torch, backend, hd, new):
+    # a step's rows may start behind others of the same matrix, which stay as they are
+    c = _attention_case(torch, 31, [(new, 60), (0, 20), (1, 33)], 4, 2, hd, 16, "float32", "float32")
+    want = _run_attention(torch, backend, c)
+    out = torch.full((new + 4, 4 * hd), 7.0, device="cuda")
+    moved = dict(c, q=torch.cat([c["q"].new_full((3, 4 * hd), float("nan")), c["q"]]), start=c["start"] + 3)
+    got = _run_attention(torch, backend, moved, out=out)
+    assert torch.equal(got[3:], want) and bool((got[:3] == 7.0).all())
+
+
 @pytest.mark.parametrize("x,cache", TYPES)
 def test_attention_extreme_scores(torch, backend, x, cache):
     # one key far ahead of the others, and scores that all lie far from 0

@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256) void paged_rows(const PagedArgs a) {
     const int64_t t = row / a.nh;
     const int h = (int)(row % a.nh);
     const int32_t b = request_of(a, (int32_t)t);
-    if (b >= a.requests) return;                 // behind the last request's rows
+    if (b >= a.requests || a.start[b] > t || a.start[b] < 0) return;   // not a request's row
     const int64_t held = min((int64_t)max(a.ctx[b], 0), (int64_t)a.most << a.shift);
     const int64_t behind = (int64_t)a.start[b + 1] - 1 - t;   // rows of the request after this one
     const int32_t last = (int32_t)min(held - 1, held - 1 - behind);   // this row's position
