@@ -309,6 +309,14 @@ def test_attention_rows_with_nothing_to_see(torch, backend, x, cache, hd):
     assert np.isfinite(out[:5]).all()                   # the other requests are not touched by it
 
 
+@pytest.mark.parametrize("x,cache", TYPES)
+def test_attention_of_chunks_without_a_position(torch, backend, x, cache):
+    # requests of many rows that hold nothing yet, beside one that does
+    c = _attention_case(torch, 30, [(90, 0), (200, 0), (70, 150), (40, 0)], 4, 2, 128, 16, x, cache)
+    got = _check_attention(torch, backend, c, x, cache)
+    assert not got[:290].any() and not got[360:].any() and got[290:360].all()
+
+
 @pytest.mark.parametrize("hd", [64, 128, 6])
 @pytest.mark.parametrize("new", [1, 5, 40])
 def test_attention_rows_before_the_first_request(torch, backend, hd, new):

@@ -657,7 +657,6 @@ __device__ __forceinline__ void split_merge(const SplitArgs &sa, uint32_t block,
     const float l = wave::sum(part && f != 0.0f ? f * mine.y : 0.0f);
     const bool any = __any(part && mine.y > 0.0f);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
     for (int s0 = 0; s0 < ct.parts; s0 += G) {
         const int s = s0 + sg;
         const float fs = __shfl(f, min(s, 63));
@@ -825,7 +824,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
 #pragma unroll
         for (int j = 0; j < NL; ++j) dma::dma16(vd + 1024 * j, vr, voff[j], 0);
     };
-    copy(0, c0, ids);
+    if (c0 < c1) copy(0, c0, ids);   // else nothing waits for it
     uint64_t blocks = __ballot((uint32_t)ids < (uint32_t)a.num_blocks);   // sub-tiles of the window that have one
 
     // this wave's rows and their positions
@@ -1062,7 +1061,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
 #pragma unroll
         for (int j = 0; j < NL; ++j) dma::dma16(vd + 1024 * j, vr, voff[j], 0);
     };
-    copy(0, c0, ids);
+    if (c0 < c1) copy(0, c0, ids);   // else nothing waits for it
     uint64_t blocks = __ballot((uint32_t)ids < (uint32_t)a.num_blocks);
 
     const int32_t wrow = gr.row0 + 16 * w, wrows = min(16, gr.row0 + gr.rows - wrow);   // may be none
