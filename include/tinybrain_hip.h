@@ -481,8 +481,8 @@ typedef struct tbh_paged_layout {
     int32_t num_kv_heads;
     int32_t head_dim;        /* 1 .. 256 */
     int32_t type;            /* TBH_F32 or TBH_BF16 */
-    int32_t max_requests;    /* rows of the block table */
-    int32_t max_blocks;      /* entries per row */
+    int32_t max_requests;    /* rows of the block table, at most 2^30 */
+    int32_t max_blocks;      /* entries per row; max_blocks * block_size <= 2^30 */
 } tbh_paged_layout;
 
 /* Plans a step.  new_lens[max_requests]: tokens each request adds (0: idle

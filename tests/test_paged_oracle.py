@@ -150,6 +150,10 @@ LAYOUTS = [
     (dict(num_blocks=1 << 27), _abi.E_INVALID), (dict(max_requests=1 << 20, max_blocks=1 << 12), _abi.E_INVALID),
     (dict(max_blocks=1 << 27, max_requests=1), _abi.E_INVALID),
 ]
+LIMITS = [
+    (dict(max_blocks=(1 << 26) + 1, max_requests=1), _abi.E_INVALID),
+    (dict(max_requests=(1 << 30) + 1, max_blocks=1), _abi.E_INVALID),
+]
 CACHES = [
     (dict(num_kv_heads=0), _abi.E_INVALID), (dict(head_dim=0), _abi.E_INVALID), (dict(type=2), _abi.E_INVALID),
     (dict(head_dim=257), _abi.E_UNSUPPORTED),
@@ -163,6 +167,13 @@ def _plan(layout, **kw):
     return _abi.lib().tbh_paged_plan_device(a["dev"], ctypes.byref(layout) if layout is not None else None, a["new"],
                                             a["ctx"], a["table"], a["free"], a["count"], a["tokens"], a["start"],
                                             a["granted"], a["out"], a["count_out"], a["slots"], a["positions"], None)
+
+
+@pytest.mark.parametrize("change,status", LIMITS)
+def test_sizes_whose_tiles_would_pass_32_bits(change, status):
+    assert _plan(_layout(**change)) == status
+    assert _attention(_layout(**change)) == status
+    assert _append(_layout(**change)) == status
 
 
 @pytest.mark.parametrize("change,status", LAYOUTS)

@@ -64,7 +64,9 @@ inline tbh_status check_layout(const char *what, const tbh_device *dev, const tb
     if ((int64_t)l->num_blocks * l->block_size > INT32_MAX) return bad("num_blocks * block_size exceeds 2^31 - 1");
     if ((int64_t)l->max_requests * l->max_blocks > INT32_MAX)
         return bad("max_requests * max_blocks exceeds 2^31 - 1");
-    if ((int64_t)l->max_blocks * l->block_size > INT32_MAX) return bad("max_blocks * block_size exceeds 2^31 - 1");
+    // positions and the tile behind the last one, and a tile of requests, in 32 bits
+    if ((int64_t)l->max_blocks * l->block_size > 1 << 30) return bad("max_blocks * block_size exceeds 2^30");
+    if (l->max_requests > 1 << 30) return bad("max_requests exceeds 2^30");
     if (!cache) return TBH_OK;
     if (l->num_kv_heads <= 0 || l->head_dim <= 0) return bad("invalid heads or head_dim");
     if (l->type != TBH_F32 && l->type != TBH_BF16) return bad("unknown cache type");

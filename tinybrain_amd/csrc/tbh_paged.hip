@@ -176,7 +176,7 @@ template <class F>
 __device__ __forceinline__ int32_t row_of(int32_t t, int32_t rows, F start) {
     int32_t lo = 0, hi = rows;   // start(lo) <= t < start(hi + 1)
     while (lo < hi) {
-        const int32_t mid = (lo + hi + 1) >> 1;
+        const int32_t mid = lo + ((hi - lo + 1) >> 1);
         if (start(mid) <= t) lo = mid;
         else hi = mid - 1;
     }

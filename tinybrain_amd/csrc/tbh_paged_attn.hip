@@ -31,7 +31,7 @@ __device__ __forceinline__ float elem(const void *p, int64_t i) {
 __device__ __forceinline__ int32_t request_of(const PagedArgs &a, int32_t t) {
     int32_t lo = 0, hi = a.requests;
     while (lo < hi) {
-        const int32_t mid = (lo + hi + 1) >> 1;
+        const int32_t mid = lo + ((hi - lo + 1) >> 1);
         if (a.start[mid] <= t) lo = mid;
         else hi = mid - 1;
     }
