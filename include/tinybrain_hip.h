@@ -523,7 +523,8 @@ typedef struct tbh_paged_rows {
     int64_t q_stride;        /* elements from one row to the next */
     int64_t k_stride;
     int64_t v_stride;
-    void *q_out;             /* [tokens][num_heads * head_dim]; may be q itself (same type and stride) */
+    void *q_out;             /* [tokens][num_heads * head_dim]; may be q itself (same type and stride), */
+                             /* else it overlaps none of q, k and v */
     int64_t q_out_stride;
     int32_t q_out_type;
     float rope_base;         /* 0: no rotation */

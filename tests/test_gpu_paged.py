@@ -385,6 +385,82 @@ def test_attention_split_partials_of_two_streams(torch, backend):
         assert all(torch.equal(g, w) for g, w in zip(got, want))
 
 
+def test_attention_captured_before_any_eager_call(torch, backend):
+    # a stream without a workspace: whole contexts, and the same formula
+    c = _attention_case(torch, 40, [(1, 3000), (60, 900)], 8, 2, 64, 16, "float32", "bfloat16")
+    args = [_ints(torch, c[k]) for k in ("table", "start", "context")]
+    out = torch.empty_like(c["q"])
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        backend.paged_attention_device(c["q"], c["keys"], c["values"], *args, c["heads"], out=out)
+    keys, values = _np(c["keys"]), _np(c["values"])
+    want, bound = P.attention(_np(c["q"]), keys, values, c["table"], c["start"], c["context"], c["heads"])
+    for _ in range(3):
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        _close(_np(out), want, _tolerance(want, bound, "float32", "bfloat16"))
+        eager = _run_attention(torch, backend, c)            # with parts
+        _close(_np(eager), want, _tolerance(want, bound, "float32", "bfloat16"))
+
+
+def test_two_captured_steps_take_turns(torch, backend):
+    # two graphs of one stream share its workspace; replayed in turn, with eager calls between
+    cs = [_attention_case(torch, 41 + i, [(1, 2500 - 700 * i), (30, 800)], 8, 2, 64, 16, "float32", "float32")
+          for i in range(2)]
+    args = [[_ints(torch, c[k]) for k in ("table", "start", "context")] for c in cs]
+    outs = [torch.empty_like(c["q"]) for c in cs]
+    stream = torch.cuda.Stream()
+
+    def call(i, out):
+        return backend.paged_attention_device(cs[i]["q"], cs[i]["keys"], cs[i]["values"], *args[i], 8, out=out)
+
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        want = [call(i, torch.empty_like(outs[i])) for i in range(2)]
+        stream.synchronize()
+        graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+        for i in range(2):
+            with torch.cuda.graph(graphs[i], stream=stream):
+                call(i, outs[i])
+        for _ in range(4):
+            for o in outs:
+                o.zero_()
+            graphs[0].replay()
+            graphs[1].replay()
+            again = call(0, torch.empty_like(outs[0]))
+            graphs[0].replay()
+            stream.synchronize()
+            assert all(torch.equal(o, w) for o, w in zip([*outs, again], [*want, want[0]]))
+
+
+def test_calls_of_nothing(torch, backend):
+    # no request, no block, no entry in the table, no row
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")      # noqa: E731
+    p = backend.paged_plan_device(i(0), i(0), i(0, 4), i(6), i(1) + 6, 16, 3)
+    assert _np(p.queryStart).tolist() == [0] and _np(p.slots).tolist() == [-1] * 3 and int(p.freeCount) == 6
+    p = backend.paged_plan_device(i(2) + 1, i(2), i(2, 0), i(0), i(1), 16, 3)
+    assert _np(p.queryStart).tolist() == [0, 1, 2] and _np(p.granted).tolist() == [0, 0]
+    assert _np(p.slots).tolist() == [-1] * 3 and _np(p.contextLens).tolist() == [0, 0]
+    q, rows = torch.randn(3, 256, device="cuda"), torch.randn(3, 128, device="cuda")
+    for blocks, entries in ((0, 2), (4, 0), (0, 0)):
+        k = torch.ones(blocks, 2, 16, 64, device="cuda")
+        for new in (1, 3):
+            start = i(3) + new
+            start[0] = 0
+            got = backend.paged_attention_device(q[:new], k, k, i(2, entries), start, i(2) + 5, 4)
+            assert not got.any()
+        assert torch.equal(backend.paged_append_device(k, k, i(3) - 1, rows, rows, q=q), q) and bool((k == 1).all())
+    k = torch.ones(4, 2, 16, 64, device="cuda")
+    assert backend.paged_attention_device(q[:0], k, k, i(2, 1), i(3), i(2), 4).shape == (0, 256)
+    assert backend.paged_append_device(k, k, i(0), rows[:0], rows[:0], q=q[:0]).shape == (0, 256)
+    out = torch.full_like(q, 7.0)
+    assert bool((backend.paged_attention_device(q, k, k, i(0, 1), i(1), i(0), 4, out=out) == 7.0).all())
+
+
 # ---------------------------------------------------------------------------
 # refusals of the Python entry points
 # ---------------------------------------------------------------------------
@@ -418,6 +494,12 @@ def test_preconditions(torch, backend):
             call()
     with pytest.raises(T.HIPBackendError):
         backend.paged_plan_device(i(3), i(3), i(3, 4), i(4), i(1), 24, 4)
+    for call in (lambda: backend.paged_plan_device(i(3), i(3), i(3, 4), i(4), i(1), 1 << 35, 4),
+                 lambda: backend.paged_attention_device(q, k, k, i(2, 4), i(3), i(2), 4, maxContextLen=1 << 31)):
+        with pytest.raises(PreconditionFailure):
+            call()
+    with pytest.raises(T.HIPBackendError):
+        backend.paged_append_device(k, k, i(3), r, r, positions=i(3), ropeBase=1e300)
 
 
 # ---------------------------------------------------------------------------

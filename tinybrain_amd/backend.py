@@ -451,7 +451,7 @@ class HIPBackend:
             raise PreconditionFailure("plan: contextOut [requests] and freeCountOut [1]")
         at = out.data_ptr()
         _check(self._lib.tbh_paged_plan_device(
-            self._dev, self._layout.pack(freeBlocks.numel(), blockSize, 0, 0, 0, b, blockTable.shape[1]),
+            self._dev, self._packed(self._layout, freeBlocks.numel(), blockSize, 0, 0, 0, b, blockTable.shape[1]),
             newLens.data_ptr(), contextLens.data_ptr(), blockTable.data_ptr(), freeBlocks.data_ptr(),
             freeCount.data_ptr(), maxTokens, at, at + 4 * (b + 1), ctx.data_ptr(), count.data_ptr(),
             at + 4 * (2 * b + 1), at + 4 * (2 * b + 1 + maxTokens), self._raw_stream(stream)))
@@ -500,9 +500,9 @@ class HIPBackend:
                 ot = self._paged_type(qOut)
             heads, qp, qs, op, os = width // hd, q.data_ptr(), q.stride(0), qOut.data_ptr(), qOut.stride(0)
         _check(self._lib.tbh_paged_append_device(
-            self._dev, self._layout.pack(n, bs, nkv, hd, ct, 0, 0),
-            self._rows.pack(tokens, xt, heads, qp, k.data_ptr(), v.data_ptr(), qs, k.stride(0), v.stride(0), op, os,
-                            ot, ropeBase, slots.data_ptr(), at),
+            self._dev, self._packed(self._layout, n, bs, nkv, hd, ct, 0, 0),
+            self._packed(self._rows, tokens, xt, heads, qp, k.data_ptr(), v.data_ptr(), qs, k.stride(0), v.stride(0),
+                         op, os, ot, ropeBase, slots.data_ptr(), at),
             keys.data_ptr(), values.data_ptr(), self._raw_stream(stream)))
         return qOut if q is not None else None
 
@@ -531,11 +531,18 @@ class HIPBackend:
         elif self._row_shape(out) != shape or out.dtype != q.dtype:
             raise PreconditionFailure("attention: out must be like the queries")
         _check(self._lib.tbh_paged_attention_device(
-            self._dev, self._layout.pack(n, bs, nkv, hd, ct, b, blockTable.shape[1]),
-            self._queries.pack(tokens, xt, numHeads, q.data_ptr(), out.data_ptr(), q.stride(0), out.stride(0),
-                               queryStart.data_ptr(), contextLens.data_ptr(), scale, maxQueryLen, maxContextLen),
+            self._dev, self._packed(self._layout, n, bs, nkv, hd, ct, b, blockTable.shape[1]),
+            self._packed(self._queries, tokens, xt, numHeads, q.data_ptr(), out.data_ptr(), q.stride(0), out.stride(0),
+                         queryStart.data_ptr(), contextLens.data_ptr(), scale, maxQueryLen, maxContextLen),
             keys.data_ptr(), values.data_ptr(), blockTable.data_ptr(), self._raw_stream(stream)))
         return out
+
+    @staticmethod
+    def _packed(packer, *values) -> bytes:
+        try:
+            return packer.pack(*values)
+        except struct.error:
+            raise PreconditionFailure("a size does not fit the call's 32 bits") from None
 
     def _raw_stream(self, stream) -> int:
         if stream is not None:
