@@ -46,13 +46,6 @@ __device__ __forceinline__ int64_t place(const PagedArgs &a, int32_t b, int32_t 
     return ((((int64_t)id * a.nkv + kvh) << a.shift) + (pos & ((1 << a.shift) - 1))) * a.hd;
 }
 
-// Orders a wave's LDS writes before later LDS reads by its other lanes.
-__device__ __forceinline__ void wave_lds_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-}
-
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // One row's part of the softmax over positions [c0, end), by one wave: 64
@@ -69,9 +62,9 @@ __device__ __forceinline__ RowPart row_part(const PagedArgs &a, int32_t b, int64
                                             float *qs) {
     const int lane = threadIdx.x & 63, kvh = head / a.rep;
     const float c2 = a.scale * 1.44269504f;
-    wave_lds_fence();
+    wave::lds_fence();
     for (int d = lane; d < a.hd; d += 64) qs[d] = elem<XT>(a.q, t * a.q_stride + (int64_t)head * a.hd + d);
-    wave_lds_fence();
+    wave::lds_fence();
     RowPart r{-INFINITY, 0.0f, {}, false};
     for (int32_t p0 = c0; p0 < end; p0 += 64) {
         const int64_t at = p0 + lane < end ? place(a, b, p0 + lane, kvh) : -1;

@@ -29,6 +29,13 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
+// Orders a wave's LDS writes before later LDS reads by its other lanes.
+__device__ __forceinline__ void lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // Sum over each aligned group of 4 lanes, in every lane of the group.
 __device__ __forceinline__ float quad_sum(float v) {
     v += dpp<kXor1>(v);
