@@ -286,6 +286,15 @@ def test_attention_lengths(torch, backend, x, cache, lens, nh, nkv, hd):
 
 
 @pytest.mark.parametrize("x,cache", TYPES)
+@pytest.mark.parametrize("nh,nkv,hd,bs", [(4, 2, 80, 16), (2, 2, 256, 16), (4, 4, 64, 8), (6, 2, 33, 32), (8, 1, 8, 1)])
+def test_attention_of_other_heads_over_several_passes(torch, backend, x, cache, nh, nkv, hd, bs):
+    # head dimensions and blocks that no matrix kernel takes, lengths around the waves' passes of 64
+    c = _attention_case(torch, 32, [(1, 64), (1, 65), (3, 256), (2, 257), (1, 700), (70, 130), (1, 1)], nh, nkv, hd, bs,
+                        x, cache, holes=bs > 1)
+    _check_attention(torch, backend, c, x, cache)
+
+
+@pytest.mark.parametrize("x,cache", TYPES)
 def test_attention_strides_holes_and_scale(torch, backend, x, cache):
     # rows of a wider matrix whose starts are not 16-byte aligned; pages that are
     # missing; a scale of the caller's

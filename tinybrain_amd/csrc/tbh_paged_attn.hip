@@ -49,47 +49,83 @@ __device__ __forceinline__ int64_t place(const PagedArgs &a, int32_t b, int32_t 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // One row's part of the softmax over positions [c0, end), by one wave: 64
-// positions a pass, a position per lane for the scores and an output dimension
-// per lane (lane, lane + 64, ...) for the values.  m: largest score in powers of
-// two, l and o: sums relative to it.  qs: the wave's LDS, head_dim floats.
+// positions a pass, every `step`, a position per lane for the scores and an output
+// dimension per lane (lane, lane + 64, ...) for the values.  m: largest score in
+// powers of two, l and o: sums relative to it.  qs: the wave's LDS, head_dim floats.
+// AHEAD: positions whose values are in flight at once, 8, or 1 where the rare row is
+// taken inside a kernel that needs the registers.
 struct RowPart {
     float m, l, o[kMaxHeadDim / 64];
     bool seen;             // a position of the range is in a block
 };
 
-template <class XT, class CT>
+template <class CT, bool VEC>
+__device__ __forceinline__ float dot_key(const PagedArgs &a, int64_t at, const float *qs) {
+    float dot = 0.0f;
+    if (VEC && a.hd % 8 == 0) {
+        const CT *k = (const CT *)a.kc + at;
+#pragma unroll 4
+        for (int d = 0; d < a.hd; d += 8) {
+            float x[8];
+            unpack(*(const Vec8<CT> *)(k + d), x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dot += qs[d + i] * x[i];
+        }
+    } else {
+        for (int d = 0; d < a.hd; ++d) dot += qs[d] * elem<CT>(a.kc, at + d);
+    }
+    return dot;
+}
+
+template <class XT, class CT, int AHEAD>
 __device__ __forceinline__ RowPart row_part(const PagedArgs &a, int32_t b, int64_t t, int head, int32_t c0, int32_t end,
-                                            float *qs) {
+                                            float *qs, int32_t step = 64) {
     const int lane = threadIdx.x & 63, kvh = head / a.rep;
     const float c2 = a.scale * 1.44269504f;
     wave::lds_fence();
     for (int d = lane; d < a.hd; d += 64) qs[d] = elem<XT>(a.q, t * a.q_stride + (int64_t)head * a.hd + d);
     wave::lds_fence();
     RowPart r{-INFINITY, 0.0f, {}, false};
-    for (int32_t p0 = c0; p0 < end; p0 += 64) {
+    for (int32_t p0 = c0; p0 < end; p0 += step) {
         const int64_t at = p0 + lane < end ? place(a, b, p0 + lane, kvh) : -1;
         const uint64_t valid = __ballot(at >= 0);
         if (!valid) continue;
         r.seen = true;
-        float s = -INFINITY;
-        if (at >= 0) {
-            float dot = 0.0f;
-            for (int d = 0; d < a.hd; ++d) dot += qs[d] * elem<CT>(a.kc, at + d);
-            s = dot * c2;
-        }
+        const float s = at >= 0 ? dot_key<CT, (AHEAD > 1)>(a, at, qs) * c2 : -INFINITY;
         const float nm = fmaxf(r.m, wave::max(s));
         const float ref = nm == -INFINITY ? 0.0f : nm;
         const float corr = exp2_fast(r.m - ref), p = at >= 0 ? exp2_fast(s - ref) : 0.0f;
         r.l = r.l * corr + wave::sum(p);
 #pragma unroll
         for (int i = 0; i < kMaxHeadDim / 64; ++i) r.o[i] *= corr;
-        for (uint64_t v = valid; v; v &= v - 1) {
-            const int j = __builtin_ctzll(v);
+        for (uint64_t left = valid; AHEAD == 1 && left; left &= left - 1) {
+            const int j = __builtin_ctzll(left);
             const float pj = wave::lane_value(p, j);
-            const int64_t vj = __shfl(at, j);
+            const int64_t from = __shfl(at, j);
 #pragma unroll
             for (int i = 0; i < kMaxHeadDim / 64; ++i)
-                if (lane + 64 * i < a.hd) r.o[i] += pj * elem<CT>(a.vc, vj + lane + 64 * i);
+                if (lane + 64 * i < a.hd) r.o[i] += pj * elem<CT>(a.vc, from + lane + 64 * i);
+        }
+        for (int j0 = 0; AHEAD > 1 && j0 < 64; j0 += AHEAD) {
+            if (!(valid >> j0 & ((1ull << AHEAD) - 1))) continue;
+            int64_t from[AHEAD];
+            float pj[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                pj[j] = wave::lane_value(p, j0 + j);
+                from[j] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), j0 + j) << 32 |
+                                    (uint32_t)__builtin_amdgcn_readlane((int)at, j0 + j));
+            }
+#pragma unroll
+            for (int i = 0; i < kMaxHeadDim / 64; ++i) {
+                if (64 * i >= a.hd) break;
+                const int d = min(lane + 64 * i, a.hd - 1);
+                float x[AHEAD];
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) x[j] = elem<CT>(a.vc, max(from[j], (int64_t)0) + d);   // block 0's: not used
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) r.o[i] += from[j] >= 0 ? pj[j] * x[j] : 0.0f;
+            }
         }
         r.m = nm;
     }
@@ -106,12 +142,18 @@ __device__ __forceinline__ void store_row(const PagedArgs &a, int64_t t, int hea
             ((XT *)a.out)[t * a.out_stride + (int64_t)head * a.hd + lane + 64 * i] = (XT)(r.seen ? r.o[i] / r.l : 0.0f);
 }
 
-// Any head dimension, block size and alignment: one wave per (token, query head).
+// Any head dimension, block size and alignment: a block per (token, query head),
+// whose four waves take passes of 64 positions in turn and meet in LDS.  Bound by
+// the latency of its loads.  us, bf16 cache, 32 heads on 8 of 80: 130 for a row over
+// 4000 positions (381 with one wave a row), 120 for 64 rows over 1000 (143), 278 for
+// 256 rows over 1024 (292); heads of 256: 210 (708), 324 (301), 641 (647).
 template <class XT, class CT>
 __global__ __launch_bounds__(256) void paged_rows(const PagedArgs a) {
-    __shared__ float qs[4][kMaxHeadDim];
-    const int w = threadIdx.x >> 6;
-    const int64_t row = (int64_t)blockIdx.x * 4 + w;
+    __shared__ float qs[4][kMaxHeadDim], so[4][kMaxHeadDim];
+    __shared__ float sm[4], sl[4];
+    __shared__ bool sseen[4];
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     if (row >= a.tokens * a.nh) return;
     const int64_t t = row / a.nh;
     const int h = (int)(row % a.nh);
@@ -120,7 +162,30 @@ __global__ __launch_bounds__(256) void paged_rows(const PagedArgs a) {
     const int64_t held = min((int64_t)max(a.ctx[b], 0), (int64_t)a.most << a.shift);
     const int64_t behind = (int64_t)a.start[b + 1] - 1 - t;   // rows of the request after this one
     const int32_t last = (int32_t)min(held - 1, held - 1 - behind);   // this row's position
-    store_row<XT>(a, t, h, row_part<XT, CT>(a, b, t, h, 0, last + 1, qs[w]));
+    const RowPart p = row_part<XT, CT, 8>(a, b, t, h, 64 * w, last + 1, qs[w], 256);
+    if (lane == 0) {
+        sm[w] = p.m;
+        sl[w] = p.l;
+        sseen[w] = p.seen;
+    }
+#pragma unroll
+    for (int i = 0; i < kMaxHeadDim / 64; ++i)
+        if (lane + 64 * i < a.hd) so[w][lane + 64 * i] = p.o[i];
+    __syncthreads();
+    if (w != 0) return;
+    RowPart r{-INFINITY, 0.0f, {}, false};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r.m = fmaxf(r.m, sm[k]);
+    for (int k = 0; k < 4; ++k) {
+        if (!sseen[k]) continue;
+        r.seen = true;
+        const float f = exp2_fast(sm[k] - (r.m == -INFINITY ? 0.0f : r.m));   // 0 for scores of -inf alone
+        r.l += f * sl[k];
+#pragma unroll
+        for (int i = 0; i < kMaxHeadDim / 64; ++i)
+            if (lane + 64 * i < a.hd) r.o[i] += f * so[k][lane + 64 * i];
+    }
+    store_row<XT>(a, t, h, r);
 }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -600,7 +665,7 @@ __device__ __forceinline__ void split_block(const SplitArgs &sa, uint32_t block,
             const int32_t tt = (row0 + rr) / a.rep;
             const int head = gr.kvh * a.rep + (row0 + rr) % a.rep;
             const int32_t end = min(c1, gr.q.base + tt + 1);
-            const RowPart x = row_part<XT, CT>(a, gr.b, gr.q.first + tt, head, c0, end, &so[w][0][0]);
+            const RowPart x = row_part<XT, CT, 1>(a, gr.b, gr.q.first + tt, head, c0, end, &so[w][0][0]);
             if (ct.parts == 1) {
                 store_row<XT>(a, gr.q.first + tt, head, x);
             } else {
@@ -700,7 +765,9 @@ SplitArgs plan_split(const PagedArgs &a, int64_t query, int64_t context, bool ti
     sa.long_rows = tiles ? 16 : INT32_MAX;
     sa.slots = (int32_t)std::min<int64_t>(16, query * a.rep);
     sa.least = split_least(units, context, cus);
-    sa.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>((context + sa.least - 1) / sa.least, kMaxSplits));
+    // at most 2^22 blocks (a grid has below 2^32 threads)
+    sa.splits = (int32_t)std::max<int64_t>(
+        1, std::min<int64_t>({(context + sa.least - 1) / sa.least, kMaxSplits, (1 << 22) / std::max<int64_t>(units, 1)}));
     return sa;
 }
 
@@ -732,7 +799,7 @@ __device__ __forceinline__ void rows_apart(const TileArgs &ta, const Group &gr, 
     for (int rr = 0; rr < wrows; ++rr) {
         const int32_t tt = (wrow + rr) / a.rep;
         const int head = gr.kvh * a.rep + (wrow + rr) % a.rep;
-        const RowPart x = row_part<XT, CT>(a, gr.b, gr.q.first + tt, head, c0, min(c1, gr.q.base + tt + 1), qs);
+        const RowPart x = row_part<XT, CT, 1>(a, gr.b, gr.q.first + tt, head, c0, min(c1, gr.q.base + tt + 1), qs);
         if (parts == 1) {
             store_row<XT>(a, gr.q.first + tt, head, x);
         } else {
@@ -1320,7 +1387,9 @@ hipError_t launch_paged(tbh_device *dev, const PagedArgs &a, int64_t query, int6
         default: break;
         }
     }
-    hipLaunchKernelGGL((paged_rows<XT, CT>), dim3((unsigned)((a.tokens * a.nh + 3) / 4)), dim3(256), 0, s, a);
+    const int64_t rows = a.tokens * a.nh, across = std::min<int64_t>(rows, 1 << 20);   // threads of a grid's x: below 2^32
+    hipLaunchKernelGGL((paged_rows<XT, CT>), dim3((unsigned)across, (unsigned)((rows + across - 1) / across)), dim3(256), 0,
+                       s, a);
     return hipGetLastError();
 }
 
