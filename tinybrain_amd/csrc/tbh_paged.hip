@@ -77,7 +77,9 @@ __device__ __forceinline__ int32_t first_above(const int32_t *v, int32_t n, int3
 // Rows of the plan: one block, a row per thread and tile of 1024 rows, its sums by
 // block scans with a carry.  Bound by its chain of dependent steps: lengths, scan,
 // blocks off the stack.  New blocks, and the tokens of a small step (solo), are
-// dealt over all threads, each finding its row in the tile's sums.
+// dealt over all threads, each finding its row in the tile's sums (a row's own thread
+// would walk a chunk's blocks alone).  7.8 us for 64 requests and tokens, 12 for 1000
+// requests, whose scans over several blocks would need a launch more.
 __global__ __launch_bounds__(kPlanThreads) void plan_rows(const PlanArgs a, bool solo) {
     __shared__ int64_t red[kPlanThreads / 64];
     __shared__ int32_t upto[kPlanThreads], have_[kPlanThreads];   // blocks asked for by the tile's rows up to this
@@ -183,7 +185,8 @@ __device__ __forceinline__ int32_t row_of(int32_t t, int32_t rows, F start) {
     return lo;
 }
 
-// Slots and positions of the step's tokens, one per thread, after plan_rows.
+// Slots and positions of the step's tokens, one per thread, after plan_rows.  Bound
+// by the latency of its search and look-ups: 4.4 us for 22000 tokens of 1000 requests.
 __global__ __launch_bounds__(256) void plan_tokens(const PlanArgs a) {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (t >= a.max_tokens) return;
@@ -216,7 +219,11 @@ __device__ __forceinline__ float load1(const void *p, int64_t i) {
 
 // The rows of one token.  The angle of pair i is position * base^(-2i / hd),
 // formed in turns in double precision and reduced to (-1/2, 1/2] before the
-// sine: at position 2^20 the reduced angle is off by 2^-31 turns.
+// sine: at position 2^20 the reduced angle is off by 2^-31 turns.  A block per
+// token, so that a pair's sine is formed once and shared by all heads through LDS;
+// VEC: eight elements, four whole pairs, per load and store.  Bound by memory: 4096
+// rows of 32 + 8 + 8 heads of 128 in bf16 17.5 us, 5.8 TB/s; by latency on few rows:
+// 8 of fp32 4.0 us.
 template <class XT, class CT, class QT, bool VEC>
 __global__ __launch_bounds__(256) void append_rows(const RowsArgs a) {
     __shared__ float2 cs[kMaxHeadDim / 2];   // (cos, sin) per pair

@@ -228,7 +228,7 @@ struct SplitArgs {
     int32_t units;         // (16 rows, key/value head) pairs
     int32_t splits, least; // see cut
     int32_t slots;         // rows of a unit in the partials, at most 16
-    int32_t long_rows;     // requests of more rows are another launch's (paged_tile)
+    int32_t long_rows;     // requests of more rows are tile_block's
     bool scan;             // units are groups of 16 rows of any request, else requests
     bool qvec;             // q rows are 16-byte aligned
     float2 *ml;            // partials [unit][split][slots]: (max, sum)
@@ -483,7 +483,12 @@ struct Step<XT, float, HD> {
 
 // Few rows per request (single tokens of grouped heads, short chunks): 16 rows
 // and one part of the positions a block, its four waves taking steps of 32
-// positions in turn and meeting in LDS at the end.  Bound by reading the cache.
+// positions in turn and meeting in LDS at the end.  Operands go from memory to
+// registers: each byte of the cache is used by one wave alone, so LDS would only
+// add a trip.  Bound by reading the cache: 64 requests of 100 .. 8192 positions, 32
+// heads on 8 of 128, fp32 rows over a bf16 cache 107 to 114 us, 470 MB at 4.1 to 4.4
+// TB/s (a large copy: 4.7); by latency where there is little: a row over 4096 fp32
+// positions of 4 heads of 64 7.4 us.
 template <int HD>
 struct SplitLds {
     float so[4][16][HD + 4];
@@ -683,9 +688,10 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
     split_block<XT, CT, HD>(sa, blockIdx.x, lds);
 }
 
-// Joins paged_split's parts: a block per unit and row, HD / 4 threads across the
+// Joins split_block's parts: a block per unit and row, HD / 4 threads across the
 // head, the parts dealt over the rest.  Every wave holds the parts' factors, one
-// per lane.
+// per lane.  Bound by latency: 4.0 us after a row over 4096 positions, 6.0 after 64
+// requests of up to 8192.
 template <class XT, int HD>
 __device__ __forceinline__ void split_merge(const SplitArgs &sa, uint32_t block, f32x4 *lds) {
     constexpr int T = HD / 4, G = 256 / T;
@@ -741,7 +747,7 @@ __global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa) {
 
 constexpr int64_t kMaxSplits = 64;   // a lane each in split_merge
 
-// Positions a part of paged_split has at least, for `units` units: enough blocks
+// Positions a part of split_block has at least, for `units` units: enough blocks
 // to fill the chip, parts no longer than 1024 (a batch's longest request would
 // else end long after the others) and no shorter than 128 (a step per wave).
 int32_t split_least(int64_t units, int64_t context, int64_t cus) {
@@ -788,7 +794,7 @@ struct TileArgs {
 template <class XT, class CT>
 constexpr int kTileRows = sizeof(XT) + sizeof(CT) == 4 ? 128 : 64;
 
-// As in paged_split: the wave's rows one at a time, where one may have met an inf
+// As in split_block: the wave's rows one at a time, where one may have met an inf
 // or NaN that it does not see.
 template <class XT, class CT, int HD>
 __device__ __forceinline__ void rows_apart(const TileArgs &ta, const Group &gr, uint32_t unit, uint32_t split,
@@ -810,7 +816,7 @@ __device__ __forceinline__ void rows_apart(const TileArgs &ta, const Group &gr, 
     }
 }
 
-// Many rows per request over a bf16 cache. A block takes kTileRows rows of one
+// Many rows per request over a bf16 cache.  A block takes kTileRows rows of one
 // key/value head and one part of the positions: four waves of 16 or 32 rows,
 // tiles of 64 positions in two LDS buffers, each wave copying 16 positions of the
 // next tile straight to LDS while this one is multiplied, one barrier a tile.
@@ -821,6 +827,11 @@ __device__ __forceinline__ void rows_apart(const TileArgs &ta, const Group &gr, 
 // read (four positions of one dimension per lane).  LDS rows are swizzled, 16-byte
 // pieces of keys by the row, 32-byte pieces of values likewise, so that both
 // reads touch every bank once; the copies permute their global addresses for it.
+// Bound by the matrix instructions and the exponentials that they wait for: 2048
+// rows over 4096 positions, 32 heads on 8 of 128, bf16 throughout 128 to 132 us, 103
+// GFLOP at 780 to 805 TFLOP/s (a large product: 1143).  Prompts of 150 .. 301 fp32
+// rows of 12 heads of 64: 17 us, in which launch, look-ups and the first tile count
+// for more than the three pieces' products.
 template <int HD>
 struct TileLds {
     __attribute__((aligned(256))) unsigned char k[2][64 * HD * 2], v[2][64 * HD * 2];   // 32 positions of fp32
@@ -1062,14 +1073,16 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
     rows_apart<XT, __bf16, HD>(ta, gr, unit, split, ct.parts, c0, c1, wrow, wrows, qs[w]);
 }
 
-// Many rows per request over an fp32 cache, as paged_tile but on the fp32 matrix
+// Many rows per request over an fp32 cache, as above but on the fp32 matrix
 // instruction (256 flop per clock and CU, which bounds it): four waves of 16
 // rows, tiles of 32 positions, a wave copying eight of them.  The products are
 // those of Step: values need no transposing read, as the instruction's reduction
 // takes one position per lane.  Outputs are dealt four consecutive dimensions of
 // every 64 to a lane, so that 16 lanes read 256 bytes of a value row at once;
 // keys' 16-byte pieces are swizzled by the row.  A tile's values are summed before
-// they join the running sums: an eighth of the roundings.
+// they join the running sums: an eighth of the roundings.  31 single tokens and a
+// chunk of 333, 32 heads on 4 of 64, fp32: 25 us with split_block's share, 7 tiles of
+// 32 positions a block, each a wait and 64 matrix instructions of 32 cycles.
 template <class XT, int HD>
 __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, TileLds<HD> &lds, float) {
     constexpr int ROWS = kTileRows<XT, float>, POS = 32;
@@ -1103,7 +1116,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
         voff[j] = 16 * (64 * j + lane);
     }
     const uint32_t kdst = dma::lds_addr(&kl[0][8 * w * HD]), vdst = dma::lds_addr(&vl[0][8 * w * HD]);
-    auto window = [&](int32_t p) {                         // as in paged_tile
+    auto window = [&](int32_t p) {                         // as above
         return p + 16 * lane < c1 ? table[(p + 16 * lane) >> a.shift] : -1;
     };
     int32_t ids = window(c0), ids_next = window(c0 + 1024);
@@ -1139,7 +1152,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
     const int32_t low = min(gr.q.base + wrow / a.rep, gr.q.held - 1);
     const int32_t high = wrows > 0 ? min(gr.q.base + (wrow + wrows - 1) / a.rep, gr.q.held - 1) : -1;
 
-    constexpr float kLag = 8.0f;                           // as in paged_tile
+    constexpr float kLag = 8.0f;                           // as above
     float mr = -INFINITY, l = 0.0f;                        // l: this lane's positions only
     int32_t first = INT32_MAX;
     f32x4 o[4 * NH];
@@ -1250,7 +1263,9 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
     rows_apart<XT, float, HD>(ta, gr, unit, split, ct.parts, c0, c1, wrow, wrows, qs[w]);
 }
 
-// Joins paged_tile's parts: HD / 4 threads a row.
+// Joins tile_block's parts: HD / 4 threads a row.  Bound by latency: 5 us after the
+// prompts above, 7 after the mixed batch, with split_merge's share.  (Eight parts'
+// loads in flight at once: no difference.)
 template <class XT, class CT, int HD>
 __device__ __forceinline__ void tile_merge(const TileArgs &ta, uint32_t block) {
     constexpr int T = HD / 4, R = 256 / T;

@@ -6,9 +6,10 @@
 // A row's prefix is found without a sort.  A histogram of the distance to the
 // largest logit, of element counts (top-k) or weights (top-p), names the bin the
 // border lies in.  If at most kCand elements lie in it and above it, they finish
-// the row among themselves in LDS: each counts those before it.  Else those of
-// the bin alone place the border, and the whole row is summed once more.  Bins of
-// more elements (equal logits, high temperatures) are narrowed by key first.
+// the row among themselves in LDS, where the bins' sums leave each only its own
+// bin's to count.  Else those of the bin alone place the border, and the whole row
+// is summed once more.  Bins of more elements (equal logits, high temperatures) are
+// narrowed by key first.
 //
 // Weights exp((l - max) / T) are summed as 64-bit integers of 2^-43: sums are
 // exact and do not depend on their order, and a token on the border of the
@@ -16,7 +17,12 @@
 // in double precision from a table of 2^(j / 64) and a polynomial of degree 5 on
 // +-1/128 (its error, (ln 2 / 128)^6 / 720, is below 2^-54).
 //
-// One block of 1024 threads takes a row, in two to four passes over it.
+// One block of 1024 threads takes a row, in two to four passes over it.  Bound by
+// the row's one CU: of 64 rows of 32000 a pass takes 5.7 us for the maximum, 13.6
+// with the weights (about 35 operations in double precision each), 10 with counts;
+// of 256 rows of 100000 16.7 (6.1 TB/s, memory), 37, 20.  us with all filters: 18 for
+// one row of 32000, of which 5 are launch and latency; 36 for 64 rows, each its own
+// settings; 121 for 256 rows of 100000 with top_p.
 #include <algorithm>
 #include <cstring>
 #include <new>
