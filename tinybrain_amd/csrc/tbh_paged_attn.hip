@@ -688,17 +688,18 @@ __global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
     split_block<XT, CT, HD>(sa, blockIdx.x, lds);
 }
 
-// Joins split_block's parts: a block per unit and row, HD / 4 threads across the
-// head, the parts dealt over the rest.  Every wave holds the parts' factors, one
-// per lane.  Bound by latency: 4.0 us after a row over 4096 positions, 6.0 after 64
-// requests of up to 8192.
+// Joins split_block's parts: a wave per unit and row, HD / 4 lanes across the head,
+// the parts dealt over its groups of lanes, four loads each in flight.  Lane i holds
+// part i's factor.  Bound by latency: 4.1 us after a row over 4096 positions, 4.8
+// after 64 requests of up to 8192 (5.9 with a block per row).
 template <class XT, int HD>
-__device__ __forceinline__ void split_merge(const SplitArgs &sa, uint32_t block, f32x4 *lds) {
-    constexpr int T = HD / 4, G = 256 / T;
-    f32x4 (*red)[T] = (f32x4 (*)[T])lds;
+__device__ __forceinline__ void split_merge(const SplitArgs &sa, uint32_t block) {
+    constexpr int T = HD / 4, G = 64 / T;
     const PagedArgs &a = sa.a;
-    const int tid = threadIdx.x, lane = tid & 63, d4 = tid % T, sg = tid / T;
-    const uint32_t rr = block % (uint32_t)sa.slots, unit = block / (uint32_t)sa.slots;
+    const int lane = threadIdx.x & 63, d4 = lane % T, sg = lane / T;
+    const uint32_t index = block * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t rr = index % (uint32_t)sa.slots, unit = index / (uint32_t)sa.slots;
+    if (unit >= (uint32_t)sa.units) return;
     const int64_t at0 = (int64_t)unit * sa.splits * sa.slots + rr;
     const float2 mine = sa.ml[at0 + (int64_t)min(lane, sa.splits - 1) * sa.slots];   // before the request is known
     Group gr;
@@ -721,28 +722,33 @@ __device__ __forceinline__ void split_merge(const SplitArgs &sa, uint32_t block,
     const float l = wave::sum(part && f != 0.0f ? f * mine.y : 0.0f);
     const bool any = __any(part && mine.y > 0.0f);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < ct.parts; s0 += G) {
-        const int s = s0 + sg;
-        const float fs = __shfl(f, min(s, 63));
-        if (s < ct.parts && sg < G) o += fs * *(const f32x4 *)(po + (int64_t)s * sa.slots * HD);
-    }
-    if (sg < G) red[sg][d4] = o;
-    __syncthreads();
-    if (sg != 0) return;
-    f32x4 v = red[0][d4];
+    for (int s0 = 0; s0 < ct.parts; s0 += 4 * G) {
+        f32x4 v[4];
 #pragma unroll
-    for (int i = 1; i < G; ++i) v += red[i][d4];
+        for (int i = 0; i < 4; ++i)
+            v[i] = *(const f32x4 *)(po + (int64_t)min(s0 + G * i + sg, ct.parts - 1) * sa.slots * HD);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + G * i + sg;
+            const float fs = __shfl(f, min(s, 63));
+            if (s < ct.parts && sg < G) o += fs * v[i];
+        }
+    }
+#pragma unroll
+    for (int w = G / 2; w; w /= 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_down(o[i], w * T);
+    if (sg != 0) return;
     const int32_t row = gr.row0 + rr;
     XT *out = (XT *)a.out + (int64_t)(gr.q.first + row / a.rep) * a.out_stride +
               (int64_t)(gr.kvh * a.rep + row % a.rep) * HD + 4 * d4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = (XT)(mm == -INFINITY ? (any ? NAN : 0.0f) : v[i] / l);
+    for (int i = 0; i < 4; ++i) out[i] = (XT)(mm == -INFINITY ? (any ? NAN : 0.0f) : o[i] / l);
 }
 
 template <class XT, int HD>
 __global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa) {
-    __shared__ f32x4 red[256];
-    split_merge<XT, HD>(sa, blockIdx.x, red);
+    split_merge<XT, HD>(sa, blockIdx.x);
 }
 
 constexpr int64_t kMaxSplits = 64;   // a lane each in split_merge
@@ -1264,7 +1270,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
 }
 
 // Joins tile_block's parts: HD / 4 threads a row.  Bound by latency: 5 us after the
-// prompts above, 7 after the mixed batch, with split_merge's share.  (Eight parts'
+// prompts above and after the mixed batch, with split_merge's share.  (Eight parts'
 // loads in flight at once: no difference.)
 template <class XT, class CT, int HD>
 __device__ __forceinline__ void tile_merge(const TileArgs &ta, uint32_t block) {
@@ -1317,9 +1323,8 @@ __global__ __launch_bounds__(256, 2) void paged_both(const TileArgs ta, const Sp
 
 template <class XT, class CT, int HD>
 __global__ __launch_bounds__(256) void paged_both_merge(const TileArgs ta, const SplitArgs sa) {
-    __shared__ f32x4 red[256];
     if (blockIdx.x < ta.merge_blocks) tile_merge<XT, CT, HD>(ta, blockIdx.x);
-    else split_merge<XT, HD>(sa, blockIdx.x - ta.merge_blocks, red);
+    else split_merge<XT, HD>(sa, blockIdx.x - ta.merge_blocks);
 }
 
 // Parts of paged_both's tiles: enough to fill two blocks per CU twice over, of at
@@ -1366,7 +1371,7 @@ hipError_t launch_matrix(tbh_device *dev, const PagedArgs &a, int64_t query, int
     }
     const int64_t tile_blocks = tiles ? (int64_t)ta.units * ta.splits : 0, split_blocks = (int64_t)sa.units * sa.splits;
     const int64_t tile_merges = tiles && ta.splits > 1 ? (int64_t)ta.units * (R * HD / 1024) : 0;
-    const int64_t split_merges = sa.splits > 1 ? (int64_t)sa.units * sa.slots : 0;
+    const int64_t split_merges = sa.splits > 1 ? ((int64_t)sa.units * sa.slots + 3) / 4 : 0;
     if (std::max(tile_blocks + split_blocks, tile_merges + split_merges) > INT32_MAX || sa.units == INT32_MAX ||
         ta.units == INT32_MAX)
         return hipErrorInvalidValue;
