@@ -755,7 +755,8 @@ constexpr int64_t kMaxSplits = 64;   // a lane each in split_merge
 
 // Positions a part of split_block has at least, for `units` units: enough blocks
 // to fill the chip, parts no longer than 1024 (a batch's longest request would
-// else end long after the others) and no shorter than 128 (a step per wave).
+// else end long after the others: 64 requests of 109 .. 7927 positions 111 us, 126
+// without, 159 with 256) and no shorter than 128 (a step per wave).
 int32_t split_least(int64_t units, int64_t context, int64_t cus) {
     const int64_t parts = std::max<int64_t>(1, 4 * cus / std::max<int64_t>(units, 1));
     const int64_t even = (context + parts - 1) / parts;
@@ -785,24 +786,26 @@ SplitArgs plan_split(const PagedArgs &a, int64_t query, int64_t context, bool ti
 
 struct TileArgs {
     PagedArgs a;
-    int32_t units;         // (kTileRows rows, key/value head) pairs
+    int32_t units;         // (ROWS rows, key/value head) pairs
     int32_t splits, least; // see cut
     bool pair_up;          // see find_group
     bool qvec;             // q rows are 16-byte aligned
     uint32_t blocks, merge_blocks;   // of the launch that takes split_block's work too
-    float2 *ml;            // partials [unit][split][kTileRows]: (max, sum)
-    float *po;             // and sums of p v, [unit][split][kTileRows][head_dim]
+    float2 *ml;            // partials [unit][split][ROWS]: (max, sum)
+    float *po;             // and sums of p v, [unit][split][ROWS][head_dim]
 };
 
-// Rows of a tile: two column groups of 16 per wave for bf16 rows over a bf16 cache;
-// one where the matrix work per LDS read is more (three pieces of fp32 rows, the
-// fp32 matrix instruction).
-template <class XT, class CT>
-constexpr int kTileRows = sizeof(XT) + sizeof(CT) == 4 ? 128 : 64;
+// Rows of a tile (ROWS): 64, 16 a wave; 128, two column groups a wave, for bf16 rows
+// over a bf16 cache whose tiles fill the chip even so, heads of 64 twice over: half
+// the LDS reads per product (us with 128 and with 64, 32 heads on 8 of 128: 2048 rows
+// over 4096 119 and 143, 1000 over 1000 47 and 28; on 4 of 64: 2048 over 2048 47 and 39,
+// 8192 over 8192 351 and 393).  With more matrix work per LDS read (three pieces of fp32
+// rows: 301 and 313; the fp32 instruction) 64 always.
+constexpr int kWideRows = 128;
 
 // As in split_block: the wave's rows one at a time, where one may have met an inf
 // or NaN that it does not see.
-template <class XT, class CT, int HD>
+template <class XT, class CT, int HD, int ROWS>
 __device__ __forceinline__ void rows_apart(const TileArgs &ta, const Group &gr, uint32_t unit, uint32_t split,
                                            int32_t parts, int32_t c0, int32_t c1, int32_t wrow, int32_t wrows,
                                            float *qs) {
@@ -815,14 +818,14 @@ __device__ __forceinline__ void rows_apart(const TileArgs &ta, const Group &gr, 
         if (parts == 1) {
             store_row<XT>(a, gr.q.first + tt, head, x);
         } else {
-            const int64_t r = ((int64_t)unit * ta.splits + split) * kTileRows<XT, CT> + wrow + rr - gr.row0;
+            const int64_t r = ((int64_t)unit * ta.splits + split) * ROWS + wrow + rr - gr.row0;
             if (lane == 0) ta.ml[r] = x.m == -INFINITY ? float2{x.m, x.seen ? 1.0f : 0.0f} : float2{x.m, x.l};
             for (int i = 0; 64 * i + lane < HD; ++i) ta.po[r * HD + 64 * i + lane] = x.o[i];
         }
     }
 }
 
-// Many rows per request over a bf16 cache.  A block takes kTileRows rows of one
+// Many rows per request over a bf16 cache.  A block takes ROWS rows of one
 // key/value head and one part of the positions: four waves of 16 or 32 rows,
 // tiles of 64 positions in two LDS buffers, each wave copying 16 positions of the
 // next tile straight to LDS while this one is multiplied, one barrier a tile.
@@ -844,9 +847,9 @@ struct TileLds {
     float qs[4][HD];
 };
 
-template <class XT, int HD>
+template <class XT, int HD, int ROWS>
 __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, TileLds<HD> &lds, __bf16) {
-    constexpr int NP = sizeof(XT) == 4 ? 3 : 1, ROWS = kTileRows<XT, __bf16>, CG = ROWS / 64;
+    constexpr int NP = sizeof(XT) == 4 ? 3 : 1, CG = ROWS / 64;
     constexpr int NJ = HD / 32, ND = HD / 16;
     constexpr int CR = HD / 8, NL = CR / 4;                // 16-byte pieces per row, copies per wave and tile
     constexpr int KD = 16 / CR, VD2 = 8 / ND;              // rows per 256 bytes of LDS, as 16- and 32-byte pieces count
@@ -1076,7 +1079,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
         }
     }
     if (low + 1 >= c1 || !__any(odd)) return;
-    rows_apart<XT, __bf16, HD>(ta, gr, unit, split, ct.parts, c0, c1, wrow, wrows, qs[w]);
+    rows_apart<XT, __bf16, HD, ROWS>(ta, gr, unit, split, ct.parts, c0, c1, wrow, wrows, qs[w]);
 }
 
 // Many rows per request over an fp32 cache, as above but on the fp32 matrix
@@ -1089,9 +1092,10 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
 // they join the running sums: an eighth of the roundings.  31 single tokens and a
 // chunk of 333, 32 heads on 4 of 64, fp32: 25 us with split_block's share, 7 tiles of
 // 32 positions a block, each a wait and 64 matrix instructions of 32 cycles.
-template <class XT, int HD>
+template <class XT, int HD, int ROWS>
 __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, TileLds<HD> &lds, float) {
-    constexpr int ROWS = kTileRows<XT, float>, POS = 32;
+    static_assert(ROWS == 64, "16 rows a wave");
+    constexpr int POS = 32;
     constexpr int NJ = HD / 16, NH = HD / 64;
     constexpr int CR = HD / 4, NL = 8 * CR / 64;           // 16-byte pieces per row, copies per wave and tile
     float (*kl)[POS * HD] = (float (*)[POS * HD])lds.k, (*vl)[POS * HD] = (float (*)[POS * HD])lds.v;
@@ -1266,28 +1270,28 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
             }
     }
     if (low + 1 >= c1 || !__any(odd)) return;
-    rows_apart<XT, float, HD>(ta, gr, unit, split, ct.parts, c0, c1, wrow, wrows, qs[w]);
+    rows_apart<XT, float, HD, ROWS>(ta, gr, unit, split, ct.parts, c0, c1, wrow, wrows, qs[w]);
 }
 
 // Joins tile_block's parts: HD / 4 threads a row.  Bound by latency: 5 us after the
 // prompts above and after the mixed batch, with split_merge's share.  (Eight parts'
 // loads in flight at once: no difference.)
-template <class XT, class CT, int HD>
+template <class XT, int HD, int ROWS>
 __device__ __forceinline__ void tile_merge(const TileArgs &ta, uint32_t block) {
     constexpr int T = HD / 4, R = 256 / T;
     const PagedArgs &a = ta.a;
-    const uint32_t unit = block / (kTileRows<XT, CT> / R);
-    const int rr = (int)(block % (kTileRows<XT, CT> / R)) * R + threadIdx.x / T, d4 = threadIdx.x % T;
+    const uint32_t unit = block / (ROWS / R);
+    const int rr = (int)(block % (ROWS / R)) * R + threadIdx.x / T, d4 = threadIdx.x % T;
     Group gr;
-    if (!find_group<kTileRows<XT, CT>>(a, unit, 16, ta.pair_up, gr)) return;
-    set_rows<kTileRows<XT, CT>>(a, gr, gr.row0);
+    if (!find_group<ROWS>(a, unit, 16, ta.pair_up, gr)) return;
+    set_rows<ROWS>(a, gr, gr.row0);
     const Cut ct = cut(gr.len, ta.splits, ta.least);
     if (ct.parts == 1 || rr >= gr.rows) return;
-    const int64_t at0 = (int64_t)unit * ta.splits * kTileRows<XT, CT> + rr;
+    const int64_t at0 = (int64_t)unit * ta.splits * ROWS + rr;
     float mm = -INFINITY, any = 0.0f;
 #pragma unroll 4
     for (int s = 0; s < ct.parts; ++s) {
-        const float2 x = ta.ml[at0 + (int64_t)s * kTileRows<XT, CT>];
+        const float2 x = ta.ml[at0 + (int64_t)s * ROWS];
         mm = fmaxf(mm, x.x);
         any = fmaxf(any, x.y);
     }
@@ -1295,7 +1299,7 @@ __device__ __forceinline__ void tile_merge(const TileArgs &ta, uint32_t block) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int s = 0; s < ct.parts; ++s) {
-        const int64_t r = at0 + (int64_t)s * kTileRows<XT, CT>;
+        const int64_t r = at0 + (int64_t)s * ROWS;
         const float2 x = ta.ml[r];
         const float f = x.x == -INFINITY ? 0.0f : exp2_fast(x.x - mm);
         if (x.x != -INFINITY) l += f * x.y;
@@ -1311,50 +1315,74 @@ __device__ __forceinline__ void tile_merge(const TileArgs &ta, uint32_t block) {
 // One launch for a batch of chunks and single tokens: the tiles' blocks, then those
 // of the requests with few rows, which fill in beside them (31 tokens and a
 // 333-token chunk over fp32: 48 us in two launches and two merges, 35 so); likewise their merges.
-template <class XT, class CT, int HD>
+template <class XT, class CT, int HD, int ROWS>
 __global__ __launch_bounds__(256, 2) void paged_both(const TileArgs ta, const SplitArgs sa) {
     __shared__ __attribute__((aligned(256))) union {
         TileLds<HD> tile;
         SplitLds<HD> split;
     } lds;
-    if (blockIdx.x < ta.blocks) tile_block<XT, HD>(ta, blockIdx.x, lds.tile, CT{});
+    if (blockIdx.x < ta.blocks) tile_block<XT, HD, ROWS>(ta, blockIdx.x, lds.tile, CT{});
     else split_block<XT, CT, HD>(sa, blockIdx.x - ta.blocks, lds.split);
 }
 
-template <class XT, class CT, int HD>
+template <class XT, int HD, int ROWS>
 __global__ __launch_bounds__(256) void paged_both_merge(const TileArgs ta, const SplitArgs sa) {
-    if (blockIdx.x < ta.merge_blocks) tile_merge<XT, CT, HD>(ta, blockIdx.x);
+    if (blockIdx.x < ta.merge_blocks) tile_merge<XT, HD, ROWS>(ta, blockIdx.x);
     else split_merge<XT, HD>(sa, blockIdx.x - ta.merge_blocks);
 }
 
-// Parts of paged_both's tiles: enough to fill two blocks per CU twice over, of at
-// least 512 positions.  (2048 rows over 4096, which fill the chip with whole
-// contexts: 168 us, 203 in two parts, 244 in four: partials of fp32 rows cost
-// more than the evener blocks gain.)
-TileArgs plan_tile(const PagedArgs &a, int64_t context, int64_t tile_rows, size_t elem, int64_t cus) {
+// Whether so many tiles fill two blocks per CU, nine in ten of them.
+bool fills(int64_t tiles, int64_t cus) { return 10 * tiles >= 9 * 2 * cus; }
+
+// Parts of tile_block's tiles: none where they fill the chip (2048 rows over 4096
+// positions: 168 us, 203 in two parts, 244 in four: partials of fp32 rows cost more than
+// evener blocks gain), else enough to fill it twice over, of at least 256 positions (a
+// chunk of 8 rows over 4096: 16 us, 71 without; 600 over 4000 81, 89 without).
+TileArgs plan_tile(const PagedArgs &a, int64_t query, int64_t context, int64_t tile_rows, size_t elem, int64_t cus) {
     TileArgs ta{};
     ta.a = a;
     ta.qvec = aligned(a.q, 16) && (a.q_stride * (int64_t)elem) % 16 == 0;
     const int64_t rows = a.tokens * a.rep;
     const int64_t units = (rows / tile_rows + std::min<int64_t>(a.requests, rows / 17 + 1)) * (int64_t)a.nkv;
     ta.units = (int32_t)std::min<int64_t>(units, INT32_MAX);
-    const int64_t full = std::max<int64_t>(1, rows / tile_rows * a.nkv);   // without the requests' last, partial tiles
-    const int64_t parts = 10 * full >= 9 * 2 * cus ? 1 : std::max<int64_t>(1, 4 * cus / full);
+    // How many there are: chunks alike, as the step's bounds tell, have a last, partial
+    // tile each (64 chunks of 5 rows over 1000: 67 us with parts for as many tiles as the
+    // rows would fill, 50 so); else those that the rows fill, as the rest may be single tokens.
+    const bool alike = 2 * a.tokens >= a.requests * query;
+    const int64_t tiles = alike ? a.requests * ((query * a.rep + tile_rows - 1) / tile_rows) : rows / tile_rows;
+    const int64_t full = std::max<int64_t>(1, tiles * a.nkv);
+    const int64_t parts = fills(full, cus) ? 1 : std::max<int64_t>(1, 4 * cus / full);
     ta.least = 256;
     ta.splits = (int32_t)std::max<int64_t>(1, std::min({parts, (context + ta.least - 1) / ta.least, kMaxSplits}));
-    // two blocks share a CU: all run at once, or the longest have to come first
-    ta.pair_up = rows / tile_rows * a.nkv <= 2 * cus;
+    // two blocks share a CU: all run at once, or the longest have to come first (512 blocks
+    // of 2048 rows over 4096: 119 us, 121 without; over 8192: 244, 250)
+    ta.pair_up = full <= 2 * cus;
     return ta;
+}
+
+template <class XT, class CT, int HD, int ROWS>
+hipError_t launch_both(const TileArgs &ta, const SplitArgs &sa, int64_t split_blocks, int64_t split_merges, hipStream_t s) {
+    hipLaunchKernelGGL((paged_both<XT, CT, HD, ROWS>), dim3((unsigned)(ta.blocks + split_blocks)), dim3(256), 0, s, ta, sa);
+    const hipError_t e = hipGetLastError();
+    const int64_t merges = ta.merge_blocks + split_merges;
+    if (e != hipSuccess || merges == 0) return e;
+    hipLaunchKernelGGL((paged_both_merge<XT, HD, ROWS>), dim3((unsigned)merges), dim3(256), 0, s, ta, sa);
+    return hipGetLastError();
 }
 
 template <class XT, class CT, int HD>
 hipError_t launch_matrix(tbh_device *dev, const PagedArgs &a, int64_t query, int64_t context, hipStream_t s) {
-    constexpr int R = kTileRows<XT, CT>;
     const int64_t cus = std::max(1, dev->cu_count);
+    // More than one group of 16 rows: tiles, or else groups apart.  us, bf16 throughout, 32
+    // heads on 8 of 128: 8 chunks of 5 rows over 2000 positions 24 in tiles and 29 in groups,
+    // 64 of 5 over 1000 50 and 56, 8 of 16 over 2000 27 and 39; fp32, 32 on 4 of 64: a chunk
+    // of 8 over 4096 23 and 21, 8 of 16 over 2000 34 and 46.
     const bool tiles = (HD == 64 || HD == 128) && query * a.rep > 16;
     SplitArgs sa = plan_split(a, query, context, tiles, sizeof(XT), cus);
     TileArgs ta{};
-    if (tiles) ta = plan_tile(a, context, R, sizeof(XT), cus);
+    int64_t R = 64;
+    if (sizeof(XT) + sizeof(CT) == 4 && fills(a.tokens * a.rep / kWideRows * a.nkv * HD / 128, cus)) R = kWideRows;
+    if (tiles) ta = plan_tile(a, query, context, R, sizeof(XT), cus);
     const int64_t tile_rows = tiles && ta.splits > 1 ? (int64_t)ta.units * ta.splits * R : 0;
     const int64_t split_rows = sa.splits > 1 ? (int64_t)sa.units * sa.splits * sa.slots : 0;
     if (tile_rows + split_rows > 0) {
@@ -1379,13 +1407,9 @@ hipError_t launch_matrix(tbh_device *dev, const PagedArgs &a, int64_t query, int
     ta.merge_blocks = (uint32_t)tile_merges;
     if constexpr (HD == 64 || HD == 128) {
         if (tiles) {
-            hipLaunchKernelGGL((paged_both<XT, CT, HD>), dim3((unsigned)(tile_blocks + split_blocks)), dim3(256), 0, s, ta,
-                               sa);
-            const hipError_t e = hipGetLastError();
-            if (e != hipSuccess || tile_merges + split_merges == 0) return e;
-            hipLaunchKernelGGL((paged_both_merge<XT, CT, HD>), dim3((unsigned)(tile_merges + split_merges)), dim3(256), 0,
-                               s, ta, sa);
-            return hipGetLastError();
+            if constexpr (sizeof(XT) + sizeof(CT) == 4)
+                if (R == kWideRows) return launch_both<XT, CT, HD, kWideRows>(ta, sa, split_blocks, split_merges, s);
+            return launch_both<XT, CT, HD, 64>(ta, sa, split_blocks, split_merges, s);
         }
     }
     hipLaunchKernelGGL((paged_split<XT, CT, HD>), dim3((unsigned)split_blocks), dim3(256), 0, s, sa);
