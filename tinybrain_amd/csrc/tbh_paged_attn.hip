@@ -1349,7 +1349,8 @@ TileArgs plan_tile(const PagedArgs &a, int64_t query, int64_t context, int64_t t
     // tile each (64 chunks of 5 rows over 1000: 67 us with parts for as many tiles as the
     // rows would fill, 50 so); else those that the rows fill, as the rest may be single tokens.
     const bool alike = 2 * a.tokens >= a.requests * query;
-    const int64_t tiles = alike ? a.requests * ((query * a.rep + tile_rows - 1) / tile_rows) : rows / tile_rows;
+    const int64_t each = (rows + a.requests - 1) / a.requests;   // rows of a request, on average
+    const int64_t tiles = alike ? a.requests * ((each + tile_rows - 1) / tile_rows) : rows / tile_rows;
     const int64_t full = std::max<int64_t>(1, tiles * a.nkv);
     const int64_t parts = fills(full, cus) ? 1 : std::max<int64_t>(1, 4 * cus / full);
     ta.least = 256;
