@@ -1314,7 +1314,8 @@ __device__ __forceinline__ void tile_merge(const TileArgs &ta, uint32_t block) {
 
 // One launch for a batch of chunks and single tokens: the tiles' blocks, then those
 // of the requests with few rows, which fill in beside them (31 tokens and a
-// 333-token chunk over fp32: 48 us in two launches and two merges, 35 so); likewise their merges.
+// 333-token chunk over fp32: 48 us in two launches and two merges, 35 when joined, 29 now); likewise
+// their merges.
 template <class XT, class CT, int HD, int ROWS>
 __global__ __launch_bounds__(256, 2) void paged_both(const TileArgs ta, const SplitArgs sa) {
     __shared__ __attribute__((aligned(256))) union {
@@ -1335,7 +1336,7 @@ __global__ __launch_bounds__(256) void paged_both_merge(const TileArgs ta, const
 bool fills(int64_t tiles, int64_t cus) { return 10 * tiles >= 9 * 2 * cus; }
 
 // Parts of tile_block's tiles: none where they fill the chip (2048 rows over 4096
-// positions: 168 us, 203 in two parts, 244 in four: partials of fp32 rows cost more than
+// positions, when they took 168 us: 203 in two parts, 244 in four: partials of fp32 rows cost more than
 // evener blocks gain), else enough to fill it twice over, of at least 256 positions (a
 // chunk of 8 rows over 4096: 16 us, 71 without; 600 over 4000 81, 89 without).
 TileArgs plan_tile(const PagedArgs &a, int64_t query, int64_t context, int64_t tile_rows, size_t elem, int64_t cus) {
