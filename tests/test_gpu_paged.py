@@ -354,6 +354,53 @@ def test_attention_extreme_scores(torch, backend, x, cache):
     assert bad[66:, :2].all() and bad[66:, 2:, 3].all() and not bad[66:, 2:, :3].any() and not bad[66:, 2:, 4:].any()
 
 
+def _attention64(torch, c, hd):
+    """The formula in float64 on the device, a head at a time: (out, sum p |v|,
+    bound of fp32 arithmetic), rows x heads x hd."""
+    q = c["q"].double().reshape(c["q"].shape[0], -1, hd)
+    rep = q.shape[1] // c["keys"].shape[1]
+    out, mass, bound = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(q)
+    for b, n in enumerate(c["context"]):
+        lo, hi, bs = int(c["start"][b]), int(c["start"][b + 1]), c["keys"].shape[2]
+        pages = torch.tensor(c["table"][b, :P.ceil_div(int(n), bs)].astype(np.int64), device="cuda")
+        see = torch.arange(int(n), device="cuda")[None] <= torch.arange(hi - lo, device="cuda")[:, None] + int(n) - (hi - lo)
+        for h in range(q.shape[1]):
+            k = c["keys"][pages, h // rep].reshape(-1, hd)[:int(n)].double()
+            v = c["values"][pages, h // rep].reshape(-1, hd)[:int(n)].double()
+            x = q[lo:hi, h]
+            s = (x @ k.T) * hd ** -0.5
+            top = s.masked_fill(~see, -float("inf")).max(1, keepdim=True).values
+            p = torch.where(see, torch.exp(s - top), torch.zeros_like(s))
+            p /= p.sum(1, keepdim=True)
+            e = ((hd + 2) * U32 * (x.abs() @ k.abs().T) * hd ** -0.5 + U32 * (s - top).abs()) * see
+            out[lo:hi, h], mass[lo:hi, h] = p @ v, p @ v.abs()
+            bound[lo:hi, h] = (2 * e.max(1, keepdim=True).values + (int(n) + 8) * U32) * mass[lo:hi, h]
+    return out.reshape(c["q"].shape), mass.reshape(c["q"].shape), bound.reshape(c["q"].shape)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 16, 128), (64, 32, 64)])
+def test_attention_of_a_long_chunk(torch, backend, nh, nkv, hd):
+    # enough rows for the widest tiles, beside a short chunk and a single token
+    lens = [(1, 300), (3800 * nkv // nh, 3900), (70, 90)]
+    c = _attention_case(torch, 50, lens, nh, nkv, hd, 16, "bfloat16", "bfloat16")
+    want, mass, bound = _attention64(torch, c, hd)
+    # the result rounded once, and each p: by U16 of sum p |v - out|, at most mass + |out|
+    tol = bound + (U32 + 2 * U16) * want.abs() + U16 * mass
+    out = torch.full(c["q"].shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    got = _run_attention(torch, backend, c, out=out).double()
+    rows = int(c["start"][-1])
+    assert bool(((got - want).abs() <= tol)[:rows].all()) and bool((got[rows:] == 7.0).all())
+    # an inf that only the chunk's last rows see
+    p = 3850
+    c["values"][int(c["table"][1, p // 16]), nkv - 1, p % 16, 5] = float("inf")
+    got = _run_attention(torch, backend, c, out=out).double()
+    first = int(c["start"][2]) - (3900 - p)                  # the first row that sees it
+    at = [h * hd + 5 for h in range(nh - nh // nkv, nh)]
+    assert bool((got[first:int(c["start"][2])][:, at] == float("inf")).all())
+    got[first:int(c["start"][2]), at] = want[first:int(c["start"][2]), at]
+    assert bool(((got - want).abs() <= tol)[:rows].all())
+
+
 def test_attention_past_32_bits(torch, backend):
     # blocks whose elements lie beyond 2^31 (and bytes beyond 2^32)
     nkv, bs, hd = 8, 16, 128

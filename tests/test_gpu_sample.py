@@ -82,6 +82,17 @@ def test_sample_large_vocab_and_batch(backend):
            p=rng.choice([0.4, 0.9, 1], 300), m=rng.choice([0, 0.1], 300))
 
 
+@pytest.mark.parametrize("std", [0.02, 0.3, 2.0])
+def test_sample_around_a_thousand_candidates(backend, std):
+    # kept sets below, at and above what a block holds, in few bins and in many
+    rng = np.random.default_rng(6)
+    k = np.array([0, 64, 500, 511, 513, 900, 1000, 1023, 1024, 1025, 1500, 2999] * 4)
+    x = (rng.normal(size=(len(k), 2999)) * std).astype(np.float32)
+    x[1::2, ::3] = x[1::2, :1]                         # a third of every other row is equal
+    _check(backend, x, rng.random(len(k)), t=np.repeat([0.7, 1.0, 1.0, 1.3], 12), k=k,
+           p=np.repeat([1.0, 0.3, 0.9, 0.35], 12), m=np.tile([0, 0, 0.2], 16))
+
+
 def test_sample_device_rows(backend):
     # strided rows and rows that start off 16 bytes give the host call's tokens
     import torch
