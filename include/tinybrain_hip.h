@@ -223,7 +223,8 @@ tbh_status tbh_matmul(tbh_device *dev, const float *x, int64_t M, int64_t K,
                       const tbh_weight *w, float *y);
 
 /* Same product on device pointers, enqueued on `stream` (a hipStream_t of the
- * weight's device; NULL = the null stream).  Returns after the launch.
+ * weight's device; NULL = the null stream).  Returns after the launch.  Host
+ * threads may call on one stream: the launches of a call stay together there.
  * Launches that split K (matrix-core GEMV, MFMA GEMM) keep their partial sums,
  * and the MFMA GEMM its 16-bit pieces of fp32 x (4 or 6 bytes per element, up
  * to 128 MiB at a time: longer x is taken in even parts) and their exponents
@@ -464,7 +465,8 @@ tbh_status tbh_attention_device(tbh_device *dev, const tbh_attention_shape *shap
  *   tbh_sample_device           logits -> tokens
  * All of them take device pointers, are enqueued on `stream` and return after
  * the launch; lengths, tables and slots are read on the device, so a captured
- * step replays with new ones.  Device-side values out of range are never
+ * step replays with new ones.  Host threads may call on one stream: the
+ * launches of a call stay together there.  Device-side values out of range are never
  * followed: a block id outside the cache holds nothing, a slot outside it is
  * not written, lengths are clamped to what the table and the rows can hold.
  *

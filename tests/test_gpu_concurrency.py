@@ -112,3 +112,54 @@ def test_threads_share_a_device():
         _run_threads(own_weights)
     finally:
         b.close()
+
+
+def test_threads_share_a_stream():
+    # Every thread enqueues on one stream: calls that keep partial results in its
+    # workspace between launches (attention in parts, split K) and a step's plan.
+    import torch
+
+    rng = np.random.default_rng(11)
+    b, bs, nkv, hd = T.HIPBackend(0), 16, 2, 64
+
+    def ints(a):
+        return torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
+
+    keys, values = torch.randn(2, 700, nkv, bs, hd, device="cuda")
+    work = []
+    for i, lens in enumerate([[(1, 5000)], [(1, 900), (40, 700), (1, 2100)], [(1, 300)] * 6, [(130, 1500)]]):
+        held = [-(-c // bs) for _, c in lens]
+        order = rng.permutation(700)
+        table = np.full((len(lens), max(held)), -1)
+        for r, h in enumerate(held):
+            table[r, :h], order = order[:h], order[h:]
+        start = np.concatenate([[0], np.cumsum([n for n, _ in lens])])
+        q = torch.randn(int(start[-1]), 8 * hd, device="cuda")
+        args = [ints(a) for a in (table, start, [c for _, c in lens])]
+        work.append(lambda q=q, a=args: b.paged_attention_device(q, keys, values, *a, 8))
+    q = torch.randn(1, 8 * hd, device="cuda")
+    k, v = torch.randn(2, 3000, nkv * hd, device="cuda")
+    work.append(lambda: b.attention_device(q, k, v, None, hd, 8, nkv))
+    w, _ = _weights()[2]
+    w = T.DeviceWeight(b, w)
+    x = torch.randn(8, w.K, device="cuda")
+    work.append(lambda: b.matmul_device(x, w))
+    new, ctx = ints([3, 0, 4000, 1, 900]), ints([20, 5, 0, 77, 64])
+    tables, stack, height = ints(np.full((5, 300), -1)), ints(np.arange(600)), ints([600])
+    work.append(lambda: b.paged_plan_device(new, ctx, tables, stack, height, bs, 4904).slots)
+    try:
+        want = [f() for f in work]
+        torch.cuda.synchronize()
+
+        def body(t):
+            got = []
+            for r in range(10):
+                got += [((i + t + r) % len(work), work[(i + t + r) % len(work)]()) for i in range(len(work))]
+            torch.cuda.synchronize()
+            for i, y in got:
+                assert torch.equal(y, want[i]), (t, i)
+
+        _run_threads(body)
+    finally:
+        w.close()
+        b.close()

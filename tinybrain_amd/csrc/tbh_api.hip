@@ -936,6 +936,7 @@ tbh_status tbh_matmul_device(const tbh_weight *w, const float *x, int64_t M, int
     if (st != TBH_OK) return st;
     Scratch scr;
     scr.dev = w->dev;
+    const auto held = hold_launches(w->dev, (hipStream_t)stream);
     return matmul_enqueue(w, x, M, y, (hipStream_t)stream, scr);
 }
 
@@ -1163,6 +1164,7 @@ tbh_status tbh_matmul_bf16_device(const tbh_weight *w, const uint16_t *x, int64_
     if (st != TBH_OK) return st;
     Scratch scr;
     scr.dev = w->dev;
+    const auto held = hold_launches(w->dev, (hipStream_t)stream);
     hipError_t e = launch_prefill(*w, x, K, M, y, w->N, (hipStream_t)stream, scr);
     if (e != hipSuccess) return hip_error(e, "prefill kernel launch");
     return TBH_OK;

@@ -87,6 +87,7 @@ struct tbh_device {
     std::mutex ws_mu;
     std::vector<Workspace> workspaces;
     std::vector<void *> retired;
+    std::mutex launches[64];     // see hold_launches
 };
 
 struct tbh_weight {
@@ -245,6 +246,15 @@ hipError_t launch_split_sum(const float *part, int splits, float *y, int64_t n, 
 // until the device closes.  Returns nullptr when it would have to grow while
 // the stream is being captured into a graph, or when the allocation fails.
 void *stream_workspace(tbh_device *dev, hipStream_t s, size_t bytes);
+
+// Keeps a call's launches together on their stream: held by a call that passes
+// results from one launch to the next (in the stream's workspace, or a plan's
+// outputs) until its last is enqueued, so that another host thread's call on the
+// same stream comes before or after all of them.  Streams share 64 locks.
+inline std::unique_lock<std::mutex> hold_launches(tbh_device *dev, hipStream_t s) {
+    const uintptr_t h = (uintptr_t)s >> 6;
+    return std::unique_lock<std::mutex>(dev->launches[(h ^ h >> 6 ^ h >> 12) & 63]);
+}
 
 // Where a launch takes its scratch memory (split-K partial sums) from: the
 // per-stream workspace of `dev`, grown on demand, or a fixed buffer that is

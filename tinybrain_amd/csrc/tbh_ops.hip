@@ -1471,6 +1471,7 @@ tbh_status tbh_attention_device(tbh_device *dev, const tbh_attention_shape *shap
     a.v = v;
     a.mask = mask;
     a.out = out;
+    const auto held = hold_launches(dev, (hipStream_t)stream);
     hipError_t e = launch_attention(dev, a, (hipStream_t)stream);
     return e == hipSuccess ? TBH_OK : hip_error(e, "attention launch");
 }

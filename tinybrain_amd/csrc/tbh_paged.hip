@@ -362,6 +362,7 @@ tbh_status tbh_paged_plan_device(tbh_device *dev, const tbh_paged_layout *layout
     a.max_tokens = max_tokens;
     const hipStream_t s = (hipStream_t)stream;
     const bool solo = B <= kPlanThreads && max_tokens <= kSoloTokens;
+    const auto held = hold_launches(dev, s);
     hipLaunchKernelGGL(plan_rows, dim3(1), dim3(kPlanThreads), 0, s, a, solo);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && max_tokens > 0 && !solo) {

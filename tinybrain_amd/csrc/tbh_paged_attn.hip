@@ -1496,6 +1496,7 @@ tbh_status tbh_paged_attention_device(tbh_device *dev, const tbh_paged_layout *l
     const int64_t query = q.max_query_len ? std::min<int64_t>(q.max_query_len, q.tokens) : q.tokens;
     const int64_t table = (int64_t)layout->max_blocks * layout->block_size;
     const int64_t context = q.max_context_len ? std::min<int64_t>(q.max_context_len, table) : table;
+    const auto held = hold_launches(dev, s);
     hipError_t e;
     switch ((q.type == TBH_BF16) * 2 + (layout->type == TBH_BF16)) {
     case 0: e = launch_paged<float, float>(dev, a, query, context, s); break;
