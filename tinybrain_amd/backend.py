@@ -196,7 +196,7 @@ class HIPBackend:
         if x.dtype != torch.float32 or not x.is_contiguous() or not x.is_cuda:
             raise PreconditionFailure("x must be a contiguous float32 device tensor")
         if out is None:
-            out = torch.empty((x.shape[0], weight.N), dtype=torch.float32, device=x.device)
+            out = self._made(stream, torch.empty, (x.shape[0], weight.N), dtype=torch.float32, device=x.device)
         s = stream if stream is not None else torch.cuda.current_stream(x.device)
         _check(self._lib.tbh_matmul_device(weight.handle, x.data_ptr(), x.shape[0], x.shape[1],
                                            out.data_ptr(), ctypes.c_void_p(s.cuda_stream)))
@@ -235,7 +235,7 @@ class HIPBackend:
             if bias.dtype != torch.float32 or not bias.is_contiguous() or not bias.is_cuda:
                 raise PreconditionFailure("bias must be a contiguous float32 device tensor")
         if out is None:
-            out = torch.empty((x.shape[0], weight.N), dtype=torch.float32, device=x.device)
+            out = self._made(stream, torch.empty, (x.shape[0], weight.N), dtype=torch.float32, device=x.device)
         s = stream if stream is not None else torch.cuda.current_stream(x.device)
         _check(self._lib.tbh_linear_device(weight.handle, x.data_ptr(), x.shape[0], x.shape[1],
                                            None if bias is None else bias.data_ptr(), out.data_ptr(),
@@ -254,7 +254,7 @@ class HIPBackend:
         if x.dtype != torch.bfloat16 or not x.is_contiguous() or not x.is_cuda:
             raise PreconditionFailure("x must be a contiguous bfloat16 device tensor")
         if out is None:
-            out = torch.empty((x.shape[0], weight.N), dtype=torch.float32, device=x.device)
+            out = self._made(stream, torch.empty, (x.shape[0], weight.N), dtype=torch.float32, device=x.device)
         s = stream if stream is not None else torch.cuda.current_stream(x.device)
         _check(self._lib.tbh_matmul_bf16_device(weight.handle, x.data_ptr(), x.shape[0], x.shape[1],
                                                 out.data_ptr(), ctypes.c_void_p(s.cuda_stream)))
@@ -264,8 +264,8 @@ class HIPBackend:
         import torch
 
         if out is None:
-            out = torch.empty((weight.K, weight.N), dtype=torch.float32,
-                              device=torch.device("cuda", self.device))
+            out = self._made(stream, torch.empty, (weight.K, weight.N), dtype=torch.float32,
+                             device=torch.device("cuda", self.device))
         s = stream if stream is not None else torch.cuda.current_stream(out.device)
         _check(self._lib.tbh_dequantize_device(weight.handle, out.data_ptr(),
                                                ctypes.c_void_p(s.cuda_stream)))
@@ -345,6 +345,20 @@ class HIPBackend:
                                        v.ctypes.data, None if m is None else m.ctypes.data, out.ctypes.data))
         return out
 
+    def _made(self, stream, make, *args, **kw):
+        """A new tensor that `stream` writes, from that stream's own memory:
+        memory freed on torch's current stream may still be used by work that
+        is queued there.  Once freed it is kept until what the current stream
+        then has queued is done, as the caller may read it there."""
+        import torch
+
+        if stream is None or stream.cuda_stream == torch._C._cuda_getCurrentRawStream(self.device):
+            return make(*args, **kw)
+        with torch.cuda.stream(stream):
+            t = make(*args, **kw)
+        t.record_stream(torch.cuda.current_stream(self.device))
+        return t
+
     # device-resident variants: contiguous float32 torch tensors on this device
     def _stream(self, t, stream):
         import torch
@@ -363,7 +377,7 @@ class HIPBackend:
         import torch
 
         x = self._dev_tensor(x)
-        out = torch.empty_like(x) if out is None else self._dev_tensor(out)
+        out = self._made(stream, torch.empty_like, x) if out is None else self._dev_tensor(out)
         if x.numel():
             cols = x.shape[-1]
             _check(self._lib.tbh_softmax_device(self._dev, x.data_ptr(), x.numel() // cols, cols,
@@ -376,7 +390,7 @@ class HIPBackend:
         x, weight = self._dev_tensor(x), self._dev_tensor(weight)
         if x.dim() != 2 or weight.numel() != x.shape[1]:
             raise PreconditionFailure("rmsnorm: x [tokens, hidden] and weight [hidden]")
-        out = torch.empty_like(x) if out is None else self._dev_tensor(out)
+        out = self._made(stream, torch.empty_like, x) if out is None else self._dev_tensor(out)
         _check(self._lib.tbh_rmsnorm_device(self._dev, x.data_ptr(), x.shape[0], x.shape[1], weight.data_ptr(),
                                             float(eps), out.data_ptr(), self._stream(x, stream)))
         return out
@@ -385,7 +399,7 @@ class HIPBackend:
         import torch
 
         x = self._dev_tensor(x)
-        out = torch.empty_like(x) if out is None else self._dev_tensor(out)
+        out = self._made(stream, torch.empty_like, x) if out is None else self._dev_tensor(out)
         _check(self._lib.tbh_silu_device(self._dev, x.data_ptr(), x.numel(), out.data_ptr(),
                                          self._stream(x, stream)))
         return out
@@ -394,7 +408,7 @@ class HIPBackend:
         import torch
 
         x = self._dev_tensor(x)
-        out = torch.empty_like(x) if out is None else self._dev_tensor(out)
+        out = self._made(stream, torch.empty_like, x) if out is None else self._dev_tensor(out)
         _check(self._lib.tbh_gelu_device(self._dev, x.data_ptr(), x.numel(), out.data_ptr(),
                                          self._stream(x, stream)))
         return out
@@ -406,7 +420,7 @@ class HIPBackend:
         q, k, v = self._dev_tensor(query), self._dev_tensor(keys), self._dev_tensor(values)
         m = None if mask is None else self._dev_tensor(mask)
         sh = self._attention_shape(q, k, v, m, headDim, numHeads, numKVHeads)
-        out = torch.empty_like(q) if out is None else self._dev_tensor(out)
+        out = self._made(stream, torch.empty_like, q) if out is None else self._dev_tensor(out)
         _check(self._lib.tbh_attention_device(self._dev, ctypes.byref(sh), q.data_ptr(), k.data_ptr(),
                                               v.data_ptr(), None if m is None else m.data_ptr(),
                                               out.data_ptr(), self._stream(q, stream)))
@@ -437,8 +451,7 @@ class HIPBackend:
             raise PreconditionFailure("plan: lengths and block table must have one row per request")
         if maxTokens < 0:
             raise PreconditionFailure("plan: maxTokens must not be negative")
-        out = newLens.new_empty(3 * b + 2 + 2 * maxTokens)
-        self._made(out, stream)
+        out = self._made(stream, newLens.new_empty, 3 * b + 2 + 2 * maxTokens)
         start, granted, slots, positions, ctx, count = torch.split_with_sizes(
             out, (b + 1, b, maxTokens, maxTokens, b, 1))
         if contextOut is not None:
@@ -495,8 +508,7 @@ class HIPBackend:
             if rows != tokens or width % hd:
                 raise PreconditionFailure("append: q must be rows [tokens, heads * headDim]")
             if qOut is None:
-                qOut = torch.empty_like(q)
-                self._made(qOut, stream)
+                qOut = self._made(stream, torch.empty_like, q)
             else:
                 if self._row_shape(qOut) != (rows, width):
                     raise PreconditionFailure("append: qOut must be shaped like q")
@@ -532,8 +544,7 @@ class HIPBackend:
             raise PreconditionFailure("attention: block table and query starts must have one row per request")
         xt = self._paged_type(q)
         if out is None:
-            out = torch.empty_like(q)
-            self._made(out, stream)
+            out = self._made(stream, torch.empty_like, q)
         elif self._row_shape(out) != shape or out.dtype != q.dtype:
             raise PreconditionFailure("attention: out must be like the queries")
         try:
@@ -568,12 +579,6 @@ class HIPBackend:
         if len(shape) != 2 or t.get_device() != self.device or (shape[1] > 1 and t.stride(1) != 1):
             raise PreconditionFailure("expected rows on this device, contiguous along the last dimension")
         return shape
-
-    @staticmethod
-    def _made(t, stream) -> None:
-        """A result allocated on torch's current stream and written on `stream`."""
-        if stream is not None:
-            t.record_stream(stream)
 
     @staticmethod
     def _paged_type(t) -> int:
@@ -635,11 +640,9 @@ class HIPBackend:
                                   or t.get_device() != self.device):
                 raise PreconditionFailure("sample: u and settings must be contiguous device tensors, one entry per row")
         if tokens is None:
-            tokens = u.new_empty(rows, dtype=torch.int32)
-            self._made(tokens, stream)
+            tokens = self._made(stream, u.new_empty, rows, dtype=torch.int32)
         if probs is None:
-            probs = u.new_empty(rows)
-            self._made(probs, stream)
+            probs = self._made(stream, u.new_empty, rows)
         _check(self._lib.tbh_sample_device(
             self._dev, logits.data_ptr(), logits.stride(0), rows, vocab,
             temperature.data_ptr() if temperature is not None else None, topK.data_ptr() if topK is not None else None,
