@@ -151,3 +151,23 @@ def test_threads_on_one_stream_do_not_mix_their_launches(stand_in):
                 ends |= {at + len(one[i]) for i in several if got[at:at + len(one[i])] == one[i]}
         assert len(got) in ends, got[max(ends):max(ends) + 4]
     """)
+
+
+def test_memory_that_cannot_be_had_fails_no_call_that_does_without(stand_in):
+    # The runtime keeps a failed allocation's error until it is read, and a launch's check reads it.
+    stand_in("""
+        import tinybrain_amd as T
+        backend = T.HIPBackend(0)
+        dev = backend._dev
+        w = T.quantize(np.random.default_rng(0).normal(size=(4096, 512)).astype(np.float32), T.QuantizationMode.perChannel)
+        d = T.DeviceWeight(backend, w)
+        S.stand_in_limits(0, ALL)
+        calls = [lambda s: attention(layout(), 4, max_query_len=1, stream=s), lambda s: attention(layout(), 300, stream=s),
+                 lambda s: contiguous_attention(1, 4096, s), lambda s: contiguous_attention(64, 2048, s),
+                 lambda s: L.tbh_matmul_device(d.handle, P, 64, d.K, P, s)]
+        for i, call in enumerate(calls):
+            assert call(0x4000 + 64 * i) == 0, (i, _abi.last_error())     # whole contexts, whole K
+        S.stand_in_limits(ALL, 0)                                         # nor page-locked memory
+        backend.matmulQuantized(np.zeros((1, 4096), np.float32), w)
+        backend.matmulQuantized(np.zeros((64, 4096), np.float32), w)
+    """)

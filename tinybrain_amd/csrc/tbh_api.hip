@@ -765,8 +765,15 @@ void *stream_workspace(tbh_device *dev, hipStream_t s, size_t bytes) {
     for (auto &e : dev->workspaces)
         if (e.stream == s) ws = &e;
     if (ws && ws->bytes >= bytes) return ws->ptr;
+    // The runtime keeps an error until it is read, and the caller, which goes on
+    // without the memory, reads it as its launch's.
+    auto none = [] {
+        (void)hipGetLastError();
+        return nullptr;
+    };
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(s, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone) return nullptr;
+    if (hipStreamIsCapturing(s, &cap) != hipSuccess) return none();
+    if (cap != hipStreamCaptureStatusNone) return nullptr;
     // Grow by replacement: work queued on this stream, and any graph captured
     // on it, may still use the old buffer, so it stays allocated (retired)
     // until tbh_device_close.  Growth doubles, so the retired bytes stay below
@@ -775,7 +782,7 @@ void *stream_workspace(tbh_device *dev, hipStream_t s, size_t bytes) {
     size_t grown = (bytes + mib - 1) & ~(mib - 1);
     if (ws) grown = std::max(grown, 2 * ws->bytes);
     void *p = nullptr;
-    if (hipMalloc(&p, grown) != hipSuccess) return nullptr;
+    if (hipMalloc(&p, grown) != hipSuccess) return none();
     if (!ws) {
         dev->workspaces.push_back({s, nullptr, 0});
         ws = &dev->workspaces.back();
@@ -1021,6 +1028,7 @@ static hipError_t host_wait(tbh_device *dev) {
                     (void)hipHostFree(p);
                 }
             }
+            if (!dev->done_flag) (void)hipGetLastError();   // kept for the next launch's check else
         }
         if (dev->done_flag) {
             const uint32_t seq = ++dev->done_seq;
@@ -1101,6 +1109,7 @@ tbh_status tbh_matmul(tbh_device *dev, const float *x, int64_t M, int64_t K, con
         } else {
             dev->pin_bytes = grown;
         }
+        if (!pinned) (void)hipGetLastError();   // not the launches' error below
     }
     float *px = pinned ? (float *)dev->pin : nullptr;
     float *py = pinned ? (float *)((char *)dev->pin + ((xb + 255) & ~size_t(255))) : nullptr;
