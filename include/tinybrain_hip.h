@@ -572,7 +572,11 @@ typedef struct tbh_paged_queries {
  * has its probabilities rounded to bf16 for the second product.
  * num_heads must be a multiple of num_kv_heads.  Calls that split a long
  * context over blocks keep partial results in the workspace of (device,
- * stream), as tbh_matmul_device does, with its rule for captured graphs. */
+ * stream), as tbh_matmul_device does, with its rule for captured graphs: at
+ * most 256 MiB, for which the bounds on the lengths count, not the lengths
+ * themselves (contexts are cut into fewer parts where more would be needed).
+ * Without a workspace (none can be had, or it would have to grow under
+ * capture) contexts are not cut. */
 tbh_status tbh_paged_attention_device(tbh_device *dev, const tbh_paged_layout *layout,
                                       const tbh_paged_queries *queries, const void *k_cache, const void *v_cache,
                                       const int32_t *block_table, void *stream);

@@ -171,3 +171,33 @@ def test_memory_that_cannot_be_had_fails_no_call_that_does_without(stand_in):
         backend.matmulQuantized(np.zeros((1, 4096), np.float32), w)
         backend.matmulQuantized(np.zeros((64, 4096), np.float32), w)
     """)
+
+
+def test_partials_stay_within_their_limit(stand_in):
+    # They are sized by what the lengths may be; 128 MiB each for tiles and for few rows.
+    stand_in("""
+        def grown(l, tokens, stream, **kw):
+            before = S.stand_in_bytes()
+            assert attention(l, tokens, stream=stream, **kw) == 0, _abi.last_error()
+            return S.stand_in_bytes() - before
+
+        most, s = 0, 0x10000
+        for requests in (1, 64, 256, 1024, 4096):
+            for positions in (1024, 8192, 131072, 1 << 20):
+                for hd in (32, 64, 96, 128):
+                    for ct in (0, 1):
+                        l = layout(max_requests=requests, max_blocks=positions // 16, head_dim=hd, type=ct)
+                        for tokens in (1, requests, requests + 511, 20000):
+                            for kw in ({}, dict(max_query_len=1), dict(max_query_len=300, max_context_len=positions)):
+                                s += 64
+                                n = grown(l, tokens, s, **kw)
+                                assert n <= 256 << 20, (requests, positions, hd, ct, tokens, kw, n)
+                                most = max(most, n)
+                                L.tbh_device_close(dev)
+                                assert L.tbh_device_open(0, ctypes.byref(dev)) == 0
+                                launches()
+        assert most > 200 << 20              # the limit is what held some of them
+        # a batch of usual size keeps its parts: 64 requests of up to 8192 positions
+        assert attention(layout(max_requests=64), 64, max_query_len=1, max_context_len=8192, stream=s + 64) == 0
+        assert launches()[0][1] == (64 * 8 * 8, 1)
+    """)

@@ -767,6 +767,20 @@ int32_t split_least(int64_t units, int64_t context, int64_t cus) {
 size_t partial_head(int64_t rows) { return ((size_t)rows * sizeof(float2) + 255) / 256 * 256; }
 size_t partial_bytes(int64_t rows, int hd) { return partial_head(rows) + ((size_t)rows * hd * sizeof(float) + 255) / 256 * 256; }
 
+// Most bytes of a launch's partials, of tiles and of few rows each: units and parts
+// are the most that the call's bounds allow, whatever its lengths are (1024 requests
+// of a table of 131072 positions, 8 heads of 128, no bounds: 4.3 GB).  Fewer parts
+// leave a request that is much longer than the others to fewer blocks, but also fewer
+// blocks without work: 256 requests of 100 .. 2000 positions and one of 131072, one
+// row each, 641 us without a limit, 624 with 256 MiB, 505 with 128, 484 with 64, 612
+// with 32; without bounds 689, 521, 654, 882, 1495; 1024 such requests 1939, 1067,
+// 1073, 1358, 1721 and 2052, 1408, 1751, 1737, 1735.
+constexpr size_t kMaxPartials = (size_t)128 << 20;
+int32_t splits_within(int64_t splits, int64_t rows, int hd) {   // rows: of one split
+    const size_t each = (size_t)rows * ((size_t)hd * sizeof(float) + sizeof(float2));
+    return (int32_t)std::max<int64_t>(1, std::min<int64_t>(splits, (int64_t)(kMaxPartials / std::max<size_t>(each, 1))));
+}
+
 SplitArgs plan_split(const PagedArgs &a, int64_t query, int64_t context, bool tiles, size_t elem, int64_t cus) {
     SplitArgs sa{};
     sa.a = a;
@@ -781,6 +795,7 @@ SplitArgs plan_split(const PagedArgs &a, int64_t query, int64_t context, bool ti
     // at most 2^22 blocks (a grid has below 2^32 threads)
     sa.splits = (int32_t)std::max<int64_t>(
         1, std::min<int64_t>({(context + sa.least - 1) / sa.least, kMaxSplits, (1 << 22) / std::max<int64_t>(units, 1)}));
+    sa.splits = splits_within(sa.splits, units * sa.slots, a.hd);
     return sa;
 }
 
@@ -1356,6 +1371,7 @@ TileArgs plan_tile(const PagedArgs &a, int64_t query, int64_t context, int64_t t
     const int64_t parts = fills(full, cus) ? 1 : std::max<int64_t>(1, 4 * cus / full);
     ta.least = 256;
     ta.splits = (int32_t)std::max<int64_t>(1, std::min({parts, (context + ta.least - 1) / ta.least, kMaxSplits}));
+    ta.splits = splits_within(ta.splits, units * tile_rows, a.hd);
     // two blocks share a CU: all run at once, or the longest have to come first (512 blocks
     // of 2048 rows over 4096: 119 us, 121 without; over 8192: 244, 250)
     ta.pair_up = full <= 2 * cus;
