@@ -495,15 +495,16 @@ typedef struct tbh_paged_layout {
  *   - released rows push their blocks (row by row, in table order);
  *   - row b with n = new_lens[b] > 0 needs ceil((context + n) / block_size) -
  *     ceil(context / block_size) blocks and is granted its tokens if context +
- *     n fits the table row and the needs of rows 0 .. b (of those that fit
- *     theirs) do not exceed the stack, or it needs none: no row overtakes one
- *     that waits for blocks;
+ *     n fits the table row, query_start[b] + n fits max_tokens, and the needs
+ *     of rows 0 .. b (of those that fit both) do not exceed the stack, or it
+ *     needs none: no row overtakes one that waits for blocks, and rows behind
+ *     one whose tokens pass max_tokens wait with it;
  *   - granted rows pop their blocks off the stack (row by row) into the table.
  * Outputs: query_start[max_requests + 1], running sums of max(new_lens, 0);
  * granted[max_requests], n or 0; context_out, free_count_out: the lengths and
  * the height after the step; slots[max_tokens], positions[max_tokens] of token
  * query_start[b] + i, position context[b] + i, and -1 for rows not granted and
- * for entries behind the last token (tokens past max_tokens get none).
+ * for entries behind the last token.
  * context_out and free_count_out may be context_lens and free_count; else a
  * plan can be dropped: entries of the table and of the stack that the old
  * lengths and height refer to are not changed.  Only the block_size, num_blocks,

@@ -35,7 +35,7 @@ def plan(new, context, table, free, count, block, max_tokens):
     asked = taken = 0
     for b, n in enumerate(new):
         more, c = max(int(n), 0), int(context[b])
-        fits = more > 0 and c + more <= table.shape[1] * block
+        fits = more > 0 and c + more <= table.shape[1] * block and start[-1] + more <= max_tokens
         need = ceil_div(c + more, block) - ceil_div(c, block) if fits else 0
         ok = fits and (need == 0 or asked + need <= height)
         if ok:
@@ -44,9 +44,8 @@ def plan(new, context, table, free, count, block, max_tokens):
             taken += need
             for i in range(more):
                 t, p = start[-1] + i, c + i
-                if t < max_tokens:
-                    slots[t] = table[b, p // block] * block + p % block
-                    positions[t] = p
+                slots[t] = table[b, p // block] * block + p % block
+                positions[t] = p
         asked += need
         granted.append(more if ok else 0)
         out.append(0 if n < 0 else c + granted[-1])

@@ -630,6 +630,38 @@ def _check_rows(got, y, nh, nkv, hd):
     _close(got, want, bound + U32 * np.abs(want) + 2 * 16 * U32 * (qm * ks + km * qs) / hd ** 0.5 * mass)
 
 
+@pytest.mark.parametrize("rows,most_tokens", [(4, 60), (1030, 1200)])
+def test_requests_past_the_steps_entries_wait(torch, backend, rows, most_tokens):
+    # A step of more tokens than it has entries: who passes them keeps its length (its keys are
+    # never stored), is served later, and no row meets a place that was not written (NaN here).
+    nh, nkv, hd, bs = 4, 2, 64, 16
+    cache = T.PagedKVCache(backend, 1, 3 * rows, bs, nkv, hd, rows, 3)
+    for a in (cache.keys[0], cache.values[0]):
+        a.fill_(float("nan"))
+    rng = np.random.default_rng(rows)
+    want_len = rng.integers(1, 40, rows)
+    history = [np.zeros((0, (nh + 2 * nkv) * hd))] * rows
+    waited = 0
+    for step in range(60):
+        new = np.where([len(h) == 0 for h in history], want_len, 0).astype(np.int32)
+        if not new.any():
+            break
+        plan = cache.plan(_ints(torch, new), most_tokens)
+        y = torch.randn(most_tokens, (nh + 2 * nkv) * hd, device="cuda")
+        nq, nk = nh * hd, nkv * hd
+        q = cache.append(0, plan, y[:, nq:nq + nk], y[:, nq + nk:], y[:, :nq], ropeBase=10000.0)
+        out, y, granted, start = _np(cache.attention(0, plan, q, nh)), _np(y), _np(plan.granted), _np(plan.queryStart)
+        np.testing.assert_array_equal(granted, np.where(start[1:] <= most_tokens, new, 0))
+        for b in np.flatnonzero(granted):
+            history[b] = y[start[b]:start[b + 1]]
+            if b % max(rows // 8, 1) == 0:
+                _check_rows(out[start[b]:start[b + 1]], history[b], nh, nkv, hd)
+        assert np.isfinite(out[:min(int(granted.sum()), most_tokens)]).all()
+        waited += int(((granted == 0) & (new > 0)).sum())
+        np.testing.assert_array_equal(_np(cache.contextLens), [len(h) for h in history])
+    assert waited > 0 and all(len(h) for h in history)
+
+
 @pytest.mark.parametrize("dtype,q_type", [("float32", None), ("bfloat16", "bfloat16")])
 def test_captured_step_replays_with_new_lengths(torch, backend, dtype, q_type):
     # plan, product, append, attention and sampling of one decode step captured

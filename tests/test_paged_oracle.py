@@ -60,6 +60,20 @@ def test_plan_waits_in_order():
     assert p["count"] == 2 and p["slots"][16] == 7 * 4 + 2 and (p["slots"] >= 0).sum() == 1
 
 
+def test_plan_grants_what_has_entries():
+    # row 1's last token would be the step's eighth: it waits, and row 2 behind it; their lengths stay
+    table = np.full((3, 4), -1, np.int32)
+    p = P.plan([3, 5, 1], [0, 2, 0], np.array([[-1] * 4, [9, -1, -1, -1], [-1] * 4], np.int32), np.arange(8), 8, 4, 7)
+    np.testing.assert_array_equal(p["granted"], [3, 0, 0])
+    np.testing.assert_array_equal(p["context"], [3, 2, 0])
+    np.testing.assert_array_equal(p["start"], [0, 3, 8, 9])
+    np.testing.assert_array_equal(p["slots"], [28, 29, 30, -1, -1, -1, -1])
+    np.testing.assert_array_equal(p["positions"], [0, 1, 2, -1, -1, -1, -1])
+    assert p["count"] == 7
+    p = P.plan([3, 5, 1], [0, 2, 0], table, np.arange(8), 8, 4, 8)
+    np.testing.assert_array_equal(p["granted"], [3, 5, 0])
+
+
 # ---------------------------------------------------------------------------
 # rotation, store, attention
 # ---------------------------------------------------------------------------

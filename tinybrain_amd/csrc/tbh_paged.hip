@@ -116,11 +116,12 @@ __global__ __launch_bounds__(kPlanThreads) void plan_rows(const PlanArgs a, bool
         const bool row = r < a.rows;
         const int32_t n = row ? a.new_lens[r] : 0, c = row ? max(a.ctx[r], 0) : 0;
         const int32_t more = max(n, 0);
-        const bool fits = more > 0 && (int64_t)c + more <= capacity;
-        const int32_t have = blocks_of(c, a.shift);
-        const int32_t need = fits ? blocks_of((int64_t)c + more, a.shift) - have : 0;
         int64_t tile_tokens, tile_need;
         const int64_t first = tokens + block_scan(more, red, tile_tokens);
+        // a token without an entry would get no slot, and its place be read unwritten
+        const bool fits = more > 0 && (int64_t)c + more <= capacity && first + more <= a.max_tokens;
+        const int32_t have = blocks_of(c, a.shift);
+        const int32_t need = fits ? blocks_of((int64_t)c + more, a.shift) - have : 0;
         const int64_t before = asked + block_scan(need, red, tile_need);
         const bool ok = fits && (need == 0 || before + need <= height);
         if (row) {

@@ -59,7 +59,9 @@ class PagedKVCache:
 
     def plan(self, newLens, maxTokens: int, stream=None) -> PagedPlan:
         """Blocks, slots and positions of the next newLens[b] tokens of each
-        request (0: idle, negative: released); advances the cache's state."""
+        request (0: idle, negative: released); advances the cache's state.  A
+        request waits (granted 0) if there are no blocks for it or the step's
+        tokens up to its own are more than maxTokens."""
         return self.backend.paged_plan_device(newLens, self.contextLens, self.blockTable, self.freeBlocks,
                                               self.freeCount, self.blockSize, maxTokens,
                                               contextOut=self.contextLens, freeCountOut=self.freeCount,
