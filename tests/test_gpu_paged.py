@@ -422,6 +422,23 @@ def test_attention_past_32_bits(torch, backend):
     assert torch.equal(big["keys"][-1, :, -1].reshape(-1), k[0]) and torch.equal(big["values"][0, :, 5].reshape(-1), v[1])
 
 
+@pytest.mark.parametrize("hd,bs", [(32, 16), (8, 1)])
+def test_more_blocks_than_a_grid_has_across(torch, backend, hd, bs):
+    # 2^20 and some rows: requests of one position, so that each row's result is its value
+    n, nkv = (1 << 20) + 7, 1
+    rows = torch.randn(n, 2 * hd, device="cuda").to(torch.bfloat16)
+    k, v = rows[:, :hd], rows[:, hd:]
+    keys, values = torch.zeros(2, n, nkv, bs, hd, dtype=torch.bfloat16, device="cuda")
+    order = torch.randperm(n, device="cuda").to(torch.int32)
+    backend.paged_append_device(keys, values, order * bs, k, v)
+    at = order.long()
+    assert torch.equal(keys[at, 0, 0], k) and torch.equal(values[at, 0, 0], v)
+    start, ones = torch.arange(n + 1, dtype=torch.int32, device="cuda"), torch.ones(n, dtype=torch.int32, device="cuda")
+    for kw in ({}, dict(maxQueryLen=1, maxContextLen=1)):
+        got = backend.paged_attention_device(k.contiguous(), keys, values, order[:, None].contiguous(), start, ones, 1, **kw)
+        assert torch.equal(got, v)
+
+
 def test_attention_split_partials_of_two_streams(torch, backend):
     # calls that split their contexts on two streams at once, each with its workspace
     c = [_attention_case(torch, 20 + i, [(1, 4000 + i)], 8, 2, 64, 16, "float32", "bfloat16") for i in range(2)]

@@ -119,6 +119,16 @@ def test_sample_device_rows(backend):
     assert (none[0] == -1).all() and (none[1] == 0).all()
 
 
+def test_sample_more_rows_than_a_grid_has_across(backend):
+    import torch
+
+    n = (1 << 20) + 3
+    want = torch.randint(0, 3, (n,), device="cuda")
+    x = torch.full((n, 3), -float("inf"), device="cuda").scatter_(1, want[:, None], 1.0)
+    tokens, probs = backend.sample_device(x, torch.rand(n, device="cuda"))
+    assert torch.equal(tokens.long(), want) and bool((probs == 1).all())
+
+
 def test_sample_preconditions(backend):
     import torch
 

@@ -201,3 +201,28 @@ def test_partials_stay_within_their_limit(stand_in):
         assert attention(layout(max_requests=64), 64, max_query_len=1, max_context_len=8192, stream=s + 64) == 0
         assert launches()[0][1] == (64 * 8 * 8, 1)
     """)
+
+
+def test_calls_of_many_blocks_are_launched(stand_in):
+    # A grid's x holds below 2^32 threads: up to 2^31 - 1 rows or requests, as the checks take them.
+    stand_in("""
+        def blocks():
+            return [x * y for _, (x, y), _, _ in launches()]
+
+        l = layout(num_kv_heads=1, head_dim=64)
+        for tokens in (5, 1 << 20, (1 << 20) + 1, 1 << 24, 1 << 31):
+            tokens = min(tokens, (1 << 31) - 1)
+            assert append(l, tokens) == 0, (tokens, _abi.last_error())
+            n, = blocks()
+            assert tokens <= n < tokens + (1 << 20)
+        for rows in (5, 1 << 22, (1 << 31) - 1):
+            assert sample(rows, 7) == 0, (rows, _abi.last_error())
+            n, = blocks()
+            assert rows <= n < rows + (1 << 20)
+        for heads, hd in ((8, 64), (8, 128), (8, 32), (8, 80)):
+            for requests, tokens in (((1 << 21) + 5, (1 << 21) + 5), (4, 1 << 27), ((1 << 27) - 1, (1 << 27) - 1)):
+                l = layout(max_requests=requests, max_blocks=2, head_dim=hd)
+                for kw in ({}, dict(max_query_len=1))[:1 + (requests == tokens)]:
+                    assert attention(l, tokens, heads=heads, **kw) == 0, (heads, hd, requests, kw, _abi.last_error())
+                    assert max(blocks()) >= tokens * heads // 128
+    """)

@@ -229,7 +229,8 @@ template <class XT, class CT, class QT, bool VEC>
 __global__ __launch_bounds__(256) void append_rows(const RowsArgs a) {
     __shared__ float2 cs[kMaxHeadDim / 2];   // (cos, sin) per pair
     const tbh_paged_rows &r = a.r;
-    const int64_t t = blockIdx.x;
+    const int64_t t = wide_block();
+    if (t >= r.tokens) return;
     const int tid = threadIdx.x, hd = a.hd;
     const bool rope = r.rope_base > 0.0f;
     if (rope) {
@@ -313,7 +314,7 @@ __global__ __launch_bounds__(256) void append_rows(const RowsArgs a) {
 
 template <class XT, class CT, class QT>
 void launch_append(const RowsArgs &a, bool vec, hipStream_t s) {
-    const dim3 grid((unsigned)a.r.tokens);
+    const dim3 grid = wide_grid(a.r.tokens);
     if (vec) hipLaunchKernelGGL((append_rows<XT, CT, QT, true>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((append_rows<XT, CT, QT, false>), grid, dim3(256), 0, s, a);
 }

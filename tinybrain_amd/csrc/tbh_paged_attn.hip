@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256) void paged_rows(const PagedArgs a) {
     __shared__ float sm[4], sl[4];
     __shared__ bool sseen[4];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    const int64_t row = wide_block();
     if (row >= a.tokens * a.nh) return;
     const int64_t t = row / a.nh;
     const int h = (int)(row % a.nh);
@@ -683,9 +683,10 @@ __device__ __forceinline__ void split_block(const SplitArgs &sa, uint32_t block,
 }
 
 template <class XT, class CT, int HD>
-__global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
+__global__ __launch_bounds__(256) void paged_split(const SplitArgs sa, uint32_t blocks) {
     __shared__ __attribute__((aligned(16))) SplitLds<HD> lds;
-    split_block<XT, CT, HD>(sa, blockIdx.x, lds);
+    const uint32_t block = (uint32_t)wide_block();
+    if (block < blocks) split_block<XT, CT, HD>(sa, block, lds);
 }
 
 // Joins split_block's parts: a wave per unit and row, HD / 4 lanes across the head,
@@ -747,8 +748,9 @@ __device__ __forceinline__ void split_merge(const SplitArgs &sa, uint32_t block)
 }
 
 template <class XT, int HD>
-__global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa) {
-    split_merge<XT, HD>(sa, blockIdx.x);
+__global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa, uint32_t blocks) {
+    const uint32_t block = (uint32_t)wide_block();
+    if (block < blocks) split_merge<XT, HD>(sa, block);
 }
 
 constexpr int64_t kMaxSplits = 64;   // a lane each in split_merge
@@ -792,7 +794,7 @@ SplitArgs plan_split(const PagedArgs &a, int64_t query, int64_t context, bool ti
     sa.long_rows = tiles ? 16 : INT32_MAX;
     sa.slots = (int32_t)std::min<int64_t>(16, query * a.rep);
     sa.least = split_least(units, context, cus);
-    // at most 2^22 blocks (a grid has below 2^32 threads)
+    // at most 2^22 blocks, most of which will have no part
     sa.splits = (int32_t)std::max<int64_t>(
         1, std::min<int64_t>({(context + sa.least - 1) / sa.least, kMaxSplits, (1 << 22) / std::max<int64_t>(units, 1)}));
     sa.splits = splits_within(sa.splits, units * sa.slots, a.hd);
@@ -1332,19 +1334,23 @@ __device__ __forceinline__ void tile_merge(const TileArgs &ta, uint32_t block) {
 // 333-token chunk over fp32: 48 us in two launches and two merges, 35 when joined, 29 now); likewise
 // their merges.
 template <class XT, class CT, int HD, int ROWS>
-__global__ __launch_bounds__(256, 2) void paged_both(const TileArgs ta, const SplitArgs sa) {
+__global__ __launch_bounds__(256, 2) void paged_both(const TileArgs ta, const SplitArgs sa, uint32_t blocks) {
     __shared__ __attribute__((aligned(256))) union {
         TileLds<HD> tile;
         SplitLds<HD> split;
     } lds;
-    if (blockIdx.x < ta.blocks) tile_block<XT, HD, ROWS>(ta, blockIdx.x, lds.tile, CT{});
-    else split_block<XT, CT, HD>(sa, blockIdx.x - ta.blocks, lds.split);
+    const uint32_t block = (uint32_t)wide_block();
+    if (block >= blocks) return;
+    if (block < ta.blocks) tile_block<XT, HD, ROWS>(ta, block, lds.tile, CT{});
+    else split_block<XT, CT, HD>(sa, block - ta.blocks, lds.split);
 }
 
 template <class XT, int HD, int ROWS>
-__global__ __launch_bounds__(256) void paged_both_merge(const TileArgs ta, const SplitArgs sa) {
-    if (blockIdx.x < ta.merge_blocks) tile_merge<XT, HD, ROWS>(ta, blockIdx.x);
-    else split_merge<XT, HD>(sa, blockIdx.x - ta.merge_blocks);
+__global__ __launch_bounds__(256) void paged_both_merge(const TileArgs ta, const SplitArgs sa, uint32_t blocks) {
+    const uint32_t block = (uint32_t)wide_block();
+    if (block >= blocks) return;
+    if (block < ta.merge_blocks) tile_merge<XT, HD, ROWS>(ta, block);
+    else split_merge<XT, HD>(sa, block - ta.merge_blocks);
 }
 
 // Whether so many tiles fill two blocks per CU, nine in ten of them.
@@ -1380,11 +1386,12 @@ TileArgs plan_tile(const PagedArgs &a, int64_t query, int64_t context, int64_t t
 
 template <class XT, class CT, int HD, int ROWS>
 hipError_t launch_both(const TileArgs &ta, const SplitArgs &sa, int64_t split_blocks, int64_t split_merges, hipStream_t s) {
-    hipLaunchKernelGGL((paged_both<XT, CT, HD, ROWS>), dim3((unsigned)(ta.blocks + split_blocks)), dim3(256), 0, s, ta, sa);
+    const int64_t blocks = ta.blocks + split_blocks;
+    hipLaunchKernelGGL((paged_both<XT, CT, HD, ROWS>), wide_grid(blocks), dim3(256), 0, s, ta, sa, (uint32_t)blocks);
     const hipError_t e = hipGetLastError();
     const int64_t merges = ta.merge_blocks + split_merges;
     if (e != hipSuccess || merges == 0) return e;
-    hipLaunchKernelGGL((paged_both_merge<XT, HD, ROWS>), dim3((unsigned)merges), dim3(256), 0, s, ta, sa);
+    hipLaunchKernelGGL((paged_both_merge<XT, HD, ROWS>), wide_grid(merges), dim3(256), 0, s, ta, sa, (uint32_t)merges);
     return hipGetLastError();
 }
 
@@ -1430,10 +1437,10 @@ hipError_t launch_matrix(tbh_device *dev, const PagedArgs &a, int64_t query, int
             return launch_both<XT, CT, HD, 64>(ta, sa, split_blocks, split_merges, s);
         }
     }
-    hipLaunchKernelGGL((paged_split<XT, CT, HD>), dim3((unsigned)split_blocks), dim3(256), 0, s, sa);
+    hipLaunchKernelGGL((paged_split<XT, CT, HD>), wide_grid(split_blocks), dim3(256), 0, s, sa, (uint32_t)split_blocks);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || split_merges == 0) return e;
-    hipLaunchKernelGGL((paged_split_merge<XT, HD>), dim3((unsigned)split_merges), dim3(256), 0, s, sa);
+    hipLaunchKernelGGL((paged_split_merge<XT, HD>), wide_grid(split_merges), dim3(256), 0, s, sa, (uint32_t)split_merges);
     return hipGetLastError();
 }
 
@@ -1449,9 +1456,7 @@ hipError_t launch_paged(tbh_device *dev, const PagedArgs &a, int64_t query, int6
         default: break;
         }
     }
-    const int64_t rows = a.tokens * a.nh, across = std::min<int64_t>(rows, 1 << 20);   // threads of a grid's x: below 2^32
-    hipLaunchKernelGGL((paged_rows<XT, CT>), dim3((unsigned)across, (unsigned)((rows + across - 1) / across)), dim3(256), 0,
-                       s, a);
+    hipLaunchKernelGGL((paged_rows<XT, CT>), wide_grid(a.tokens * a.nh), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
