@@ -129,6 +129,21 @@ def test_sample_more_rows_than_a_grid_has_across(backend):
     assert torch.equal(tokens.long(), want) and bool((probs == 1).all())
 
 
+@pytest.mark.parametrize("s", [dict(), dict(k=2), dict(k=40), dict(k=1500, p=0.9), dict(p=0.7), dict(p=0.999), dict(m=0.02),
+                               dict(k=30, p=0.8, m=0.01)])
+@pytest.mark.parametrize("t", [1.0, 2.0, 1e37, 4e37, 1e38, 3e38, float("inf")])
+def test_sample_differences_past_the_largest_float(backend, s, t):
+    # logits whose distance to the largest is past fp32's range, at temperatures at which that counts
+    rng = np.random.default_rng(7)
+    x = (rng.uniform(-3.4, 3.4, (5, 3000)) * 1e38).astype(np.float32)
+    x[1, :2900] = -3.3e38
+    x[2] = np.float32(-3.4e38)
+    x[2, [3, 50]] = 3.4e38, 3.3e38
+    x[3, ::2] = -np.inf
+    x[4, 5] = np.inf
+    _check(backend, x, [0.2, 0.6, 0.99, 0.5, 0.3], t=t, **s)
+
+
 def test_sample_preconditions(backend):
     import torch
 

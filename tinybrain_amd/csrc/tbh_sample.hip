@@ -134,7 +134,9 @@ struct Row {
     const float *x;
     int32_t vocab;
     float cap;              // largest logit; of a row with inf: the largest finite float, standing for inf
-    float bins;             // 64 / temperature
+    float half;             // 1/2 at temperatures above 1, where a distance past the largest float can count; else 1
+    float cap_half;         // cap * half
+    float bins;             // 64 / (temperature * half)
     double c;               // log2(e) / temperature
     const double *pow2;
     uint32_t top;           // the largest logit's key
@@ -149,7 +151,7 @@ struct Row {
     }
     // Distance to the largest logit in 1/64 of a power of e: from 2^-46 down the last bin.
     __device__ __forceinline__ uint32_t bin(float l) const {
-        return (uint32_t)min(kBins - 1, (int)((cap - fminf(l, cap)) * bins));
+        return (uint32_t)min(kBins - 1, (int)(fmaf(-half, fminf(l, cap), cap_half) * bins));
     }
     __device__ __forceinline__ uint64_t weight_of(double t) const {   // round(2^(43 + t)), -64 <= t <= 0
         constexpr double kShift = 6755399441055744.0;                 // 1.5 2^52: rounds to whole numbers
@@ -384,7 +386,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
     const float largest = logit_of(row.top);
     const bool inf = largest == INFINITY;
     row.cap = inf ? 3.40282347e38f : largest;
-    row.bins = 64.0f / t;
+    row.half = t > 1.0f ? 0.5f : 1.0f;
+    row.cap_half = row.cap * row.half;
+    row.bins = 64.0f / row.half / t;
     row.c = 1.4426950408889634 / (double)t;
     row.least = inf ? row.cap : -INFINITY;    // everything above -inf, or the infinities alone ...
     row.idx = -1;
