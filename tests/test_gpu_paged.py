@@ -480,6 +480,68 @@ def test_attention_captured_before_any_eager_call(torch, backend):
         _close(_np(eager), want, _tolerance(want, bound, "float32", "bfloat16"))
 
 
+@pytest.mark.parametrize("x,cache", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 32])
+def test_attention_of_long_contexts_in_one_part(torch, x, cache, hd):
+    # without a workspace a block takes a whole context: past the 4096 positions whose blocks it
+    # looks up at once (single tokens), the 1024 of a tile's window, and with pages missing
+    c = _attention_case(torch, 43, [(1, 9000), (40, 2600), (1, 4097), (3, 4230)], 4, 2, hd, 16, x, cache, holes=True)
+    c["table"][0, [255, 256, 300]] = -1                    # of the positions around the 4096th
+    args = [_ints(torch, c[k]) for k in ("table", "start", "context")]
+    out = torch.empty_like(c["q"])
+    fresh, stream, graph = T.HIPBackend(0), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    try:
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            fresh.paged_attention_device(c["q"], c["keys"], c["values"], *args, c["heads"], out=out)
+        keys, values = _np(c["keys"]), _np(c["values"])
+        want, bound = P.attention(_np(c["q"]), keys, values, c["table"], c["start"], c["context"], c["heads"])
+        tol = _tolerance(want, bound, x, cache)
+        if x == cache == "bfloat16":
+            tol = tol + U16 * P.attention(_np(c["q"]), keys, np.abs(values), c["table"], c["start"], c["context"], 4)[0]
+        for _ in range(2):
+            out.fill_(7.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            _close(_np(out), want, tol)
+        _check_attention(torch, fresh, c, x, cache)        # and in parts
+    finally:
+        fresh.close()
+
+
+@pytest.mark.parametrize("x,cache", TYPES)
+@pytest.mark.parametrize("requests", [64, 65, 129, 200])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (4, 1, 96), (4, 2, 32), (3, 3, 40)])
+def test_attention_of_many_requests(torch, backend, x, cache, requests, nh, nkv, hd):
+    # chunks and single tokens among more requests than a wave looks over at once
+    rng = np.random.default_rng(requests)
+    lens = [(1, int(rng.integers(1, 120))) for _ in range(requests)]
+    for b in {3, 40, 63, 64, 70, 127, 128, 150, requests - 1} & set(range(requests)):
+        n = int(rng.integers(2, 40))
+        lens[b] = (n, n + int(rng.integers(0, 90)))
+    for b in {0, 62, 65, 126} & set(range(requests)):
+        lens[b] = (0, int(rng.integers(0, 50)))
+    c = _attention_case(torch, requests + hd, lens, nh, nkv, hd, 16, x, cache, extra_rows=2)
+    got = _check_attention(torch, backend, c, x, cache)
+    again = _check_attention(torch, backend, c, x, cache, maxQueryLen=40, maxContextLen=130)
+    np.testing.assert_array_equal(got[-2:], again[-2:])
+
+
+@pytest.mark.parametrize("x,cache", TYPES)
+def test_attention_past_parts_of_1024_positions(torch, backend, x, cache):
+    # contexts past 65536 positions: 64 parts hold more than 1024 each
+    hd = 64
+    c = _attention_case(torch, 45, [(1, 70001), (1, 300), (20, 66000)], 4, 2, hd, 1024, x, cache)
+    want, mass, bound = _attention64(torch, c, hd)
+    tol = bound + (U32 + (2 * U16 if x == "bfloat16" else 0)) * want.abs()
+    if x == cache == "bfloat16":
+        tol = tol + U16 * mass
+    for kw in ({}, dict(maxQueryLen=20, maxContextLen=70001), dict(maxQueryLen=1)):
+        got = _run_attention(torch, backend, c, **kw).double()
+        assert bool(((got - want).abs() <= tol).all())
+
+
 def test_two_captured_steps_take_turns(torch, backend):
     # two graphs of one stream share its workspace; replayed in turn, with eager calls between
     cs = [_attention_case(torch, 41 + i, [(1, 2500 - 700 * i), (30, 800)], 8, 2, 64, 16, "float32", "float32")
