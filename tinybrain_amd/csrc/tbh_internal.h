@@ -241,13 +241,10 @@ hipError_t launch_gemm(const tbh_weight &w, const void *x, bool f32, int pieces,
                        int64_t ldy, hipStream_t s, const Scratch &scr);
 hipError_t launch_split_sum(const float *part, int splits, float *y, int64_t n, int64_t cus, hipStream_t s);
 
-// A grid of `blocks` blocks, and a block's number in it (the last may be past
-// them): a grid's x holds below 2^32 threads.
-inline dim3 wide_grid(int64_t blocks) {
-    const int64_t across = blocks < 1 << 20 ? blocks : 1 << 20;
-    return dim3((unsigned)across, (unsigned)((blocks + across - 1) / across));
-}
-__device__ __forceinline__ int64_t wide_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+// Blocks of one launch at most (a grid's x holds below 2^32 threads): calls of more
+// make several.  One launch of two dimensions cost every small call 0.4 us, as a
+// block has to know its number and the grid's end before it loads anything else.
+constexpr int64_t kMostBlocks = 1 << 20;
 
 // Device workspace of at least `bytes` owned by (dev, stream), grown on
 // demand (tbh_api.hip).  Growing allocates a new buffer and keeps the old one

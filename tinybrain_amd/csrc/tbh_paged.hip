@@ -229,8 +229,7 @@ template <class XT, class CT, class QT, bool VEC>
 __global__ __launch_bounds__(256) void append_rows(const RowsArgs a) {
     __shared__ float2 cs[kMaxHeadDim / 2];   // (cos, sin) per pair
     const tbh_paged_rows &r = a.r;
-    const int64_t t = wide_block();
-    if (t >= r.tokens) return;
+    const int64_t t = blockIdx.x;
     const int tid = threadIdx.x, hd = a.hd;
     const bool rope = r.rope_base > 0.0f;
     if (rope) {
@@ -313,10 +312,24 @@ __global__ __launch_bounds__(256) void append_rows(const RowsArgs a) {
 }
 
 template <class XT, class CT, class QT>
-void launch_append(const RowsArgs &a, bool vec, hipStream_t s) {
-    const dim3 grid = wide_grid(a.r.tokens);
-    if (vec) hipLaunchKernelGGL((append_rows<XT, CT, QT, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((append_rows<XT, CT, QT, false>), grid, dim3(256), 0, s, a);
+hipError_t launch_append(RowsArgs a, bool vec, hipStream_t s) {
+    tbh_paged_rows &r = a.r;
+    for (int64_t left = r.tokens;;) {
+        const int64_t n = std::min(left, kMostBlocks);
+        const dim3 grid((unsigned)n);
+        if (vec) hipLaunchKernelGGL((append_rows<XT, CT, QT, true>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((append_rows<XT, CT, QT, false>), grid, dim3(256), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        left -= n;
+        if (e != hipSuccess || left == 0) return e;
+        r.k = (const XT *)r.k + n * r.k_stride;
+        r.v = (const XT *)r.v + n * r.v_stride;
+        r.slots += n;
+        if (r.positions) r.positions += n;
+        if (!r.q) continue;
+        r.q = (const XT *)r.q + n * r.q_stride;
+        r.q_out = (QT *)r.q_out + n * r.q_out_stride;
+    }
 }
 
 int log2_of(int32_t v) { return __builtin_ctz((unsigned)v); }
@@ -418,17 +431,17 @@ tbh_status tbh_paged_append_device(tbh_device *dev, const tbh_paged_layout *layo
                      (!r.q || (rows16(r.q, r.q_stride, xs) && rows16(r.q_out, r.q_out_stride, qs)));
     const hipStream_t s = (hipStream_t)stream;
     const int sel = (r.x_type == TBH_BF16) * 4 + (layout->type == TBH_BF16) * 2 + (r.q && r.q_out_type == TBH_BF16);
+    hipError_t e;
     switch (sel) {
-    case 0: launch_append<float, float, float>(a, vec, s); break;
-    case 1: launch_append<float, float, __bf16>(a, vec, s); break;
-    case 2: launch_append<float, __bf16, float>(a, vec, s); break;
-    case 3: launch_append<float, __bf16, __bf16>(a, vec, s); break;
-    case 4: launch_append<__bf16, float, float>(a, vec, s); break;
-    case 5: launch_append<__bf16, float, __bf16>(a, vec, s); break;
-    case 6: launch_append<__bf16, __bf16, float>(a, vec, s); break;
-    default: launch_append<__bf16, __bf16, __bf16>(a, vec, s); break;
+    case 0: e = launch_append<float, float, float>(a, vec, s); break;
+    case 1: e = launch_append<float, float, __bf16>(a, vec, s); break;
+    case 2: e = launch_append<float, __bf16, float>(a, vec, s); break;
+    case 3: e = launch_append<float, __bf16, __bf16>(a, vec, s); break;
+    case 4: e = launch_append<__bf16, float, float>(a, vec, s); break;
+    case 5: e = launch_append<__bf16, float, __bf16>(a, vec, s); break;
+    case 6: e = launch_append<__bf16, __bf16, float>(a, vec, s); break;
+    default: e = launch_append<__bf16, __bf16, __bf16>(a, vec, s); break;
     }
-    const hipError_t e = hipGetLastError();
     return e == hipSuccess ? TBH_OK : hip_error(e, "paged append launch");
 }
 

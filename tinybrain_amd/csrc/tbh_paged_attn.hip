@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256) void paged_rows(const PagedArgs a) {
     __shared__ float sm[4], sl[4];
     __shared__ bool sseen[4];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t row = wide_block();
+    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     if (row >= a.tokens * a.nh) return;
     const int64_t t = row / a.nh;
     const int h = (int)(row % a.nh);
@@ -231,6 +231,7 @@ struct SplitArgs {
     int32_t long_rows;     // requests of more rows are tile_block's
     bool scan;             // units are groups of 16 rows of any request, else requests
     bool qvec;             // q rows are 16-byte aligned
+    uint32_t base;         // the launch's first block, of both kinds
     float2 *ml;            // partials [unit][split][slots]: (max, sum)
     float *po;             // and sums of p v, [unit][split][slots][head_dim]
 };
@@ -683,10 +684,9 @@ __device__ __forceinline__ void split_block(const SplitArgs &sa, uint32_t block,
 }
 
 template <class XT, class CT, int HD>
-__global__ __launch_bounds__(256) void paged_split(const SplitArgs sa, uint32_t blocks) {
+__global__ __launch_bounds__(256) void paged_split(const SplitArgs sa) {
     __shared__ __attribute__((aligned(16))) SplitLds<HD> lds;
-    const uint32_t block = (uint32_t)wide_block();
-    if (block < blocks) split_block<XT, CT, HD>(sa, block, lds);
+    split_block<XT, CT, HD>(sa, sa.base + blockIdx.x, lds);
 }
 
 // Joins split_block's parts: a wave per unit and row, HD / 4 lanes across the head,
@@ -748,9 +748,8 @@ __device__ __forceinline__ void split_merge(const SplitArgs &sa, uint32_t block)
 }
 
 template <class XT, int HD>
-__global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa, uint32_t blocks) {
-    const uint32_t block = (uint32_t)wide_block();
-    if (block < blocks) split_merge<XT, HD>(sa, block);
+__global__ __launch_bounds__(256) void paged_split_merge(const SplitArgs sa) {
+    split_merge<XT, HD>(sa, sa.base + blockIdx.x);
 }
 
 constexpr int64_t kMaxSplits = 64;   // a lane each in split_merge
@@ -1334,21 +1333,19 @@ __device__ __forceinline__ void tile_merge(const TileArgs &ta, uint32_t block) {
 // 333-token chunk over fp32: 48 us in two launches and two merges, 35 when joined, 29 now); likewise
 // their merges.
 template <class XT, class CT, int HD, int ROWS>
-__global__ __launch_bounds__(256, 2) void paged_both(const TileArgs ta, const SplitArgs sa, uint32_t blocks) {
+__global__ __launch_bounds__(256, 2) void paged_both(const TileArgs ta, const SplitArgs sa) {
     __shared__ __attribute__((aligned(256))) union {
         TileLds<HD> tile;
         SplitLds<HD> split;
     } lds;
-    const uint32_t block = (uint32_t)wide_block();
-    if (block >= blocks) return;
+    const uint32_t block = sa.base + blockIdx.x;
     if (block < ta.blocks) tile_block<XT, HD, ROWS>(ta, block, lds.tile, CT{});
     else split_block<XT, CT, HD>(sa, block - ta.blocks, lds.split);
 }
 
 template <class XT, int HD, int ROWS>
-__global__ __launch_bounds__(256) void paged_both_merge(const TileArgs ta, const SplitArgs sa, uint32_t blocks) {
-    const uint32_t block = (uint32_t)wide_block();
-    if (block >= blocks) return;
+__global__ __launch_bounds__(256) void paged_both_merge(const TileArgs ta, const SplitArgs sa) {
+    const uint32_t block = sa.base + blockIdx.x;
     if (block < ta.merge_blocks) tile_merge<XT, HD, ROWS>(ta, block);
     else split_merge<XT, HD>(sa, block - ta.merge_blocks);
 }
@@ -1384,15 +1381,27 @@ TileArgs plan_tile(const PagedArgs &a, int64_t query, int64_t context, int64_t t
     return ta;
 }
 
+// launch(grid) for all of them, from sa.base on.
+template <class F>
+hipError_t launch_blocks(int64_t blocks, SplitArgs &sa, F launch) {
+    hipError_t e = hipSuccess;
+    for (int64_t b = 0; e == hipSuccess && b < blocks; b += kMostBlocks) {
+        sa.base = (uint32_t)b;
+        launch(dim3((unsigned)std::min(blocks - b, kMostBlocks)));
+        e = hipGetLastError();
+    }
+    return e;
+}
+
 template <class XT, class CT, int HD, int ROWS>
-hipError_t launch_both(const TileArgs &ta, const SplitArgs &sa, int64_t split_blocks, int64_t split_merges, hipStream_t s) {
-    const int64_t blocks = ta.blocks + split_blocks;
-    hipLaunchKernelGGL((paged_both<XT, CT, HD, ROWS>), wide_grid(blocks), dim3(256), 0, s, ta, sa, (uint32_t)blocks);
-    const hipError_t e = hipGetLastError();
-    const int64_t merges = ta.merge_blocks + split_merges;
-    if (e != hipSuccess || merges == 0) return e;
-    hipLaunchKernelGGL((paged_both_merge<XT, HD, ROWS>), wide_grid(merges), dim3(256), 0, s, ta, sa, (uint32_t)merges);
-    return hipGetLastError();
+hipError_t launch_both(const TileArgs &ta, SplitArgs &sa, int64_t split_blocks, int64_t split_merges, hipStream_t s) {
+    const hipError_t e = launch_blocks(ta.blocks + split_blocks, sa, [&](dim3 grid) {
+        hipLaunchKernelGGL((paged_both<XT, CT, HD, ROWS>), grid, dim3(256), 0, s, ta, sa);
+    });
+    if (e != hipSuccess) return e;
+    return launch_blocks(ta.merge_blocks + split_merges, sa, [&](dim3 grid) {
+        hipLaunchKernelGGL((paged_both_merge<XT, HD, ROWS>), grid, dim3(256), 0, s, ta, sa);
+    });
 }
 
 template <class XT, class CT, int HD>
@@ -1437,11 +1446,13 @@ hipError_t launch_matrix(tbh_device *dev, const PagedArgs &a, int64_t query, int
             return launch_both<XT, CT, HD, 64>(ta, sa, split_blocks, split_merges, s);
         }
     }
-    hipLaunchKernelGGL((paged_split<XT, CT, HD>), wide_grid(split_blocks), dim3(256), 0, s, sa, (uint32_t)split_blocks);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || split_merges == 0) return e;
-    hipLaunchKernelGGL((paged_split_merge<XT, HD>), wide_grid(split_merges), dim3(256), 0, s, sa, (uint32_t)split_merges);
-    return hipGetLastError();
+    const hipError_t e = launch_blocks(split_blocks, sa, [&](dim3 grid) {
+        hipLaunchKernelGGL((paged_split<XT, CT, HD>), grid, dim3(256), 0, s, sa);
+    });
+    if (e != hipSuccess) return e;
+    return launch_blocks(split_merges, sa, [&](dim3 grid) {
+        hipLaunchKernelGGL((paged_split_merge<XT, HD>), grid, dim3(256), 0, s, sa);
+    });
 }
 
 template <class XT, class CT>
@@ -1456,7 +1467,9 @@ hipError_t launch_paged(tbh_device *dev, const PagedArgs &a, int64_t query, int6
         default: break;
         }
     }
-    hipLaunchKernelGGL((paged_rows<XT, CT>), wide_grid(a.tokens * a.nh), dim3(256), 0, s, a);
+    const int64_t rows = a.tokens * a.nh, across = std::min(rows, kMostBlocks);
+    hipLaunchKernelGGL((paged_rows<XT, CT>), dim3((unsigned)across, (unsigned)((rows + across - 1) / across)), dim3(256), 0,
+                       s, a);
     return hipGetLastError();
 }
 

@@ -48,7 +48,7 @@ struct SampleArgs {
     const int32_t *top_k;
     int32_t *tokens;
     float *probs;
-    int64_t ld, rows;
+    int64_t ld;
     int32_t vocab;
 };
 
@@ -335,8 +335,7 @@ template <bool VEC>
 __global__ __launch_bounds__(kThreads) void sample_rows(const SampleArgs a) {
     __shared__ Shared sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t r = wide_block();
-    if (r >= a.rows) return;
+    const int64_t r = blockIdx.x;
     Row row;
     row.x = a.logits + r * a.ld;
     row.vocab = a.vocab;
@@ -707,12 +706,24 @@ tbh_status check_sample(const char *what, tbh_device *dev, const float *logits, 
     return TBH_OK;
 }
 
-hipError_t launch_sample(const SampleArgs &a, hipStream_t s) {
-    const dim3 grid = wide_grid(a.rows), block(kThreads);
-    const bool vec = ((uintptr_t)a.logits & 15) == 0 && (a.ld % 4 == 0 || a.rows == 1);
-    if (vec) hipLaunchKernelGGL((sample_rows<true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((sample_rows<false>), grid, block, 0, s, a);
-    return hipGetLastError();
+hipError_t launch_sample(SampleArgs a, int64_t rows, hipStream_t s) {
+    const bool vec = ((uintptr_t)a.logits & 15) == 0 && (a.ld % 4 == 0 || rows == 1);
+    while (rows > 0) {
+        const int64_t n = std::min(rows, kMostBlocks);
+        if (vec) hipLaunchKernelGGL((sample_rows<true>), dim3((unsigned)n), dim3(kThreads), 0, s, a);
+        else hipLaunchKernelGGL((sample_rows<false>), dim3((unsigned)n), dim3(kThreads), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        rows -= n;
+        if (rows == 0) break;
+        a.logits += n * a.ld;
+        for (const float **p : {&a.temperature, &a.top_p, &a.min_p, &a.u})
+            if (*p) *p += n;
+        if (a.top_k) a.top_k += n;
+        if (a.probs) a.probs += n;
+        a.tokens += n;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
@@ -728,8 +739,8 @@ tbh_status tbh_sample_device(tbh_device *dev, const float *logits, int64_t ld, i
     tbh_status st = check_sample("tbh_sample", dev, logits, ld, rows, vocab, u, tokens);
     if (st != TBH_OK || rows == 0) return st;
     if ((st = use_device(dev->ordinal)) != TBH_OK) return st;
-    SampleArgs a{logits, temperature, top_p, min_p, u, top_k, tokens, probs, ld, rows, (int32_t)vocab};
-    const hipError_t e = launch_sample(a, (hipStream_t)stream);
+    SampleArgs a{logits, temperature, top_p, min_p, u, top_k, tokens, probs, ld, (int32_t)vocab};
+    const hipError_t e = launch_sample(a, rows, (hipStream_t)stream);
     return e == hipSuccess ? TBH_OK : hip_error(e, "sample launch");
 }
 
@@ -751,8 +762,8 @@ tbh_status tbh_sample(tbh_device *dev, const float *logits, int64_t rows, int64_
                        out.data(), 2 * n, [&](const std::vector<const void *> &d, void *o, hipStream_t s) {
                            SampleArgs a{(const float *)d[0], (const float *)d[1], (const float *)d[3],
                                         (const float *)d[4], (const float *)d[5], (const int32_t *)d[2],
-                                        (int32_t *)o, (float *)o + rows, vocab, rows, (int32_t)vocab};
-                           return launch_sample(a, s);
+                                        (int32_t *)o, (float *)o + rows, vocab, (int32_t)vocab};
+                           return launch_sample(a, rows, s);
                        });
         if (st != TBH_OK) return st;
         std::copy(out.begin(), out.begin() + rows, tokens);
