@@ -1,5 +1,6 @@
 // tbh_paged_attn.hip -- attention of a step's new tokens over a paged cache
-// (tbh_paged_attention_device).
+// (tbh_paged_attention_device).  Figures: us a call among others, both of its
+// launches; where a trace is named, one launch from its first wave to its last.
 #include <algorithm>
 #include <cmath>
 
@@ -145,8 +146,8 @@ __device__ __forceinline__ void store_row(const PagedArgs &a, int64_t t, int hea
 // Any head dimension, block size and alignment: a block per (token, query head),
 // whose four waves take passes of 64 positions in turn and meet in LDS.  Bound by
 // the latency of its loads.  us, bf16 cache, 32 heads on 8 of 80: 130 for a row over
-// 4000 positions (381 with one wave a row), 120 for 64 rows over 1000 (143), 278 for
-// 256 rows over 1024 (292); heads of 256: 210 (708), 324 (301), 641 (647).
+// 4000 positions (381 with one wave a row), 119 for 64 rows over 1000 (143), 265 for
+// 256 rows over 1024 (292); heads of 256: 210 (708), 313 (301), 630 (647).
 template <class XT, class CT>
 __global__ __launch_bounds__(256) void paged_rows(const PagedArgs a) {
     __shared__ float qs[4][kMaxHeadDim], so[4][kMaxHeadDim];
@@ -317,6 +318,13 @@ __device__ __forceinline__ float row4_sum(float v) {
 }
 
 // x as a sum of NP bf16 values: exact for NP = 3 (8 + 8 + 8 bits), rounded for 1.
+// One for bf16 rows, whose q is exact so and whose probabilities are rounded, each
+// off by at most 2^-8 of itself.  The sum that divides is that of the rounded ones
+// (split_block: of the exact ones), so a result is off by at most 2^-8 of sum p |v -
+// out| (of sum p |v|), as much as its own rounding to bf16 where values are about as
+// large as their mean, more where they cancel: against 64 bits 2.2e-3 over 2048 rows
+// over 4096 positions, 1.7e-3 with exact probabilities, whose three products take
+// 253 us for 116.  fp32 rows keep fp32's precision.
 template <int NP>
 __device__ __forceinline__ void pieces(float x, __bf16 (&p)[NP]) {
     p[0] = (__bf16)x;
@@ -853,10 +861,12 @@ __device__ __forceinline__ void rows_apart(const TileArgs &ta, const Group &gr, 
 // pieces of keys by the row, 32-byte pieces of values likewise, so that both
 // reads touch every bank once; the copies permute their global addresses for it.
 // Bound by the matrix instructions and the exponentials that they wait for: 2048
-// rows over 4096 positions, 32 heads on 8 of 128, bf16 throughout 128 to 132 us, 103
-// GFLOP at 780 to 805 TFLOP/s (a large product: 1143).  Prompts of 150 .. 301 fp32
-// rows of 12 heads of 64: 17 us, in which launch, look-ups and the first tile count
-// for more than the three pieces' products.
+// rows over 4096 positions, 32 heads on 8 of 128, bf16 throughout 116 to 120 us, 103
+// GFLOP at 860 to 890 TFLOP/s (a large product: 1143); in a trace 133, of whose cycles
+// matrix instructions take 38 in a hundred and vector instructions 40, with no LDS
+// conflicts.  Prompts of 150 .. 301 fp32 rows of 12 heads of 64: 17 us in a trace, in
+// which launch, look-ups and the first tile count for more than the three pieces'
+// products.
 template <int HD>
 struct TileLds {
     __attribute__((aligned(256))) unsigned char k[2][64 * HD * 2], v[2][64 * HD * 2];   // 32 positions of fp32
@@ -1106,8 +1116,8 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
 // every 64 to a lane, so that 16 lanes read 256 bytes of a value row at once;
 // keys' 16-byte pieces are swizzled by the row.  A tile's values are summed before
 // they join the running sums: an eighth of the roundings.  31 single tokens and a
-// chunk of 333, 32 heads on 4 of 64, fp32: 25 us with split_block's share, 7 tiles of
-// 32 positions a block, each a wait and 64 matrix instructions of 32 cycles.
+// chunk of 333, 32 heads on 4 of 64, fp32: 26 us in a trace with split_block's share, 7
+// tiles of 32 positions a block, each a wait and 64 matrix instructions of 32 cycles.
 template <class XT, int HD, int ROWS>
 __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, TileLds<HD> &lds, float) {
     static_assert(ROWS == 64, "16 rows a wave");
@@ -1289,7 +1299,7 @@ __device__ __forceinline__ void tile_block(const TileArgs &ta, uint32_t block, T
     rows_apart<XT, float, HD, ROWS>(ta, gr, unit, split, ct.parts, c0, c1, wrow, wrows, qs[w]);
 }
 
-// Joins tile_block's parts: HD / 4 threads a row.  Bound by latency: 5 us after the
+// Joins tile_block's parts: HD / 4 threads a row.  Bound by latency: 5 us in a trace after the
 // prompts above and after the mixed batch, with split_merge's share.  (Eight parts'
 // loads in flight at once: no difference.)
 template <class XT, int HD, int ROWS>
@@ -1354,8 +1364,8 @@ __global__ __launch_bounds__(256) void paged_both_merge(const TileArgs ta, const
 bool fills(int64_t tiles, int64_t cus) { return 10 * tiles >= 9 * 2 * cus; }
 
 // Parts of tile_block's tiles: none where they fill the chip (2048 rows over 4096
-// positions, when they took 168 us: 203 in two parts, 244 in four: partials of fp32 rows cost more than
-// evener blocks gain), else enough to fill it twice over, of at least 256 positions (a
+// positions, on an earlier tile: 1.2 times the time in two parts, 1.45 in four: partials of fp32 rows
+// cost more than evener blocks gain), else enough to fill it twice over, of at least 256 positions (a
 // chunk of 8 rows over 4096: 16 us, 71 without; 600 over 4000 81, 89 without).
 TileArgs plan_tile(const PagedArgs &a, int64_t query, int64_t context, int64_t tile_rows, size_t elem, int64_t cus) {
     TileArgs ta{};
@@ -1409,8 +1419,12 @@ hipError_t launch_matrix(tbh_device *dev, const PagedArgs &a, int64_t query, int
     const int64_t cus = std::max(1, dev->cu_count);
     // More than one group of 16 rows: tiles, or else groups apart.  us, bf16 throughout, 32
     // heads on 8 of 128: 8 chunks of 5 rows over 2000 positions 24 in tiles and 29 in groups,
-    // 64 of 5 over 1000 50 and 56, 8 of 16 over 2000 27 and 39; fp32, 32 on 4 of 64: a chunk
-    // of 8 over 4096 23 and 21, 8 of 16 over 2000 34 and 46.
+    // 64 of 5 over 1000 50 and 56, 8 of 16 over 2000 27 and 39, a chunk of 32 over 1024 14 and
+    // 17.  fp32, 32 on 4 of 64, gains from more rows on and loses before: a chunk of 8 over 4096
+    // 23.0 and 20.5, one of 32 over 1024 21.1 and 15.9, 64 chunks of 5 over 1000 60.8 and 58.9, 8
+    // of 5 and of 8 over 2000 30.6 and 30.0, 31.5 and 31.8, 8 of 16 33.9 and 45.9.  Heads of 32 and
+    // 96 have no tile kernel: every 16 rows read the context (2048 rows over 4096: 188 and 375 us,
+    // 82 at heads of 64, 116 at 128).
     const bool tiles = (HD == 64 || HD == 128) && query * a.rep > 16;
     SplitArgs sa = plan_split(a, query, context, tiles, sizeof(XT), cus);
     TileArgs ta{};
