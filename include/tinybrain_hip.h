@@ -475,7 +475,7 @@ tbh_status tbh_attention_device(tbh_device *dev, const tbh_attention_shape *shap
  * Request b is row b of block_table [max_requests][max_blocks]; its position p
  * lies in block block_table[b][p / block_size] at row p % block_size, and the
  * slot of that place is block * block_size + p % block_size. */
-enum { TBH_F32 = 0, TBH_BF16 = 1 };   /* element types of the cache and of rows */
+enum { TBH_F32 = 0, TBH_BF16 = 1 };   /* element types of the cache, of rows and of activations */
 
 typedef struct tbh_paged_layout {
     int32_t num_blocks;      /* blocks in each array; num_blocks * block_size < 2^31 */
@@ -582,6 +582,87 @@ tbh_status tbh_paged_attention_device(tbh_device *dev, const tbh_paged_layout *l
                                       const tbh_paged_queries *queries, const void *k_cache, const void *v_cache,
                                       const int32_t *block_table, void *stream);
 
+/* ---- products with block-scaled FP8 weights ------------------------------ */
+/* A third stored format beside INT8 and INT4 (no reference counterpart: its
+ * weights are INT8 or INT4): e4m3 bytes (1 sign, 4 exponent, 3 mantissa bits,
+ * largest value 448, no infinities; 0x7F and 0xFF are NaN) with one fp32 scale
+ * for each block of 128 outputs by 128 inputs.  Element (k, n) of the [K, N]
+ * weight is data[n * K + k] * scales[(n / 128) * ceil(K / 128) + k / 128].
+ * data and scales may be host or device pointers; device data has to be there
+ * before the call.  Copied and repacked once. */
+typedef struct tbh_fp8_desc {
+    int64_t K;                  /* up to 2^20 */
+    int64_t N;                  /* up to 2^24 */
+    const uint8_t *data;        /* [N][K] */
+    const float *scales;        /* [ceil(N / 128)][ceil(K / 128)] */
+} tbh_fp8_desc;
+typedef struct tbh_fp8_weight tbh_fp8_weight;
+tbh_status tbh_fp8_weight_create(tbh_device *dev, const tbh_fp8_desc *desc, tbh_fp8_weight **out);
+/* Destroy before the device is closed, as weights are. */
+tbh_status tbh_fp8_weight_destroy(tbh_fp8_weight *w);
+
+/* y[M, N] = x[M, K] . W[K, N] in 8-bit floating point: x (TBH_F32 or TBH_BF16,
+ * rows x_stride elements apart) is quantized to e4m3 as well, with a scale for each row and block b of 128 inputs: s = the least power of two
+ * (at least 2^-126) with |x| <= 448 s over the block's finite elements, q =
+ * x / s rounded once, ties to even; an infinity or NaN becomes NaN.
+ *   y[m][n] = sum over b of s[m][b] * scale[n / 128][b] * (q . w of block b)
+ * summed in fp32, rounded once to y_type.  A TBH_BF16 result of more than 32
+ * rows takes q . w from the FP8 matrix instruction, which cuts its sums (about
+ * 2^-15 of their size; rounding to bf16 then does 2^-9); all others have fp32
+ * sums on the bf16 instruction, to which q and w are widened exactly.  (Products of two scales outside
+ * fp32's normal range lose precision or overflow.)
+ * Past 32 rows x is quantized into `workspace` (256-byte aligned,
+ * tbh_fp8_matmul_workspace bytes for M rows), or, if that is NULL, into the
+ * workspace of (device, stream), with tbh_matmul_device's rule for captured
+ * graphs; where none can be had (a capture before any eager call on its
+ * stream) the rows run 16 at a time without it. */
+tbh_status tbh_fp8_matmul_workspace(const tbh_fp8_weight *w, int64_t M, int64_t *bytes);
+tbh_status tbh_fp8_matmul_device(const tbh_fp8_weight *w, const void *x, int32_t x_type, int64_t M, int64_t K,
+                                 int64_t x_stride, void *y, int32_t y_type, int64_t y_stride, void *workspace,
+                                 int64_t workspace_bytes, void *stream);
+
+/* ---- mixture-of-experts layer ---------------------------------------------- */
+/* The feed-forward layer of a mixture-of-experts model on block-scaled FP8
+ * weights, beside the dense one of the decode step (no reference counterpart:
+ * its FFN is dense, ModelRunner.swift:445-457).  For a token's row x:
+ *   z = x . router^T in 64-bit sums; its experts are the top_k largest z (of
+ *   equal ones the lowest), with weights p_e = exp(z_e) / sum of exp(z) over
+ *   all experts, or over the chosen ones (normalize)
+ *   y = sum over its experts of p_e (silu(x . G_e) * (x . U_e)) . D_e
+ * Activations are not quantized: bf16 rows are taken as they are (h is rounded
+ * to bf16 once, y once from fp32), fp32 rows keep fp32's precision throughout.
+ * Made for few tokens, where reading the chosen experts is what takes time: an
+ * expert's weights are read once for up to 64 tokens, more run 64 at a time.
+ * A row that holds an infinity or NaN gets NaN; which experts it is given then
+ * means nothing.  Other rows are not touched by it. */
+typedef struct tbh_moe_desc {
+    int32_t hidden;             /* H, up to 2^17 */
+    int32_t intermediate;       /* I, up to 2^17 */
+    int32_t experts;            /* E, up to 512 */
+    int32_t reserved;           /* 0 */
+    const float *router;        /* [E][H] */
+    const uint8_t *gate;        /* [E][I][H] e4m3, each expert as a tbh_fp8_desc's data */
+    const uint8_t *up;          /* [E][I][H] */
+    const uint8_t *down;        /* [E][H][I] */
+    const float *gate_scales;   /* [E][ceil(I / 128)][ceil(H / 128)] */
+    const float *up_scales;
+    const float *down_scales;   /* [E][ceil(H / 128)][ceil(I / 128)] */
+} tbh_moe_desc;
+typedef struct tbh_moe tbh_moe;
+/* Host or device pointers, copied and repacked once (as tbh_fp8_weight_create). */
+tbh_status tbh_moe_create(tbh_device *dev, const tbh_moe_desc *desc, tbh_moe **out);
+tbh_status tbh_moe_destroy(tbh_moe *m);
+/* x and y: [tokens][H] of x_type, rows x_stride and y_stride elements apart; y
+ * does not overlap x.  experts, weights [tokens][top_k] (each may be NULL):
+ * what the router chose, largest first.  top_k up to 32.  workspace:
+ * 256-byte aligned, tbh_moe_workspace bytes, or NULL for the one of (device,
+ * stream), with tbh_matmul_device's rule for captured graphs; a capture before
+ * any eager call on its stream finds none (TBH_E_OOM). */
+tbh_status tbh_moe_workspace(const tbh_moe *m, int32_t x_type, int64_t tokens, int32_t top_k, int64_t *bytes);
+tbh_status tbh_moe_device(const tbh_moe *m, const void *x, int32_t x_type, int64_t tokens, int64_t x_stride,
+                          int32_t top_k, int32_t normalize, void *y, int64_t y_stride, int32_t *experts,
+                          float *weights, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- sampling ---------------------------------------------------------- */
 /* Sampler (Sampler.swift) with the random numbers given by the caller: one
  * token per row of `logits` [rows][ld] (ld >= vocab).  With w_i =
@@ -607,6 +688,56 @@ tbh_status tbh_sample(tbh_device *dev, const float *logits, int64_t rows, int64_
 tbh_status tbh_sample_device(tbh_device *dev, const float *logits, int64_t ld, int64_t rows, int64_t vocab,
                              const float *temperature, const int32_t *top_k, const float *top_p,
                              const float *min_p, const float *u, int32_t *tokens, float *probs, void *stream);
+
+/* ---- beam search -------------------------------------------------------------- */
+/* Beside sampling, the other way to go on (no reference counterpart: its Sampler
+ * draws one token).  Request r has the rows r * beams .. r * beams + beams - 1
+ * of logits [requests * beams][ld] (ld >= vocab), scores (the sums of log
+ * probabilities so far) and done (nonzero: the row has ended; NULL: none).  Its
+ * candidates are, of each row b,
+ *   not done: every token j, with scores[b] + logit_j - log(sum of exp(logit))
+ *   done:     the token eos, with scores[b]
+ * and the k best of them, best first, are its tokens, parents (rows, as
+ * counted over the whole call) and scores_out, [requests][k] each; equal ones:
+ * the lowest row, then the lowest token.  Sums and comparisons are in 64 bits.
+ * done_out (or NULL) [requests][k]: 1 for the token eos and children of a done
+ * row.  NaN and -inf logits are never taken and weigh nothing (+inf ones share
+ * all of the weight); a row whose score is not finite has no candidates.  Where
+ * there are fewer than k: token and parent -1, score -inf, not done.
+ * With scores, done and parents of one call as the next one's, k = beams.
+ * The outputs overlap no input.  beams and k up to 64, vocab and rows up to
+ * 2^20 (TBH_E_UNSUPPORTED).  workspace: 256-byte aligned,
+ * tbh_beam_select_workspace bytes, or NULL for the one of (device, stream), with
+ * tbh_matmul_device's rule for captured graphs; a capture before any eager call
+ * on its stream finds none (TBH_E_OOM). */
+tbh_status tbh_beam_select_workspace(tbh_device *dev, int64_t requests, int32_t beams, int64_t vocab, int32_t k,
+                                     int64_t *bytes);
+tbh_status tbh_beam_select_device(tbh_device *dev, const float *logits, int64_t ld, int64_t requests, int32_t beams,
+                                  int64_t vocab, const float *scores, const int32_t *done, int32_t eos, int32_t k,
+                                  int32_t *tokens, int32_t *parents, float *scores_out, int32_t *done_out,
+                                  void *workspace, int64_t workspace_bytes, void *stream);
+
+/* The paged cache after a selection: row i of the block table goes on where row
+ * parents[i] stood.  Rows come in groups of `beams` (up to 64), parents lie in
+ * their own group; -1: nobody's child.  In each group
+ *   - a parent's table row goes to itself if it is its own child, else to its
+ *     first child;
+ *   - the other rows get the table rows that no parent holds, in order, and the
+ *     contents of their parent's positions shared_lens[group] (rounded down to
+ *     whole blocks; NULL: 0) .. context are copied into those blocks, in every
+ *     layer's arrays.  Positions before shared_lens are taken to be the same in
+ *     the whole group: a prompt's.
+ * So blocks stay with the group and nothing is allocated.  The rows of a group
+ * hold equally many tokens (context_lens); a group whose rows do not, or with a
+ * parent outside it, is left as it is.  reordered[groups] (or NULL): 1, or 0 for
+ * such a group.  table_out [max_requests][max_blocks] is block_table itself or
+ * does not overlap it.  k_caches and v_caches: host arrays of `layers` device
+ * pointers.  Places behind a context are not touched.  Block ids outside the
+ * cache are not followed. */
+tbh_status tbh_paged_reorder_device(tbh_device *dev, const tbh_paged_layout *layout, int32_t beams,
+                                    const int32_t *parents, const int32_t *context_lens, const int32_t *shared_lens,
+                                    const int32_t *block_table, int32_t *table_out, int32_t layers,
+                                    void *const *k_caches, void *const *v_caches, int32_t *reordered, void *stream);
 
 #ifdef __cplusplus
 }

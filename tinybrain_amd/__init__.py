@@ -14,6 +14,7 @@ from .quantized import (Layout, PreconditionFailure, QuantizationMode,  # noqa: 
                         quantize, quantize_int4_flat, unpackInt4,
                         unpack_int4_array, pack_int4_array)
 from .backend import DeviceWeight, HIPBackend, HIPBackendError  # noqa: F401
+from .fp8 import FP8Tensor, FP8Weight, MoELayer, quantize_fp8  # noqa: F401
 from .decoder import Decoder, DecoderConfig  # noqa: F401
 from .linear import LinearLayerWeights  # noqa: F401
 from .paged import PagedKVCache, PagedPlan  # noqa: F401
@@ -21,7 +22,7 @@ from .tbf import TBFFile  # noqa: F401
 
 __all__ = [
     "HIPBackend", "HIPBackendError", "DeviceWeight", "QuantizedTensor", "LinearLayerWeights", "Decoder", "DecoderConfig", "TBFFile",
-    "PagedKVCache", "PagedPlan",
+    "PagedKVCache", "PagedPlan", "FP8Tensor", "FP8Weight", "MoELayer", "quantize_fp8",
     "QuantizationMode", "QuantizationPrecision", "Layout", "PreconditionFailure",
     "quantize", "quantize_int4_flat", "packInt4", "unpackInt4",
 ]

@@ -40,7 +40,10 @@ EXPORTS = [
     "tbh_silu", "tbh_silu_device", "tbh_gelu", "tbh_gelu_device",
     "tbh_attention", "tbh_attention_device",
     "tbh_paged_plan_device", "tbh_paged_append_device", "tbh_paged_attention_device",
+    "tbh_fp8_weight_create", "tbh_fp8_weight_destroy", "tbh_fp8_matmul_workspace", "tbh_fp8_matmul_device",
+    "tbh_moe_create", "tbh_moe_destroy", "tbh_moe_workspace", "tbh_moe_device",
     "tbh_sample", "tbh_sample_device",
+    "tbh_beam_select_workspace", "tbh_beam_select_device", "tbh_paged_reorder_device",
 ]
 
 
@@ -95,6 +98,20 @@ class PagedQueries(ctypes.Structure):
         ("max_query_len", ctypes.c_int32),
         ("max_context_len", ctypes.c_int32),
     ]
+
+
+class FP8Desc(ctypes.Structure):
+    _fields_ = [
+        ("K", ctypes.c_int64),
+        ("N", ctypes.c_int64),
+        ("data", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+    ]
+
+
+class MoEDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("hidden", "intermediate", "experts", "reserved")] + \
+        [(n, ctypes.c_void_p) for n in ("router", "gate", "up", "down", "gate_scales", "up_scales", "down_scales")]
 
 
 class QTensorDesc(ctypes.Structure):
@@ -243,6 +260,22 @@ def lib() -> ctypes.CDLL:
     L.tbh_paged_attention_device.argtypes = [vp] * 7
     L.tbh_sample.argtypes = [vp, vp, i64, i64] + [vp] * 7
     L.tbh_sample_device.argtypes = [vp, vp, i64, i64, i64] + [vp] * 8
+    pi64 = ctypes.POINTER(i64)
+    L.tbh_fp8_weight_create.argtypes = [vp, ctypes.POINTER(FP8Desc), pp]
+    L.tbh_fp8_weight_destroy.argtypes = [vp]
+    L.tbh_fp8_matmul_workspace.argtypes = [vp, i64, pi64]
+    L.tbh_fp8_matmul_device.argtypes = [vp, vp, i32, i64, i64, i64, vp, i32, i64, vp, i64, vp]
+    L.tbh_moe_create.argtypes = [vp, ctypes.POINTER(MoEDesc), pp]
+    L.tbh_moe_destroy.argtypes = [vp]
+    L.tbh_moe_workspace.argtypes = [vp, i32, i64, i32, pi64]
+    L.tbh_moe_device.argtypes = [vp, vp, i32, i64, i64, i32, i32, vp, i64, vp, vp, vp, i64, vp]
+    L.tbh_beam_select_workspace.argtypes = [vp, i64, i32, i64, i32, pi64]
+    L.tbh_beam_select_device.argtypes = [vp, vp, i64, i64, i32, i64, vp, vp, i32, i32] + [vp] * 5 + [i64, vp]
+    L.tbh_paged_reorder_device.argtypes = [vp, vp, i32] + [vp] * 5 + [i32] + [vp] * 4
+    for name in ("tbh_fp8_weight_create", "tbh_fp8_weight_destroy", "tbh_fp8_matmul_workspace",
+                 "tbh_fp8_matmul_device", "tbh_moe_create", "tbh_moe_destroy", "tbh_moe_workspace", "tbh_moe_device",
+                 "tbh_beam_select_workspace", "tbh_beam_select_device", "tbh_paged_reorder_device"):
+        getattr(L, name).restype = i32
     for name in ("tbh_paged_plan_device", "tbh_paged_append_device", "tbh_paged_attention_device",
                  "tbh_sample", "tbh_sample_device"):
         getattr(L, name).restype = i32

@@ -37,6 +37,7 @@ from typing import Dict, Optional, Sequence
 import numpy as np
 
 from . import _abi
+from .fp8 import FP8Weight, MoELayer
 from .paged import PagedPlan
 from .quantized import PreconditionFailure, QuantizedTensor
 
@@ -601,6 +602,86 @@ class HIPBackend:
         n, nkv, bs, hd = shape
         return n, nkv, bs, hd, self._paged_type(keys)
 
+    # -- products with block-scaled FP8 weights, mixture of experts (see fp8.py) ----
+    def fp8_weight(self, data, scales=None) -> FP8Weight:
+        """An FP8 weight, repacked once: an FP8Tensor, or e4m3 data [N, K] with
+        scales [ceil(N / 128), ceil(K / 128)] (numpy arrays, or torch tensors)."""
+        return FP8Weight(self, data, scales)
+
+    def fp8_matmul_device(self, x, weight: FP8Weight, dtype=None, out=None, stream=None):
+        """tbh_fp8_matmul_device: y = x . W with x [M, K] (float32 or bfloat16;
+        rows may be strided) quantized to e4m3 per row and 128 inputs; y [M, N]
+        of `dtype` (x's unless given) or like out."""
+        import torch
+
+        rows, k = self._row_shape(x)
+        if k != weight.K:
+            raise PreconditionFailure("Dimensions must match")
+        if out is None:
+            out = self._made(stream, x.new_empty, (rows, weight.N), dtype=x.dtype if dtype is None else dtype)
+        elif self._row_shape(out) != (rows, weight.N) or (dtype is not None and out.dtype != dtype):
+            raise PreconditionFailure("fp8: out must be [M, N] of the type asked for")
+        xt, yt = self._paged_type(x), self._paged_type(out)
+        room, size = None, 0
+        if rows > 32 and torch.cuda.is_current_stream_capturing():
+            need = ctypes.c_int64()
+            _check(self._lib.tbh_fp8_matmul_workspace(weight.handle, rows, ctypes.byref(need)))
+            room, size = self._room(stream, x, need.value)
+        _check(self._lib.tbh_fp8_matmul_device(
+            weight.handle, x.data_ptr(), xt, rows, k, x.stride(0), out.data_ptr(), yt, out.stride(0),
+            None if room is None else room.data_ptr(), size, self._raw_stream(stream)))
+        return out
+
+    def moe_layer(self, router, gate, gateScales, up, upScales, down, downScales) -> MoELayer:
+        """A mixture-of-experts layer, repacked once: router float32 [experts,
+        hidden], e4m3 gate and up [experts, intermediate, hidden] and down
+        [experts, hidden, intermediate], each with its scales per block of 128 x 128
+        (numpy arrays, or torch tensors)."""
+        return MoELayer(self, router, gate, gateScales, up, upScales, down, downScales)
+
+    def moe_device(self, x, layer: MoELayer, topK: int, normalize: bool = True, out=None, experts=None, weights=None,
+                   stream=None):
+        """tbh_moe_device on rows x [tokens, hidden] (float32 or bfloat16, may be
+        strided): (y like x, experts int32 [tokens, topK], weights float32
+        [tokens, topK]); normalize: a token's weights sum to 1."""
+        import torch
+
+        tokens, width = shape = self._row_shape(x)
+        if width != layer.hidden:
+            raise PreconditionFailure("moe: x must be [tokens, hidden]")
+        xt = self._paged_type(x)
+        if not 0 < topK <= layer.experts:
+            raise PreconditionFailure("moe: topK must be 1 .. experts")
+        if out is None:
+            out = self._made(stream, x.new_empty, shape)
+        elif self._row_shape(out) != shape or out.dtype != x.dtype:
+            raise PreconditionFailure("moe: out must be like x")
+        if experts is None:
+            experts = self._made(stream, x.new_empty, (tokens, topK), dtype=torch.int32)
+        if weights is None:
+            weights = self._made(stream, x.new_empty, (tokens, topK), dtype=torch.float32)
+        for t, dtype in ((experts, torch.int32), (weights, torch.float32)):
+            if t.dtype != dtype or tuple(t.shape) != (tokens, topK) or not t.is_contiguous() \
+                    or t.get_device() != self.device:
+                raise PreconditionFailure("moe: experts int32 and weights float32 must be contiguous [tokens, topK]")
+        room, size = None, 0
+        if torch.cuda.is_current_stream_capturing():
+            need = ctypes.c_int64()
+            _check(self._lib.tbh_moe_workspace(layer.handle, xt, tokens, topK, ctypes.byref(need)))
+            room, size = self._room(stream, x, need.value)
+        _check(self._lib.tbh_moe_device(
+            layer.handle, x.data_ptr(), xt, tokens, x.stride(0), topK, bool(normalize), out.data_ptr(), out.stride(0),
+            experts.data_ptr(), weights.data_ptr(), None if room is None else room.data_ptr(), size,
+            self._raw_stream(stream)))
+        return out, experts, weights
+
+    def _room(self, stream, like, size: int):
+        """A graph under capture gets memory of its own (its pool's), so that it
+        needs no eager call before it and shares nothing with other graphs."""
+        import torch
+
+        return self._made(stream, like.new_empty, max(size, 1), dtype=torch.uint8), size
+
     # -- Sampler (Sampler.swift) with the caller's random numbers ----------------
     def sample(self, logits: np.ndarray, u, temperature=1.0, topK=0, topP=1.0, minP=0.0):
         """tbh_sample on host arrays: logits [rows, vocab] or [vocab], u and
@@ -649,6 +730,90 @@ class HIPBackend:
             topP.data_ptr() if topP is not None else None, minP.data_ptr() if minP is not None else None, u.data_ptr(),
             tokens.data_ptr(), probs.data_ptr(), self._raw_stream(stream)))
         return tokens, probs
+
+    # -- beam search ----------------------------------------------------------------
+    def beam_select_device(self, logits, scores, beams: int, k: Optional[int] = None, done=None, eos: int = -1,
+                           stream=None):
+        """tbh_beam_select_device: the k (beams unless given) best continuations of
+        each request's `beams` rows of logits float32 [requests * beams, vocab]
+        (rows may be strided), scores float32 and done int32 (or None)
+        [requests * beams].  Returns (tokens int32, parents int32, scores float32,
+        done int32), each [requests, k]; a missing one is -1, -1, -inf, 0."""
+        import torch
+
+        if logits.dtype != torch.float32:
+            raise PreconditionFailure("beam search: logits must be float32")
+        rows, vocab = self._row_shape(logits)
+        k = beams if k is None else k
+        if beams <= 0 or rows % beams or k <= 0:
+            raise PreconditionFailure("beam search: rows must be a multiple of beams, k positive")
+        if max(beams, k, abs(eos)) >= 1 << 31:
+            raise self._past_32_bits()
+        for t, dtype in ((scores, torch.float32), (done, torch.int32)):
+            if t is not None and (t.dtype != dtype or t.numel() != rows or not t.is_contiguous()
+                                  or t.get_device() != self.device):
+                raise PreconditionFailure("beam search: scores float32 and done int32 must be contiguous, one entry per row")
+        n = rows // beams
+        ints = self._made(stream, scores.new_empty, (3, n, k), dtype=torch.int32)
+        best = self._made(stream, scores.new_empty, (n, k))
+        room, size = None, 0
+        if torch.cuda.is_current_stream_capturing():
+            need = ctypes.c_int64()
+            _check(self._lib.tbh_beam_select_workspace(self._dev, n, beams, vocab, k, ctypes.byref(need)))
+            room, size = self._room(stream, scores, need.value)
+        at, step = ints.data_ptr(), 4 * n * k
+        _check(self._lib.tbh_beam_select_device(
+            self._dev, logits.data_ptr(), logits.stride(0), n, beams, vocab, scores.data_ptr(),
+            None if done is None else done.data_ptr(), eos, k, at, at + step, best.data_ptr(), at + 2 * step,
+            None if room is None else room.data_ptr(), size, self._raw_stream(stream)))
+        tokens, parents, ended = ints.unbind(0)
+        return tokens, parents, best, ended
+
+    def paged_reorder_device(self, keys, values, blockTable, contextLens, parents, beams: int, sharedLens=None,
+                             tableOut=None, reordered=None, stream=None):
+        """tbh_paged_reorder_device: rows of blockTable [requests, blocks] (groups of
+        `beams`) go on where their parents [requests] stood, in the cache arrays of
+        every layer (sequences keys and values).  sharedLens [requests / beams]:
+        positions that are the same in a group, not copied.  Returns the new table:
+        tableOut (blockTable itself: in place), else a new tensor."""
+        import torch
+
+        if len(keys) != len(values) or not len(keys):
+            raise PreconditionFailure("reorder: one array of keys and one of values per layer")
+        n, nkv, bs, hd, ct = self._kv_arrays(keys[0], values[0])
+        shape, dtype = keys[0].shape, keys[0].dtype
+        for a in (*keys[1:], *values[1:]):
+            if a.shape != shape or a.dtype != dtype or not a.is_contiguous() or a.get_device() != self.device:
+                raise PreconditionFailure("reorder: every layer's arrays must be alike")
+        self._ints(torch.int32, blockTable, contextLens, parents)
+        b = contextLens.numel()
+        if beams <= 0 or b % beams:
+            raise PreconditionFailure("reorder: requests must be a multiple of beams")
+        if blockTable.dim() != 2 or blockTable.shape[0] != b or parents.numel() != b:
+            raise PreconditionFailure("reorder: parents and block table must have one row per request")
+        for t in (sharedLens, reordered):
+            if t is not None:
+                self._ints(torch.int32, t)
+                if t.numel() != b // beams:
+                    raise PreconditionFailure("reorder: sharedLens and reordered must have one entry per group")
+        if tableOut is None:
+            tableOut = self._made(stream, torch.empty_like, blockTable)
+        else:
+            self._ints(torch.int32, tableOut)
+            if tableOut.shape != blockTable.shape:
+                raise PreconditionFailure("reorder: tableOut must be like the block table")
+        try:
+            layout = self._layout.pack(n, bs, nkv, hd, ct, b, blockTable.shape[1])
+        except struct.error:
+            raise self._past_32_bits() from None
+        layers = len(keys)
+        pointers = ctypes.c_void_p * layers
+        _check(self._lib.tbh_paged_reorder_device(
+            self._dev, layout, beams, parents.data_ptr(), contextLens.data_ptr(),
+            None if sharedLens is None else sharedLens.data_ptr(), blockTable.data_ptr(), tableOut.data_ptr(), layers,
+            pointers(*[a.data_ptr() for a in keys]), pointers(*[a.data_ptr() for a in values]),
+            None if reordered is None else reordered.data_ptr(), self._raw_stream(stream)))
+        return tableOut
 
     def close(self) -> None:
         with self._lock:

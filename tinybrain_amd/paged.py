@@ -80,3 +80,14 @@ class PagedKVCache:
                                                    plan.queryStart, plan.contextLens, numHeads, scale=scale,
                                                    maxQueryLen=maxQueryLen, maxContextLen=maxContextLen, out=out,
                                                    stream=stream)
+
+    def reorder(self, parents, beams: int, sharedLens=None, reordered=None, stream=None) -> None:
+        """Lets row i of every group of `beams` requests go on where row parents[i]
+        stood (a beam search's selection), in place: the block table, and in every
+        layer the contents of rows that several follow.  sharedLens [groups]: lengths
+        of the prompts that a group's rows share.  The rows of a group hold
+        equally many tokens; else, or with a parent outside its group, it is left
+        as it is (reordered [groups], if given: 0)."""
+        self.backend.paged_reorder_device(self.keys, self.values, self.blockTable, self.contextLens, parents, beams,
+                                          sharedLens=sharedLens, tableOut=self.blockTable, reordered=reordered,
+                                          stream=stream)
