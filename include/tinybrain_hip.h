@@ -655,9 +655,11 @@ tbh_status tbh_moe_destroy(tbh_moe *m);
 /* x and y: [tokens][H] of x_type, rows x_stride and y_stride elements apart; y
  * does not overlap x.  experts, weights [tokens][top_k] (each may be NULL):
  * what the router chose, largest first.  top_k up to 32.  workspace:
- * 256-byte aligned, tbh_moe_workspace bytes, or NULL for the one of (device,
- * stream), with tbh_matmul_device's rule for captured graphs; a capture before
- * any eager call on its stream finds none (TBH_E_OOM). */
+ * 256-byte aligned, tbh_moe_workspace bytes, of which the first
+ * TBH_WORKSPACE_COUNTERS are zero (calls leave them so), or NULL for the one of
+ * (device, stream), with tbh_matmul_device's rule for captured graphs; a capture
+ * before any eager call on its stream finds none (TBH_E_OOM). */
+enum { TBH_WORKSPACE_COUNTERS = 32768 };
 tbh_status tbh_moe_workspace(const tbh_moe *m, int32_t x_type, int64_t tokens, int32_t top_k, int64_t *bytes);
 tbh_status tbh_moe_device(const tbh_moe *m, const void *x, int32_t x_type, int64_t tokens, int64_t x_stride,
                           int32_t top_k, int32_t normalize, void *y, int64_t y_stride, int32_t *experts,

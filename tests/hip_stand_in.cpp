@@ -155,6 +155,15 @@ hipError_t hipMemcpyAsync(void *to, const void *from, size_t n, hipMemcpyKind, h
     std::memcpy(to, from, n);
     return hipSuccess;
 }
+hipError_t hipMemcpy2DAsync(void *to, size_t tp, const void *from, size_t fp, size_t width, size_t rows, hipMemcpyKind,
+                            hipStream_t) {
+    for (size_t r = 0; r < rows; ++r) std::memcpy((char *)to + r * tp, (const char *)from + r * fp, width);
+    return hipSuccess;
+}
+hipError_t hipMemsetAsync(void *p, int v, size_t n, hipStream_t) {
+    std::memset(p, v, n);
+    return hipSuccess;
+}
 hipError_t hipMemset(void *p, int v, size_t n) {
     std::memset(p, v, n);
     return hipSuccess;

@@ -23,6 +23,8 @@ OPT_SGEMV_MIN_ROWS, OPT_NOALLOC_SCRATCH_BYTES, OPT_MFMA_MIN_ROWS, OPT_HOST_ENTRY
 
 # element types of the paged cache and of rows
 F32, BF16 = 0, 1
+# bytes of a workspace that are zero before and after a call
+WORKSPACE_COUNTERS = 32768
 
 # every symbol the header declares
 EXPORTS = [

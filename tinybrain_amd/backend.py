@@ -680,7 +680,12 @@ class HIPBackend:
         needs no eager call before it and shares nothing with other graphs."""
         import torch
 
-        return self._made(stream, like.new_empty, max(size, 1), dtype=torch.uint8), size
+        def make():
+            room = like.new_empty(max(size, 1), dtype=torch.uint8)
+            room[:_abi.WORKSPACE_COUNTERS].zero_()
+            return room
+
+        return self._made(stream, make), size
 
     # -- Sampler (Sampler.swift) with the caller's random numbers ----------------
     def sample(self, logits: np.ndarray, u, temperature=1.0, topK=0, topP=1.0, minP=0.0):

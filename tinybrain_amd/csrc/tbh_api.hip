@@ -152,6 +152,7 @@ tbh_status tbh_device_close(tbh_device *dev) {
     if (dev->done_flag) (void)hipHostFree(dev->done_flag);
     for (auto &ws : dev->workspaces) (void)hipFree(ws.ptr);
     for (void *p : dev->retired) (void)hipFree(p);
+    for (auto &c : dev->counters) (void)hipFree(c.ptr);
     if (dev->stream) (void)hipStreamDestroy(dev->stream);
     delete dev;
     return TBH_OK;
@@ -791,6 +792,27 @@ void *stream_workspace(tbh_device *dev, hipStream_t s, size_t bytes) {
     ws->ptr = p;
     ws->bytes = grown;
     return ws->ptr;
+}
+
+uint32_t *stream_counters(tbh_device *dev, hipStream_t s) {
+    std::lock_guard<std::mutex> lock(dev->ws_mu);
+    for (auto &e : dev->counters)
+        if (e.stream == s) return (uint32_t *)e.ptr;
+    auto none = [] {
+        (void)hipGetLastError();
+        return nullptr;
+    };
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &cap) != hipSuccess) return none();
+    if (cap != hipStreamCaptureStatusNone) return nullptr;
+    void *p = nullptr;
+    if (hipMalloc(&p, kCounterBytes) != hipSuccess) return none();
+    if (hipMemsetAsync(p, 0, kCounterBytes, s) != hipSuccess) {
+        (void)hipFree(p);
+        return none();
+    }
+    dev->counters.push_back({s, p, kCounterBytes});
+    return (uint32_t *)p;
 }
 }  // namespace tbh
 

@@ -6,6 +6,7 @@
 // result is multiplied by both scales and added in fp32.
 #include <algorithm>
 #include <memory>
+#include <new>
 
 #include "tbh_dma.h"
 #include "tbh_fp8.h"

@@ -87,6 +87,7 @@ struct tbh_device {
     std::mutex ws_mu;
     std::vector<Workspace> workspaces;
     std::vector<void *> retired;
+    std::vector<Workspace> counters;   // see stream_counters
     std::mutex launches[64];     // see hold_launches
 };
 
@@ -251,6 +252,24 @@ constexpr int64_t kMostBlocks = 1 << 20;
 // until the device closes.  Returns nullptr when it would have to grow while
 // the stream is being captured into a graph, or when the allocation fails.
 void *stream_workspace(tbh_device *dev, hipStream_t s, size_t bytes);
+
+// kCounters words of (dev, stream), all zero: counters of blocks that work on one
+// result, which every launch leaves as it found them (tbh_join.h).  nullptr as above.
+constexpr int64_t kCounters = 8192;
+constexpr size_t kCounterBytes = kCounters * 4;
+uint32_t *stream_counters(tbh_device *dev, hipStream_t s);
+
+// Counters and memory of a call: the caller's workspace, which begins with zeroed
+// counters, or those of (dev, stream); counters is nullptr where there is none.
+struct Room {
+    uint32_t *counters;
+    char *data;
+};
+inline Room room_of(tbh_device *dev, hipStream_t s, void *workspace, size_t bytes) {
+    if (workspace) return {(uint32_t *)workspace, (char *)workspace + kCounterBytes};
+    void *p = stream_workspace(dev, s, bytes ? bytes : 1);
+    return {p ? stream_counters(dev, s) : nullptr, (char *)p};
+}
 
 // Keeps a call's launches together on their stream: held by a call that passes
 // results from one launch to the next (in the stream's workspace, or a plan's

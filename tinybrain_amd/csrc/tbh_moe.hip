@@ -10,14 +10,17 @@
 #include <algorithm>
 #include <cmath>
 #include <memory>
+#include <new>
 
 #include "tbh_fp8.h"
+#include "tbh_join.h"
+#include "tbh_wave.h"
 
 struct tbh_moe {
     tbh_device *dev = nullptr;
     int64_t H = 0, I = 0, hb = 0, ib = 0;     // blocks of 128
     int32_t E = 0;
-    float *router = nullptr;                  // [E][H]
+    float *router = nullptr;                  // [E][hb * 128], padded with zeros
     uint8_t *gate_up = nullptr;               // [E][ib * 8][gate, up][hb][2048]
     uint8_t *down = nullptr;                  // [E][hb * 8][ib][2048]
     float *gate_scales = nullptr, *up_scales = nullptr;   // [E][ib][hb]
@@ -39,22 +42,26 @@ using fp8::bf16x8;
 
 constexpr int kMaxExperts = 512, kMaxTopK = 32;
 constexpr int kMaxTokens = 64;      // of one part of a call
+constexpr int kSplits = 4;          // parts of the inputs of a router's product
 constexpr int kListHead = 2;        // expert, number of its tokens
 
 struct Args {
     const void *x;
     void *y;
     int64_t ldx, ldy;
-    const float *router;
+    const float *router;     // [E][hb * 128]
     const uint8_t *gate_up, *down;
     const float *gate_scales, *up_scales, *down_scales;
     int32_t *ids;            // [T][top_k]
     float *weights;          // [T][top_k]
+    uint32_t *counters;
+    double *logits;          // [splits][T][E]
+    float *sums;             // [tiles of 32 outputs][parts][T][32]
     __bf16 *xp;              // [P][T][hb * 128]
     __bf16 *hp;              // [P][T * top_k][ib * 128]
     int32_t *lists;          // [used][kListHead + kMaxTokens]: an expert, its tokens' places in ids
-    int T, E, H, I, hb, ib, top_k, used;
-    bool normalize;
+    int T, E, H, hb, ib, top_k, used, splits, parts;
+    bool normalize, vec;     // vec: rows of x can be read four elements at a time
 };
 
 // v as P pieces that sum to it: bf16 as it is, fp32 cut after 8 bits, twice.
@@ -72,61 +79,178 @@ __device__ __forceinline__ void pieces_of(float v, __bf16 (&p)[P]) {
     }
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// Four consecutive elements of a row, those at and behind `left` 0.
+template <class T>
+__device__ __forceinline__ void load4(const T *p, int left, bool vec, float (&x)[4]) {
+    if (vec && left >= 4) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 v = *(const f32x4 *)p;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+            for (int i = 0; i < 4; ++i) x[i] = v[i];
+        } else {
+            const bf16x4 v = *(const bf16x4 *)p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = (float)v[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = i < left ? (float)p[i] : 0.0f;
+    }
 }
 
-// A block takes a token: its pieces, its experts and their weights.  Logits are
-// summed in 64 bits: which of two near ones is the larger decides an expert.
-template <class T, int P>
-__global__ __launch_bounds__(256) void moe_route(Args a) {
-    __shared__ double z[kMaxExperts];
-    __shared__ int32_t chosen[kMaxTopK];
-    __shared__ float part[kMaxTopK];
-    __shared__ float sums[4];
-    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const T *x = (const T *)a.x + (int64_t)t * a.ldx;
-    const int hp = a.hb * kBlock;
-    for (int k = tid; k < hp; k += 256) {
-        __bf16 p[P];
-        pieces_of<P>(k < a.H ? (float)x[k] : 0.0f, p);
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_most(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) {
+    v = dpp_most<wave::kXor1>(v);
+    v = dpp_most<wave::kXor2>(v);
+    v = dpp_most<wave::kHalfMirror>(v);
+    v = dpp_most<wave::kRowMirror>(v);
+    const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)v, 0), b = (uint32_t)__builtin_amdgcn_readlane((int)v, 16);
+    const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)v, 32), d = (uint32_t)__builtin_amdgcn_readlane((int)v, 48);
+    return max(max(a, b), max(c, d));
+}
+
+// The double whose key (sign flipped, or all bits of a negative one) is u.
+__device__ __forceinline__ double from_key(uint64_t u) {
+    return __builtin_bit_cast(double, u ^ (u >> 63 ? 1ull << 63 : ~0ull));
+}
+
+// A wave picks a token's experts, one after the other, from the a.splits parts of its
+// logits: of up to 64 N experts, lane l holds l + 64 i.  Logits are compared as whole
+// numbers in the same order, 32 bits at a time (0.75 us an expert with 64-bit maxima, 0.1 so).
+template <int N>
+__device__ __forceinline__ void choose(const Args &a, int t) {
+    const int lane = threadIdx.x & 63;
+    // all of the loads, which take a trip past the caches, before the first is used
+    double z[N][kSplits];
 #pragma unroll
-        for (int i = 0; i < P; ++i) a.xp[((int64_t)i * a.T + t) * hp + k] = p[i];
+    for (int i = 0; i < N; ++i) {
+        const double *p = a.logits + (int64_t)t * a.E + min(lane + 64 * i, a.E - 1);
+#pragma unroll
+        for (int s = 0; s < kSplits; ++s) z[i][s] = s < a.splits ? handed_over(p + (int64_t)s * a.T * a.E) : 0.0;
     }
-    for (int e = wave; e < a.E; e += 4) {
-        const float *r = a.router + (int64_t)e * a.H;
-        double s = 0.0;
-        for (int k = lane; k < a.H; k += 64) s = __builtin_fma((double)(float)x[k], (double)r[k], s);
-        s = wave_sum(s);
-        // NaN is in no order: an expert like any other, behind the rest
-        if (lane == 0) z[e] = s != s ? -HUGE_VAL : s;
+    uint32_t hi[N], lo[N];        // 0: none, or taken
+    float all = 0.0f;
+    uint32_t first_hi = 0, first_lo = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        double sum = z[i][0];
+#pragma unroll
+        for (int s = 1; s < kSplits; ++s) sum += z[i][s];
+        // NaN is in no order: an expert like any other, behind the rest; zeros are equal
+        if (sum != sum) sum = -HUGE_VAL;
+        if (sum == 0.0) sum = 0.0;
+        z[i][0] = sum;
+        uint64_t u = __builtin_bit_cast(uint64_t, sum);
+        u ^= (int64_t)u < 0 ? ~0ull : 1ull << 63;
+        const bool in = lane + 64 * i < a.E;
+        hi[i] = in ? (uint32_t)(u >> 32) : 0, lo[i] = in ? (uint32_t)u : 0;
     }
-    __syncthreads();
-    double most = -HUGE_VAL;
-    for (int e = 0; e < a.E; ++e) most = fmax(most, z[e]);
-    float sum = 0.0f;
-    for (int e = tid; e < a.E; e += 256) {
-        const double v = z[e];
-        int rank = 0;
-        for (int o = 0; o < a.E; ++o) rank += z[o] > v || (z[o] == v && o < e);
-        const float w = expf((float)(v - most));
-        if (rank < a.top_k) chosen[rank] = e, part[rank] = w;
-        sum += w;
-    }
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    if (tid < a.top_k) {
-        float all = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-        if (a.normalize) {
-            all = 0.0f;
-            for (int i = 0; i < a.top_k; ++i) all += part[i];
+    int id = 0;
+    double own = 0.0;             // lane j: the logit of the j-th
+    for (int j = 0; j < a.top_k; ++j) {
+        uint32_t h = 0, l = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) h = max(h, hi[i]);
+        h = wave_most(h);
+#pragma unroll
+        for (int i = 0; i < N; ++i) l = max(l, hi[i] == h ? lo[i] : 0u);
+        l = wave_most(l);
+        int e = -1;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint64_t m = __ballot(hi[i] == h && lo[i] == l);
+            if (m && e < 0) {
+                const int at = __builtin_ctzll(m);
+                e = 64 * i + at;
+                if (lane == at) hi[i] = lo[i] = 0;
+            }
         }
-        a.ids[t * a.top_k + tid] = chosen[tid];
-        a.weights[t * a.top_k + tid] = part[tid] / all;
+        if (j == 0) first_hi = h, first_lo = l;
+        if (lane == j) id = e, own = from_key((uint64_t)h << 32 | l);
     }
+    const double most = from_key((uint64_t)first_hi << 32 | first_lo);
+    const float weight = lane < a.top_k ? expf((float)(own - most)) : 0.0f;
+    if (a.normalize) {
+        all = weight;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (lane + 64 * i < a.E) all += expf((float)(z[i][0] - most));
+    }
+    all = wave::sum(all);
+    if (lane < a.top_k) {
+        a.ids[t * a.top_k + lane] = id;
+        a.weights[t * a.top_k + lane] = weight / all;
+    }
+}
+
+// Logits of 16 tokens and 16 experts over a part of the inputs, on the 64-bit matrix
+// instruction: products of two floats are exact there, and which of two near logits
+// is the larger decides an expert.  Lane (g, r) has inputs 4 g .. 4 g + 3 of each 16 of
+// token r and of expert r; of the result, experts 4 i + g of token r.  The instruction
+// takes 64 cycles, so that a tile is parted over 16 waves and a.splits blocks; the block
+// that finishes a tile of tokens picks their experts, a wave a token.  Blocks of the
+// first experts also write the rows' pieces.
+template <class T, int P>
+__global__ __launch_bounds__(1024) void moe_route(Args a) {
+    __shared__ double part[16][256];
+    __shared__ uint32_t seen;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4, t0 = blockIdx.y * 16, e0 = blockIdx.x * 16, hp = a.hb * kBlock;
+    const int steps = a.hb * (kBlock / 16), w = blockIdx.z * 16 + wave, ws = a.splits * 16;
+    const int s0 = steps * w / ws, s1 = steps * (w + 1) / ws;
+    const bool live = t0 + r < a.T;
+    const T *x = (const T *)a.x + (int64_t)(t0 + r) * a.ldx + 4 * g;
+    const float *router = a.router + (int64_t)min(e0 + r, a.E - 1) * hp + 4 * g;
+    f64x4 z{0.0, 0.0, 0.0, 0.0};
+    constexpr int D = 4;
+    for (int s = s0; s < s1; s += D) {
+        float xv[D][4];
+        f32x4 rv[D];
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const int k = (s + d) * 16;
+            const bool in = s + d < s1;
+            rv[d] = in ? *(const f32x4 *)(router + k) : f32x4{0.f, 0.f, 0.f, 0.f};
+            load4(x + k, in && live ? a.H - k - 4 * g : 0, a.vec, xv[d]);
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            if (e0 == 0 && live && s + d < s1) {
+                bf16x4 o[P];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    __bf16 p[P];
+                    pieces_of<P>(xv[d][i], p);
+#pragma unroll
+                    for (int j = 0; j < P; ++j) o[j][i] = p[j];
+                }
+#pragma unroll
+                for (int j = 0; j < P; ++j)
+                    *(bf16x4 *)(a.xp + ((int64_t)j * a.T + t0 + r) * hp + (s + d) * 16 + 4 * g) = o[j];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                z = __builtin_amdgcn_mfma_f64_16x16x4f64((double)rv[d][i], (double)xv[d][i], z, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[wave][r * 16 + 4 * j + g] = z[j];
+    __syncthreads();
+    const int t = t0 + (threadIdx.x >> 4), e = e0 + (threadIdx.x & 15);
+    if (threadIdx.x < 256 && t < a.T && e < a.E) {
+        double v = 0.0;
+        for (int i = 0; i < 16; ++i) v += part[i][threadIdx.x];
+        hand_over(a.logits + ((int64_t)blockIdx.z * a.T + t) * a.E + e, v);
+    }
+    if (!last_to_arrive(a.counters + blockIdx.y, gridDim.x * gridDim.z, &seen) || t0 + wave >= a.T) return;
+    if (a.E <= 64) choose<1>(a, t0 + wave);
+    else choose<kMaxExperts / 64>(a, t0 + wave);
 }
 
 // The number of the y-th expert that some token has chosen and the places of
@@ -167,66 +291,101 @@ __device__ __forceinline__ int find_expert(const Args &a, int y, uint32_t (&used
     return e;
 }
 
-// One 128-deep block: acc[c] += scale * (tile . rows), for CT columns tiles of rows.
-// row[c]: the lane's row of column tile c at input 16 g of the block; stride: from one
-// piece to the next.
-template <int P, int CT>
-__device__ __forceinline__ void block_product(const uint8_t *tile, float scale, const __bf16 *const (&row)[CT],
-                                              int64_t stride, f32x4 (&acc)[CT]) {
-    const i32x4 w[2] = {*(const i32x4 *)tile, *(const i32x4 *)(tile + 1024)};
-    f32x4 part[CT];
+// The rows of a matrix instruction's other operand: P pieces of kTokens<P> tokens side by
+// side, so that an fp32 row costs no more instructions and loads than its pieces fill.
+template <int P>
+constexpr int kTokens = P == 1 ? 16 : 5;
+// Column r16's token among them (P == 3: the last column repeats, and is not used).
+template <int P>
+__device__ __forceinline__ int token_of(int r16) {
+    return P == 1 ? r16 : min(r16 / 3, kTokens<P> - 1);
+}
+template <int P>
+__device__ __forceinline__ int piece_of(int r16) {
+    return P == 1 ? 0 : r16 % 3;
+}
+// A token's sum over its pieces, in the column of its first.
+template <int P>
+__device__ __forceinline__ f32x4 over_pieces(f32x4 v) {
+    if constexpr (P == 3) {
 #pragma unroll
-    for (int c = 0; c < CT; ++c) part[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        bf16x8 o[2];
-        fp8::widen(w[h], o);
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const bf16x8 x = *(const bf16x8 *)(row[c] + p * stride + 64 * h + 8 * s);
-                    part[c] = fp8::mfma_wide(o[s], x, part[c]);
-                }
+        for (int i = 0; i < 4; ++i) v[i] += wave::dpp<0x101>(v[i]) + wave::dpp<0x102>(v[i]);   // columns + 1, + 2
     }
+    return v;
+}
+template <int P>
+__device__ __forceinline__ bool first_piece(int r16) {
+    return P == 1 || (r16 % 3 == 0 && r16 < 15);
+}
+
+// acc[t][c] += scale[t] * (tile t . rows c) of one 128-deep block, for RT tiles and CT column
+// tiles; row[c]: the lane's row at input 16 g of the block.
+template <int RT, int CT>
+__device__ __forceinline__ void block_product(const i32x4 (&w)[RT][2], const float (&scale)[RT], const __bf16 *const (&row)[CT],
+                                              f32x4 (&acc)[RT][CT]) {
+    bf16x8 x[CT][4];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[c][i] = __builtin_fmaf(part[c][i], scale, acc[c][i]);
+        for (int i = 0; i < 4; ++i) x[c][i] = *(const bf16x8 *)(row[c] + 64 * (i >> 1) + 8 * (i & 1));
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        f32x4 part[CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) part[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            bf16x8 o[2];
+            fp8::widen(w[t][h], o);
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) part[c] = fp8::mfma_wide(o[s], x[c][2 * h + s], part[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][c][i] = __builtin_fmaf(part[c][i], scale[t], acc[t][c][i]);
+    }
 }
 
-// h of 16 inner columns for an expert's tokens c0 .. c0 + 16 CT.
+__device__ __forceinline__ void load_tile(i32x4 (&w)[2], const uint8_t *p) {
+    w[0] = *(const i32x4 *)p, w[1] = *(const i32x4 *)(p + 1024);
+}
+
+// h of 16 inner columns for an expert's tokens c0 .. c0 + CT kTokens.
 template <int P, int CT>
 __device__ __forceinline__ void up_tokens(const Args &a, int e, int tile, const int32_t *slots, int c0, int count,
                                           f32x4 (*red)[64]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
     const int hp = a.hb * kBlock;
     const __bf16 *row[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         // a column past the last token repeats it; its result is not stored
-        const int slot = slots[min(c0 + c * 16 + r16, count - 1)];
-        row[c] = a.xp + (int64_t)(slot / a.top_k) * hp + 16 * g;
+        const int slot = slots[min(c0 + c * kTokens<P> + token_of<P>(r16), count - 1)];
+        row[c] = a.xp + ((int64_t)piece_of<P>(r16) * a.T + slot / a.top_k) * hp + 16 * g;
     }
-    f32x4 gate[CT], up[CT];
+    f32x4 acc[2][CT];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) gate[c] = up[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < CT; ++c) acc[0][c] = acc[1][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     const uint8_t *wt = a.gate_up + ((int64_t)e * a.ib * 8 + tile) * 2 * a.hb * kTileBytes + lane * 16;
-    const int64_t sb = ((int64_t)e * a.ib + tile / 8) * a.hb, stride = (int64_t)a.T * hp;
+    const int64_t sb = ((int64_t)e * a.ib + tile / 8) * a.hb;
     const int b0 = a.hb * wave / 4, b1 = a.hb * (wave + 1) / 4;
     for (int b = b0; b < b1; ++b) {
+        i32x4 w[2][2];
+        load_tile(w[0], wt + (int64_t)b * kTileBytes);
+        load_tile(w[1], wt + (int64_t)(a.hb + b) * kTileBytes);
+        const float s[2] = {a.gate_scales[sb + b], a.up_scales[sb + b]};
         const __bf16 *at[CT];
 #pragma unroll
         for (int c = 0; c < CT; ++c) at[c] = row[c] + b * kBlock;
-        block_product<P, CT>(wt + (int64_t)b * kTileBytes, a.gate_scales[sb + b], at, stride, gate);
-        block_product<P, CT>(wt + (int64_t)(a.hb + b) * kTileBytes, a.up_scales[sb + b], at, stride, up);
+        block_product(w, s, at, acc);
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-        red[wave * 2 * CT + 2 * c][lane] = gate[c];
-        red[wave * 2 * CT + 2 * c + 1][lane] = up[c];
+        red[wave * 2 * CT + 2 * c][lane] = acc[0][c];
+        red[wave * 2 * CT + 2 * c + 1][lane] = acc[1][c];
     }
     __syncthreads();
     if (wave < CT) {
@@ -237,8 +396,9 @@ __device__ __forceinline__ void up_tokens(const Args &a, int e, int tile, const 
             gv += red[w * 2 * CT + 2 * c][lane];
             uv += red[w * 2 * CT + 2 * c + 1][lane];
         }
-        const int at = c0 + c * 16 + r16;
-        if (at < count) {
+        gv = over_pieces<P>(gv), uv = over_pieces<P>(uv);
+        const int at = c0 + c * kTokens<P> + token_of<P>(r16);
+        if (at < count && first_piece<P>(r16)) {
             const int ip = a.ib * kBlock;
             bf16x4 o[P];
 #pragma unroll
@@ -272,71 +432,153 @@ __global__ __launch_bounds__(256) void moe_up(Args a) {
     }
     if (e < 0) return;
     int c0 = 0;
-    for (; count - c0 > 16; c0 += 32) up_tokens<P, 2>(a, e, blockIdx.x, slots, c0, count, red);
+    for (; count - c0 > kTokens<P>; c0 += 2 * kTokens<P>) up_tokens<P, 2>(a, e, blockIdx.x, slots, c0, count, red);
     if (c0 < count) up_tokens<P, 1>(a, e, blockIdx.x, slots, c0, count, red);
 }
 
-// 16 outputs of all tokens: the waves part the (expert, block of inputs) pairs and
-// each adds its share of a token's sum to its own row in LDS; joined in order.
+// 32 outputs of all tokens: the waves of a.parts blocks part the units of kUnit blocks
+// of inputs of the active experts, the next unit's tiles in flight while one is
+// multiplied; each wave adds its share of a token's sum to its own row in LDS, once an
+// expert.  Joined in order, and over the blocks by the one that is last.  (A tile for one
+// token needs twice as many loads of h as of weights, so that a wave takes two tiles a
+// load of h.)
+constexpr int kDownWaves = 8, kUnit = 2;
+
 template <class T, int P>
-__global__ __launch_bounds__(512) void moe_down(Args a) {
-    extern __shared__ f32x4 sums[];       // [8][T][4]
+__global__ __launch_bounds__(64 * kDownWaves) void moe_down(Args a) {
+    extern __shared__ f32x4 sums[];       // [waves][8 quads of outputs][T], then the experts' heads
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r16 = lane & 15, g = lane >> 4, tile = blockIdx.x;
-    f32x4 *own = sums + wave * a.T * 4;
-    for (int i = lane; i < a.T * 4; i += 64) own[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int r16 = lane & 15, g = lane >> 4, tile = blockIdx.x * 2, w = blockIdx.y * kDownWaves + wave;
+    f32x4 *own = sums + wave * a.T * 8;
+    int2 *heads = (int2 *)(sums + kDownWaves * a.T * 8);      // expert, number of its tokens
+    for (int y = tid; y < a.used; y += 64 * kDownWaves) heads[y] = *(const int2 *)(a.lists + y * (kListHead + kMaxTokens));
+    for (int i = lane; i < a.T * 8; i += 64) own[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
     int active = 0;
-    for (int y = 0; y < a.used; y += 64)
-        active += __builtin_popcountll(__ballot(y + lane < a.used && a.lists[(y + lane) * (kListHead + kMaxTokens) + 1] > 0));
-    const int total = active * a.ib;
-    int i = (int)((int64_t)total * wave / 8);
-    const int end = (int)((int64_t)total * (wave + 1) / 8);
+    for (int y = 0; y < a.used; y += 64) active += __builtin_popcountll(__ballot(y + lane < a.used && heads[y + lane].y > 0));
+    const int per = (a.ib + kUnit - 1) / kUnit, total = active * per, ws = a.parts * kDownWaves;
+    const int first = (int)((int64_t)total * w / ws), end = (int)((int64_t)total * (w + 1) / ws);
     const int ip = a.ib * kBlock;
-    const int64_t stride = (int64_t)a.T * a.top_k * ip;
-    __builtin_amdgcn_wave_barrier();
-    while (i < end) {
-        const int y = i / a.ib, b0 = i - y * a.ib, b1 = min(a.ib, b0 + end - i);
-        const int32_t *l = a.lists + y * (kListHead + kMaxTokens);
-        const int e = l[0], count = l[1];
-        const uint8_t *wt = a.down + ((int64_t)e * a.hb * 8 + tile) * a.ib * kTileBytes + lane * 16;
-        const float *sw = a.down_scales + ((int64_t)e * a.hb + tile / 8) * a.ib;
-        for (int c0 = 0; c0 < count; c0 += 16) {
-            const int at = c0 + r16, slot = l[kListHead + min(at, count - 1)];
-            const __bf16 *row = a.hp + (int64_t)slot * ip + 16 * g;
-            f32x4 acc[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
-            for (int b = b0; b < b1; ++b) {
-                const __bf16 *const rows[1] = {row + b * kBlock};
-                block_product<P, 1>(wt + (int64_t)b * kTileBytes, sw[b], rows, stride, acc);
-            }
-            if (at < count) {
-                const float p = a.weights[slot];
-                f32x4 *to = own + (slot / a.top_k) * 4 + g;
-                f32x4 v = *to;
+    i32x4 next[kUnit][2][2];
+    float next_s[kUnit];
+    int y = first / per, b0 = (first - y * per) * kUnit;      // of the unit that is loaded next
+    auto load = [&]() {
+        const int e = __builtin_amdgcn_readfirstlane(heads[y].x);
+        const int64_t row = ((int64_t)e * a.hb * 8 + tile) * a.ib;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = __builtin_fmaf(acc[0][j], p, v[j]);
-                *to = v;
-            }
+        for (int u = 0; u < kUnit; ++u) {
+            const int b = min(b0 + u, a.ib - 1);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) load_tile(next[u][t], a.down + (row + (int64_t)t * a.ib + b) * kTileBytes + lane * 16);
+            next_s[u] = a.down_scales[((int64_t)e * a.hb + tile / 8) * a.ib + b];
         }
-        i += b1 - b0;
+    };
+    auto slot_of = [&](int c0, int count) {
+        return a.lists[y * (kListHead + kMaxTokens) + kListHead + min(c0 + token_of<P>(r16), count - 1)];
+    };
+    auto add = [&](int slot, bool some, f32x4 (&acc)[2][1]) {
+        const float p = a.weights[slot];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const f32x4 sum = over_pieces<P>(acc[t][0]);
+            if (!some || !first_piece<P>(r16)) continue;
+            f32x4 *to = own + (4 * t + g) * a.T + slot / a.top_k;
+            f32x4 v = *to;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __builtin_fmaf(sum[j], p, v[j]);
+            *to = v;
+        }
+    };
+    const __bf16 *hrow = a.hp + (int64_t)piece_of<P>(r16) * a.T * a.top_k * ip + 16 * g;
+    f32x4 acc[2][1];
+    int count = 0, slot = 0;
+    bool fresh = true;
+    if (first < end) load();
+    for (int i = first; i < end; ++i) {
+        i32x4 now[kUnit][2][2];
+        float s[kUnit];
+#pragma unroll
+        for (int u = 0; u < kUnit; ++u) {
+            s[u] = next_s[u];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) now[u][t][0] = next[u][t][0], now[u][t][1] = next[u][t][1];
+        }
+        if (fresh) {
+            count = __builtin_amdgcn_readfirstlane(heads[y].y);
+            slot = slot_of(0, count);
+            acc[0][0] = acc[1][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        const int yi = y, bi = b0;
+        b0 += kUnit;
+        fresh = b0 >= a.ib;
+        if (fresh) ++y, b0 = 0;
+        if (i + 1 < end) load();
+        for (int c0 = 0; c0 < count; c0 += kTokens<P>) {
+            int sl = slot;
+            if (c0 > 0) {
+                sl = a.lists[yi * (kListHead + kMaxTokens) + kListHead + min(c0 + token_of<P>(r16), count - 1)];
+                acc[0][0] = acc[1][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int u = 0; u < kUnit; ++u) {
+                if (bi + u >= a.ib) break;
+                const __bf16 *const rows[1] = {hrow + (int64_t)sl * ip + (bi + u) * kBlock};
+                const float sc[2] = {s[u], s[u]};
+                block_product(now[u], sc, rows, acc);
+            }
+            // one column tile: its sums stay in registers until the expert's last unit
+            if (count > kTokens<P> || fresh || i + 1 == end) add(sl, c0 + token_of<P>(r16) < count, acc);
+        }
+        if (count > kTokens<P>) acc[0][0] = acc[1][0] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     __syncthreads();
-    for (int j = tid; j < a.T * 16; j += 512) {
-        const int t = j >> 4, n = tile * 16 + (j & 15);
-        float v = 0.0f;
-        for (int w = 0; w < 8; ++w) v += ((const float *)sums)[w * a.T * 16 + j];
+    auto store = [&](int j, float v) {
+        const int t = j >> 5, n = tile * 16 + (j & 31);
         if (n < a.H) ((T *)a.y)[(int64_t)t * a.ldy + n] = (T)v;
+    };
+    float *part = a.sums + (int64_t)blockIdx.x * a.parts * a.T * 32;
+    for (int j = tid; j < a.T * 32; j += 64 * kDownWaves) {
+        const int at = ((j & 31) / 4 * a.T + (j >> 5)) * 4 + (j & 3);
+        float v = 0.0f;
+        for (int i = 0; i < kDownWaves; ++i) v += ((const float *)sums)[i * a.T * 32 + at];
+        if (a.parts == 1) store(j, v);
+        else hand_over(part + (int64_t)blockIdx.y * a.T * 32 + j, v);
+    }
+    if (a.parts == 1 || !last_to_arrive(a.counters + blockIdx.x, a.parts, (uint32_t *)sums)) return;
+    for (int j = tid; j < a.T * 32; j += 64 * kDownWaves) {
+        float v = 0.0f;
+        for (int i = 0; i < a.parts; ++i) v += handed_over(part + (int64_t)i * a.T * 32 + j);
+        store(j, v);
     }
 }
 
 template <class T, int P>
 hipError_t launch(const Args &a, hipStream_t s) {
-    hipLaunchKernelGGL((moe_route<T, P>), dim3((unsigned)a.T), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((moe_route<T, P>), dim3((unsigned)(a.E + 15) / 16, (unsigned)(a.T + 15) / 16, (unsigned)a.splits),
+                       dim3(1024), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((moe_up<P>), dim3((unsigned)(a.ib * 8), (unsigned)a.used), dim3(256), 0, s, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL((moe_down<T, P>), dim3((unsigned)((a.H + 15) / 16)), dim3(512), (size_t)a.T * 8 * 64, s, a);
+    hipLaunchKernelGGL((moe_down<T, P>), dim3((unsigned)((a.H + 31) / 32), (unsigned)a.parts), dim3(64 * kDownWaves),
+                       (size_t)a.T * kDownWaves * 128 + (size_t)a.used * 8, s, a);
     return hipGetLastError();
+}
+
+// Sizes of a part of T tokens and the launch shapes that follow from them.
+void size_up(Args &a, const tbh_moe &m, int64_t tokens, int32_t top_k) {
+    a.T = (int)std::min<int64_t>(kMaxTokens, tokens);
+    a.top_k = top_k;
+    a.E = m.E;
+    a.H = (int)m.H;
+    a.hb = (int)m.hb;
+    a.ib = (int)m.ib;
+    a.used = std::min(m.E, a.T * top_k);
+    // two steps of 16 inputs a wave
+    a.splits = std::max(1, std::min(kSplits, a.hb * (kBlock / 16) / 32));
+    // a block a CU, of waves that have a unit at the least
+    const int tiles = (a.H + 31) / 32, units = a.used * ((a.ib + kUnit - 1) / kUnit);
+    a.parts = std::max(1, std::min((m.dev->cu_count + tiles - 1) / tiles, units / kDownWaves));
 }
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -352,6 +594,8 @@ size_t carve(Args &a, int P, char *base) {
     const size_t rows = (size_t)a.T * a.top_k;
     a.ids = (int32_t *)take(rows * 4);
     a.weights = (float *)take(rows * 4);
+    a.logits = (double *)take((size_t)a.splits * a.T * a.E * 8);
+    a.sums = (float *)take(a.parts > 1 ? (size_t)((a.H + 31) / 32) * a.parts * a.T * 128 : 0);
     a.lists = (int32_t *)take((size_t)a.used * (kListHead + kMaxTokens) * 4);
     a.xp = (__bf16 *)take((size_t)P * a.T * a.hb * kBlock * 2);
     a.hp = (__bf16 *)take((size_t)P * rows * a.ib * kBlock * 2);
@@ -360,12 +604,15 @@ size_t carve(Args &a, int P, char *base) {
 
 size_t workspace_of(const tbh_moe &m, int32_t x_type, int64_t tokens, int32_t top_k) {
     Args a{};
-    a.T = (int)std::min<int64_t>(tokens, kMaxTokens);
-    a.top_k = top_k;
-    a.hb = (int)m.hb;
-    a.ib = (int)m.ib;
-    a.used = std::min(m.E, a.T * top_k);
-    return carve(a, x_type == TBH_BF16 ? 1 : 3, nullptr);
+    size_up(a, m, tokens, top_k);
+    // (more tokens have fewer parts of a tile, and a last part of few tokens may have more)
+    size_t most = 0;
+    for (int64_t t : {(int64_t)a.T, tokens % kMaxTokens}) {
+        if (t == 0) continue;
+        size_up(a, m, t, top_k);
+        most = std::max(most, carve(a, x_type == TBH_BF16 ? 1 : 3, nullptr));
+    }
+    return most;
 }
 
 constexpr int64_t kMaxWidth = 1 << 17;
@@ -419,7 +666,11 @@ tbh_status tbh_moe_create(tbh_device *dev, const tbh_moe_desc *desc, tbh_moe **o
     const size_t tiles = E * m->hb * m->ib * 8 * kTileBytes;
     std::lock_guard<std::mutex> lock(dev->mu);
     const hipStream_t s = dev->stream;
-    hipError_t e = fp8::copy_in((void **)&m->router, d.router, E * m->H * 4, s);
+    const size_t row = (size_t)m->hb * kBlock * 4;
+    hipError_t e = hipMalloc((void **)&m->router, E * row);
+    if (e == hipSuccess) e = hipMemsetAsync(m->router, 0, E * row, s);
+    if (e == hipSuccess)
+        e = hipMemcpy2DAsync(m->router, row, d.router, (size_t)m->H * 4, (size_t)m->H * 4, E, hipMemcpyDefault, s);
     if (e == hipSuccess) e = fp8::copy_in((void **)&m->gate_scales, d.gate_scales, scales, s);
     if (e == hipSuccess) e = fp8::copy_in((void **)&m->up_scales, d.up_scales, scales, s);
     if (e == hipSuccess) e = fp8::copy_in((void **)&m->down_scales, d.down_scales, scales, s);
@@ -458,7 +709,7 @@ tbh_status tbh_moe_workspace(const tbh_moe *m, int32_t x_type, int64_t tokens, i
     const tbh_status st = check_moe("tbh_moe_workspace", m, x_type, tokens, top_k);
     if (st != TBH_OK) return st;
     if (!bytes) return set_error(TBH_E_INVALID, "tbh_moe_workspace: NULL pointer");
-    *bytes = (int64_t)workspace_of(*m, x_type, tokens, top_k);
+    *bytes = (int64_t)(kCounterBytes + workspace_of(*m, x_type, tokens, top_k));
     return TBH_OK;
 }
 
@@ -477,27 +728,23 @@ tbh_status tbh_moe_device(const tbh_moe *m, const void *x, int32_t x_type, int64
         return bad("a pointer is not aligned to its type");
     if (workspace && ((uintptr_t)workspace & 255)) return bad("the workspace must be 256-byte aligned");
     const size_t need = workspace_of(*m, x_type, tokens, top_k);
-    if (workspace && (workspace_bytes < 0 || (size_t)workspace_bytes < need)) return bad("the workspace is too small");
+    if (workspace && (workspace_bytes < 0 || (size_t)workspace_bytes < need + kCounterBytes)) return bad("the workspace is too small");
     if ((st = use_device(m->dev->ordinal)) != TBH_OK) return st;
     const hipStream_t s = (hipStream_t)stream;
+    const bool vec = (uintptr_t)x % (4 * size) == 0 && (tokens == 1 || x_stride % 4 == 0);
     const auto held = hold_launches(m->dev, s);
-    char *room = (char *)(workspace ? workspace : stream_workspace(m->dev, s, need));
-    if (!room)
+    const Room room = room_of(m->dev, s, workspace, need);
+    if (!room.counters)
         return set_error(TBH_E_OOM, std::string(what) + ": no workspace (a captured stream needs an earlier eager call, or a "
                                                         "workspace of the caller's)");
     hipError_t e = hipSuccess;
     for (int64_t at = 0; at < tokens && e == hipSuccess; at += kMaxTokens) {
         Args a{};
-        a.T = (int)std::min<int64_t>(kMaxTokens, tokens - at);
-        a.top_k = top_k;
-        a.E = m->E;
-        a.H = (int)m->H;
-        a.I = (int)m->I;
-        a.hb = (int)m->hb;
-        a.ib = (int)m->ib;
-        a.used = std::min(m->E, a.T * top_k);
+        size_up(a, *m, tokens - at, top_k);
         a.normalize = normalize != 0;
-        carve(a, x_type == TBH_BF16 ? 1 : 3, room);
+        a.vec = vec;
+        a.counters = room.counters;
+        carve(a, x_type == TBH_BF16 ? 1 : 3, room.data);
         if (experts) a.ids = experts + at * top_k;
         if (weights) a.weights = weights + at * top_k;
         a.x = (const char *)x + at * x_stride * size;
