@@ -708,10 +708,8 @@ tbh_status tbh_sample_device(tbh_device *dev, const float *logits, int64_t ld, i
  * there are fewer than k: token and parent -1, score -inf, not done.
  * With scores, done and parents of one call as the next one's, k = beams.
  * The outputs overlap no input.  beams and k up to 64, vocab and rows up to
- * 2^20 (TBH_E_UNSUPPORTED).  workspace: 256-byte aligned,
- * tbh_beam_select_workspace bytes, or NULL for the one of (device, stream), with
- * tbh_matmul_device's rule for captured graphs; a capture before any eager call
- * on its stream finds none (TBH_E_OOM). */
+ * 2^20 (TBH_E_UNSUPPORTED).  workspace: as tbh_moe_device's, of
+ * tbh_beam_select_workspace bytes. */
 tbh_status tbh_beam_select_workspace(tbh_device *dev, int64_t requests, int32_t beams, int64_t vocab, int32_t k,
                                      int64_t *bytes);
 tbh_status tbh_beam_select_device(tbh_device *dev, const float *logits, int64_t ld, int64_t requests, int32_t beams,

@@ -183,7 +183,7 @@ def test_select_limits():
     f = _abi.lib().tbh_beam_select_workspace
     assert f(DEV, 3, 4, 32000, 4, ctypes.byref(n)) == _abi.OK and n.value > 0
     for requests, beams, vocab, k in ((1, 64, 1 << 20, 64), (1 << 14, 64, 1 << 20, 64), (1 << 20, 1, 1, 1)):
-        assert f(DEV, requests, beams, vocab, k, ctypes.byref(n)) == _abi.OK and 0 < n.value <= 128 << 20
+        assert f(DEV, requests, beams, vocab, k, ctypes.byref(n)) == _abi.OK and 0 < n.value <= (128 << 20) + _abi.WORKSPACE_COUNTERS
     assert f(DEV, 3, 4, 32000, 4, None) == _abi.E_INVALID
 
 
@@ -331,7 +331,7 @@ assert reorder(layout(max_requests=1 << 22, max_blocks=8)) == _abi.E_UNSUPPORTED
 
 def test_threads_on_one_stream(stand_in):  # noqa: F811
     stand_in(MAKE + """
-calls = [lambda: fp8(70), lambda: moe(5), lambda: select(3), lambda: reorder(layout())]
+calls = [lambda: fp8(70), lambda: moe(5), lambda: select(20000), lambda: reorder(layout())]
 launches()
 one = []
 for c in calls:

@@ -3,19 +3,21 @@
 #include <algorithm>
 #include <cmath>
 
+#include "tbh_join.h"
 #include "tbh_paged.h"
+#include "tbh_wave.h"
 
 namespace tbh {
 namespace beam {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxBeams = 64, kMaxPick = 64;
 constexpr int64_t kMaxVocab = 1 << 20, kMaxRows = 1 << 20;
 constexpr size_t kMaxPartials = (size_t)128 << 20;
-constexpr int kPer = 16, kChunk = 256 * kPer;     // elements of a row that a block takes
 
 struct SelectArgs {
     const float *logits;
@@ -24,212 +26,453 @@ struct SelectArgs {
     const int32_t *done;
     int32_t *tokens, *parents, *done_out;
     float *scores_out;
+    uint32_t *counters;     // [requests], then [rows]
     uint64_t *best;         // [rows][splits][k]: an element's key, largest first; 0: none
+    double *sum;            // [rows][splits]: of exp(logit - most)
     float *most;            // [rows][splits]
-    double *sum;            // [rows][splits]
-    int vocab, splits, beams, k, eos;
+    int vocab, splits, part, beams, k, eos;   // part: elements of a split
     int row0;               // the first row of the call's part
+    bool vec;               // rows can be read four elements at a time
 };
 
-// (logit, index) as one number: the larger logit, then the lower index.
+// (logit, index) as one number: the larger logit, then the lower index; 0 for what is never taken.
 __device__ __forceinline__ uint64_t key_of(float v, uint32_t i) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v == 0.0f ? 0.0f : v);
-    return (uint64_t)(u ^ ((int32_t)u < 0 ? 0xFFFFFFFFu : 0x80000000u)) << 32 | (0xFFFFFFFFu - i);
+    const uint64_t key = (uint64_t)(u ^ ((int32_t)u < 0 ? 0xFFFFFFFFu : 0x80000000u)) << 32 | (0xFFFFFFFFu - i);
+    return v > -HUGE_VALF ? key : 0;
 }
 __device__ __forceinline__ float logit_of(uint64_t key) {
     const uint32_t u = (uint32_t)(key >> 32);
     return __builtin_bit_cast(float, u ^ ((int32_t)u < 0 ? 0x80000000u : 0xFFFFFFFFu));
 }
-
-// A chunk of a row: its largest logit, the sum of exp(logit - largest) in 64
-// bits, and its k best elements.
-__global__ __launch_bounds__(256) void beam_chunk(SelectArgs a) {
-    __shared__ uint64_t heads[256], found[kMaxPick * kPer];
-    __shared__ uint64_t floor_key;
-    __shared__ int count;
-    __shared__ float wave_most[4];
-    __shared__ double wave_sum[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row = blockIdx.x, split = blockIdx.y;
-    const int64_t at = (int64_t)row * a.splits + split;
-    if (a.done && a.done[row]) return;       // its one candidate is no logit
-    const float *x = a.logits + (int64_t)row * a.ld + (int64_t)split * kChunk;
-    const int n = min(kChunk, a.vocab - split * kChunk);
-    float v[kPer];
-    float most = -HUGE_VALF;
-    uint64_t head = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int i = j * 256 + tid;
-        v[j] = i < n ? x[i] : -HUGE_VALF;
-        if (v[j] != v[j]) v[j] = -HUGE_VALF;
-        most = fmaxf(most, v[j]);
-        const uint64_t key = v[j] > -HUGE_VALF ? key_of(v[j], (uint32_t)(split * kChunk + i)) : 0;
-        head = key > head ? key : head;
-    }
-    heads[tid] = head;
-    if (tid == 0) floor_key = 0, count = 0;
-    for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-    if (lane == 0) wave_most[wave] = most;
-    __syncthreads();
-    most = fmaxf(fmaxf(wave_most[0], wave_most[1]), fmaxf(wave_most[2], wave_most[3]));
-    double s = 0.0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        if (v[j] == most) s += most > -HUGE_VALF ? 1.0 : 0.0;
-        else if (most < HUGE_VALF) s += exp((double)v[j] - (double)most);
-    }
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (lane == 0) wave_sum[wave] = s;
-    // the k-th largest of the threads' best: at least k elements are no smaller
-    if (head) {
-        int better = 0;
-        for (int i = 0; i < 256; ++i) better += heads[i] > head;
-        if (better == a.k - 1) floor_key = head;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        a.most[at] = most;
-        a.sum[at] = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
-    }
-    const uint64_t least = floor_key;
-    // threads whose best is below it have none; the k others at most all of theirs
-    if (head && head >= least) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            if (!(v[j] > -HUGE_VALF)) continue;
-            const uint64_t key = key_of(v[j], (uint32_t)(split * kChunk + j * 256 + tid));
-            if (key >= least) found[atomicAdd(&count, 1)] = key;
-        }
-    }
-    __syncthreads();
-    uint64_t *best = a.best + at * a.k;
-    const int c = count;
-    for (int i = tid; i < c; i += 256) {
-        const uint64_t key = found[i];
-        int rank = 0;
-        for (int o = 0; o < c; ++o) rank += found[o] > key;
-        if (rank < a.k) best[rank] = key;
-    }
-    for (int i = c + tid; i < a.k; i += 256) best[i] = 0;
+__device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
 
-struct Candidate {
-    double key;        // score + log probability
-    uint64_t element;  // (logit, token) within the row
-    int32_t row;
+// exp(d) for d in -700 .. 0: 2^n times Taylor's series of exp(f ln 2) for the fraction f of
+// d / ln 2, |f| <= 1/2, up to f^8, the rest of which is below 2e-10.  (n from the low bits of
+// a sum with 1.5 * 2^52, and into the exponent: conversions and scalings of 64-bit numbers
+// are slower than their sums.)
+constexpr double kLeastExp = -690.0;
+__device__ __forceinline__ double exp_low(double d) {
+    constexpr double kLog2E = 1.4426950408889634, kShift = 6755399441055744.0;
+    const double u = __builtin_fma(d, kLog2E, kShift), f = __builtin_fma(d, kLog2E, -(u - kShift));
+    double p = 1.3215486790144309e-06;            // ln(2)^8 / 8!
+    p = __builtin_fma(p, f, 1.5252733804059841e-05);
+    p = __builtin_fma(p, f, 1.5403530393381608e-04);
+    p = __builtin_fma(p, f, 1.3333558146428443e-03);
+    p = __builtin_fma(p, f, 9.6181291076284772e-03);
+    p = __builtin_fma(p, f, 5.5504108664821580e-02);
+    p = __builtin_fma(p, f, 2.4022650695910072e-01);
+    p = __builtin_fma(p, f, 6.9314718055994531e-01);
+    p = __builtin_fma(p, f, 1.0);
+    u32x2 w = __builtin_bit_cast(u32x2, p);
+    w[1] += __builtin_bit_cast(u32x2, u)[0] << 20;
+    return __builtin_bit_cast(double, w);
+}
+// exp(v - most), v <= most, both finite or v -inf; below exp(kLeastExp) nothing counts
+__device__ __forceinline__ double exp_below(float v, float most) {
+    return exp_low(fmax((double)v - (double)most, kLeastExp));
+}
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = dpp_add<wave::kXor1>(v);
+    v = dpp_add<wave::kXor2>(v);
+    v = dpp_add<wave::kHalfMirror>(v);
+    v = dpp_add<wave::kRowMirror>(v);
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    auto row = [&](int l) { return __builtin_bit_cast(double, lane_key(u, l)); };
+    return (row(0) + row(16)) + (row(32) + row(48));
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_most(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) {
+    v = dpp_most<wave::kXor1>(v);
+    v = dpp_most<wave::kXor2>(v);
+    v = dpp_most<wave::kHalfMirror>(v);
+    v = dpp_most<wave::kRowMirror>(v);
+    auto row = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+    return max(max(row(0), row(16)), max(row(32), row(48)));
+}
+
+// A running sum of exp(x - most); an infinite most counts the infinite x alone.
+struct Total {
+    float most;
+    double sum;
+    __device__ __forceinline__ void rescale(float to) {      // to >= most
+        if (to > most) sum = to < HUGE_VALF && most > -HUGE_VALF ? sum * exp_below(most, to) : 0.0;
+        most = to;
+    }
 };
-// in the order of the selection: ties to the lowest row, then token
-__device__ __forceinline__ bool before(const Candidate &a, const Candidate &b) {
-    if (a.key != b.key) return a.key > b.key;
-    if (a.row != b.row) return a.row < b.row;
-    return a.element > b.element;
+
+// A list's length at which it is cut down to its k best, and elements that one step adds
+// at most: fewer heads than few_heads pass as they are, of more at most k a wave.  W: waves
+// of a block.
+constexpr int kPer = 16, kLong = 128;
+__host__ __device__ constexpr int few_heads(int W) { return 16 * W; }
+__host__ __device__ constexpr int list_room(int k, int W) {
+    return kLong + k + (W * k > few_heads(W) ? W * k : few_heads(W)) * kPer;
 }
 
-constexpr int kRoom = kMaxPick + 256 + 64;
+// Sum over each aligned group of 8 lanes, in all of them.
+__device__ __forceinline__ int sum_of_8(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, wave::kXor1, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, wave::kXor2, 0xF, 0xF, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, wave::kHalfMirror, 0xF, 0xF, false);
+}
 
-// Keeps the k first of n candidates, in order.
-__device__ __forceinline__ int prune(Candidate *c, Candidate *tmp, int n, int k) {
+// Keeps the k largest of n distinct keys, in order (tmp: k keys).  Eight lanes find a key's rank.
+template <int W>
+__device__ __forceinline__ int prune(uint64_t *c, uint64_t *tmp, int n, int k) {
+    const int part = threadIdx.x & 7;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += 256) {
+    for (int i = threadIdx.x >> 3; i < n; i += W * 8) {
+        const uint64_t mine = c[i];
         int rank = 0;
-        const Candidate mine = c[i];
-        for (int o = 0; o < n; ++o) rank += before(c[o], mine);
-        if (rank < k) tmp[rank] = mine;
+#pragma unroll 4
+        for (int o = part; o < n; o += 8) rank += c[o] > mine;
+        rank = sum_of_8(rank);
+        if (rank < k && part == 0) tmp[rank] = mine;
     }
     __syncthreads();
     n = min(n, k);
-    for (int i = threadIdx.x; i < n; i += 256) c[i] = tmp[i];
+    for (int i = threadIdx.x; i < n; i += W * 64) c[i] = tmp[i];
     __syncthreads();
     return n;
 }
 
-// A request: its chunks' lists joined, best elements of all lists first.
-__global__ __launch_bounds__(256) void beam_join(SelectArgs a) {
-    __shared__ Candidate held[kRoom], tmp[kMaxPick];
-    __shared__ double total[kMaxBeams];       // log of the sum of exp(logit)
-    __shared__ int alive[kMaxBeams];          // 1: continued by its logits, 2: done, 0: neither
-    __shared__ int fresh;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row0 = blockIdx.x * a.beams;
-    for (int b = wave; b < a.beams; b += 4) {
-        const int row = row0 + b;
-        const float score = a.scores[row];
-        int state = a.done && a.done[row] ? 2 : 1;
-        if (!(score > -HUGE_VALF && score < HUGE_VALF)) state = 0;
-        double sum = 0.0;
-        float most = -HUGE_VALF;
-        if (state == 1) {
-            const float *m = a.most + (int64_t)row * a.splits;
-            const double *s = a.sum + (int64_t)row * a.splits;
-            for (int i = lane; i < a.splits; i += 64) most = fmaxf(most, m[i]);
-            for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-            for (int i = lane; i < a.splits; i += 64)
-                if (m[i] > -HUGE_VALF) sum += m[i] == most ? s[i] : most < HUGE_VALF ? s[i] * exp((double)m[i] - (double)most) : 0.0;
-            for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
-            if (!(most > -HUGE_VALF)) state = 0;
-        }
-        if (lane == 0) {
-            alive[b] = state;
-            // infinite logits share all of the weight: total holds their log count
-            total[b] = state == 1 ? (most < HUGE_VALF ? (double)most : 0.0) + log(sum) : 0.0;
-        }
+// A key that k of a wave's 64 (one a lane, 0: none) are not below; 0 where there are fewer.
+__device__ __forceinline__ uint64_t kth_of_wave(uint64_t key, int k) {
+    int better = 0;
+#pragma unroll
+    for (int l = 0; l < 64; ++l) better += lane_key(key, l) > key;
+    const uint64_t m = __ballot(key && better == k - 1);
+    return m ? lane_key(key, (int)__builtin_ctzll(m)) : 0;
+}
+
+// A value that those of k of a wave's lanes are not below, as key_of's upper half; 0 where
+// there are fewer.  Equal ones may make it more than k.
+__device__ __forceinline__ uint32_t kth_value(uint32_t value, int k) {
+    uint32_t most = 0;
+    for (int left = k; left > 0;) {
+        most = wave_most(value);
+        const uint64_t m = __ballot(value == most);
+        left -= __builtin_popcountll(m);
+        if (!most) break;
+        value = value == most ? 0 : value;
     }
-    if (tid == 0) fresh = 0;
+    return most;
+}
+
+// Candidates of a request's rows, in LDS.
+template <int N>
+struct Candidates {
+    double key[N];          // score + log probability
+    uint64_t element[N];    // (logit, token) within the row
+    int32_t row[N];
+};
+
+// Keeps the k first of n candidates, in order: the larger key, then the lower row, then the
+// larger element.
+template <int W, int N>
+__device__ __forceinline__ int prune(Candidates<N> &c, Candidates<kMaxPick> &tmp, int n, int k) {
+    const int part = threadIdx.x & 7;
+    __syncthreads();
+    for (int i = threadIdx.x >> 3; i < n; i += W * 8) {
+        const double mine = c.key[i];
+        int rank = 0, equal = 0;
+#pragma unroll 4
+        for (int o = part; o < n; o += 8) rank += c.key[o] > mine, equal += c.key[o] == mine;
+        if (sum_of_8(equal) > 1)
+            for (int o = part; o < n; o += 8)
+                rank += c.key[o] == mine && (c.row[o] < c.row[i] || (c.row[o] == c.row[i] && c.element[o] > c.element[i]));
+        rank = sum_of_8(rank);
+        if (rank < k && part == 0) tmp.key[rank] = mine, tmp.element[rank] = c.element[i], tmp.row[rank] = c.row[i];
+    }
+    __syncthreads();
+    n = min(n, k);
+    for (int i = threadIdx.x; i < n; i += W * 64) c.key[i] = tmp.key[i], c.element[i] = tmp.element[i], c.row[i] = tmp.row[i];
+    __syncthreads();
+    return n;
+}
+
+// A wave's totals as one, in every lane.
+__device__ __forceinline__ Total over_wave(Total t) {
+    t.rescale(wave::max(t.most));
+    t.sum = wave_sum(t.sum);
+    return t;
+}
+
+// Everything of a block in LDS but its list, whose length depends on k.
+template <int W>
+struct Shared {
+    Candidates<kMaxPick + 64 * W> held;
+    Candidates<kMaxPick> tmp;
+    Total wave_total[W];
+    uint64_t wave_key[W];
+    int heads[3][W];
+    double total[kMaxBeams];      // log of the sum of exp(logit)
+    int state[kMaxBeams];
+    int count;
+    uint32_t seen;
+};
+
+// The request's last block: the lists of its rows joined.
+template <int W>
+__device__ __forceinline__ void join_rows(const SelectArgs &a, int request, Shared<W> &sh) {
+    constexpr int NT = 64 * W;
+    const int tid = threadIdx.x, row0 = request * a.beams, all = a.beams * a.k;
+    // all rows' best first, then their next
+    auto load = [&](int i) {
+        return i < all ? handed_over(a.best + (int64_t)(row0 + i % a.beams) * a.splits * a.k + i / a.beams) : 0;
+    };
+    uint64_t next = load(tid);
+    if (tid < a.beams) {
+        const int row = row0 + tid;
+        const float score = a.scores[row];
+        // 1: goes on by its logits, 2: done, 3: as 1, by its infinite logits alone; 0: no candidates
+        int st = a.done && a.done[row] ? 2 : 1;
+        double total = 0.0;
+        if (!(score > -HUGE_VALF && score < HUGE_VALF)) st = 0;
+        if (st == 1) {
+            const float most = handed_over(a.most + (int64_t)row * a.splits);
+            const double sum = handed_over(a.sum + (int64_t)row * a.splits);
+            st = !(most > -HUGE_VALF) ? 0 : most == HUGE_VALF ? 3 : 1;
+            // infinite logits share all of the weight: the logarithm of their number
+            total = (st == 1 ? (double)most : 0.0) + log(sum);
+        }
+        sh.state[tid] = st;
+        sh.total[tid] = total;
+    }
+    if (tid == 0) sh.count = 0;
     __syncthreads();
     int n = 0;
-    const int lists = a.beams * a.splits;
-    for (int level = 0; level < a.k; ++level) {
-        bool more = false;
-        for (int base = 0; base < lists; base += 256) {
-            const int i = base + tid, b = i / a.splits, split = i - b * a.splits;
-            Candidate c{};
-            bool in = false;
-            if (i < lists) {
-                const int row = row0 + b;
-                c.row = row;
-                if (alive[b] == 1) {
-                    c.element = a.best[((int64_t)row * a.splits + split) * a.k + level];
-                    if (c.element) {
-                        const float v = logit_of(c.element);
-                        // beside infinite logits a finite one weighs nothing
-                        const bool inf = v == HUGE_VALF, infs = a.most[(int64_t)row * a.splits + split] == HUGE_VALF;
-                        c.key = (double)a.scores[row] + ((inf ? 0.0 : (double)v) - total[b]);
-                        in = inf || !infs;
-                        if (in && !inf)
-                            for (int o = 0; o < a.splits && in; ++o) in = a.most[(int64_t)row * a.splits + o] < HUGE_VALF;
-                    }
-                } else if (alive[b] == 2 && level == 0 && split == 0) {
-                    c.key = (double)a.scores[row];
-                    c.element = 0xFFFFFFFFu - (uint32_t)a.eos;
-                    in = true;
-                }
-                if (in && n == a.k) in = before(c, held[a.k - 1]);
+    for (int base = 0; base < all; base += NT) {
+        const int i = base + tid, b = i % a.beams, level = i / a.beams;
+        double key = 0.0;
+        uint64_t element = next;
+        bool in = false;
+        if (base + NT < all) next = load(i + NT);
+        if (i < all) {
+            const int row = row0 + b, st = sh.state[b];
+            const float score = a.scores[row];
+            if (st == 1 || st == 3) {
+                const float v = logit_of(element);
+                key = (double)score + ((st == 3 ? 0.0 : (double)v) - sh.total[b]);
+                in = element && (st == 1 || v == HUGE_VALF);
+            } else if (st == 2 && level == 0) {
+                key = (double)score;
+                element = 0xFFFFFFFFu - (uint32_t)a.eos;
+                in = true;
             }
-            if (in) held[n + atomicAdd(&fresh, 1)] = c;
+            // (one equal to the last held is sorted out by prune)
+            if (in && n == a.k) in = key >= sh.held.key[a.k - 1];
+        }
+        if (in) {
+            const int to = n + atomicAdd(&sh.count, 1);
+            sh.held.key[to] = key, sh.held.element[to] = element, sh.held.row[to] = row0 + b;
+        }
+        __syncthreads();
+        const int got = sh.count;
+        if (got) n = prune<W>(sh.held, sh.tmp, n + got, a.k);
+        __syncthreads();
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+    }
+    const int64_t to = (int64_t)request * a.k;
+    for (int i = tid; i < a.k; i += NT) {
+        const bool some = i < n;
+        const int32_t token = some ? (int32_t)(0xFFFFFFFFu - (uint32_t)sh.held.element[i]) : -1;
+        a.tokens[to + i] = token;
+        a.parents[to + i] = some ? sh.held.row[i] + a.row0 : -1;
+        a.scores_out[to + i] = some ? (float)sh.held.key[i] : -HUGE_VALF;
+        if (a.done_out) a.done_out[to + i] = some && (token == a.eos || sh.state[sh.held.row[i] - row0] == 2);
+    }
+}
+
+// The row's last block: the lists and sums of its parts joined, to where its first part's stand.
+template <int W>
+__device__ __forceinline__ void join_parts(const SelectArgs &a, int row, uint64_t *list, Shared<W> &sh) {
+    constexpr int NT = 64 * W;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t at = (int64_t)row * a.splits;
+    uint64_t *best = a.best + at * a.k;
+    const int all = a.splits * a.k;
+    auto load = [&](int i) { return i < all ? handed_over(best + (int64_t)(i % a.splits) * a.k + i / a.splits) : 0; };
+    uint64_t next = load(tid);
+    Total t{-HUGE_VALF, 0.0};
+    if (wave == 0) {
+        for (int i = lane; i < a.splits; i += 64) {
+            Total o{handed_over(a.most + at + i), handed_over(a.sum + at + i)};
+            const float top = fmaxf(t.most, o.most);
+            t.rescale(top), o.rescale(top);
+            t.sum += o.sum;
+        }
+        t = over_wave(t);
+    }
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    int n = 0;
+    uint64_t least = 0;
+    for (int base = 0; base < all; base += NT) {       // all parts' best first, then their next
+        const uint64_t key = next;
+        if (base + NT < all) next = load(base + NT + tid);
+        if (key > least) list[atomicAdd(&sh.count, 1)] = key;
+        __syncthreads();
+        n = sh.count;
+        __syncthreads();
+        if (n > kLong || base + NT >= all) {
+            n = prune<W>(list, (uint64_t *)sh.tmp.key, n, a.k);
+            if (n == a.k) least = list[a.k - 1];
+            if (tid == 0) sh.count = n;
             __syncthreads();
-            const int got = fresh;
-            __syncthreads();
-            if (tid == 0) fresh = 0;
-            if (got) {
-                more = true;
-                n = prune(held, tmp, n + got, a.k);
-            } else {
+        }
+    }
+    // every load of the parts is done
+    for (int i = tid; i < a.k; i += NT) hand_over(best + i, i < n ? list[i] : 0);
+    if (tid == 0) {
+        hand_over(a.most + at, t.most);
+        hand_over(a.sum + at, t.sum);
+    }
+}
+
+// A part of a row, 16 elements a thread at a time: the largest logit, the sum of
+// exp(logit - largest) in 64 bits, and the k best elements.  These are kept by a list:
+// an element has to pass a key that k elements before it are not below.  The row's last
+// block joins its parts, the request's last its rows (a counter takes some 70 ns an
+// arrival, so that they are counted in two steps).
+template <int W>
+__global__ __launch_bounds__(64 * W) void beam_select(SelectArgs a) {
+    constexpr int NT = 64 * W, kChunk = NT * kPer;
+    extern __shared__ uint64_t list[];       // [list_room]
+    __shared__ Shared<W> sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x, split = blockIdx.y, request = row / a.beams;
+    const int64_t at = (int64_t)row * a.splits + split;
+    const bool live = !a.done || !a.done[row];
+    if (!live && split > 0) return;                // (a done row has one part)
+    if (live) {
+        const float *x = a.logits + (int64_t)row * a.ld;
+        const int begin = split * a.part, end = min(a.vocab, begin + a.part);
+        auto load = [&](int from, float (&v)[kPer]) {
+#pragma unroll
+            for (int j = 0; j < kPer / 4; ++j) {
+                const int i = from + (j * NT + tid) * 4;
+                if (a.vec && i + 4 <= end) {
+                    const f32x4 q = *(const f32x4 *)(x + i);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[4 * j + c] = q[c];
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[4 * j + c] = i + c < end ? x[i + c] : -HUGE_VALF;
+                }
+            }
+        };
+        Total t{-HUGE_VALF, 0.0};        // a thread's sum, on its wave's maximum
+        uint64_t least = 0;
+        float next[kPer];
+        load(begin, next);
+        if (tid == 0) sh.count = 0;
+        int turn = 0;
+        for (int from = begin; from < end; from += kChunk, turn ^= 1) {
+            float v[kPer];
+            float top = -HUGE_VALF;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                v[j] = fmaxf(next[j], -HUGE_VALF);       // NaN: never taken
+                top = fmaxf(top, v[j]);
+            }
+            if (from + kChunk < end) load(from + kChunk, next);
+            auto index = [&](int j) { return (uint32_t)(from + ((j / 4) * NT + tid) * 4 + j % 4); };
+            // how many threads may have elements for the list (their places decide among equal ones)
+            auto count_heads = [&](int *words) {
+                const uint64_t lanes = __ballot(top > -HUGE_VALF && key_of(top, 0) > least);
+                if (lane == 0) words[wave] = __builtin_popcountll(lanes);
                 __syncthreads();
+                int n = 0;
+#pragma unroll
+                for (int w = 0; w < W; ++w) n += words[w];
+                return n;
+            };
+            const int heads = count_heads(sh.heads[turn]);
+            if (heads) {
+                auto raise = [&](uint64_t key) {      // to the largest of the waves' k-th best
+                    if (lane == 0) sh.wave_key[wave] = key;
+                    __syncthreads();
+#pragma unroll
+                    for (int w = 0; w < W; ++w) least = sh.wave_key[w] > least + 1 ? sh.wave_key[w] - 1 : least;
+                };
+                if (heads > few_heads(W)) {
+                    const uint64_t best = key_of(top, 0);
+                    raise((uint64_t)kth_value((uint32_t)(best >> 32), a.k) << 32);
+                    if (count_heads(sh.heads[2]) > max(W * a.k, few_heads(W))) {
+                        // many equal ones: by their places, too
+                        uint32_t at = 0;
+#pragma unroll
+                        for (int j = kPer - 1; j >= 0; --j) at = v[j] == top ? index(j) : at;
+                        raise(kth_of_wave(key_of(top, at), a.k));
+                    }
+                }
+                const float low = least ? logit_of(least) : -HUGE_VALF;
+                if (top >= low) {
+#pragma unroll
+                    for (int j = 0; j < kPer; ++j) {
+                        if (!(v[j] >= low)) continue;
+                        const uint64_t key = key_of(v[j], index(j));
+                        if (key > least) list[atomicAdd(&sh.count, 1)] = key;
+                    }
+                }
+                __syncthreads();
+                const int n = sh.count;
+                if (n > kLong) {
+                    const int left = prune<W>(list, (uint64_t *)sh.tmp.key, n, a.k);
+                    if (left == a.k) least = list[a.k - 1];
+                    if (tid == 0) sh.count = left;
+                }
+            }
+            // the sum
+            const float wave_top = wave::max(top);
+            if (wave_top > t.most) t.rescale(wave_top);
+            if (t.most == HUGE_VALF) {
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) t.sum += v[j] == HUGE_VALF ? 1.0 : 0.0;
+            } else if (t.most > -HUGE_VALF) {
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) t.sum += exp_below(v[j], t.most);
             }
         }
-        // lists go down: where no list's next element is among the best, none behind it is
-        if (!more) break;
+        t.sum = wave_sum(t.sum);
+        if (lane == 0) sh.wave_total[wave] = t;
+        __syncthreads();
+        const int n = prune<W>(list, (uint64_t *)sh.tmp.key, sh.count, a.k);
+        for (int i = tid; i < a.k; i += NT) hand_over(a.best + at * a.k + i, i < n ? list[i] : 0);
+        if (tid == 0) {
+            Total s = sh.wave_total[0];
+            for (int w = 1; w < W; ++w) {
+                Total u = sh.wave_total[w];
+                const float top = fmaxf(s.most, u.most);
+                s.rescale(top), u.rescale(top);
+                s.sum += u.sum;
+            }
+            hand_over(a.most + at, s.most);
+            hand_over(a.sum + at, s.sum);
+        }
+        if (a.splits > 1) {
+            if (!last_to_arrive(a.counters + gridDim.x / a.beams + row, (uint32_t)a.splits, &sh.seen)) return;
+            join_parts<W>(a, row, list, sh);
+        }
     }
-    const int64_t to = (int64_t)blockIdx.x * a.k;
-    for (int i = tid; i < a.k; i += 256) {
-        const bool some = i < n;
-        const int32_t token = some ? (int32_t)(0xFFFFFFFFu - (uint32_t)held[i].element) : -1;
-        a.tokens[to + i] = token;
-        a.parents[to + i] = some ? held[i].row + a.row0 : -1;
-        a.scores_out[to + i] = some ? (float)held[i].key : -HUGE_VALF;
-        if (a.done_out) a.done_out[to + i] = some && (token == a.eos || alive[held[i].row - row0] == 2);
-    }
+    if (last_to_arrive(a.counters + request, (uint32_t)a.beams, &sh.seen)) join_rows<W>(a, request, sh);
 }
 
 // ---- reordering the cache ------------------------------------------------------
@@ -342,13 +585,23 @@ void launch_copy(const ReorderArgs &a, dim3 grid, hipStream_t s) {
     hipLaunchKernelGGL((reorder_copy<V>), grid, dim3(256), 0, s, a);
 }
 
-int64_t splits_of(int64_t vocab) { return (vocab + kChunk - 1) / kChunk; }
-size_t request_bytes(int64_t beams, int64_t vocab, int64_t k) {
-    return (size_t)(beams * splits_of(vocab)) * (size_t)(k * 8 + 16);
+// How a call's rows are parted.  Rows for every second CU and more: a block of 16 waves
+// a row.  Fewer: blocks of four waves, of 4096 elements at the least, until there are
+// some four a CU.
+struct Parts {
+    int waves, part, splits;
+};
+Parts parts_of(const tbh_device *dev, int64_t rows, int64_t vocab) {
+    const int64_t cus = std::max(1, dev->cu_count);
+    if (2 * rows >= cus && vocab > 4096) return {16, (int)vocab, 1};
+    const int64_t chunks = (vocab + 4095) / 4096, most = std::max<int64_t>(1, std::min(chunks, (4 * cus + rows - 1) / rows));
+    const int64_t each = (chunks + most - 1) / most;
+    return {4, (int)(each * 4096), (int)((chunks + each - 1) / each)};
 }
+size_t request_bytes(int64_t beams, int64_t splits, int64_t k) { return (size_t)(beams * splits) * (size_t)(k * 8 + 12); }
 // requests of one part of a call
-int64_t part_of(int64_t requests, int64_t beams, int64_t vocab, int64_t k) {
-    return std::max<int64_t>(1, std::min<int64_t>(requests, (int64_t)(kMaxPartials / request_bytes(beams, vocab, k))));
+int64_t part_of(int64_t requests, int64_t beams, int64_t splits, int64_t k) {
+    return std::max<int64_t>(1, std::min({requests, kCounters / (beams + 1), (int64_t)(kMaxPartials / request_bytes(beams, splits, k))}));
 }
 
 tbh_status check_select(const char *what, const tbh_device *dev, int64_t requests, int64_t beams, int64_t vocab, int64_t k) {
@@ -377,7 +630,9 @@ tbh_status tbh_beam_select_workspace(tbh_device *dev, int64_t requests, int32_t 
     const tbh_status st = check_select(what, dev, requests, beams, vocab, k);
     if (st != TBH_OK) return st;
     if (!bytes) return set_error(TBH_E_INVALID, std::string(what) + ": NULL pointer");
-    *bytes = requests ? part_of(requests, beams, vocab, k) * (int64_t)request_bytes(beams, vocab, k) : 0;
+    const Parts p = parts_of(dev, requests * beams, vocab);
+    *bytes = (int64_t)kCounterBytes;
+    if (requests) *bytes += part_of(requests, beams, p.splits, k) * (int64_t)request_bytes(beams, p.splits, k);
     return TBH_OK;
 }
 
@@ -394,14 +649,16 @@ tbh_status tbh_beam_select_device(tbh_device *dev, const float *logits, int64_t 
     if (ld < vocab && requests * beams > 1) return bad("ld is shorter than vocab");
     if (done && (eos < 0 || eos >= vocab)) return bad("done rows need an eos within the vocabulary");
     if (workspace && ((uintptr_t)workspace & 255)) return bad("the workspace must be 256-byte aligned");
-    const int64_t part = part_of(requests, beams, vocab, k);
-    const size_t need = (size_t)part * request_bytes(beams, vocab, k);
-    if (workspace && (workspace_bytes < 0 || (size_t)workspace_bytes < need)) return bad("the workspace is too small");
+    const Parts p = parts_of(dev, requests * beams, vocab);
+    const int64_t part = part_of(requests, beams, p.splits, k);
+    const size_t need = (size_t)part * request_bytes(beams, p.splits, k);
+    if (workspace && (workspace_bytes < 0 || (size_t)workspace_bytes < need + kCounterBytes))
+        return bad("the workspace is too small");
     if ((st = use_device(dev->ordinal)) != TBH_OK) return st;
     const hipStream_t s = (hipStream_t)stream;
     const auto held = hold_launches(dev, s);
-    char *room = (char *)(workspace ? workspace : stream_workspace(dev, s, need));
-    if (!room)
+    const Room room = room_of(dev, s, workspace, need);
+    if (!room.counters)
         return set_error(TBH_E_OOM, std::string(what) + ": no workspace (a captured stream needs an earlier eager call, or a "
                                                         "workspace of the caller's)");
     hipError_t e = hipSuccess;
@@ -409,12 +666,14 @@ tbh_status tbh_beam_select_device(tbh_device *dev, const float *logits, int64_t 
         const int64_t some = std::min(part, requests - at), rows = some * beams;
         SelectArgs a{};
         a.vocab = (int)vocab;
-        a.splits = (int)splits_of(vocab);
+        a.splits = p.splits;
+        a.part = p.part;
         a.beams = beams;
         a.k = k;
         a.eos = eos;
         a.row0 = (int)(at * beams);
         a.ld = ld;
+        a.vec = (uintptr_t)logits % 16 == 0 && (requests * beams == 1 || ld % 4 == 0);
         a.logits = logits + at * beams * ld;
         a.scores = scores + at * beams;
         a.done = done ? done + at * beams : nullptr;
@@ -422,12 +681,14 @@ tbh_status tbh_beam_select_device(tbh_device *dev, const float *logits, int64_t 
         a.parents = parents + at * k;
         a.scores_out = scores_out + at * k;
         a.done_out = done_out ? done_out + at * k : nullptr;
-        a.sum = (double *)room;
+        a.counters = room.counters;
+        a.sum = (double *)room.data;
         a.best = (uint64_t *)(a.sum + rows * a.splits);
         a.most = (float *)(a.best + rows * a.splits * k);
-        hipLaunchKernelGGL(beam_chunk, dim3((unsigned)rows, (unsigned)a.splits), dim3(256), 0, s, a);
-        if ((e = hipGetLastError()) != hipSuccess) break;
-        hipLaunchKernelGGL(beam_join, dim3((unsigned)some), dim3(256), 0, s, a);
+        const dim3 grid((unsigned)rows, (unsigned)a.splits);
+        const size_t lds = (size_t)list_room(k, p.waves) * 8;
+        if (p.waves == 16) hipLaunchKernelGGL((beam_select<16>), grid, dim3(1024), lds, s, a);
+        else hipLaunchKernelGGL((beam_select<4>), grid, dim3(256), lds, s, a);
         e = hipGetLastError();
     }
     return e == hipSuccess ? TBH_OK : hip_error(e, "beam select launch");
