@@ -71,7 +71,7 @@ __device__ __forceinline__ double exp_low(double d) {
     w[1] += __builtin_bit_cast(u32x2, u)[0] << 20;
     return __builtin_bit_cast(double, w);
 }
-// exp(v - most), v <= most, both finite or v -inf; below exp(kLeastExp) nothing counts
+// exp(v - most) of a v <= most, which is finite; below exp(kLeastExp) nothing counts, nor -inf and NaN
 __device__ __forceinline__ double exp_below(float v, float most) {
     return exp_low(fmax((double)v - (double)most, kLeastExp));
 }
@@ -103,6 +103,13 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
     v = dpp_most<wave::kRowMirror>(v);
     auto row = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
     return max(max(row(0), row(16)), max(row(32), row(48)));
+}
+
+// exp(v - most) in 32 bits, off by at most (2 + |v - most|) 2^-23 of itself: an element's, of
+// which a sum has so many that 64-bit ones, at eight cycles an operation, took half of the
+// call (256 rows of 100000: 44 us, 34 so).  0 for -inf and NaN.
+__device__ __forceinline__ float exp_step(float v, float most) {
+    return __builtin_amdgcn_exp2f(fmaxf(v - most, -1000.0f) * 1.44269504f);
 }
 
 // A running sum of exp(x - most); an infinite most counts the infinite x alone.
@@ -220,7 +227,7 @@ struct Shared {
     Candidates<kMaxPick> tmp;
     Total wave_total[W];
     uint64_t wave_key[W];
-    int heads[3][W];
+    int heads[2][W];
     double total[kMaxBeams];      // log of the sum of exp(logit)
     int state[kMaxBeams];
     int count;
@@ -347,8 +354,8 @@ __device__ __forceinline__ void join_parts(const SelectArgs &a, int row, uint64_
 }
 
 // A part of a row, 16 elements a thread at a time: the largest logit, the sum of
-// exp(logit - largest) in 64 bits, and the k best elements.  These are kept by a list:
-// an element has to pass a key that k elements before it are not below.  The row's last
+// exp(logit - largest), 64 bits over 32-bit steps, and the k best elements, by a list of those that pass a
+// key that k elements before them are not below.  The row's last
 // block joins its parts, the request's last its rows (a counter takes some 70 ns an
 // arrival, so that they are counted in two steps).
 template <int W>
@@ -380,20 +387,9 @@ __global__ __launch_bounds__(64 * W) void beam_select(SelectArgs a) {
         };
         Total t{-HUGE_VALF, 0.0};        // a thread's sum, on its wave's maximum
         uint64_t least = 0;
-        float next[kPer];
-        load(begin, next);
-        if (tid == 0) sh.count = 0;
-        int turn = 0;
-        for (int from = begin; from < end; from += kChunk, turn ^= 1) {
-            float v[kPer];
-            float top = -HUGE_VALF;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                v[j] = fmaxf(next[j], -HUGE_VALF);       // NaN: never taken
-                top = fmaxf(top, v[j]);
-            }
-            if (from + kChunk < end) load(from + kChunk, next);
-            auto index = [&](int j) { return (uint32_t)(from + ((j / 4) * NT + tid) * 4 + j % 4); };
+        auto index = [&](int from, int j) { return (uint32_t)(from + ((j / 4) * NT + tid) * 4 + j % 4); };
+        // what of a step passes the list's threshold, by the whole block
+        auto take = [&](const float (&v)[kPer], float top, int from) {
             // how many threads may have elements for the list (their places decide among equal ones)
             auto count_heads = [&](int *words) {
                 const uint64_t lanes = __ballot(top > -HUGE_VALF && key_of(top, 0) > least);
@@ -404,51 +400,121 @@ __global__ __launch_bounds__(64 * W) void beam_select(SelectArgs a) {
                 for (int w = 0; w < W; ++w) n += words[w];
                 return n;
             };
-            const int heads = count_heads(sh.heads[turn]);
-            if (heads) {
-                auto raise = [&](uint64_t key) {      // to the largest of the waves' k-th best
-                    if (lane == 0) sh.wave_key[wave] = key;
-                    __syncthreads();
+            auto raise = [&](uint64_t key) { least = key > least + 1 ? key - 1 : least; };
+            constexpr int kFew = few_heads(W);
+            const int limit = max(W * a.k, kFew);
+            if (count_heads(sh.heads[0]) > kFew) {
+                const uint32_t best = (uint32_t)(key_of(top, 0) >> 32);
+                // the least of the waves' (k / W)-th best: k elements are no smaller.  Some three
+                // times as many pass as have to
+                const uint32_t value = kth_value(best, (a.k + W - 1) / W);
+                if (lane == 0) sh.wave_key[wave] = (uint64_t)value << 32;
+                __syncthreads();
+                uint64_t key = ~0ull;
 #pragma unroll
-                    for (int w = 0; w < W; ++w) least = sh.wave_key[w] > least + 1 ? sh.wave_key[w] - 1 : least;
-                };
-                if (heads > few_heads(W)) {
-                    const uint64_t best = key_of(top, 0);
-                    raise((uint64_t)kth_value((uint32_t)(best >> 32), a.k) << 32);
-                    if (count_heads(sh.heads[2]) > max(W * a.k, few_heads(W))) {
+                for (int w = 0; w < W; ++w) key = min(key, sh.wave_key[w]);
+                raise(key);
+                if (count_heads(sh.heads[1]) > limit) {
+                    // unlike waves: the largest of their k-th best
+                    const uint32_t kth = kth_value(best, a.k);
+                    if (lane == 0) sh.wave_key[wave] = (uint64_t)kth << 32;
+                    __syncthreads();
+                    key = 0;
+#pragma unroll
+                    for (int w = 0; w < W; ++w) key = max(key, sh.wave_key[w]);
+                    raise(key);
+                    if (count_heads(sh.heads[0]) > limit) {
                         // many equal ones: by their places, too
                         uint32_t at = 0;
 #pragma unroll
-                        for (int j = kPer - 1; j >= 0; --j) at = v[j] == top ? index(j) : at;
-                        raise(kth_of_wave(key_of(top, at), a.k));
-                    }
-                }
-                const float low = least ? logit_of(least) : -HUGE_VALF;
-                if (top >= low) {
+                        for (int j = kPer - 1; j >= 0; --j) at = v[j] == top ? index(from, j) : at;
+                        const uint64_t exact = kth_of_wave(key_of(top, at), a.k);
+                        if (lane == 0) sh.wave_key[wave] = exact;
+                        __syncthreads();
+                        key = 0;
 #pragma unroll
-                    for (int j = 0; j < kPer; ++j) {
-                        if (!(v[j] >= low)) continue;
-                        const uint64_t key = key_of(v[j], index(j));
-                        if (key > least) list[atomicAdd(&sh.count, 1)] = key;
+                        for (int w = 0; w < W; ++w) key = max(key, sh.wave_key[w]);
+                        raise(key);
                     }
-                }
-                __syncthreads();
-                const int n = sh.count;
-                if (n > kLong) {
-                    const int left = prune<W>(list, (uint64_t *)sh.tmp.key, n, a.k);
-                    if (left == a.k) least = list[a.k - 1];
-                    if (tid == 0) sh.count = left;
                 }
             }
-            // the sum
+            const float low = least ? logit_of(least) : -HUGE_VALF;
+            if (top >= low) {
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) {
+                    if (!(v[j] >= low)) continue;
+                    const uint64_t key = key_of(v[j], index(from, j));
+                    if (key > least) list[atomicAdd(&sh.count, 1)] = key;
+                }
+            }
+            __syncthreads();
+            const int n = sh.count;
+            const int left = n > a.k ? prune<W>(list, (uint64_t *)sh.tmp.key, n, a.k) : n;
+            if (left == a.k && n > a.k) least = list[a.k - 1];
+            if (tid == 0) sh.count = left;
+            __syncthreads();
+        };
+        // (NaN is in no comparison below, and in no maximum)
+        auto largest = [&](const float (&v)[kPer]) {
+            float top = -HUGE_VALF;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) top = fmaxf(top, v[j]);
+            return top;
+        };
+        auto sum = [&](const float (&v)[kPer], float top) {
             const float wave_top = wave::max(top);
             if (wave_top > t.most) t.rescale(wave_top);
             if (t.most == HUGE_VALF) {
 #pragma unroll
                 for (int j = 0; j < kPer; ++j) t.sum += v[j] == HUGE_VALF ? 1.0 : 0.0;
-            } else if (t.most > -HUGE_VALF) {
+            } else {
+                const float most = t.most > -HUGE_VALF ? t.most : 0.0f;
+                float step = 0.0f;
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) t.sum += exp_below(v[j], t.most);
+                for (int j = 0; j < kPer; ++j) step += exp_step(v[j], most);
+                t.sum += (double)step;
+            }
+        };
+        float v[kPer], next[kPer];
+        load(begin, v);
+        if (tid == 0) sh.count = 0;
+        if (begin + kChunk < end) load(begin + kChunk, next);
+        // the first step's k best are the threshold for the others, which no barrier holds up: a wave
+        // adds what passes to the list
+        const float first = largest(v);
+        take(v, first, begin);
+        sum(v, first);
+        const float low = least ? logit_of(least) : -HUGE_VALF;
+        const int room = list_room(a.k, W);
+        for (int from = begin + kChunk; from < end; from += kChunk) {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) v[j] = next[j];
+            if (from + kChunk < end) load(from + kChunk, next);
+            const float top = largest(v);
+            if (__ballot(top >= low && top > -HUGE_VALF)) {
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) {
+                    if (!__ballot(v[j] >= low)) continue;
+                    const uint64_t key = key_of(v[j], index(from, j));
+                    if (key > least) {
+                        const int to = atomicAdd(&sh.count, 1);
+                        if (to < room) list[to] = key;
+                    }
+                }
+            }
+            sum(v, top);
+        }
+        __syncthreads();
+        if (sh.count > room) {
+            // more than the list holds: the whole part again, step by step
+            __syncthreads();
+            if (tid == 0) sh.count = 0;
+            least = 0;
+            __syncthreads();
+            for (int from = begin; from < end; from += kChunk) {
+                load(from, v);
+                const float top = largest(v);
+                take(v, top, from);
             }
         }
         t.sum = wave_sum(t.sum);
