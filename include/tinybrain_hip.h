@@ -602,16 +602,17 @@ tbh_status tbh_fp8_weight_create(tbh_device *dev, const tbh_fp8_desc *desc, tbh_
 tbh_status tbh_fp8_weight_destroy(tbh_fp8_weight *w);
 
 /* y[M, N] = x[M, K] . W[K, N] in 8-bit floating point: x (TBH_F32 or TBH_BF16,
- * rows x_stride elements apart) is quantized to e4m3 as well, with a scale for each row and block b of 128 inputs: s = the least power of two
- * (at least 2^-126) with |x| <= 448 s over the block's finite elements, q =
- * x / s rounded once, ties to even; an infinity or NaN becomes NaN.
+ * rows x_stride elements apart) is quantized to e4m3 as well, with a scale for
+ * each row and block b of 128 inputs: s = the least power of two (at least
+ * 2^-126) with |x| <= 448 s over the block's finite elements, q = x / s rounded
+ * once, ties to even; an infinity or NaN becomes NaN.
  *   y[m][n] = sum over b of s[m][b] * scale[n / 128][b] * (q . w of block b)
- * summed in fp32, rounded once to y_type.  A TBH_BF16 result of more than 32
- * rows takes q . w from the FP8 matrix instruction, which cuts its sums (about
- * 2^-15 of their size; rounding to bf16 then does 2^-9); all others have fp32
- * sums on the bf16 instruction, to which q and w are widened exactly.  (Products of two scales outside
+ * summed in fp32, rounded once to y_type.  For TBH_BF16 q . w comes from the FP8
+ * matrix instruction, which cuts its sums (about 2^-15 of their size; rounding to
+ * bf16 then does 2^-9); TBH_F32 results have fp32 sums, on the bf16 instruction, to
+ * which q and w are widened exactly.  (Products of two scales outside
  * fp32's normal range lose precision or overflow.)
- * Past 32 rows x is quantized into `workspace` (256-byte aligned,
+ * Past 16 rows x is quantized into `workspace` (256-byte aligned,
  * tbh_fp8_matmul_workspace bytes for M rows), or, if that is NULL, into the
  * workspace of (device, stream), with tbh_matmul_device's rule for captured
  * graphs; where none can be had (a capture before any eager call on its

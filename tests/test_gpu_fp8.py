@@ -3,7 +3,7 @@ oracle/experts_ref.py in float64.  x's quantization is exact up to its one
 rounding, so that results differ by sums alone: at most 2^-23 of the sum of
 magnitudes for each of 128 additions inside the matrix instructions (which may
 cut), each block's addition and scale, and half a step of the result's type.  A
-bf16 result of more than 32 rows comes from the FP8 instruction, which aligns its
+bf16 result comes from the FP8 instruction, which aligns its
 products to the largest and keeps some 17 bits of each: 128 cuts of 2^-17 of the
 largest product of a block at the most."""
 import numpy as np
@@ -49,7 +49,7 @@ def _check(y, x, w, dtype):
     want, size, largest = E.fp8_matmul(_np(x), w.data, w.scales)
     k = w.shape[0]
     tol = (128 + 3 * (-(-k // 128)) + 4) * 2.0 ** -23 * size
-    if dtype == "bfloat16" and len(want) > 32:
+    if dtype == "bfloat16":
         tol = tol + 128 * 2.0 ** -17 * largest
     tol += HALF[dtype] * (np.abs(want) + tol)
     err = np.abs(_np(y) - want)
@@ -73,6 +73,20 @@ def test_product(torch, backend, m, k, n, xt, yt):
     y = backend.fp8_matmul_device(x, backend.fp8_weight(w), dtype=getattr(torch, yt))
     assert y.dtype == getattr(torch, yt) and tuple(y.shape) == (m, n)
     _check(y, x, w, yt)
+
+
+# enough results to fill the device with blocks of 128 x 256, with larger ones, and with
+# larger ones over more than 64 blocks of 128 inputs
+@pytest.mark.parametrize("xt,yt", [("float32", "float32"), ("bfloat16", "bfloat16"), ("float32", "bfloat16"),
+                                   ("bfloat16", "float32")])
+@pytest.mark.parametrize("m,k,n", [(700, 130, 7000), (1100, 300, 7000), (1500, 8330, 4500)])
+def test_large_product(torch, backend, m, k, n, xt, yt):
+    rng = np.random.default_rng(m + k + n)
+    w = _weight(rng, k, n)
+    x = _rows(torch, rng, m, k, xt)
+    y = backend.fp8_matmul_device(x, backend.fp8_weight(w), dtype=getattr(torch, yt))
+    for at in (0, 250, m // 2, m - 24):
+        _check(y[at:at + 24], x[at:at + 24], w, yt)
 
 
 def _one_at(n):
@@ -151,11 +165,11 @@ def test_weights_of_device_and_host_tensors_are_one(torch, backend):
 
 def test_rows_past_one_part(torch, backend):
     rng = np.random.default_rng(9)
-    w = backend.fp8_weight(_weight(rng, 130, 33))
+    w = _weight(rng, 130, 33)
     x = _rows(torch, rng, (1 << 14) + 77, 130, "float32")
-    y = backend.fp8_matmul_device(x, w)
+    y = backend.fp8_matmul_device(x, backend.fp8_weight(w))
     for at in (0, 1000, (1 << 14) - 40, (1 << 14), (1 << 14) + 37):
-        assert torch.equal(y[at:at + 40], backend.fp8_matmul_device(x[at:at + 40].clone(), w)[:len(y) - at])
+        _check(y[at:at + 40], x[at:at + 40], w, "float32")
 
 
 @pytest.mark.parametrize("m", [5, 70])

@@ -623,7 +623,7 @@ class HIPBackend:
             raise PreconditionFailure("fp8: out must be [M, N] of the type asked for")
         xt, yt = self._paged_type(x), self._paged_type(out)
         room, size = None, 0
-        if rows > 32 and torch.cuda.is_current_stream_capturing():
+        if rows > 16 and torch.cuda.is_current_stream_capturing():
             need = ctypes.c_int64()
             _check(self._lib.tbh_fp8_matmul_workspace(weight.handle, rows, ctypes.byref(need)))
             room, size = self._room(stream, x, need.value)

@@ -2,8 +2,9 @@
 // their kernels share (tbh_fp8.hip, tbh_moe.hip).
 //
 // A matrix of N outputs by K inputs is stored as tiles of 16 outputs x 128
-// inputs, 2 KiB each, [ceil(N / 16)][ceil(K / 128)], padded with zeros to 128
-// outputs.  In a tile, byte i of 16-byte piece (h, g, r) is output r, input
+// inputs, 2 KiB each, padded with zeros to whole blocks of 128 outputs, the eight
+// tiles of a block (what shares a scale) together: [ceil(N / 128)][ceil(K / 128)][8].
+// In a tile, byte i of 16-byte piece (h, g, r) is output r, input
 // 64 h + 16 g + i, pieces in the order h, g, r: lane (g, r) = 16 g + r of a
 // wave finds both halves of its matrix operand with two loads that each cover
 // 1 KiB, and both operands of a product use the same order, so that which
@@ -32,15 +33,20 @@ inline int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
 
 // A matrix in that layout on the device.
 struct Matrix {
-    const uint8_t *tiles;      // [row_blocks * 8][k_blocks][2048]
+    const uint8_t *tiles;      // [row_blocks][k_blocks][8][2048]
     const float *scales;       // [row_blocks][k_blocks]
 };
 
-// Writes `count` matrices of N x K e4m3 bytes (row-major, one after the other) as tiles;
-// tile row t of matrix i goes to tiles + (i * row_tiles + t * step) * k_blocks * 2048, with
-// row_tiles tile rows per matrix in the result (tbh_fp8.hip).
-hipError_t launch_repack(const uint8_t *data, int64_t N, int64_t K, int64_t count, int64_t row_tiles, int64_t step,
+// Writes `count` matrices of N x K e4m3 bytes (row-major, one after the other) as tiles,
+// one matrix after the other: tile t of block b goes to place (t / group * k_blocks + b) *
+// group * step + t % group * step of its matrix's (places of `step` tiles; tbh_fp8.hip).
+hipError_t launch_repack(const uint8_t *data, int64_t N, int64_t K, int64_t count, int64_t group, int64_t step,
                          uint8_t *tiles, hipStream_t s);
+
+// Where tile t of block b of a matrix in groups of eight tiles starts.
+__device__ __forceinline__ int64_t tile_at(int64_t t, int64_t b, int64_t k_blocks) {
+    return ((t >> 3) * k_blocks + b) * (8 * kTileBytes) + (t & 7) * kTileBytes;
+}
 
 // Copies `bytes` from host or device memory into a new device allocation.
 hipError_t copy_in(void **out, const void *from, size_t bytes, hipStream_t s);
@@ -73,34 +79,6 @@ __device__ __forceinline__ f32x4 mfma_wide(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// 16 elements of a row as float: those at and behind `left` are 0.
-template <class T>
-__device__ __forceinline__ void load16(const T *p, int left, bool vec, float (&x)[16]) {
-    if (vec && left >= 16) {
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 v = *(const f32x4 *)(p + 4 * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const u32x4 v = *(const u32x4 *)(p + 8 * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    x[8 * i + 2 * j] = __builtin_bit_cast(float, v[j] << 16);
-                    x[8 * i + 2 * j + 1] = __builtin_bit_cast(float, v[j] & 0xFFFF0000u);
-                }
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = i < left ? (float)p[i] : 0.0f;
-    }
-}
-
 // The largest of the four lanes that hold one row's block (lane, and those 16, 32 and 48 away).
 __device__ __forceinline__ uint32_t row_most(uint32_t v) {
     const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
@@ -109,45 +87,99 @@ __device__ __forceinline__ uint32_t row_most(uint32_t v) {
     return max(b[0], b[1]);
 }
 
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// A lane's 32 elements of a row's block as they are stored: inputs 16 g .. 16 g + 15 of both halves.
+template <class T>
+struct Block {
+    static constexpr int kWords = sizeof(T) == 4 ? 16 : 8;      // of a half
+    uint32_t v[2][kWords];
+};
+
+// p: the row at input 16 g of the block; elements at and behind `left` are 0.
+template <class T>
+__device__ __forceinline__ void load_block(Block<T> &x, const T *p, int left, bool vec) {
+    constexpr int N = Block<T>::kWords;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int rest = left - 64 * h;
+        if (vec && rest >= 16) {
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i) {
+                const u32x4 q = *(const u32x4 *)((const uint32_t *)(p + 64 * h) + 4 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x.v[h][4 * i + j] = q[j];
+            }
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x.v[h][i] = i < rest ? __builtin_bit_cast(uint32_t, p[64 * h + i]) : 0u;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint16_t *u = (const uint16_t *)p + 64 * h + 2 * i;
+                x.v[h][i] = (2 * i < rest ? u[0] : 0u) | (2 * i + 1 < rest ? (uint32_t)u[1] << 16 : 0u);
+            }
+        }
+    }
+}
+
 // Quantizes a row's block of 128, of which this lane holds 32 and the three
 // lanes 16, 32 and 48 away the others: scale s, the least power of two (at
 // least 2^-126) with max |x| <= 448 s over the finite elements, and e4m3(x / s),
-// ties to even.  x / s is exact, so that the one rounding is the last.  Not
-// finite: NaN.
-__device__ __forceinline__ float quantize_block(const float (&x)[2][16], i32x8 &q) {
+// ties to even: the conversion scales exactly and rounds once, and makes NaN of
+// what is not finite.
+template <class T>
+__device__ __forceinline__ float quantize_block(const Block<T> &x, i32x8 &q) {
     uint32_t most = 0;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const uint32_t u = __builtin_bit_cast(uint32_t, x[h][i]) & 0x7FFFFFFFu;
-            most = max(most, u >= 0x7F800000u ? 0u : u);
-        }
+            for (int i = 0; i < 16; ++i) most = max(most, x.v[h][i] & 0x7FFFFFFFu);
+    } else {
+        u16x2 m{0, 0};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x.v[h][i] & 0x7FFF7FFFu));
+        most = (uint32_t)max(m[0], m[1]) << 16;
+    }
+    if (most >= 0x7F800000u) {        // rare: the largest of what is finite
+        most = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < Block<T>::kWords; ++i) {
+                const uint32_t w = x.v[h][i];
+                const uint32_t a = (sizeof(T) == 4 ? w : w << 16) & 0x7FFFFFFFu, b = sizeof(T) == 4 ? 0u : w & 0x7FFF0000u;
+                most = max(most, max(a < 0x7F800000u ? a : 0u, b < 0x7F800000u ? b : 0u));
+            }
+    }
     most = row_most(most);
     // 448 = 1.75 * 2^8: a mantissa above 1.75 needs the next power
     int e = (int)(most >> 23) - 127 - 8 + ((most & 0x7FFFFFu) > 0x600000u ? 1 : 0);
     e = max(e, -126);
-    const float inv = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);   // 2^-e, e in -126 .. 120
+    const float s = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);      // e in -126 .. 120
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float v[4];
+            s16x2 w{0, 0};
+            if constexpr (sizeof(T) == 4) {
+                float f[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = x[h][4 * i + j] * inv;
-                // (the conversion takes an infinity to 448 or NaN by a mode of the wave)
-                if (__builtin_isinf(v[j])) v[j] = __builtin_nanf("");
+                for (int j = 0; j < 4; ++j) f[j] = __builtin_bit_cast(float, x.v[h][4 * i + j]);
+                w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, f[0], f[1], s, false);
+                w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, f[2], f[3], s, true);
+            } else {
+                w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2, x.v[h][2 * i]), s, false);
+                w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2, x.v[h][2 * i + 1]), s, true);
             }
-            int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-            q[4 * h + i] = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
+            q[4 * h + i] = __builtin_bit_cast(int, w);
         }
-    return __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
-}
-
-template <class T>
-__device__ __forceinline__ T rounded(float v) {
-    return (T)v;
+    return s;
 }
 
 // Four results of one row from column n on: those at and behind N are left out.
@@ -157,7 +189,6 @@ __device__ __forceinline__ void store4(T *p, f32x4 v, int64_t left, bool vec) {
         if constexpr (sizeof(T) == 4) {
             *(f32x4 *)p = v;
         } else {
-            typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
             *(bf16x4 *)p = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
         }
     } else {
@@ -174,6 +205,6 @@ struct tbh_fp8_weight {
     tbh_device *dev = nullptr;
     int64_t K = 0, N = 0;
     int64_t kb = 0, nb = 0;          // blocks of 128 along K and N
-    uint8_t *tiles = nullptr;        // [nb * 8][kb][2048]
+    uint8_t *tiles = nullptr;        // [nb][kb][8][2048]
     float *scales = nullptr;         // [nb][kb]
 };

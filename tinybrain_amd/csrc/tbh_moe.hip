@@ -21,7 +21,7 @@ struct tbh_moe {
     int64_t H = 0, I = 0, hb = 0, ib = 0;     // blocks of 128
     int32_t E = 0;
     float *router = nullptr;                  // [E][hb * 128], padded with zeros
-    uint8_t *gate_up = nullptr;               // [E][ib * 8][gate, up][hb][2048]
+    uint8_t *gate_up = nullptr;               // [E][ib * 8][hb][gate, up][2048]
     uint8_t *down = nullptr;                  // [E][hb * 8][ib][2048]
     float *gate_scales = nullptr, *up_scales = nullptr;   // [E][ib][hb]
     float *down_scales = nullptr;             // [E][hb][ib]
@@ -374,8 +374,8 @@ __device__ __forceinline__ void up_tokens(const Args &a, int e, int tile, const 
     const int b0 = a.hb * wave / 4, b1 = a.hb * (wave + 1) / 4;
     for (int b = b0; b < b1; ++b) {
         i32x4 w[2][2];
-        load_tile(w[0], wt + (int64_t)b * kTileBytes);
-        load_tile(w[1], wt + (int64_t)(a.hb + b) * kTileBytes);
+        load_tile(w[0], wt + (int64_t)b * (2 * kTileBytes));
+        load_tile(w[1], wt + (int64_t)b * (2 * kTileBytes) + kTileBytes);
         const float s[2] = {a.gate_scales[sb + b], a.up_scales[sb + b]};
         const __bf16 *at[CT];
 #pragma unroll
@@ -676,17 +676,17 @@ tbh_status tbh_moe_create(tbh_device *dev, const tbh_moe_desc *desc, tbh_moe **o
     if (e == hipSuccess) e = fp8::copy_in((void **)&m->down_scales, d.down_scales, scales, s);
     if (e == hipSuccess) e = hipMalloc((void **)&m->gate_up, 2 * tiles);
     if (e == hipSuccess) e = hipMalloc((void **)&m->down, tiles);
-    auto repack = [&](const uint8_t *from, int64_t N, int64_t K, int64_t row_tiles, int64_t step, uint8_t *to) {
+    auto repack = [&](const uint8_t *from, int64_t N, int64_t K, int64_t step, uint8_t *to) {
         void *raw = nullptr;
         if (e == hipSuccess) e = fp8::copy_in(&raw, from, bytes, s);
-        if (e == hipSuccess) e = fp8::launch_repack((const uint8_t *)raw, N, K, m->E, row_tiles, step, to, s);
+        if (e == hipSuccess) e = fp8::launch_repack((const uint8_t *)raw, N, K, m->E, 1, step, to, s);
         const hipError_t waited = hipStreamSynchronize(s);
         if (e == hipSuccess) e = waited;
         if (raw) (void)hipFree(raw);
     };
-    repack(d.gate, m->I, m->H, m->ib * 16, 2, m->gate_up);
-    repack(d.up, m->I, m->H, m->ib * 16, 2, m->gate_up ? m->gate_up + m->hb * kTileBytes : nullptr);
-    repack(d.down, m->H, m->I, m->hb * 8, 1, m->down);
+    repack(d.gate, m->I, m->H, 2, m->gate_up);
+    repack(d.up, m->I, m->H, 2, m->gate_up ? m->gate_up + kTileBytes : nullptr);
+    repack(d.down, m->H, m->I, 1, m->down);
     if (e != hipSuccess) {
         (void)hipGetLastError();
         return hip_error(e, what);
