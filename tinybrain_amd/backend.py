@@ -42,6 +42,9 @@ from .paged import PagedPlan
 from .quantized import PreconditionFailure, QuantizedTensor
 
 
+_PAGED_TYPES: Dict = {}          # the types of _paged_type, once there was a tensor
+
+
 class HIPBackendError(RuntimeError):
     """A non-zero tbh_status (the reference backend's `throws`)."""
 
@@ -583,13 +586,15 @@ class HIPBackend:
 
     @staticmethod
     def _paged_type(t) -> int:
-        import torch
+        code = _PAGED_TYPES.get(t.dtype)
+        if code is None:
+            import torch
 
-        if t.dtype == torch.float32:
-            return _abi.F32
-        if t.dtype == torch.bfloat16:
-            return _abi.BF16
-        raise PreconditionFailure("expected float32 or bfloat16")
+            _PAGED_TYPES.update({torch.float32: _abi.F32, torch.bfloat16: _abi.BF16})
+            code = _PAGED_TYPES.get(t.dtype)
+            if code is None:
+                raise PreconditionFailure("expected float32 or bfloat16")
+        return code
 
     def _kv_arrays(self, keys, values):
         """blocks, kvHeads, blockSize, headDim, type of the cache arrays."""
@@ -786,10 +791,11 @@ class HIPBackend:
         if len(keys) != len(values) or not len(keys):
             raise PreconditionFailure("reorder: one array of keys and one of values per layer")
         n, nkv, bs, hd, ct = self._kv_arrays(keys[0], values[0])
-        shape, dtype = keys[0].shape, keys[0].dtype
-        for a in (*keys[1:], *values[1:]):
-            if a.shape != shape or a.dtype != dtype or not a.is_contiguous() or a.get_device() != self.device:
-                raise PreconditionFailure("reorder: every layer's arrays must be alike")
+        layers, shape, dtype, device = len(keys), keys[0].shape, keys[0].dtype, self.device
+        if layers > 1:
+            for a in (*keys[1:], *values[1:]):
+                if a.shape != shape or a.dtype != dtype or not a.is_contiguous() or a.get_device() != device:
+                    raise PreconditionFailure("reorder: every layer's arrays must be alike")
         self._ints(torch.int32, blockTable, contextLens, parents)
         b = contextLens.numel()
         if beams <= 0 or b % beams:
@@ -811,12 +817,11 @@ class HIPBackend:
             layout = self._layout.pack(n, bs, nkv, hd, ct, b, blockTable.shape[1])
         except struct.error:
             raise self._past_32_bits() from None
-        layers = len(keys)
-        pointers = ctypes.c_void_p * layers
+        pointers = "%dP" % layers
         _check(self._lib.tbh_paged_reorder_device(
             self._dev, layout, beams, parents.data_ptr(), contextLens.data_ptr(),
             None if sharedLens is None else sharedLens.data_ptr(), blockTable.data_ptr(), tableOut.data_ptr(), layers,
-            pointers(*[a.data_ptr() for a in keys]), pointers(*[a.data_ptr() for a in values]),
+            struct.pack(pointers, *[a.data_ptr() for a in keys]), struct.pack(pointers, *[a.data_ptr() for a in values]),
             None if reordered is None else reordered.data_ptr(), self._raw_stream(stream)))
         return tableOut
 
