@@ -56,7 +56,7 @@ def _compare(got, want, vocab=1 << 20):
 @pytest.mark.parametrize("requests,beams,k,vocab", [
     (1, 1, 1, 1), (1, 1, 1, 2), (1, 4, 4, 5), (3, 2, 4, 3), (1, 4, 4, 32000), (5, 3, 6, 1000), (2, 8, 16, 4096),
     (2, 8, 8, 4095), (2, 5, 5, 4097), (1, 64, 64, 9000), (3, 1, 64, 50), (40, 4, 8, 700), (1, 2, 2, 1 << 20),
-    (7, 16, 32, 20001),
+    (7, 16, 32, 20001), (64, 4, 40, 30011),
 ])
 @pytest.mark.parametrize("ended", [False, True])
 def test_selection(torch, backend, requests, beams, k, vocab, ended):
@@ -97,10 +97,11 @@ def test_values_that_are_not_finite(torch, backend):
                 _select(torch, backend, x, s, 4, k, done, 0)
 
 
-@pytest.mark.parametrize("rows,vocab", [(2, 20000), (100, 30000), (128, 40000), (132, 16385)])
+@pytest.mark.parametrize("rows,vocab,k", [(2, 20000, 8), (100, 30000, 8), (128, 40000, 8), (132, 16385, 8),
+                                          (256, 40000, 32), (260, 16385, 64)])
 @pytest.mark.parametrize("order", ["ascending", "descending", "constant", "late", "nan", "waves"])
-def test_orders_that_fill_the_lists(torch, backend, rows, vocab, order):
-    # 2 rows in many parts, 100 in parts of several steps, 128 and more in one
+def test_orders_that_fill_the_lists(torch, backend, rows, vocab, k, order):
+    # 2 rows in many parts, 100 and more in parts of several steps, 256 and more in one
     rng = np.random.default_rng(rows + vocab)
     x = np.sort(rng.normal(size=(rows, vocab)).astype(np.float32), 1)
     if order == "descending":
@@ -115,7 +116,7 @@ def test_orders_that_fill_the_lists(torch, backend, rows, vocab, order):
     elif order == "waves":                       # some waves' elements all above the others'
         x += 50.0 * ((np.arange(vocab) // 256) % 4 == 1)
     s = -rng.random(rows).astype(np.float32)
-    _select(torch, backend, x, s, 4 if rows % 4 == 0 else 2, 8)
+    _select(torch, backend, x, s, 4 if rows % 4 == 0 else 2, k)
 
 
 def test_first_step_of_a_search(torch, backend):

@@ -357,7 +357,10 @@ __device__ __forceinline__ void join_parts(const SelectArgs &a, int row, uint64_
 // exp(logit - largest), 64 bits over 32-bit steps, and the k best elements, by a list of those that pass a
 // key that k elements before them are not below.  The row's last
 // block joins its parts, the request's last its rows (a counter takes some 70 ns an
-// arrival, so that they are counted in two steps).
+// arrival, so that they are counted in two steps).  Bound by the latency of one step, its
+// ranking and the two joins for few rows (4 of 32000, k = 4: 12 us, of which the loads are
+// 2.5), by memory and the instructions of a step, some 60 for 16 elements, for many: 256 rows
+// of 100000, k = 16 33.5 us, 3.1 TB/s.
 template <int W>
 __global__ __launch_bounds__(64 * W) void beam_select(SelectArgs a) {
     constexpr int NT = 64 * W, kChunk = NT * kPer;
@@ -651,15 +654,18 @@ void launch_copy(const ReorderArgs &a, dim3 grid, hipStream_t s) {
     hipLaunchKernelGGL((reorder_copy<V>), grid, dim3(256), 0, s, a);
 }
 
-// How a call's rows are parted.  Rows for every second CU and more: a block of 16 waves
-// a row.  Fewer: blocks of four waves, of 4096 elements at the least, until there are
-// some four a CU.
+// How a call's rows are parted.  Blocks of four waves, of 4096 elements at the least, until
+// there are some four a CU; but a block of 16 waves a row, which ranks one list where the parts'
+// lists would be ranked and joined, where each CU has a row and vocab * k is 2^20 or more.  Four
+// waves / 16 in us: 256 rows of 100000, k = 16 43.6 / 36.6, k = 8 37.1 / 35.2, of 150000, k = 8
+// 49.1 / 45.5; 128 rows of 100000, k = 16 30.1 / 31.0; 1024 rows of 16000, k = 8 24.5 / 56.3, of
+// 64000, k = 16 91.4 / 98.5, of 100000, k = 16 150 / 128; 4 rows of 32000, k = 4 13.1 / 17.8.
 struct Parts {
     int waves, part, splits;
 };
-Parts parts_of(const tbh_device *dev, int64_t rows, int64_t vocab) {
+Parts parts_of(const tbh_device *dev, int64_t rows, int64_t vocab, int64_t k) {
     const int64_t cus = std::max(1, dev->cu_count);
-    if (2 * rows >= cus && vocab > 4096) return {16, (int)vocab, 1};
+    if (rows >= cus && vocab * k >= 1 << 20) return {16, (int)vocab, 1};
     const int64_t chunks = (vocab + 4095) / 4096, most = std::max<int64_t>(1, std::min(chunks, (4 * cus + rows - 1) / rows));
     const int64_t each = (chunks + most - 1) / most;
     return {4, (int)(each * 4096), (int)((chunks + each - 1) / each)};
@@ -696,7 +702,7 @@ tbh_status tbh_beam_select_workspace(tbh_device *dev, int64_t requests, int32_t 
     const tbh_status st = check_select(what, dev, requests, beams, vocab, k);
     if (st != TBH_OK) return st;
     if (!bytes) return set_error(TBH_E_INVALID, std::string(what) + ": NULL pointer");
-    const Parts p = parts_of(dev, requests * beams, vocab);
+    const Parts p = parts_of(dev, requests * beams, vocab, k);
     *bytes = (int64_t)kCounterBytes;
     if (requests) *bytes += part_of(requests, beams, p.splits, k) * (int64_t)request_bytes(beams, p.splits, k);
     return TBH_OK;
@@ -715,7 +721,7 @@ tbh_status tbh_beam_select_device(tbh_device *dev, const float *logits, int64_t 
     if (ld < vocab && requests * beams > 1) return bad("ld is shorter than vocab");
     if (done && (eos < 0 || eos >= vocab)) return bad("done rows need an eos within the vocabulary");
     if (workspace && ((uintptr_t)workspace & 255)) return bad("the workspace must be 256-byte aligned");
-    const Parts p = parts_of(dev, requests * beams, vocab);
+    const Parts p = parts_of(dev, requests * beams, vocab, k);
     const int64_t part = part_of(requests, beams, p.splits, k);
     const size_t need = (size_t)part * request_bytes(beams, p.splits, k);
     if (workspace && (workspace_bytes < 0 || (size_t)workspace_bytes < need + kCounterBytes))
