@@ -611,7 +611,7 @@ tbh_status tbh_fp8_weight_destroy(tbh_fp8_weight *w);
  * matrix instruction, which cuts its sums (about 2^-15 of their size; rounding to
  * bf16 then does 2^-9); TBH_F32 results have fp32 sums, on the bf16 instruction, to
  * which q and w are widened exactly.  (Products of two scales outside
- * fp32's normal range lose precision or overflow.)
+ * fp32's normal range lose precision or overflow.)  y does not overlap x.
  * Past 16 rows x is quantized into `workspace` (256-byte aligned,
  * tbh_fp8_matmul_workspace bytes for M rows), or, if that is NULL, into the
  * workspace of (device, stream), with tbh_matmul_device's rule for captured
@@ -729,7 +729,8 @@ tbh_status tbh_beam_select_device(tbh_device *dev, const float *logits, int64_t 
  *     contents of their parent's positions shared_lens[group] (rounded down to
  *     whole blocks; NULL: 0) .. context are copied into those blocks, in every
  *     layer's arrays.  Positions before shared_lens are taken to be the same in
- *     the whole group: a prompt's.
+ *     the whole group: a prompt's, whose whole blocks rows may share; of the
+ *     others each stands in one place of the table only.
  * So blocks stay with the group and nothing is allocated.  The rows of a group
  * hold equally many tokens (context_lens); a group whose rows do not, or with a
  * parent outside it, is left as it is.  reordered[groups] (or NULL): 1, or 0 for

@@ -6,6 +6,8 @@ cut), each block's addition and scale, and half a step of the result's type.  A
 bf16 result comes from the FP8 instruction, which aligns its
 products to the largest and keeps some 17 bits of each: 128 cuts of 2^-17 of the
 largest product of a block at the most."""
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 
@@ -234,6 +236,12 @@ def test_preconditions(torch, backend):
                dict(out=torch.zeros(2, 32, device="cuda"), dtype=torch.bfloat16)):
         with pytest.raises(PreconditionFailure):
             backend.fp8_matmul_device(x, w, **kw)
+    elsewhere = SimpleNamespace(K=64, N=32, backend=SimpleNamespace(device=1))
+    with pytest.raises(PreconditionFailure):
+        backend.fp8_matmul_device(x, elsewhere)
+    square = backend.fp8_weight(_weight(np.random.default_rng(13), 64, 64))
+    with pytest.raises(T.HIPBackendError):
+        backend.fp8_matmul_device(x, square, out=x)
     data, scales = torch.zeros(32, 64, dtype=torch.uint8), torch.ones(1, 1)
     for d, s in ((data[0], scales), (data, scales[0]), (data.float(), scales), (data, scales.double()),
                  (data.t(), scales), (data, torch.ones(1, 2)), (data.numpy(), scales), (data[:0], scales)):

@@ -1,5 +1,7 @@
 """GPU tests of the mixture-of-experts layer (tbh_moe_device) against
 oracle/experts_ref.py in float64, whose bound says how far fp32 sums may be."""
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 
@@ -187,6 +189,10 @@ def test_preconditions(torch, backend):
                dict(topK=2, weights=torch.zeros(2, 2, dtype=torch.float64, device="cuda"))):
         with pytest.raises(PreconditionFailure):
             backend.moe_device(x, model.layer, **kw)
+    with pytest.raises(PreconditionFailure):
+        backend.moe_device(x, SimpleNamespace(hidden=32, experts=3, backend=SimpleNamespace(device=1)), 1)
+    with pytest.raises(T.HIPBackendError):
+        backend.moe_device(x, model.layer, 1, out=x)
     a = model.args
     for i, bad in ((0, a[0][:2]), (0, a[0].astype(np.float64)), (1, a[1][:, :15]), (2, a[2][:2]),
                    (3, a[3][:, :, :31]), (5, a[3]), (6, a[6][:, :, :0])):

@@ -622,6 +622,8 @@ class HIPBackend:
         rows, k = self._row_shape(x)
         if k != weight.K:
             raise PreconditionFailure("Dimensions must match")
+        if weight.backend.device != self.device:
+            raise PreconditionFailure("fp8: the weight is on another device")
         if out is None:
             out = self._made(stream, x.new_empty, (rows, weight.N), dtype=x.dtype if dtype is None else dtype)
         elif self._row_shape(out) != (rows, weight.N) or (dtype is not None and out.dtype != dtype):
@@ -654,6 +656,8 @@ class HIPBackend:
         tokens, width = shape = self._row_shape(x)
         if width != layer.hidden:
             raise PreconditionFailure("moe: x must be [tokens, hidden]")
+        if layer.backend.device != self.device:
+            raise PreconditionFailure("moe: the layer is on another device")
         xt = self._paged_type(x)
         if not 0 < topK <= layer.experts:
             raise PreconditionFailure("moe: topK must be 1 .. experts")

@@ -604,6 +604,7 @@ tbh_status tbh_fp8_matmul_device(const tbh_fp8_weight *w, const void *x, int32_t
     if (K != w->K) return bad("Dimensions must match");
     if (M == 0) return TBH_OK;
     if (!x || !y) return bad("NULL x or y");
+    if (x == y) return bad("y overlaps x");
     if (M > 1 && (x_stride < K || y_stride < w->N)) return bad("a stride is shorter than its row");
     if (workspace && ((uintptr_t)workspace & 255)) return bad("the workspace must be 256-byte aligned");
     if (workspace_bytes < 0) return bad("negative workspace_bytes");

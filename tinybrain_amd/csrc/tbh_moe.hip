@@ -7,6 +7,14 @@
 // and h stay as exact as they came, as bf16 or as three bf16 pieces of an fp32,
 // and the weights are widened to bf16 (exactly) on their way to the matrix
 // instruction.
+//   Three launches, as every chosen expert's h has to be whole before D_e, and the
+// choice before either.  Their times in us (route, up, down; floor: the chosen experts'
+// bytes at the 4.8 TB/s of a large copy):
+//   1 token, 2 of 8 experts of 2048 x 5632, fp32 rows      8.4  11.4  10.8   (14.5)
+//   13 tokens, 6 of 64 experts of 2048 x 1000, bf16       11.7  41.2  28.6   (59)
+//   64 tokens, 4 of 32 experts of 4096 x 2048, bf16       13.5  110   67.8   (168)
+// What is above the floor is the latency of launches and of loads that depend on
+// one another (ids, lists, weights, the join), not the work.
 #include <algorithm>
 #include <cmath>
 #include <memory>
@@ -195,7 +203,9 @@ __device__ __forceinline__ void choose(const Args &a, int t) {
 // token r and of expert r; of the result, experts 4 i + g of token r.  The instruction
 // takes 64 cycles, so that a tile is parted over 16 waves and a.splits blocks; the block
 // that finishes a tile of tokens picks their experts, a wave a token.  Blocks of the
-// first experts also write the rows' pieces.
+// first experts also write the rows' pieces.  Bound by latency: of 8.4 us for one token
+// and 8 experts, 2.6 are the loads and products, 1.9 the sums over waves, 0.9 the count of
+// the blocks, 1.0 the choice.
 template <class T, int P>
 __global__ __launch_bounds__(1024) void moe_route(Args a) {
     __shared__ double part[16][256];
@@ -417,7 +427,10 @@ __device__ __forceinline__ void up_tokens(const Args &a, int e, int tile, const 
 }
 
 // Gate and up products of 16 inner columns of one expert and h = silu(gate) * up;
-// the waves part the inputs.
+// the waves part the inputs.  Gate's and up's tiles lie side by side, so that a wave
+// reads 4 KiB in a row a step.  Bound by memory: 32 experts of 4096 x 2048 (537 MB) in 105 us,
+// 5.1 TB/s, 2 of 2048 x 5632 (46 MB) in 9.6 behind the 1.0 of the search for the expert.  (Two
+// or four steps' loads ahead of the products: no faster, the blocks of a CU hide each other's.)
 template <int P>
 __global__ __launch_bounds__(256) void moe_up(Args a) {
     __shared__ uint32_t used[kMaxExperts / 32];
@@ -431,6 +444,8 @@ __global__ __launch_bounds__(256) void moe_up(Args a) {
         if (e >= 0 && (int)threadIdx.x < count) l[kListHead + threadIdx.x] = slots[threadIdx.x];
     }
     if (e < 0) return;
+    // two column tiles to a load of the weights while there are more than one's tokens (64 tokens, 2
+    // of 8 experts of 4096 x 4096: 120 us against 128 one at a time, of fp32 231 and 252)
     int c0 = 0;
     for (; count - c0 > kTokens<P>; c0 += 2 * kTokens<P>) up_tokens<P, 2>(a, e, blockIdx.x, slots, c0, count, red);
     if (c0 < count) up_tokens<P, 1>(a, e, blockIdx.x, slots, c0, count, red);
@@ -441,7 +456,9 @@ __global__ __launch_bounds__(256) void moe_up(Args a) {
 // multiplied; each wave adds its share of a token's sum to its own row in LDS, once an
 // expert.  Joined in order, and over the blocks by the one that is last.  (A tile for one
 // token needs twice as many loads of h as of weights, so that a wave takes two tiles a
-// load of h.)
+// load of h.)  Bound by memory where there are many experts (268 MB in 60 us, 4.5 TB/s), by the
+// latency of the join for one token: 4.6 of 10.8 us are products.  (kUnit 1, 2 or 4: a whole call on
+// 1 token 29.1, 28.9, 31.4 us, on 64 177, 169, 169.)
 constexpr int kDownWaves = 8, kUnit = 2;
 
 template <class T, int P>
@@ -547,7 +564,14 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down(Args a) {
     if (a.parts == 1 || !last_to_arrive(a.counters + blockIdx.x, a.parts, (uint32_t *)sums)) return;
     for (int j = tid; j < a.T * 32; j += 64 * kDownWaves) {
         float v = 0.0f;
-        for (int i = 0; i < a.parts; ++i) v += handed_over(part + (int64_t)i * a.T * 32 + j);
+        // (four at a time: a load past the caches takes a third of a microsecond)
+        for (int i = 0; i < a.parts; i += 4) {
+            float u[4];
+#pragma unroll
+            for (int o = 0; o < 4; ++o) u[o] = i + o < a.parts ? handed_over(part + (int64_t)(i + o) * a.T * 32 + j) : 0.0f;
+#pragma unroll
+            for (int o = 0; o < 4; ++o) v += u[o];
+        }
         store(j, v);
     }
 }
@@ -574,9 +598,11 @@ void size_up(Args &a, const tbh_moe &m, int64_t tokens, int32_t top_k) {
     a.hb = (int)m.hb;
     a.ib = (int)m.ib;
     a.used = std::min(m.E, a.T * top_k);
-    // two steps of 16 inputs a wave
+    // two steps of 16 inputs a wave at the least (1, 2 or 4 parts: a whole call on 1 token 33.3,
+    // 30.5, 28.9 us, on 64 of width 4096 184, 174, 169)
     a.splits = std::max(1, std::min(kSplits, a.hb * (kBlock / 16) / 32));
-    // a block a CU, of waves that have a unit at the least
+    // a block a CU, of waves that have a unit at the least (one part a tile: 13 tokens of width 2048
+    // 106 us, 73 so, 64 of 4096 194 and 169)
     const int tiles = (a.H + 31) / 32, units = a.used * ((a.ib + kUnit - 1) / kUnit);
     a.parts = std::max(1, std::min((m.dev->cu_count + tiles - 1) / tiles, units / kDownWaves));
 }
@@ -722,6 +748,7 @@ tbh_status tbh_moe_device(const tbh_moe *m, const void *x, int32_t x_type, int64
     if (st != TBH_OK) return st;
     if (tokens == 0) return TBH_OK;
     if (!x || !y) return bad("NULL x or y");
+    if (x == y) return bad("y overlaps x");
     if (tokens > 1 && (x_stride < m->H || y_stride < m->H)) return bad("a stride is shorter than its row");
     const size_t size = fp8::type_size(x_type);
     if ((uintptr_t)x % size || (uintptr_t)y % size || (uintptr_t)experts % 4 || (uintptr_t)weights % 4)
