@@ -230,6 +230,7 @@ struct Shared {
     int heads[2][W];
     double total[kMaxBeams];      // log of the sum of exp(logit)
     int state[kMaxBeams];
+    float score[kMaxBeams];
     int count;
     uint32_t seen;
 };
@@ -246,19 +247,20 @@ __device__ __forceinline__ void join_rows(const SelectArgs &a, int request, Shar
     uint64_t next = load(tid);
     if (tid < a.beams) {
         const int row = row0 + tid;
-        const float score = a.scores[row];
+        // (all loads before the first is used; a done row's sums are nothing)
+        const float score = a.scores[row], most = handed_over(a.most + (int64_t)row * a.splits);
+        const double sum = handed_over(a.sum + (int64_t)row * a.splits);
         // 1: goes on by its logits, 2: done, 3: as 1, by its infinite logits alone; 0: no candidates
         int st = a.done && a.done[row] ? 2 : 1;
         double total = 0.0;
         if (!(score > -HUGE_VALF && score < HUGE_VALF)) st = 0;
         if (st == 1) {
-            const float most = handed_over(a.most + (int64_t)row * a.splits);
-            const double sum = handed_over(a.sum + (int64_t)row * a.splits);
             st = !(most > -HUGE_VALF) ? 0 : most == HUGE_VALF ? 3 : 1;
             // infinite logits share all of the weight: the logarithm of their number
             total = (st == 1 ? (double)most : 0.0) + log(sum);
         }
         sh.state[tid] = st;
+        sh.score[tid] = score;
         sh.total[tid] = total;
     }
     if (tid == 0) sh.count = 0;
@@ -271,8 +273,8 @@ __device__ __forceinline__ void join_rows(const SelectArgs &a, int request, Shar
         bool in = false;
         if (base + NT < all) next = load(i + NT);
         if (i < all) {
-            const int row = row0 + b, st = sh.state[b];
-            const float score = a.scores[row];
+            const int st = sh.state[b];
+            const float score = sh.score[b];
             if (st == 1 || st == 3) {
                 const float v = logit_of(element);
                 key = (double)score + ((st == 3 ? 0.0 : (double)v) - sh.total[b]);
@@ -357,10 +359,12 @@ __device__ __forceinline__ void join_parts(const SelectArgs &a, int row, uint64_
 // exp(logit - largest), 64 bits over 32-bit steps, and the k best elements, by a list of those that pass a
 // key that k elements before them are not below.  The row's last
 // block joins its parts, the request's last its rows (a counter takes some 70 ns an
-// arrival, so that they are counted in two steps).  Bound by the latency of one step, its
-// ranking and the two joins for few rows (4 of 32000, k = 4: 12 us, of which the loads are
-// 2.5), by memory and the instructions of a step, some 60 for 16 elements, for many: 256 rows
-// of 100000, k = 16 33.5 us, 3.1 TB/s.
+// arrival, so that they are counted in two steps; all parts of four rows of 32000 counted
+// and joined at once: 13.1 us against 13.5 in a graph, of 16 requests of them 18.4 against
+// 15.2).  Bound by the latency of one step, its
+// ranking and the two joins for few rows (4 of 32000, k = 4: 10.5 us, of which the loads are
+// 2), by memory and the instructions of a step, some 60 for 16 elements, for many: 256 rows
+// of 100000, k = 16 31 us, 3.3 TB/s; its loads are done after 21.
 template <int W>
 __global__ __launch_bounds__(64 * W) void beam_select(SelectArgs a) {
     constexpr int NT = 64 * W, kChunk = NT * kPer;
@@ -525,16 +529,13 @@ __global__ __launch_bounds__(64 * W) void beam_select(SelectArgs a) {
         __syncthreads();
         const int n = prune<W>(list, (uint64_t *)sh.tmp.key, sh.count, a.k);
         for (int i = tid; i < a.k; i += NT) hand_over(a.best + at * a.k + i, i < n ? list[i] : 0);
-        if (tid == 0) {
-            Total s = sh.wave_total[0];
-            for (int w = 1; w < W; ++w) {
-                Total u = sh.wave_total[w];
-                const float top = fmaxf(s.most, u.most);
-                s.rescale(top), u.rescale(top);
-                s.sum += u.sum;
+        // (a lane a wave's: one after the other they took 2.7 us)
+        if (wave == W - 1) {
+            t = over_wave(lane < W ? sh.wave_total[lane] : Total{-HUGE_VALF, 0.0});
+            if (lane == 0) {
+                hand_over(a.most + at, t.most);
+                hand_over(a.sum + at, t.sum);
             }
-            hand_over(a.most + at, s.most);
-            hand_over(a.sum + at, s.sum);
         }
         if (a.splits > 1) {
             if (!last_to_arrive(a.counters + gridDim.x / a.beams + row, (uint32_t)a.splits, &sh.seen)) return;
@@ -598,7 +599,11 @@ __device__ __forceinline__ Moves plan_moves(const ReorderArgs &a, int group) {
 }
 
 // Copies what a row does not inherit; V: the unit of a copy.  With a table of
-// its own to write, the launch writes that too.
+// its own to write, the launch writes that too.  Every block works out its group's moves
+// by itself (a few ballots), so that nothing is handed from launch to launch.  Bound by memory:
+// eight groups of eight rows, 800 positions of 8 x 128 bf16 of two layers, 315 MB
+// read and written, 64 to 68 us (4.8 TB/s, a large copy's rate); by its launch for one
+// group of four: 4.4 us.
 template <class V>
 __global__ __launch_bounds__(256) void reorder_copy(ReorderArgs a) {
     const int row = blockIdx.x / a.steps, step = blockIdx.x % a.steps, group = row / a.beams;
@@ -812,7 +817,9 @@ tbh_status tbh_paged_reorder_device(tbh_device *dev, const tbh_paged_layout *lay
         for (int i = 0; i < b.count / 2; ++i) b.arrays[2 * i] = k_caches[at + i], b.arrays[2 * i + 1] = v_caches[at + i];
         if (in_place || at > 0) b.table_out = nullptr;
         if (at > 0) b.reordered = nullptr;
-        // a row's blocks parted so that there are some thousands of thread blocks
+        // a row's blocks parted so that there are some thousands of thread blocks (1024, 2048, 8192
+        // or 32768 of them: the 64 rows above 103, 91, 64, 71 us, 64 rows of 100 positions 6.1,
+        // 7.4, 8.8, 8.6; how much there is to copy is known on the device alone)
         const int64_t ys = std::max(1, b.count);
         const int64_t steps = std::max<int64_t>(1, std::min<int64_t>(a.most, 8192 / std::min<int64_t>(8192, a.rows * ys)));
         b.steps = (int)steps;

@@ -214,7 +214,8 @@ struct TilesArgs {
 // from memory straight to registers: no barrier but that of the join.  For products that
 // do not fill the device with blocks of 128 x 256, bound by the latency of the loads and then by
 // the caches, which serve x to every block of outputs and the weight to every block of rows:
-// 4096 x 11008 on 32 rows 17.4 us (2.6 TB/s of weight), 5632 x 2048 on 333 rows 19 us.
+// 21 rows by 4096 x 11008 10.4 us (4.3 TB/s of weight) behind the quantizing's 3.4, 333 of fp32
+// by 5632 x 2048 14 behind 4.
 template <class YT, int W, int RT, int KW, int CT>
 __global__ __launch_bounds__(64 * W) void fp8_few(TilesArgs a) {
     __shared__ f32x4 red[W][RT * CT][64];
@@ -283,9 +284,12 @@ constexpr uint32_t kPast = 0x7FFFFFF0u;   // past every buffer: reads as zeros
 // half as fast, with x widened by the pass that quantized it (WIDE) and the weight here.
 // Two steps of 128 inputs in LDS: a step's one barrier says that its tiles have landed and
 // that every wave is done with the step before, whose place the loads issued then take.
-// Bound by LDS and the matrix instructions together, which one barrier a step leaves too
-// little to do beside each other: 4096 rows by 4096 x 11008 202 us of this kernel (1.83
-// PFLOP/s; loads alone 115, products alone 170), fp32 results 384 us with the quantizing.
+// 4096 rows by 4096 x 11008: 193 us of this kernel (1.9 PFLOP/s; loads alone 115, products
+// alone 170), fp32 results 384 us with the quantizing.  Bound by power as much as by LDS
+// (1536 cycles of reads a step beside 2048 of products): matrix instructions alone, out of
+// registers, with these fp32 sums, run such data at 3.0 PFLOP/s and 1.6 GHz, zeros at 4.1
+// and 2.2.  (Two halves of a block's waves, one at LDS while the other multiplies: 1.4 us
+// slower of 203; cache lines touched two to four steps ahead: 20 us slower.)
 template <class YT, int WN, int WM, int TN, int TM>
 __global__ __launch_bounds__(64 * WN * WM) void fp8_tiles(TilesArgs a) {
     constexpr bool WIDE = sizeof(YT) == 4;
