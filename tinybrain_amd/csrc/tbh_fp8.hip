@@ -285,19 +285,20 @@ constexpr uint32_t kPast = 0x7FFFFFF0u;   // past every buffer: reads as zeros
 // Two steps of 128 inputs in LDS: a step's one barrier says that its tiles have landed and
 // that every wave is done with the step before, whose place the loads issued then take.
 // 4096 rows by 4096 x 11008: 193 us of this kernel (1.9 PFLOP/s; loads alone 115, products
-// alone 170), fp32 results 384 us with the quantizing.  Bound by power as much as by LDS
-// (1536 cycles of reads a step beside 2048 of products): matrix instructions alone, out of
-// registers, with these fp32 sums, run such data at 3.0 PFLOP/s and 1.6 GHz, zeros at 4.1
-// and 2.2.  (Two halves of a block's waves, one at LDS while the other multiplies: 1.4 us
-// slower of 203; cache lines touched two to four steps ahead: 20 us slower.)
+// alone 170), fp32 results 384 us with the quantizing.  Bound by the step: of its some 4500
+// cycles the matrix instructions are busy for 40 % (2050), LDS reads take 1536, loads 2800,
+// and a barrier joins them; 160 KiB of LDS hold no third step.  (Two halves of a block's
+// waves, one at LDS while the other multiplies: 210 us; cache lines touched two to four
+// steps ahead: 233.  Matrix instructions alone, out of registers and with these fp32 sums, run
+// such data at 3.0 PFLOP/s, where power brings the clock down to 1.6 GHz.)
 template <class YT, int WN, int WM, int TN, int TM>
 __global__ __launch_bounds__(64 * WN * WM) void fp8_tiles(TilesArgs a) {
     constexpr bool WIDE = sizeof(YT) == 4;
     constexpr int W = WN * WM, NT = WN * TN, MT = WM * TM, XB = (WIDE ? 2 : 1) * kTileBytes, XL = XB / 1024;
     constexpr int LOADS = (NT * 2 + MT * XL) / W;
-    static_assert((NT * 2 + MT * XL) % W == 0 && TM * 64 <= 1024, "");
+    static_assert((NT * 2 + MT * XL) % W == 0 && MT * 64 <= 1024, "");
     static_assert(NT % 8 == 0 && MT % 8 == 0 && 8 % TN == 0, "whole groups of tiles; a wave's outputs share a scale");
-    constexpr int kScales = NT * kTileBytes + MT * XB, kStage = kScales + W * 1024;
+    constexpr int kScales = NT * kTileBytes + MT * XB, kStage = kScales + 1024;
     static_assert(2 * kStage <= 160 * 1024, "");
     __shared__ __align__(16) char sm[2 * kStage];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -332,10 +333,10 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tiles(TilesArgs a) {
                        (uint32_t)((t >> 3) * (of_w ? row : xrow)) + (t & 7) * (of_w ? kTileBytes : XB) + part * 1024 + lane * 16,
                        b * (8 * (of_w ? kTileBytes : XB)));
         }
-        // the scales of the wave's rows
-        dma::dma16(__builtin_amdgcn_readfirstlane(lds + kScales + wave * 1024), sr,
-                   lane < TM * 4 && sm0 + lane * 4 < mp ? (uint32_t)(sm0 * 4 + lane * 16) : kPast,
-                   b * (uint32_t)(mp * 4));
+        // the scales of the block's rows
+        if (wave == 0)
+            dma::dma16(__builtin_amdgcn_readfirstlane(lds + kScales), sr,
+                       lane < MT * 4 && m0 * 16 + lane * 4 < mp ? (uint32_t)(m0 * 64 + lane * 16) : kPast, b * (uint32_t)(mp * 4));
     };
     f32x4 acc[TN][TM];
 #pragma unroll
@@ -343,27 +344,18 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tiles(TilesArgs a) {
 #pragma unroll
         for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     // (a wave's outputs lie in one block of 128)
-    const float *sw = a.w.scales + min((n0 + wn * TN) / 8, (int64_t)a.w_tiles / 8 - 1) * a.kb;
-    // 64 steps' scales, a lane each.  (Waited for at once: the compiler does not know of the
-    // copies to LDS, and a wait of its own in the loop would be for all of them.)
-    auto hold = [&](int b) {
-        float v = b + lane < a.kb ? sw[b + lane] : 0.0f;
-        asm volatile("s_waitcnt vmcnt(0)" : "+v"(v)::"memory");
-        return v;
-    };
-    float held = hold(0);
+    const auto *sw = (const __attribute__((address_space(4))) float *)(a.w.scales + min((n0 + wn * TN) / 8, (int64_t)a.w_tiles / 8 - 1) * a.kb);
     issue(0, 0);
     for (int b = 0; b < a.kb; ++b) {
         const int buf = b & 1;
-        if (b && (b & 63) == 0) held = hold(b);
+        const float s = sw[b];
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
         issue(b + 1, buf ^ 1);
         const char *st = sm + buf * kStage;
         const char *wt = st + wn * TN * kTileBytes + lane * 16, *xt = st + NT * kTileBytes + wm * TM * XB + lane * 16;
-        const float s = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), b & 63));
         float f[TM];
 #pragma unroll
-        for (int j = 0; j < TM; ++j) f[j] = s * *(const float *)(st + kScales + wave * 1024 + (j * 16 + r16) * 4);
+        for (int j = 0; j < TM; ++j) f[j] = s * *(const float *)(st + kScales + ((wm * TM + j) * 16 + r16) * 4);
         auto add = [&](int i, int j, f32x4 part) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(part[e], f[j], acc[i][j][e]);
@@ -392,12 +384,13 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tiles(TilesArgs a) {
                 const i32x4 lo = *(const i32x4 *)p, hi = *(const i32x4 *)(p + 1024);
                 return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             };
-            i32x8 x[TM];
+            i32x8 x[TM], next = operand(wt);
 #pragma unroll
             for (int j = 0; j < TM; ++j) x[j] = operand(xt + j * kTileBytes);
 #pragma unroll
             for (int i = 0; i < TN; ++i) {
-                const i32x8 w = operand(wt + i * kTileBytes);
+                const i32x8 w = next;
+                if (i + 1 < TN) next = operand(wt + (i + 1) * kTileBytes);
 #pragma unroll
                 for (int j = 0; j < TM; ++j) add(i, j, mfma_block(w, x[j]));
             }
