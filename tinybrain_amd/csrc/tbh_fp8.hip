@@ -284,10 +284,10 @@ constexpr uint32_t kPast = 0x7FFFFFF0u;   // past every buffer: reads as zeros
 // half as fast, with x widened by the pass that quantized it (WIDE) and the weight here.
 // Two steps of 128 inputs in LDS: a step's one barrier says that its tiles have landed and
 // that every wave is done with the step before, whose place the loads issued then take.
-// 4096 rows by 4096 x 11008: 193 us of this kernel (1.9 PFLOP/s; loads alone 115, products
-// alone 170), fp32 results 384 us with the quantizing.  Bound by the step: of its some 4500
-// cycles the matrix instructions are busy for 40 % (2050), LDS reads take 1536, loads 2800,
-// and a barrier joins them; 160 KiB of LDS hold no third step.  (Two halves of a block's
+// 4096 rows by 4096 x 11008: 191 us of this kernel (1.9 PFLOP/s; loads alone 115, products
+// alone 170), fp32 results 371 us with the quantizing.  Bound by the step: of its some 4300
+// cycles the matrix instructions are busy for 2050 (42 % of all), LDS reads take 1536, loads
+// 2800, and a barrier joins them; 160 KiB of LDS hold no third step.  (Two halves of a block's
 // waves, one at LDS while the other multiplies: 210 us; cache lines touched two to four
 // steps ahead: 233.  Matrix instructions alone, out of registers and with these fp32 sums, run
 // such data at 3.0 PFLOP/s, where power brings the clock down to 1.6 GHz.)
