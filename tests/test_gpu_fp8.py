@@ -62,7 +62,10 @@ def _check(y, x, w, dtype):
 
 SHAPES = [(1, 1, 1), (1, 128, 16), (1, 2048, 512), (2, 130, 17), (5, 127, 129), (15, 1000, 300), (16, 256, 128),
           (17, 384, 200), (31, 640, 48), (32, 129, 257), (33, 1000, 300), (48, 128, 128), (64, 129, 128),
-          (100, 2048, 130), (129, 520, 1000), (300, 5632, 256), (700, 256, 520)]
+          (100, 2048, 130), (129, 520, 1000), (300, 5632, 256), (700, 256, 520),
+          # outputs past one, and past two, blocks a CU, in each count of rows
+          (1, 300, 4500), (3, 1300, 8200), (16, 260, 9000), (20, 300, 4500), (32, 140, 9000), (60, 300, 9000),
+          (60, 140, 21000), (90, 140, 20000), (330, 400, 2048), (330, 140, 5000)]
 
 
 @pytest.mark.parametrize("xt,yt", [("float32", "float32"), ("bfloat16", "bfloat16"), ("float32", "bfloat16"),

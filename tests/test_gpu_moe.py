@@ -75,7 +75,7 @@ def _rows(torch, seed, tokens, hidden, dtype):
     (1, 1, 1, 1, 1, True), (1, 4, 2, 256, 128, True), (1, 8, 8, 130, 72, False), (2, 7, 3, 100, 260, True),
     (5, 60, 4, 384, 17, False), (13, 64, 6, 256, 200, False), (16, 3, 2, 129, 128, True), (17, 2, 1, 640, 384, True),
     (33, 2, 2, 128, 130, True), (50, 16, 4, 200, 100, False), (64, 8, 8, 130, 260, True), (65, 5, 2, 128, 128, False),
-    (130, 9, 3, 64, 300, True), (6, 512, 32, 64, 40, True), (64, 100, 32, 48, 40, False), (3, 5, 5, 1000, 1400, True),
+    (130, 9, 3, 64, 300, True), (6, 512, 32, 64, 40, True), (66, 512, 30, 40, 24, True), (64, 100, 32, 48, 40, False), (3, 5, 5, 1000, 1400, True),
 ])
 def test_layer(torch, backend, dtype, tokens, experts, top_k, hidden, inner, normalize):
     model = Model(backend, tokens * 31 + experts, experts, hidden, inner)
