@@ -354,9 +354,11 @@ class HIPBackend:
         memory freed on torch's current stream may still be used by work that
         is queued there.  Once freed it is kept until what the current stream
         then has queued is done, as the caller may read it there."""
+        if stream is None:
+            return make(*args, **kw)
         import torch
 
-        if stream is None or stream.cuda_stream == torch._C._cuda_getCurrentRawStream(self.device):
+        if stream.cuda_stream == torch._C._cuda_getCurrentRawStream(self.device):
             return make(*args, **kw)
         with torch.cuda.stream(stream):
             t = make(*args, **kw)
@@ -617,8 +619,6 @@ class HIPBackend:
         """tbh_fp8_matmul_device: y = x . W with x [M, K] (float32 or bfloat16;
         rows may be strided) quantized to e4m3 per row and 128 inputs; y [M, N]
         of `dtype` (x's unless given) or like out."""
-        import torch
-
         rows, k = self._row_shape(x)
         if k != weight.K:
             raise PreconditionFailure("Dimensions must match")
@@ -630,10 +630,13 @@ class HIPBackend:
             raise PreconditionFailure("fp8: out must be [M, N] of the type asked for")
         xt, yt = self._paged_type(x), self._paged_type(out)
         room, size = None, 0
-        if rows > 16 and torch.cuda.is_current_stream_capturing():
-            need = ctypes.c_int64()
-            _check(self._lib.tbh_fp8_matmul_workspace(weight.handle, rows, ctypes.byref(need)))
-            room, size = self._room(stream, x, need.value)
+        if rows > 16:
+            import torch
+
+            if torch.cuda.is_current_stream_capturing():
+                need = ctypes.c_int64()
+                _check(self._lib.tbh_fp8_matmul_workspace(weight.handle, rows, ctypes.byref(need)))
+                room, size = self._room(stream, x, need.value)
         _check(self._lib.tbh_fp8_matmul_device(
             weight.handle, x.data_ptr(), xt, rows, k, x.stride(0), out.data_ptr(), yt, out.stride(0),
             None if room is None else room.data_ptr(), size, self._raw_stream(stream)))
@@ -800,23 +803,19 @@ class HIPBackend:
             for a in (*keys[1:], *values[1:]):
                 if a.shape != shape or a.dtype != dtype or not a.is_contiguous() or a.get_device() != device:
                     raise PreconditionFailure("reorder: every layer's arrays must be alike")
-        self._ints(torch.int32, blockTable, contextLens, parents)
+        self._ints(torch.int32, blockTable, contextLens, parents, *(t for t in (sharedLens, reordered, tableOut) if t is not None))
         b = contextLens.numel()
         if beams <= 0 or b % beams:
             raise PreconditionFailure("reorder: requests must be a multiple of beams")
         if blockTable.dim() != 2 or blockTable.shape[0] != b or parents.numel() != b:
             raise PreconditionFailure("reorder: parents and block table must have one row per request")
         for t in (sharedLens, reordered):
-            if t is not None:
-                self._ints(torch.int32, t)
-                if t.numel() != b // beams:
-                    raise PreconditionFailure("reorder: sharedLens and reordered must have one entry per group")
+            if t is not None and t.numel() != b // beams:
+                raise PreconditionFailure("reorder: sharedLens and reordered must have one entry per group")
         if tableOut is None:
             tableOut = self._made(stream, torch.empty_like, blockTable)
-        else:
-            self._ints(torch.int32, tableOut)
-            if tableOut.shape != blockTable.shape:
-                raise PreconditionFailure("reorder: tableOut must be like the block table")
+        elif tableOut.shape != blockTable.shape:
+            raise PreconditionFailure("reorder: tableOut must be like the block table")
         try:
             layout = self._layout.pack(n, bs, nkv, hd, ct, b, blockTable.shape[1])
         except struct.error:
