@@ -283,11 +283,12 @@ constexpr uint32_t kPast = 0x7FFFFFF0u;   // past every buffer: reads as zeros
 // A result of bf16 comes from the FP8 instruction; one of fp32 from the bf16 one,
 // half as fast, with x widened by the pass that quantized it (WIDE) and the weight here.
 // Two steps of 128 inputs in LDS: a step's one barrier says that its tiles have landed and
-// that every wave is done with the step before, whose place the loads issued then take.
-// 4096 rows by 4096 x 11008: 191 us of this kernel (1.9 PFLOP/s; loads alone 115, products
-// alone 170), fp32 results 371 us with the quantizing.  Bound by the step: of its some 4300
-// cycles the matrix instructions are busy for 2050 (42 % of all), LDS reads take 1536, loads
-// 2800, and a barrier joins them; 160 KiB of LDS hold no third step.  (Two halves of a block's
+// that every wave is done with the step before, whose place the loads issued then take, a few
+// behind each row of products (all at the step's start: 196 us and 364 of the 190 and 345 below).
+// 4096 rows by 4096 x 11008: 180 us of this kernel (2.05 PFLOP/s; loads alone 115, products
+// alone 170), fp32 results 345 us with the quantizing.  Bound by the step: of its some 4100
+// cycles the matrix instructions are busy for 2050, LDS reads take 1536, loads 2800, and a
+// barrier joins them; 160 KiB of LDS hold no third step.  (Two halves of a block's
 // waves, one at LDS while the other multiplies: 210 us; cache lines touched two to four
 // steps ahead: 233.  Matrix instructions alone, out of registers and with these fp32 sums, run
 // such data at 3.0 PFLOP/s, where power brings the clock down to 1.6 GHz.)
@@ -320,12 +321,12 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tiles(TilesArgs a) {
     const int64_t mp = a.row_tiles * 16, sm0 = m0 * 16 + wm * TM * 16;
     const dma::i32x4 sr = dma::make_rsrc(a.xs, (int)((int64_t)a.kb * mp * 4));
     const uint32_t lds0 = dma::lds_addr(sm);
-    // (The step past the last is the last again: every step issues, and waits for, as many.)
-    auto issue = [&](int step, int buf) {
+    // Loads i0 .. i1 - 1 of a wave for a step.  (The step past the last is the last again.)
+    auto issue = [&](int step, int buf, int i0, int i1) {
         const uint32_t lds = lds0 + buf * kStage;
         const uint32_t b = (uint32_t)__builtin_amdgcn_readfirstlane(min(step, a.kb - 1));
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
+        for (int i = i0; i < i1; ++i) {
             const int j = i * W + wave;      // 1 KiB of a tile
             const bool of_w = j < 2 * NT;
             const int t = of_w ? j >> 1 : (j - 2 * NT) / XL, part = of_w ? j & 1 : (j - 2 * NT) % XL;
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tiles(TilesArgs a) {
                        b * (8 * (of_w ? kTileBytes : XB)));
         }
         // the scales of the block's rows
-        if (wave == 0)
+        if (i0 == 0 && wave == 0)
             dma::dma16(__builtin_amdgcn_readfirstlane(lds + kScales), sr,
                        lane < MT * 4 && m0 * 16 + lane * 4 < mp ? (uint32_t)(m0 * 64 + lane * 16) : kPast, b * (uint32_t)(mp * 4));
     };
@@ -345,12 +346,11 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tiles(TilesArgs a) {
         for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     // (a wave's outputs lie in one block of 128)
     const auto *sw = (const __attribute__((address_space(4))) float *)(a.w.scales + min((n0 + wn * TN) / 8, (int64_t)a.w_tiles / 8 - 1) * a.kb);
-    issue(0, 0);
+    issue(0, 0, 0, LOADS);
     for (int b = 0; b < a.kb; ++b) {
         const int buf = b & 1;
         const float s = sw[b];
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        issue(b + 1, buf ^ 1);
         const char *st = sm + buf * kStage;
         const char *wt = st + wn * TN * kTileBytes + lane * 16, *xt = st + NT * kTileBytes + wm * TM * XB + lane * 16;
         float f[TM];
@@ -369,6 +369,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tiles(TilesArgs a) {
 #pragma unroll
             for (int i = 0; i < TN; ++i) {
                 bf16x8 w[2][2];
+                issue(b + 1, buf ^ 1, i * LOADS / TN, (i + 1) * LOADS / TN);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) widen(*(const i32x4 *)(wt + i * kTileBytes + h * 1024), w[h]);
 #pragma unroll
@@ -390,6 +391,7 @@ __global__ __launch_bounds__(64 * WN * WM) void fp8_tiles(TilesArgs a) {
 #pragma unroll
             for (int i = 0; i < TN; ++i) {
                 const i32x8 w = next;
+                issue(b + 1, buf ^ 1, i * LOADS / TN, (i + 1) * LOADS / TN);
                 if (i + 1 < TN) next = operand(wt + (i + 1) * kTileBytes);
 #pragma unroll
                 for (int j = 0; j < TM; ++j) add(i, j, mfma_block(w, x[j]));
