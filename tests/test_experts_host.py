@@ -202,7 +202,7 @@ def _reorder(layout=None, **kw):
 @pytest.mark.parametrize("change", [
     dict(dev=None), dict(beams=0), dict(beams=3), dict(beams=65), dict(parents=None), dict(ctx=None), dict(table=None),
     dict(out=None), dict(layers=-1), dict(k=None), dict(v=None), dict(k=[None]), dict(v=[None]), dict(k=[PTR + 8]),
-    dict(v=[PTR + 4]),
+    dict(v=[PTR + 4]), dict(out=PTR + 60), dict(out=PTR - 60),
 ])
 def test_reorder_refuses(change):
     assert _reorder(**change) == _abi.E_INVALID
@@ -250,15 +250,17 @@ def test_calls_refuse_arguments(stand_in):  # noqa: F811
 I, U = _abi.E_INVALID, _abi.E_UNSUPPORTED
 for kw in (dict(m=-1), dict(xt=2), dict(yt=-1), dict(k=299), dict(x=None), dict(y=None), dict(xs=299), dict(ys=199),
            dict(ws=P + 8, size=1 << 30), dict(ws=P, size=10, m=40), dict(ws=P, size=-1, m=40), dict(x=P + 2), dict(y=P + 1),
-           dict(xt=1, x=P + 1)):
+           dict(xt=1, x=P + 1), dict(y=P), dict(y=P + 2396), dict(y=P - 1596), dict(xs=500, y=P)):
     assert fp8(**{"m": 2, **kw}) == I, kw
     assert "tbh_fp8_matmul" in _abi.last_error()
 assert fp8(0, x=None) == 0 and fp8(1, xs=0, ys=0) == 0
+assert fp8(2, y=P + 2400) == 0 and fp8(2, y=P - 1600) == 0 and fp8(2, xs=500, y=P + 1200, ys=500) == 0
 for kw in (dict(t=-1), dict(xt=2), dict(k=0), dict(k=7), dict(x=None), dict(y=None), dict(xs=39), dict(ys=39),
-           dict(ws=P + 8, size=1 << 30), dict(ws=P, size=10), dict(x=P + 2), dict(e=P + 2), dict(p=P + 1)):
+           dict(ws=P + 8, size=1 << 30), dict(ws=P, size=10), dict(x=P + 2), dict(e=P + 2), dict(p=P + 1),
+           dict(y=P), dict(y=P + 316), dict(y=P - 316)):
     assert moe(**{"t": 2, **kw}) == I, kw
     assert "tbh_moe" in _abi.last_error()
-assert moe(0, x=None) == 0
+assert moe(0, x=None) == 0 and moe(2, y=P + 320) == 0 and moe(2, xs=80, ys=80, y=P + 160) == 0
 n = ctypes.c_int64()
 assert L.tbh_moe_workspace(layer.handle, 0, 5, 2, None) == I and L.tbh_fp8_matmul_workspace(w.handle, 5, None) == I
 assert L.tbh_moe_workspace(layer.handle, 0, 5, 9, ctypes.byref(n)) == I

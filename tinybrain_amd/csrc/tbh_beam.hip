@@ -791,6 +791,9 @@ tbh_status tbh_paged_reorder_device(tbh_device *dev, const tbh_paged_layout *lay
     if (layout->max_requests == 0) return TBH_OK;
     if (!parents || !context_lens) return bad("NULL parents or context_lens");
     if (layout->max_blocks > 0 && (!block_table || !table_out)) return bad("NULL block_table");
+    const uintptr_t t0 = (uintptr_t)block_table, t1 = (uintptr_t)table_out;
+    if (t0 != t1 && (t0 < t1 ? t1 - t0 : t0 - t1) < (size_t)layout->max_requests * layout->max_blocks * 4)
+        return bad("table_out overlaps block_table");
     if ((st = use_device(dev->ordinal)) != TBH_OK) return st;
     const hipStream_t s = (hipStream_t)stream;
     ReorderArgs a{};

@@ -603,11 +603,11 @@ tbh_status tbh_fp8_matmul_device(const tbh_fp8_weight *w, const void *x, int32_t
     if (K != w->K) return bad("Dimensions must match");
     if (M == 0) return TBH_OK;
     if (!x || !y) return bad("NULL x or y");
-    if (x == y) return bad("y overlaps x");
     if (M > 1 && (x_stride < K || y_stride < w->N)) return bad("a stride is shorter than its row");
     if (workspace && ((uintptr_t)workspace & 255)) return bad("the workspace must be 256-byte aligned");
     if (workspace_bytes < 0) return bad("negative workspace_bytes");
     const size_t xs = type_size(x_type), ys = type_size(y_type);
+    if (rows_overlap(x, x_stride, K, xs, y, y_stride, w->N, ys, M)) return bad("y overlaps x");
     if ((uintptr_t)x % xs || (uintptr_t)y % ys) return bad("x or y is not aligned to its type");
     tbh_status st = use_device(w->dev->ordinal);
     if (st != TBH_OK) return st;
