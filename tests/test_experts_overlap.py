@@ -1,0 +1,42 @@
+"""Outputs that share memory with inputs are refused by the FP8 product and the
+mixture-of-experts layer, also where rows are strided; rows side by side in one wider
+matrix are not.  Over the stand-in for the HIP runtime."""
+from test_experts_host import MAKE
+from test_host_launches import stand_in  # noqa: F401
+
+ROWS = """
+def shared(x0, sx, nx, y0, sy, ny, rows):      # byte by byte
+    bytes_of = lambda at, stride, width: {at + r * stride + i for r in range(rows) for i in range(width)}
+    return bool(bytes_of(x0, sx, nx) & bytes_of(y0, sy, ny))
+"""
+
+
+def test_strided_rows(stand_in):  # noqa: F811
+    # 300 inputs, 200 outputs of the FP8 product; 40 of the layer
+    stand_in(MAKE + ROWS + """
+I = _abi.E_INVALID
+some = [0, 0]
+for rows in (1, 2, 3, 5):
+    for xs, ys in ((300, 200), (300, 500), (500, 200), (500, 500), (700, 500), (500, 703), (300, 201), (1000, 1000)):
+        for off in (4, 296, 299, 300, 301, 495, 500, 504, 700, 800, 1199, 1200, 1500, 1999, 2000, 3000, 5000,
+                    -4, -199, -200, -201, -300, -496, -500, -700, -1000, -1200, -2000, -5000):
+            want = shared(0, 4 * xs, 1200, 4 * off, 4 * ys, 800, rows)
+            got = fp8(rows, xs=xs, ys=ys, y=P + 4 * off)
+            assert got == (I if want else 0), (rows, xs, ys, off, got)
+            some[want] += 1
+assert min(some) > 50
+for rows in (1, 2, 4):
+    for xs, ys in ((40, 40), (40, 80), (80, 40), (80, 80), (100, 80)):
+        for off in (4, 36, 39, 40, 41, 60, 80, 120, 160, 400, -4, -39, -40, -41, -80, -120, -400):
+            want = shared(0, 4 * xs, 160, 4 * off, 4 * ys, 160, rows)
+            got = moe(rows, xs=xs, ys=ys, y=P + 4 * off)
+            assert got == (I if want else 0), (rows, xs, ys, off, got)
+# x of bf16 within rows of fp32 and beside them
+assert fp8(9, xt=1, xs=1400, y=P + 600, ys=700) == 0 and fp8(9, xt=1, xs=1400, y=P + 596, ys=700) == I
+assert fp8(9, xt=1, xs=1400, y=P + 2000, ys=700) == 0 and fp8(9, xt=1, xs=1400, y=P + 2004, ys=700) == I
+# the last of very many rows
+n = 1 << 22
+assert fp8(n, xs=300, y=P + 1200 * n - 4, ys=999) == I and fp8(n, xs=300, y=P + 1200 * n, ys=999) == 0
+assert fp8(n, xs=500, y=P + 2000 * n, ys=200) == 0 and fp8(n, xs=500, y=P + 2000 * n - 804, ys=200) == I
+""")
+

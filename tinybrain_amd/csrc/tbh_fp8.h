@@ -53,16 +53,6 @@ hipError_t copy_in(void **out, const void *from, size_t bytes, hipStream_t s);
 
 inline size_t type_size(int32_t t) { return t == TBH_BF16 ? 2 : 4; }
 
-// Whether rows x and y share memory, as far as addresses tell: rows side by side in one wider
-// matrix may lie between each other without.
-inline bool rows_overlap(const void *x, int64_t ldx, int64_t nx, size_t sx, const void *y, int64_t ldy, int64_t ny, size_t sy,
-                         int64_t rows) {
-    const uintptr_t x0 = (uintptr_t)x, y0 = (uintptr_t)y;
-    if (x0 == y0) return true;
-    if (rows > 1 && (ldx != nx || ldy != ny)) return false;
-    return x0 < y0 + (size_t)(rows * ny) * sy && y0 < x0 + (size_t)(rows * nx) * sx;
-}
-
 // a . b of a whole 128-deep block on the FP8 instruction: A's row r16 and B's
 // column r16 per lane; the result's lane holds rows 4 (lane / 16) + 0 .. 3 of
 // column r16.  The instruction cuts its sums: 1.4e-5 .. 5e-5 of the result's

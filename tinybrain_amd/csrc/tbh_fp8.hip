@@ -607,7 +607,7 @@ tbh_status tbh_fp8_matmul_device(const tbh_fp8_weight *w, const void *x, int32_t
     if (workspace && ((uintptr_t)workspace & 255)) return bad("the workspace must be 256-byte aligned");
     if (workspace_bytes < 0) return bad("negative workspace_bytes");
     const size_t xs = type_size(x_type), ys = type_size(y_type);
-    if (rows_overlap(x, x_stride, K, xs, y, y_stride, w->N, ys, M)) return bad("y overlaps x");
+    if (overlap(Span(x, K, x_stride, xs, M), Span(y, w->N, y_stride, ys, M))) return bad("y overlaps x");
     if ((uintptr_t)x % xs || (uintptr_t)y % ys) return bad("x or y is not aligned to its type");
     tbh_status st = use_device(w->dev->ordinal);
     if (st != TBH_OK) return st;

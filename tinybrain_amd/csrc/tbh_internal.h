@@ -271,6 +271,38 @@ inline Room room_of(tbh_device *dev, hipStream_t s, void *workspace, size_t byte
     return {p ? stream_counters(dev, s) : nullptr, (char *)p};
 }
 
+// Rows in memory: `rows` of `width` bytes, `step` bytes apart (step >= width).
+struct Span {
+    uintptr_t at;
+    size_t width;
+    int64_t rows;
+    size_t step;
+    Span(const void *p, size_t bytes) : at((uintptr_t)p), width(bytes), rows(1), step(bytes) {}
+    Span(const void *p, int64_t n, int64_t stride, size_t size, int64_t count)
+        : at((uintptr_t)p), width((size_t)n * size), rows(count), step((size_t)stride * size) {
+        if (rows > 1 && step == width) width *= (size_t)rows, rows = 1;      // no gaps
+        if (rows == 1) step = width;
+    }
+};
+
+// Whether two of them share a byte.  (Rows side by side in one wider matrix lie between
+// each other without.)
+inline bool overlap(const Span &x, const Span &y) {
+    const auto at = [](const Span &s, int64_t i) { return s.at + (size_t)i * s.step; };
+    if (at(x, x.rows - 1) + x.width <= y.at || at(y, y.rows - 1) + y.width <= x.at) return false;
+    // Rows in their order: of two that share nothing the lower gives way to the first of its span that
+    // ends behind the other's start.  With equal steps the third pair lies as the second or the first.
+    int64_t i = 0, j = 0;
+    for (int trip = 0; i < x.rows && j < y.rows; ++trip) {
+        const uintptr_t a = at(x, i), b = at(y, j);
+        if (a + x.width <= b) i += (int64_t)((b - a - x.width) / x.step) + 1;
+        else if (b + y.width <= a) j += (int64_t)((a - b - y.width) / y.step) + 1;
+        else return true;
+        if (trip >= 2 && x.step == y.step) return false;
+    }
+    return false;
+}
+
 // Keeps a call's launches together on their stream: held by a call that passes
 // results from one launch to the next (in the stream's workspace, or a plan's
 // outputs) until its last is enqueued, so that another host thread's call on the

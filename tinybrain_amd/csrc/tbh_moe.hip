@@ -750,7 +750,8 @@ tbh_status tbh_moe_device(const tbh_moe *m, const void *x, int32_t x_type, int64
     if (!x || !y) return bad("NULL x or y");
     if (tokens > 1 && (x_stride < m->H || y_stride < m->H)) return bad("a stride is shorter than its row");
     const size_t size = fp8::type_size(x_type);
-    if (fp8::rows_overlap(x, x_stride, m->H, size, y, y_stride, m->H, size, tokens)) return bad("y overlaps x");
+    const Span of_x(x, m->H, x_stride, size, tokens), of_y(y, m->H, y_stride, size, tokens);
+    if (overlap(of_x, of_y)) return bad("y overlaps x");
     if ((uintptr_t)x % size || (uintptr_t)y % size || (uintptr_t)experts % 4 || (uintptr_t)weights % 4)
         return bad("a pointer is not aligned to its type");
     if (workspace && ((uintptr_t)workspace & 255)) return bad("the workspace must be 256-byte aligned");
