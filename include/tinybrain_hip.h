@@ -635,7 +635,8 @@ tbh_status tbh_fp8_matmul_device(const tbh_fp8_weight *w, const void *x, int32_t
  * Made for few tokens, where reading the chosen experts is what takes time: an
  * expert's weights are read once for up to 64 tokens, more run 64 at a time.
  * A row that holds an infinity or NaN gets NaN; which experts it is given then
- * means nothing.  Other rows are not touched by it. */
+ * means nothing.  Other rows are not touched by it.  An h past the largest fp32
+ * number is an infinity and weighs like one. */
 typedef struct tbh_moe_desc {
     int32_t hidden;             /* H, up to 2^17 */
     int32_t intermediate;       /* I, up to 2^17 */

@@ -72,7 +72,8 @@ struct Args {
     bool normalize, vec;     // vec: rows of x can be read four elements at a time
 };
 
-// v as P pieces that sum to it: bf16 as it is, fp32 cut after 8 bits, twice.
+// v as P pieces that sum to it: bf16 as it is, fp32 cut after 8 bits, twice.  (An infinity
+// is its first piece and zeros, not infinity less infinity.)
 template <int P>
 __device__ __forceinline__ void pieces_of(float v, __bf16 (&p)[P]) {
     if constexpr (P == 1) {
@@ -82,7 +83,8 @@ __device__ __forceinline__ void pieces_of(float v, __bf16 (&p)[P]) {
         for (int i = 0; i < P; ++i) {
             const uint32_t u = __builtin_bit_cast(uint32_t, v) & 0xFFFF0000u;
             p[i] = __builtin_bit_cast(__bf16, (uint16_t)(u >> 16));
-            v -= __builtin_bit_cast(float, u);
+            const float cut = __builtin_bit_cast(float, u);
+            v = v == cut ? 0.0f : v - cut;
         }
     }
 }
