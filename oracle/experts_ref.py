@@ -111,7 +111,7 @@ def beam_select(logits, scores, beams, k, done=None, eos=-1):
             if not math.isfinite(score):
                 continue
             if done is not None and done[b]:
-                found.append((-score, b, 0.0, eos))
+                found.append((-score, b, eos))
                 continue
             v = np.where(np.isnan(x[b]), -np.inf, x[b])
             top = v.max()
@@ -122,14 +122,15 @@ def beam_select(logits, scores, beams, k, done=None, eos=-1):
                 total = math.log(np.count_nonzero(v == 0.0))
             else:
                 total = top + math.log(np.exp(v - top).sum())
-            best = np.lexsort((np.arange(vocab), -v))[:k]
-            found += [(-(score + (v[j] - total)), b, -v[j], int(j)) for j in best if v[j] > -np.inf]
+            key = score + (v - total)
+            best = np.lexsort((np.arange(vocab), -key))[:k]
+            found += [(-key[j], b, int(j)) for j in best if v[j] > -np.inf]
         found = sorted(found)[:k]
-        ended = [j == eos or bool(done is not None and done[b]) for _, b, _, j in found]
+        ended = [j == eos or bool(done is not None and done[b]) for _, b, j in found]
         rest = k - len(found)
-        out[0].append([j for _, _, _, j in found] + [-1] * rest)
-        out[1].append([b for _, b, _, _ in found] + [-1] * rest)
-        out[2].append([-f for f, _, _, _ in found] + [-math.inf] * rest)
+        out[0].append([j for _, _, j in found] + [-1] * rest)
+        out[1].append([b for _, b, _ in found] + [-1] * rest)
+        out[2].append([-f for f, _, _ in found] + [-math.inf] * rest)
         out[3].append([int(e) for e in ended] + [0] * rest)
     return tuple(np.array(o).reshape(-1, k) for o in out)
 

@@ -185,12 +185,12 @@ __device__ __forceinline__ uint32_t kth_value(uint32_t value, int k) {
 template <int N>
 struct Candidates {
     double key[N];          // score + log probability
-    uint64_t element[N];    // (logit, token) within the row
+    uint64_t element[N];    // (logit, token) within the row; of equal keys the token counts
     int32_t row[N];
 };
 
 // Keeps the k first of n candidates, in order: the larger key, then the lower row, then the
-// larger element.
+// lower token.
 template <int W, int N>
 __device__ __forceinline__ int prune(Candidates<N> &c, Candidates<kMaxPick> &tmp, int n, int k) {
     const int part = threadIdx.x & 7;
@@ -202,7 +202,8 @@ __device__ __forceinline__ int prune(Candidates<N> &c, Candidates<kMaxPick> &tmp
         for (int o = part; o < n; o += 8) rank += c.key[o] > mine, equal += c.key[o] == mine;
         if (sum_of_8(equal) > 1)
             for (int o = part; o < n; o += 8)
-                rank += c.key[o] == mine && (c.row[o] < c.row[i] || (c.row[o] == c.row[i] && c.element[o] > c.element[i]));
+                rank += c.key[o] == mine &&
+                        (c.row[o] < c.row[i] || (c.row[o] == c.row[i] && (uint32_t)c.element[o] > (uint32_t)c.element[i]));
         rank = sum_of_8(rank);
         if (rank < k && part == 0) tmp.key[rank] = mine, tmp.element[rank] = c.element[i], tmp.row[rank] = c.row[i];
     }
@@ -234,6 +235,63 @@ struct Shared {
     int count;
     uint32_t seen;
 };
+
+// A candidate's score, from its row's and the logarithm of its row's sum.
+__device__ __forceinline__ double score_of(float score, float logit, double total) {
+    return (double)score + ((double)logit - total);
+}
+
+// The n candidates of a request with the tokens that they should have.  A row's list holds its
+// largest logits, but where a score absorbs the difference of logits (they are tiny, or the
+// score is huge) lower ones may be equal, at lower tokens.  Then the row is searched for its
+// first ones of that score; how many of them there are is right as it is, since all that is
+// above them is in the list.  No candidate of ordinary logits comes here.
+template <int W>
+__device__ __forceinline__ void take_lowest(const SelectArgs &a, int row0, int n, Shared<W> &sh) {
+    constexpr int NT = 64 * W;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    bool absorbed = false;
+    if (lane < n) {
+        const int b = sh.held.row[lane] - row0;
+        const float v = logit_of(sh.held.element[lane]);
+        if (sh.state[b] == 1) {
+            const float below = v == 0.0f ? -1.4e-45f : logit_of(sh.held.element[lane] - (1ull << 32));
+            absorbed = score_of(sh.score[b], below, sh.total[b]) == sh.held.key[lane];
+        }
+    }
+    const uint64_t some = __ballot(absorbed);      // the same in all waves
+    if (!some) return;
+    int turn = 0;          // of two sets of counts, which no two searches in a row share
+    for (int i = 0; i < n;) {
+        const double key = sh.held.key[i];
+        const int row = sh.held.row[i], b = row - row0;
+        int end = i + 1;
+        while (end < n && sh.held.key[end] == key && sh.held.row[end] == row) ++end;
+        const uint64_t group = (end < 64 ? 1ull << end : 0) - (1ull << i);
+        if (some & group) {
+            const float *x = a.logits + (int64_t)row * a.ld, score = sh.score[b];
+            const double total = sh.total[b];
+            int found = 0;
+            for (int from = 0; from < a.vocab && found < end - i; from += NT, turn ^= 1) {
+                const int j = from + tid;
+                const float v = j < a.vocab ? x[j] : -HUGE_VALF;
+                const bool equal = v > -HUGE_VALF && score_of(score, v, total) == key;
+                const uint64_t lanes = __ballot(equal);
+                if (lane == 0) sh.heads[turn][wave] = __builtin_popcountll(lanes);
+                __syncthreads();
+                int at = found + __builtin_popcountll(lanes & ((1ull << lane) - 1));
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    at += w < wave ? sh.heads[turn][w] : 0;
+                    found += sh.heads[turn][w];
+                }
+                if (equal && i + at < end) sh.held.element[i + at] = key_of(v, (uint32_t)j);
+            }
+        }
+        i = end;
+    }
+    __syncthreads();
+}
 
 // The request's last block: the lists of its rows joined.
 template <int W>
@@ -277,7 +335,7 @@ __device__ __forceinline__ void join_rows(const SelectArgs &a, int request, Shar
             const float score = sh.score[b];
             if (st == 1 || st == 3) {
                 const float v = logit_of(element);
-                key = (double)score + ((st == 3 ? 0.0 : (double)v) - sh.total[b]);
+                key = score_of(score, st == 3 ? 0.0f : v, sh.total[b]);
                 in = element && (st == 1 || v == HUGE_VALF);
             } else if (st == 2 && level == 0) {
                 key = (double)score;
@@ -298,6 +356,7 @@ __device__ __forceinline__ void join_rows(const SelectArgs &a, int request, Shar
         if (tid == 0) sh.count = 0;
         __syncthreads();
     }
+    take_lowest<W>(a, row0, n, sh);
     const int64_t to = (int64_t)request * a.k;
     for (int i = tid; i < a.k; i += NT) {
         const bool some = i < n;
