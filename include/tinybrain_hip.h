@@ -703,9 +703,8 @@ tbh_status tbh_sample_device(tbh_device *dev, const float *logits, int64_t ld, i
  *   done:     the token eos, with scores[b]
  * and the k best of them, best first, are its tokens, parents (rows, as
  * counted over the whole call) and scores_out, [requests][k] each; equal ones:
- * the lowest row, then the lowest token.  Candidates are compared in 64 bits; the
- * sum of exp is good to some 1e-7 (fp32 terms, 64-bit sums), and the same for
- * equal rows.
+ * the lowest row, then the lowest token.  Candidates are computed and compared in
+ * 64 bits (exp to some 1e-12), the same for equal rows.
  * done_out (or NULL) [requests][k]: 1 for the token eos and children of a done
  * row.  NaN and -inf logits are never taken and weigh nothing (+inf ones share
  * all of the weight); a row whose score is not finite has no candidates.  Where

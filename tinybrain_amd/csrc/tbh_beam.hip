@@ -50,22 +50,22 @@ __device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {
            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
 
-// exp(d) for d in -700 .. 0: 2^n times Taylor's series of exp(f ln 2) for the fraction f of
-// d / ln 2, |f| <= 1/2, up to f^8, the rest of which is below 2e-10.  (n from the low bits of
+// exp(d) for d in -700 .. 0: 2^n times 2^f for the fraction f of d / ln 2, |f| <= 1/2, by the
+// polynomial of degree 8 that is 1 at 0 and of the least relative error, 1.1e-12.  (n from the low bits of
 // a sum with 1.5 * 2^52, and into the exponent: conversions and scalings of 64-bit numbers
 // are slower than their sums.)
 constexpr double kLeastExp = -690.0;
 __device__ __forceinline__ double exp_low(double d) {
     constexpr double kLog2E = 1.4426950408889634, kShift = 6755399441055744.0;
     const double u = __builtin_fma(d, kLog2E, kShift), f = __builtin_fma(d, kLog2E, -(u - kShift));
-    double p = 1.3215486790144309e-06;            // ln(2)^8 / 8!
-    p = __builtin_fma(p, f, 1.5252733804059841e-05);
-    p = __builtin_fma(p, f, 1.5403530393381608e-04);
-    p = __builtin_fma(p, f, 1.3333558146428443e-03);
-    p = __builtin_fma(p, f, 9.6181291076284772e-03);
-    p = __builtin_fma(p, f, 5.5504108664821580e-02);
-    p = __builtin_fma(p, f, 2.4022650695910072e-01);
-    p = __builtin_fma(p, f, 6.9314718055994531e-01);
+    double p = 1.33441836556714563e-06;
+    p = __builtin_fma(p, f, 1.53142092288029329e-05);
+    p = __builtin_fma(p, f, 1.54030982856375782e-04);
+    p = __builtin_fma(p, f, 1.33334341575339402e-03);
+    p = __builtin_fma(p, f, 9.61812955884047173e-03);
+    p = __builtin_fma(p, f, 5.55041095922884711e-02);
+    p = __builtin_fma(p, f, 2.40226506947425839e-01);
+    p = __builtin_fma(p, f, 6.93147180541232699e-01);
     p = __builtin_fma(p, f, 1.0);
     u32x2 w = __builtin_bit_cast(u32x2, p);
     w[1] += __builtin_bit_cast(u32x2, u)[0] << 20;
@@ -103,13 +103,6 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
     v = dpp_most<wave::kRowMirror>(v);
     auto row = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
     return max(max(row(0), row(16)), max(row(32), row(48)));
-}
-
-// exp(v - most) in 32 bits, off by at most (2 + |v - most|) 2^-23 of itself: an element's, of
-// which a sum has so many that 64-bit ones, at eight cycles an operation, took half of the
-// call (256 rows of 100000: 44 us, 34 so).  0 for -inf and NaN.
-__device__ __forceinline__ float exp_step(float v, float most) {
-    return __builtin_amdgcn_exp2f(fmaxf(v - most, -1000.0f) * 1.44269504f);
 }
 
 // A running sum of exp(x - most); an infinite most counts the infinite x alone.
@@ -415,15 +408,17 @@ __device__ __forceinline__ void join_parts(const SelectArgs &a, int row, uint64_
 }
 
 // A part of a row, 16 elements a thread at a time: the largest logit, the sum of
-// exp(logit - largest), 64 bits over 32-bit steps, and the k best elements, by a list of those that pass a
+// exp(logit - largest), and the k best elements, by a list of those that pass a
 // key that k elements before them are not below.  The row's last
 // block joins its parts, the request's last its rows (a counter takes some 70 ns an
 // arrival, so that they are counted in two steps; all parts of four rows of 32000 counted
 // and joined at once: 13.1 us against 13.5 in a graph, of 16 requests of them 18.4 against
-// 15.2).  Bound by the latency of one step, its
-// ranking and the two joins for few rows (4 of 32000, k = 4: 10.5 us, of which the loads are
-// 2), by memory and the instructions of a step, some 60 for 16 elements, for many: 256 rows
-// of 100000, k = 16 31 us, 3.3 TB/s; its loads are done after 21.
+// 15.2).  The sum decides which of two rows' candidates is the better, so that its terms have
+// 64 bits, at some 16 64-bit operations each (with terms of 32 bits, off by up to 6e-7, 256 rows of
+// 100000 took 30.5 us; with other orders of the same operations, or fewer of them, no less than so).
+// Bound by the latency of one step, its
+// ranking and the two joins for few rows (4 of 32000, k = 4: 11.7 us, of which the loads are
+// 2), by these operations beside memory for many: 256 rows of 100000, k = 16 38.6 us, 2.65 TB/s.
 template <int W>
 __global__ __launch_bounds__(64 * W) void beam_select(SelectArgs a) {
     constexpr int NT = 64 * W, kChunk = NT * kPer;
@@ -535,10 +530,8 @@ __global__ __launch_bounds__(64 * W) void beam_select(SelectArgs a) {
                 for (int j = 0; j < kPer; ++j) t.sum += v[j] == HUGE_VALF ? 1.0 : 0.0;
             } else {
                 const float most = t.most > -HUGE_VALF ? t.most : 0.0f;
-                float step = 0.0f;
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) step += exp_step(v[j], most);
-                t.sum += (double)step;
+                for (int j = 0; j < kPer; ++j) t.sum += exp_below(v[j], most);
             }
         };
         float v[kPer], next[kPer];
@@ -721,9 +714,10 @@ void launch_copy(const ReorderArgs &a, dim3 grid, hipStream_t s) {
 // How a call's rows are parted.  Blocks of four waves, of 4096 elements at the least, until
 // there are some four a CU; but a block of 16 waves a row, which ranks one list where the parts'
 // lists would be ranked and joined, where each CU has a row and vocab * k is 2^20 or more.  Four
-// waves / 16 in us: 256 rows of 100000, k = 16 43.6 / 36.6, k = 8 37.1 / 35.2, of 150000, k = 8
-// 49.1 / 45.5; 128 rows of 100000, k = 16 30.1 / 31.0; 1024 rows of 16000, k = 8 24.5 / 56.3, of
-// 64000, k = 16 91.4 / 98.5, of 100000, k = 16 150 / 128; 4 rows of 32000, k = 4 13.1 / 17.8.
+// waves / 16 in us: 256 rows of 100000, k = 16 49.1 / 42.1, k = 8 41.9 / 40.0, of 150000, k = 8
+// 52.6 / 50.6, of 66000, k = 16 36.5 / 33.3; 512 of 50000, k = 16 45.1 / 52.6; 128 rows of 100000,
+// k = 16 32.4 / 37.5; 1024 rows of 16000, k = 8 29.6 / 52.6, of 64000, k = 16 101 / 104, of 100000,
+// k = 16 176 / 145; 4 rows of 32000, k = 4 11.7 / 16.7.
 struct Parts {
     int waves, part, splits;
 };
