@@ -656,7 +656,8 @@ tbh_status tbh_moe_create(tbh_device *dev, const tbh_moe_desc *desc, tbh_moe **o
 tbh_status tbh_moe_destroy(tbh_moe *m);
 /* x and y: [tokens][H] of x_type, rows x_stride and y_stride elements apart; y
  * does not overlap x.  experts, weights [tokens][top_k] (each may be NULL):
- * what the router chose, largest first.  top_k up to 32.  workspace:
+ * what the router chose, largest first; they overlap neither x, y nor each
+ * other.  top_k up to 32.  workspace:
  * 256-byte aligned, tbh_moe_workspace bytes, of which the first
  * TBH_WORKSPACE_COUNTERS are zero (calls leave them so), or NULL for the one of
  * (device, stream), with tbh_matmul_device's rule for captured graphs; a capture

@@ -40,3 +40,20 @@ assert fp8(n, xs=300, y=P + 1200 * n - 4, ys=999) == I and fp8(n, xs=300, y=P + 
 assert fp8(n, xs=500, y=P + 2000 * n, ys=200) == 0 and fp8(n, xs=500, y=P + 2000 * n - 804, ys=200) == I
 """)
 
+
+def test_choices_of_the_layer(stand_in):  # noqa: F811
+    # 5 tokens of 40 fp32; two experts a token: 40 bytes each
+    stand_in(MAKE + """
+I, far = _abi.E_INVALID, P + (1 << 37)
+X, Y, n = P, P + (1 << 38), 5 * 160
+for at in (X, Y):
+    for kw in (dict(e=at), dict(p=at), dict(e=at + n - 4), dict(p=at + n - 4), dict(e=at - 36), dict(p=at - 36)):
+        assert moe(5, **kw) == I, kw
+        assert "overlap" in _abi.last_error()
+    for kw in (dict(e=at + n), dict(p=at - 40), dict(e=at + n, p=at - 40)):
+        assert moe(5, **kw) == 0, kw
+assert moe(5, e=far, p=far) == moe(5, e=far, p=far + 36) == moe(5, e=far, p=far - 36) == I
+assert moe(5, e=far, p=far + 40) == moe(5, e=far + 40, p=far) == 0
+# between the rows of a wider matrix
+assert moe(5, xs=80, e=X + 160) == 0 and moe(5, xs=80, e=X + 124) == I and moe(5, ys=80, p=Y + 300) == I
+""")

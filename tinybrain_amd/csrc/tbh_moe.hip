@@ -754,6 +754,10 @@ tbh_status tbh_moe_device(const tbh_moe *m, const void *x, int32_t x_type, int64
     const size_t size = fp8::type_size(x_type);
     const Span of_x(x, m->H, x_stride, size, tokens), of_y(y, m->H, y_stride, size, tokens);
     if (overlap(of_x, of_y)) return bad("y overlaps x");
+    const Span chosen[2] = {Span(experts, (size_t)tokens * top_k * 4), Span(weights, (size_t)tokens * top_k * 4)};
+    for (const Span &c : chosen)
+        if (c.at && (overlap(c, of_x) || overlap(c, of_y))) return bad("experts or weights overlap x or y");
+    if (experts && weights && overlap(chosen[0], chosen[1])) return bad("experts and weights overlap");
     if ((uintptr_t)x % size || (uintptr_t)y % size || (uintptr_t)experts % 4 || (uintptr_t)weights % 4)
         return bad("a pointer is not aligned to its type");
     if (workspace && ((uintptr_t)workspace & 255)) return bad("the workspace must be 256-byte aligned");
