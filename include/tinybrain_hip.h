@@ -711,7 +711,8 @@ tbh_status tbh_sample_device(tbh_device *dev, const float *logits, int64_t ld, i
  * all of the weight); a row whose score is not finite has no candidates.  Where
  * there are fewer than k: token and parent -1, score -inf, not done.
  * With scores, done and parents of one call as the next one's, k = beams.
- * The outputs overlap no input.  beams and k up to 64, vocab and rows up to
+ * The outputs overlap no input and no other output, but for scores_out, which
+ * may be scores where k = beams.  beams and k up to 64, vocab and rows up to
  * 2^20 (TBH_E_UNSUPPORTED).  workspace: as tbh_moe_device's, of
  * tbh_beam_select_workspace bytes. */
 tbh_status tbh_beam_select_workspace(tbh_device *dev, int64_t requests, int32_t beams, int64_t vocab, int32_t k,

@@ -1,6 +1,6 @@
-"""Outputs that share memory with inputs are refused by the FP8 product and the
-mixture-of-experts layer, also where rows are strided; rows side by side in one wider
-matrix are not.  Over the stand-in for the HIP runtime."""
+"""Outputs that share memory with inputs are refused by the FP8 product, the
+mixture-of-experts layer and beam selection, also where rows are strided; rows side by
+side in one wider matrix are not.  Over the stand-in for the HIP runtime."""
 from test_experts_host import MAKE
 from test_host_launches import stand_in  # noqa: F401
 
@@ -56,4 +56,34 @@ assert moe(5, e=far, p=far) == moe(5, e=far, p=far + 36) == moe(5, e=far, p=far 
 assert moe(5, e=far, p=far + 40) == moe(5, e=far + 40, p=far) == 0
 # between the rows of a wider matrix
 assert moe(5, xs=80, e=X + 160) == 0 and moe(5, xs=80, e=X + 124) == I and moe(5, ys=80, p=Y + 300) == I
+""")
+
+
+def test_outputs_of_a_selection(stand_in):  # noqa: F811
+    # 3 requests of 4 rows, k = 4: 48 bytes of everything but the logits, of 12 rows of 900 in 1000
+    stand_in(MAKE + """
+I = _abi.E_INVALID
+NAMES = ("tokens", "parents", "scores_out", "done_out")
+def call(k=4, **kw):
+    a = dict(logits=P, scores=P + (1 << 30), done=P + (2 << 30), tokens=P + (3 << 30), parents=P + (4 << 30),
+             scores_out=P + (5 << 30), done_out=P + (6 << 30))
+    a.update(kw)
+    return L.tbh_beam_select_device(dev, a["logits"], 1000, 3, 4, 900, a["scores"], a["done"], 2, k, *(a[n] for n in NAMES),
+                                    None, 0, STREAM)
+assert call() == 0 and call(done=None) == 0 and call(done_out=None) == 0
+SCORES, DONE = P + (1 << 30), P + (2 << 30)
+for n in NAMES:                                # what all blocks of a row read
+    for off in (0, 44, -44):
+        assert call(**{n: DONE + off}) == I, (n, off)
+        assert "overlap" in _abi.last_error()
+    assert call(**{n: DONE + 48}) == call(**{n: DONE - 48}) == 0
+    assert call(done=None, **{n: DONE}) == 0
+for off in (4, -4, 44, -44):
+    assert call(scores_out=SCORES + off) == I
+for off in (0, 4, -4, 44, -44):
+    assert call(done_out=SCORES + off) == I and call(done_out=P + 40000 + off) == I
+    for n in ("tokens", "parents", "scores_out"):
+        assert call(done_out=P + (7 << 30) + off, **{n: P + (7 << 30)}) == I
+assert call(scores_out=SCORES) == 0            # a request's scores in place
+assert call(k=3, scores_out=SCORES) == call(k=8, scores_out=SCORES) == I
 """)

@@ -101,3 +101,19 @@ def test_a_callers_workspace(torch, requests, vocab):
         tokens, parents, scores, ended = made.unbind(0)
         _check((tokens, parents, scores.view(torch.float32), ended), case, 4)
     backend.close()
+
+
+def test_scores_in_place(torch):
+    """A request's scores written over those it came with, where k = beams."""
+    backend, lib = T.HIPBackend(0), _abi.lib()
+    for requests, vocab in SHAPES:
+        x, s, done = _case(torch, 50, requests, vocab)
+        want = backend.beam_select_device(x, s, BEAMS, done=done, eos=EOS)
+        made = torch.full((3, requests, BEAMS), -9, dtype=torch.int32, device="cuda")
+        at = [made[i].data_ptr() for i in range(3)]
+        assert lib.tbh_beam_select_device(backend._dev, x.data_ptr(), vocab, requests, BEAMS, vocab, s.data_ptr(),
+                                          done.data_ptr(), EOS, BEAMS, at[0], at[1], s.data_ptr(), at[2], None, 0,
+                                          backend._raw_stream(None)) == _abi.OK, _abi.last_error()
+        for a, b in zip(want, (made[0], made[1], s.view(requests, BEAMS), made[2])):
+            assert torch.equal(a, b)
+    backend.close()

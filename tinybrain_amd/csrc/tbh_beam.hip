@@ -779,6 +779,22 @@ tbh_status tbh_beam_select_device(tbh_device *dev, const float *logits, int64_t 
     if (ld < vocab && requests * beams > 1) return bad("ld is shorter than vocab");
     if (done && (eos < 0 || eos >= vocab)) return bad("done rows need an eos within the vocabulary");
     if (workspace && ((uintptr_t)workspace & 255)) return bad("the workspace must be 256-byte aligned");
+    // What blocks read while others write.  (A request's scores are read by its last block alone,
+    // before it writes.)
+    const int64_t all_rows = requests * beams;
+    const size_t in_bytes = (size_t)all_rows * 4, out_bytes = (size_t)(requests * k) * 4;
+    if (done)
+        for (const void *p : {(void *)tokens, (void *)parents, (void *)scores_out, (void *)done_out})
+            if (p && overlap(Span(p, out_bytes), Span(done, in_bytes))) return bad("an output overlaps done");
+    if ((k != beams || scores_out != scores) && overlap(Span(scores_out, out_bytes), Span(scores, in_bytes)))
+        return bad("scores_out overlaps scores, and is not the same with k = beams");
+    if (done_out) {
+        const Span ended(done_out, out_bytes);
+        if (overlap(ended, Span(scores, in_bytes)) || overlap(ended, Span(logits, vocab, ld, 4, all_rows)))
+            return bad("done_out overlaps an input");
+        for (const void *p : {(void *)tokens, (void *)parents, (void *)scores_out})
+            if (overlap(ended, Span(p, out_bytes))) return bad("done_out overlaps another output");
+    }
     const Parts p = parts_of(dev, requests * beams, vocab, k);
     const int64_t part = part_of(requests, beams, p.splits, k);
     const size_t need = (size_t)part * request_bytes(beams, p.splits, k);
