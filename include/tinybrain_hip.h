@@ -630,8 +630,9 @@ tbh_status tbh_fp8_matmul_device(const tbh_fp8_weight *w, const void *x, int32_t
  *   equal ones the lowest), with weights p_e = exp(z_e) / sum of exp(z) over
  *   all experts, or over the chosen ones (normalize)
  *   y = sum over its experts of p_e (silu(x . G_e) * (x . U_e)) . D_e
- * Activations are not quantized: bf16 rows are taken as they are (h is rounded
- * to bf16 once, y once from fp32), fp32 rows keep fp32's precision throughout.
+ * Activations are not quantized: bf16 rows are taken as they are (h is held to
+ * 2^-16 of itself, y is rounded to bf16 once, from fp32), fp32 rows keep fp32's
+ * precision throughout.
  * Made for few tokens, where reading the chosen experts is what takes time: an
  * expert's weights are read once for up to 64 tokens, more run 64 at a time.
  * A row that holds an infinity or NaN gets NaN; which experts it is given then

@@ -4,15 +4,15 @@
 //   weights p = softmax(z) (over all experts, or over the chosen ones)
 //   y = sum over its experts e of p_e (silu(x . G_e) * (x . U_e)) . D_e
 // Few tokens are bound by reading the chosen experts' weights once: rows of x
-// and h stay as exact as they came, as bf16 or as three bf16 pieces of an fp32,
-// and the weights are widened to bf16 (exactly) on their way to the matrix
-// instruction.
+// stay as exact as they came, as bf16 or as three bf16 pieces of an fp32, h is two
+// pieces of 16 bits together (bf16 rows, whose y is rounded to 8) or three, and the
+// weights are widened to bf16 (exactly) on their way to the matrix instruction.
 //   Three launches, as every chosen expert's h has to be whole before D_e, and the
 // choice before either.  Their times in us (route, up, down; floor: the chosen experts'
 // bytes at the 4.8 TB/s of a large copy):
 //   1 token, 2 of 8 experts of 2048 x 5632, fp32 rows      8.4  11.4  10.8   (14.5)
-//   13 tokens, 6 of 64 experts of 2048 x 1000, bf16       11.7  41.2  28.6   (59)
-//   64 tokens, 4 of 32 experts of 4096 x 2048, bf16       13.5  110   67.8   (168)
+//   13 tokens, 6 of 64 experts of 2048 x 1000, bf16       11.6  42.2  29.8   (59)
+//   64 tokens, 4 of 32 experts of 4096 x 2048, bf16       13.6   113  69.9   (168)
 // What is above the floor is the latency of launches and of loads that depend on
 // one another (ids, lists, weights, the join), not the work.
 #include <algorithm>
@@ -65,28 +65,27 @@ struct Args {
     uint32_t *counters;
     double *logits;          // [splits][T][E]
     float *sums;             // [tiles of 32 outputs][parts][T][32]
-    __bf16 *xp;              // [P][T][hb * 128]
-    __bf16 *hp;              // [P][T * top_k][ib * 128]
+    __bf16 *xp;              // [P][T][hb * 128], see pieces_of
+    __bf16 *hp;              // [PH][T * top_k][ib * 128]
     int32_t *lists;          // [used][kListHead + kMaxTokens]: an expert, its tokens' places in ids
     int T, E, H, hb, ib, top_k, used, splits, parts;
+    int tiles;               // of 16 outputs that a wave of moe_down takes
     bool normalize, vec;     // vec: rows of x can be read four elements at a time
 };
 
-// v as P pieces that sum to it: bf16 as it is, fp32 cut after 8 bits, twice.  (An infinity
-// is its first piece and zeros, not infinity less infinity.)
+// v as P pieces that sum to it: a bf16 as it is; of an fp32 what is cut after 8 bits, and the rest
+// in the same way, the last piece rounded.  Three hold all of an fp32, two are off by at most 2^-16
+// of it.  (An infinity is its first piece and zeros, not infinity less infinity.)
 template <int P>
 __device__ __forceinline__ void pieces_of(float v, __bf16 (&p)[P]) {
-    if constexpr (P == 1) {
-        p[0] = (__bf16)v;
-    } else {
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const uint32_t u = __builtin_bit_cast(uint32_t, v) & 0xFFFF0000u;
-            p[i] = __builtin_bit_cast(__bf16, (uint16_t)(u >> 16));
-            const float cut = __builtin_bit_cast(float, u);
-            v = v == cut ? 0.0f : v - cut;
-        }
+    for (int i = 0; i + 1 < P; ++i) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v) & 0xFFFF0000u;
+        const float cut = __builtin_bit_cast(float, u);
+        p[i] = __builtin_bit_cast(__bf16, (uint16_t)(u >> 16));
+        v = v == cut ? 0.0f : v - cut;
     }
+    p[P - 1] = (__bf16)v;
 }
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
@@ -306,40 +305,45 @@ __device__ __forceinline__ int find_expert(const Args &a, int y, uint32_t (&used
 // The rows of a matrix instruction's other operand: P pieces of kTokens<P> tokens side by
 // side, so that an fp32 row costs no more instructions and loads than its pieces fill.
 template <int P>
-constexpr int kTokens = P == 1 ? 16 : 5;
+constexpr int kTokens = 16 / P;
 // Column r16's token among them (P == 3: the last column repeats, and is not used).
 template <int P>
 __device__ __forceinline__ int token_of(int r16) {
-    return P == 1 ? r16 : min(r16 / 3, kTokens<P> - 1);
+    return min(r16 / P, kTokens<P> - 1);
 }
 template <int P>
 __device__ __forceinline__ int piece_of(int r16) {
-    return P == 1 ? 0 : r16 % 3;
+    return r16 % P;
 }
 // A token's sum over its pieces, in the column of its first.
 template <int P>
 __device__ __forceinline__ f32x4 over_pieces(f32x4 v) {
-    if constexpr (P == 3) {
+    // columns + 1, + 2
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += wave::dpp<0x101>(v[i]) + wave::dpp<0x102>(v[i]);   // columns + 1, + 2
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (P == 2) v[i] += wave::dpp<0x101>(v[i]);
+        if constexpr (P == 3) v[i] += wave::dpp<0x101>(v[i]) + wave::dpp<0x102>(v[i]);
     }
     return v;
 }
 template <int P>
 __device__ __forceinline__ bool first_piece(int r16) {
-    return P == 1 || (r16 % 3 == 0 && r16 < 15);
+    return r16 % P == 0 && r16 / P < kTokens<P>;
 }
 
 // acc[t][c] += scale[t] * (tile t . rows c) of one 128-deep block, for RT tiles and CT column
-// tiles; row[c]: the lane's row at input 16 g of the block.
-template <int RT, int CT>
+// tiles of rows that are the sum of PK pieces; row[c]: the lane's row at input 16 g of the block,
+// its pieces `step` elements apart.
+template <int PK, int RT, int CT>
 __device__ __forceinline__ void block_product(const i32x4 (&w)[RT][2], const float (&scale)[RT], const __bf16 *const (&row)[CT],
-                                              f32x4 (&acc)[RT][CT]) {
-    bf16x8 x[CT][4];
+                                              int64_t step, f32x4 (&acc)[RT][CT]) {
+    bf16x8 x[CT][PK][4];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[c][i] = *(const bf16x8 *)(row[c] + 64 * (i >> 1) + 8 * (i & 1));
+        for (int q = 0; q < PK; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[c][q][i] = *(const bf16x8 *)(row[c] + q * step + 64 * (i >> 1) + 8 * (i & 1));
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         f32x4 part[CT];
@@ -352,7 +356,9 @@ __device__ __forceinline__ void block_product(const i32x4 (&w)[RT][2], const flo
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int s = 0; s < 2; ++s) part[c] = fp8::mfma_wide(o[s], x[c][2 * h + s], part[c]);
+                for (int q = 0; q < PK; ++q)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) part[c] = fp8::mfma_wide(o[s], x[c][q][2 * h + s], part[c]);
         }
 #pragma unroll
         for (int c = 0; c < CT; ++c)
@@ -366,7 +372,7 @@ __device__ __forceinline__ void load_tile(i32x4 (&w)[2], const uint8_t *p) {
 }
 
 // h of 16 inner columns for an expert's tokens c0 .. c0 + CT kTokens.
-template <int P, int CT>
+template <int P, int PH, int CT>
 __device__ __forceinline__ void up_tokens(const Args &a, int e, int tile, const int32_t *slots, int c0, int count,
                                           f32x4 (*red)[64]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
@@ -392,7 +398,7 @@ __device__ __forceinline__ void up_tokens(const Args &a, int e, int tile, const 
         const __bf16 *at[CT];
 #pragma unroll
         for (int c = 0; c < CT; ++c) at[c] = row[c] + b * kBlock;
-        block_product(w, s, at, acc);
+        block_product<1>(w, s, at, 0, acc);
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -412,16 +418,16 @@ __device__ __forceinline__ void up_tokens(const Args &a, int e, int tile, const 
         const int at = c0 + c * kTokens<P> + token_of<P>(r16);
         if (at < count && first_piece<P>(r16)) {
             const int ip = a.ib * kBlock;
-            bf16x4 o[P];
+            bf16x4 o[PH];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                __bf16 p[P];
-                pieces_of<P>(gv[i] / (1.0f + expf(-gv[i])) * uv[i], p);
+                __bf16 p[PH];
+                pieces_of<PH>(gv[i] / (1.0f + expf(-gv[i])) * uv[i], p);
 #pragma unroll
-                for (int j = 0; j < P; ++j) o[j][i] = p[j];
+                for (int j = 0; j < PH; ++j) o[j][i] = p[j];
             }
 #pragma unroll
-            for (int j = 0; j < P; ++j)
+            for (int j = 0; j < PH; ++j)
                 *(bf16x4 *)(a.hp + ((int64_t)j * a.T * a.top_k + slots[at]) * ip + tile * 16 + 4 * g) = o[j];
         }
     }
@@ -433,7 +439,7 @@ __device__ __forceinline__ void up_tokens(const Args &a, int e, int tile, const 
 // reads 4 KiB in a row a step.  Bound by memory: 32 experts of 4096 x 2048 (537 MB) in 105 us,
 // 5.1 TB/s, 2 of 2048 x 5632 (46 MB) in 9.6 behind the 1.0 of the search for the expert.  (Two
 // or four steps' loads ahead of the products: no faster, the blocks of a CU hide each other's.)
-template <int P>
+template <int P, int PH>
 __global__ __launch_bounds__(256) void moe_up(Args a) {
     __shared__ uint32_t used[kMaxExperts / 32];
     __shared__ int32_t slots[kMaxTokens];
@@ -449,36 +455,37 @@ __global__ __launch_bounds__(256) void moe_up(Args a) {
     // two column tiles to a load of the weights while there are more than one's tokens (64 tokens, 2
     // of 8 experts of 4096 x 4096: 120 us against 128 one at a time, of fp32 231 and 252)
     int c0 = 0;
-    for (; count - c0 > kTokens<P>; c0 += 2 * kTokens<P>) up_tokens<P, 2>(a, e, blockIdx.x, slots, c0, count, red);
-    if (c0 < count) up_tokens<P, 1>(a, e, blockIdx.x, slots, c0, count, red);
+    for (; count - c0 > kTokens<P>; c0 += 2 * kTokens<P>) up_tokens<P, PH, 2>(a, e, blockIdx.x, slots, c0, count, red);
+    if (c0 < count) up_tokens<P, PH, 1>(a, e, blockIdx.x, slots, c0, count, red);
 }
 
-// 32 outputs of all tokens: the waves of a.parts blocks part the units of kUnit blocks
+// 16 RT outputs of all tokens: the waves of a.parts blocks part the units of kUnit blocks
 // of inputs of the active experts, the next unit's tiles in flight while one is
 // multiplied; each wave adds its share of a token's sum to its own row in LDS, once an
 // expert.  Joined in order, and over the blocks by the one that is last.  (A tile for one
-// token needs twice as many loads of h as of weights, so that a wave takes two tiles a
-// load of h.)  Bound by memory where there are many experts (268 MB in 60 us, 4.5 TB/s), by the
+// token needs twice as many loads of h as of weights, so that a wave takes two or four tiles a
+// load of h, see size_up.)  Bound by memory where there are many experts (268 MB in 70 us, 3.8 TB/s, which
+// with h in one piece of bf16 took 67), by the
 // latency of the join for one token: 4.6 of 10.8 us are products.  (kUnit 1, 2 or 4: a whole call on
-// 1 token 29.1, 28.9, 31.4 us, on 64 177, 169, 169.)
+// 1 token 29.1, 28.9, 31.4 us, on 64, h in one piece, 177, 169, 169.)
 constexpr int kDownWaves = 8, kUnit = 2;
 
-template <class T, int P>
+template <class T, int P, int PK, int RT>
 __global__ __launch_bounds__(64 * kDownWaves) void moe_down(Args a) {
-    extern __shared__ f32x4 sums[];       // [waves][8 quads of outputs][T], then the experts' heads
+    extern __shared__ f32x4 sums[];       // [waves][4 RT quads of outputs][T], then the experts' heads
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r16 = lane & 15, g = lane >> 4, tile = blockIdx.x * 2, w = blockIdx.y * kDownWaves + wave;
-    f32x4 *own = sums + wave * a.T * 8;
-    int2 *heads = (int2 *)(sums + kDownWaves * a.T * 8);      // expert, number of its tokens
+    const int r16 = lane & 15, g = lane >> 4, tile = blockIdx.x * RT, w = blockIdx.y * kDownWaves + wave;
+    f32x4 *own = sums + wave * a.T * (4 * RT);
+    int2 *heads = (int2 *)(sums + kDownWaves * a.T * (4 * RT));      // expert, number of its tokens
     for (int y = tid; y < a.used; y += 64 * kDownWaves) heads[y] = *(const int2 *)(a.lists + y * (kListHead + kMaxTokens));
-    for (int i = lane; i < a.T * 8; i += 64) own[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = lane; i < a.T * (4 * RT); i += 64) own[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     __syncthreads();
     int active = 0;
     for (int y = 0; y < a.used; y += 64) active += __builtin_popcountll(__ballot(y + lane < a.used && heads[y + lane].y > 0));
     const int per = (a.ib + kUnit - 1) / kUnit, total = active * per, ws = a.parts * kDownWaves;
     const int first = (int)((int64_t)total * w / ws), end = (int)((int64_t)total * (w + 1) / ws);
     const int ip = a.ib * kBlock;
-    i32x4 next[kUnit][2][2];
+    i32x4 next[kUnit][RT][2];
     float next_s[kUnit];
     int y = first / per, b0 = (first - y * per) * kUnit;      // of the unit that is loaded next
     auto load = [&]() {
@@ -488,17 +495,17 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down(Args a) {
         for (int u = 0; u < kUnit; ++u) {
             const int b = min(b0 + u, a.ib - 1);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) load_tile(next[u][t], a.down + (row + (int64_t)t * a.ib + b) * kTileBytes + lane * 16);
+            for (int t = 0; t < RT; ++t) load_tile(next[u][t], a.down + (row + (int64_t)t * a.ib + b) * kTileBytes + lane * 16);
             next_s[u] = a.down_scales[((int64_t)e * a.hb + tile / 8) * a.ib + b];
         }
     };
     auto slot_of = [&](int c0, int count) {
         return a.lists[y * (kListHead + kMaxTokens) + kListHead + min(c0 + token_of<P>(r16), count - 1)];
     };
-    auto add = [&](int slot, bool some, f32x4 (&acc)[2][1]) {
+    auto add = [&](int slot, bool some, f32x4 (&acc)[RT][1]) {
         const float p = a.weights[slot];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < RT; ++t) {
             const f32x4 sum = over_pieces<P>(acc[t][0]);
             if (!some || !first_piece<P>(r16)) continue;
             f32x4 *to = own + (4 * t + g) * a.T + slot / a.top_k;
@@ -508,24 +515,29 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down(Args a) {
             *to = v;
         }
     };
-    const __bf16 *hrow = a.hp + (int64_t)piece_of<P>(r16) * a.T * a.top_k * ip + 16 * g;
-    f32x4 acc[2][1];
+    const int64_t step = (int64_t)a.T * a.top_k * ip;         // a piece of all rows
+    const __bf16 *hrow = a.hp + piece_of<P>(r16) * step + 16 * g;
+    f32x4 acc[RT][1];
+    auto clear = [&]() {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[t][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
     int count = 0, slot = 0;
     bool fresh = true;
     if (first < end) load();
     for (int i = first; i < end; ++i) {
-        i32x4 now[kUnit][2][2];
+        i32x4 now[kUnit][RT][2];
         float s[kUnit];
 #pragma unroll
         for (int u = 0; u < kUnit; ++u) {
             s[u] = next_s[u];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) now[u][t][0] = next[u][t][0], now[u][t][1] = next[u][t][1];
+            for (int t = 0; t < RT; ++t) now[u][t][0] = next[u][t][0], now[u][t][1] = next[u][t][1];
         }
         if (fresh) {
             count = __builtin_amdgcn_readfirstlane(heads[y].y);
             slot = slot_of(0, count);
-            acc[0][0] = acc[1][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+            clear();
         }
         const int yi = y, bi = b0;
         b0 += kUnit;
@@ -536,41 +548,44 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down(Args a) {
             int sl = slot;
             if (c0 > 0) {
                 sl = a.lists[yi * (kListHead + kMaxTokens) + kListHead + min(c0 + token_of<P>(r16), count - 1)];
-                acc[0][0] = acc[1][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+                clear();
             }
 #pragma unroll
             for (int u = 0; u < kUnit; ++u) {
                 if (bi + u >= a.ib) break;
                 const __bf16 *const rows[1] = {hrow + (int64_t)sl * ip + (bi + u) * kBlock};
-                const float sc[2] = {s[u], s[u]};
-                block_product(now[u], sc, rows, acc);
+                float sc[RT];
+#pragma unroll
+                for (int t = 0; t < RT; ++t) sc[t] = s[u];
+                block_product<PK>(now[u], sc, rows, step, acc);
             }
             // one column tile: its sums stay in registers until the expert's last unit
             if (count > kTokens<P> || fresh || i + 1 == end) add(sl, c0 + token_of<P>(r16) < count, acc);
         }
-        if (count > kTokens<P>) acc[0][0] = acc[1][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (count > kTokens<P>) clear();
     }
     __syncthreads();
+    constexpr int kWide = 16 * RT;
     auto store = [&](int j, float v) {
-        const int t = j >> 5, n = tile * 16 + (j & 31);
+        const int t = j / kWide, n = tile * 16 + j % kWide;
         if (n < a.H) ((T *)a.y)[(int64_t)t * a.ldy + n] = (T)v;
     };
-    float *part = a.sums + (int64_t)blockIdx.x * a.parts * a.T * 32;
-    for (int j = tid; j < a.T * 32; j += 64 * kDownWaves) {
-        const int at = ((j & 31) / 4 * a.T + (j >> 5)) * 4 + (j & 3);
+    float *part = a.sums + (int64_t)blockIdx.x * a.parts * a.T * kWide;
+    for (int j = tid; j < a.T * kWide; j += 64 * kDownWaves) {
+        const int at = (j % kWide / 4 * a.T + j / kWide) * 4 + (j & 3);
         float v = 0.0f;
-        for (int i = 0; i < kDownWaves; ++i) v += ((const float *)sums)[i * a.T * 32 + at];
+        for (int i = 0; i < kDownWaves; ++i) v += ((const float *)sums)[i * a.T * kWide + at];
         if (a.parts == 1) store(j, v);
-        else hand_over(part + (int64_t)blockIdx.y * a.T * 32 + j, v);
+        else hand_over(part + (int64_t)blockIdx.y * a.T * kWide + j, v);
     }
     if (a.parts == 1 || !last_to_arrive(a.counters + blockIdx.x, a.parts, (uint32_t *)sums)) return;
-    for (int j = tid; j < a.T * 32; j += 64 * kDownWaves) {
+    for (int j = tid; j < a.T * kWide; j += 64 * kDownWaves) {
         float v = 0.0f;
         // (four at a time: a load past the caches takes a third of a microsecond)
         for (int i = 0; i < a.parts; i += 4) {
             float u[4];
 #pragma unroll
-            for (int o = 0; o < 4; ++o) u[o] = i + o < a.parts ? handed_over(part + (int64_t)(i + o) * a.T * 32 + j) : 0.0f;
+            for (int o = 0; o < 4; ++o) u[o] = i + o < a.parts ? handed_over(part + (int64_t)(i + o) * a.T * kWide + j) : 0.0f;
 #pragma unroll
             for (int o = 0; o < 4; ++o) v += u[o];
         }
@@ -578,21 +593,22 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down(Args a) {
     }
 }
 
-template <class T, int P>
+// x in P pieces, h in PC * PK: PC side by side as columns, PK one after the other; RT output tiles a wave.
+template <class T, int P, int PC, int PK, int RT>
 hipError_t launch(const Args &a, hipStream_t s) {
     hipLaunchKernelGGL((moe_route<T, P>), dim3((unsigned)(a.E + 15) / 16, (unsigned)(a.T + 15) / 16, (unsigned)a.splits),
                        dim3(1024), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((moe_up<P>), dim3((unsigned)(a.ib * 8), (unsigned)a.used), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((moe_up<P, PC * PK>), dim3((unsigned)(a.ib * 8), (unsigned)a.used), dim3(256), 0, s, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL((moe_down<T, P>), dim3((unsigned)((a.H + 31) / 32), (unsigned)a.parts), dim3(64 * kDownWaves),
-                       (size_t)a.T * kDownWaves * 128 + (size_t)a.used * 8, s, a);
+    hipLaunchKernelGGL((moe_down<T, PC, PK, RT>), dim3((unsigned)((a.H + 16 * RT - 1) / (16 * RT)), (unsigned)a.parts),
+                       dim3(64 * kDownWaves), (size_t)a.T * kDownWaves * (64 * RT) + (size_t)a.used * 8, s, a);
     return hipGetLastError();
 }
 
 // Sizes of a part of T tokens and the launch shapes that follow from them.
-void size_up(Args &a, const tbh_moe &m, int64_t tokens, int32_t top_k) {
+void size_up(Args &a, const tbh_moe &m, int32_t x_type, int64_t tokens, int32_t top_k) {
     a.T = (int)std::min<int64_t>(kMaxTokens, tokens);
     a.top_k = top_k;
     a.E = m.E;
@@ -605,14 +621,21 @@ void size_up(Args &a, const tbh_moe &m, int64_t tokens, int32_t top_k) {
     a.splits = std::max(1, std::min(kSplits, a.hb * (kBlock / 16) / 32));
     // a block a CU, of waves that have a unit at the least (one part a tile: 13 tokens of width 2048
     // 106 us, 73 so, 64 of 4096 194 and 169)
-    const int tiles = (a.H + 31) / 32, units = a.used * ((a.ib + kUnit - 1) / kUnit);
+    // An h of bf16 rows has two pieces.  Side by side they are free while an expert has few tokens; past
+    // four on the average they would ask for a second column tile, and follow one another in one of 16
+    // tokens, with four output tiles to a load of h.  Side by side / one after the other in us, a whole
+    // call: 13 tokens, 6 of 64 experts of 2048 x 1000 74.4 / 76.8, 5 tokens, 2 of 8 of 4096 x 14336 226 / 230,
+    // 64 tokens, 8 of 128 of 2048 x 768 153 / 153, 4 of 32 of 4096 x 2048 204 / 175, 2 of 8 of 4096 x 4096 136 / 126.
+    a.tiles = x_type == TBH_BF16 && a.T * top_k > 4 * m.E ? 4 : 2;
+    const int tiles = (a.H + 16 * a.tiles - 1) / (16 * a.tiles), units = a.used * ((a.ib + kUnit - 1) / kUnit);
     a.parts = std::max(1, std::min((m.dev->cu_count + tiles - 1) / tiles, units / kDownWaves));
 }
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Workspace of a part of T tokens; sets the pointers when `base` is given.
-size_t carve(Args &a, int P, char *base) {
+size_t carve(Args &a, int32_t x_type, char *base) {
+    const size_t P = x_type == TBH_BF16 ? 1 : 3, PH = x_type == TBH_BF16 ? 2 : 3;
     size_t at = 0;
     auto take = [&](size_t n) {
         char *p = base ? base + at : nullptr;
@@ -623,22 +646,22 @@ size_t carve(Args &a, int P, char *base) {
     a.ids = (int32_t *)take(rows * 4);
     a.weights = (float *)take(rows * 4);
     a.logits = (double *)take((size_t)a.splits * a.T * a.E * 8);
-    a.sums = (float *)take(a.parts > 1 ? (size_t)((a.H + 31) / 32) * a.parts * a.T * 128 : 0);
+    a.sums = (float *)take(a.parts > 1 ? (size_t)((a.H + 16 * a.tiles - 1) / (16 * a.tiles)) * a.parts * a.T * (64 * a.tiles) : 0);
     a.lists = (int32_t *)take((size_t)a.used * (kListHead + kMaxTokens) * 4);
-    a.xp = (__bf16 *)take((size_t)P * a.T * a.hb * kBlock * 2);
-    a.hp = (__bf16 *)take((size_t)P * rows * a.ib * kBlock * 2);
+    a.xp = (__bf16 *)take(P * a.T * a.hb * kBlock * 2);
+    a.hp = (__bf16 *)take(PH * rows * a.ib * kBlock * 2);
     return at;
 }
 
 size_t workspace_of(const tbh_moe &m, int32_t x_type, int64_t tokens, int32_t top_k) {
     Args a{};
-    size_up(a, m, tokens, top_k);
+    size_up(a, m, x_type, tokens, top_k);
     // (more tokens have fewer parts of a tile, and a last part of few tokens may have more)
     size_t most = 0;
     for (int64_t t : {(int64_t)a.T, tokens % kMaxTokens}) {
         if (t == 0) continue;
-        size_up(a, m, t, top_k);
-        most = std::max(most, carve(a, x_type == TBH_BF16 ? 1 : 3, nullptr));
+        size_up(a, m, x_type, t, top_k);
+        most = std::max(most, carve(a, x_type, nullptr));
     }
     return most;
 }
@@ -774,11 +797,11 @@ tbh_status tbh_moe_device(const tbh_moe *m, const void *x, int32_t x_type, int64
     hipError_t e = hipSuccess;
     for (int64_t at = 0; at < tokens && e == hipSuccess; at += kMaxTokens) {
         Args a{};
-        size_up(a, *m, tokens - at, top_k);
+        size_up(a, *m, x_type, tokens - at, top_k);
         a.normalize = normalize != 0;
         a.vec = vec;
         a.counters = room.counters;
-        carve(a, x_type == TBH_BF16 ? 1 : 3, room.data);
+        carve(a, x_type, room.data);
         if (experts) a.ids = experts + at * top_k;
         if (weights) a.weights = weights + at * top_k;
         a.x = (const char *)x + at * x_stride * size;
@@ -791,7 +814,8 @@ tbh_status tbh_moe_device(const tbh_moe *m, const void *x, int32_t x_type, int64
         a.gate_scales = m->gate_scales;
         a.up_scales = m->up_scales;
         a.down_scales = m->down_scales;
-        e = x_type == TBH_BF16 ? launch<__bf16, 1>(a, s) : launch<float, 3>(a, s);
+        if (x_type == TBH_F32) e = launch<float, 3, 3, 1, 2>(a, s);
+        else e = a.tiles == 4 ? launch<__bf16, 1, 1, 2, 4>(a, s) : launch<__bf16, 1, 2, 1, 2>(a, s);
     }
     return e == hipSuccess ? TBH_OK : hip_error(e, "moe launch");
 }
