@@ -608,9 +608,9 @@ tbh_status tbh_fp8_weight_destroy(tbh_fp8_weight *w);
  * once, ties to even; an infinity or NaN becomes NaN.
  *   y[m][n] = sum over b of s[m][b] * scale[n / 128][b] * (q . w of block b)
  * summed in fp32, rounded once to y_type.  For TBH_BF16 q . w comes from the FP8
- * matrix instruction, which cuts its sums (about 2^-15 of their size; rounding to
- * bf16 then does 2^-9); TBH_F32 results have fp32 sums, on the bf16 instruction, to
- * which q and w are widened exactly.  (Products of two scales outside
+ * matrix instruction, which cuts its sums (about 2^-15 of their size, at most 2^-10
+ * of a block's largest product; rounding to bf16 then does 2^-9); TBH_F32 results
+ * have fp32 sums, on the bf16 instruction, to which q and w are widened exactly.  (Products of two scales outside
  * fp32's normal range lose precision or overflow.)  y does not overlap x.
  * Past 16 rows x is quantized into `workspace` (256-byte aligned,
  * tbh_fp8_matmul_workspace bytes for M rows), or, if that is NULL, into the
@@ -634,7 +634,8 @@ tbh_status tbh_fp8_matmul_device(const tbh_fp8_weight *w, const void *x, int32_t
  * 2^-16 of itself, y is rounded to bf16 once, from fp32), fp32 rows keep fp32's
  * precision throughout.
  * Made for few tokens, where reading the chosen experts is what takes time: an
- * expert's weights are read once for up to 64 tokens, more run 64 at a time.
+ * expert's weights are read from memory once for up to 64 tokens, more run 64 at a
+ * time.
  * A row that holds an infinity or NaN gets NaN; which experts it is given then
  * means nothing.  Other rows are not touched by it.  An h past the largest fp32
  * number is an infinity and weighs like one. */

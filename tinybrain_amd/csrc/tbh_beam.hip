@@ -654,8 +654,9 @@ __device__ __forceinline__ Moves plan_moves(const ReorderArgs &a, int group) {
 // its own to write, the launch writes that too.  Every block works out its group's moves
 // by itself (a few ballots), so that nothing is handed from launch to launch.  Bound by memory:
 // eight groups of eight rows, 800 positions of 8 x 128 bf16 of two layers, 315 MB
-// read and written, 64 to 68 us (4.8 TB/s, a large copy's rate); by its launch for one
-// group of four: 4.4 us.
+// read and written, 64 to 69 us (4.8 TB/s, a large copy's rate; cache blocks of 32 and 64
+// positions, of which one thread block copies each, 75 and 78); by its launch for one
+// group of four: 4.8 us.
 template <class V>
 __global__ __launch_bounds__(256) void reorder_copy(ReorderArgs a) {
     const int row = blockIdx.x / a.steps, step = blockIdx.x % a.steps, group = row / a.beams;
@@ -691,7 +692,8 @@ __global__ __launch_bounds__(256) void reorder_copy(ReorderArgs a) {
     }
 }
 
-// The table in place: a thread takes one column of a group, and holds it.
+// The table in place: a thread takes one column of a group, and holds it.  Some 3 to 8 us of a call
+// (eight groups of eight rows 71.6 us, into a second table 63.6).
 __global__ __launch_bounds__(64) void reorder_table(ReorderArgs a) {
     __shared__ int32_t column[kMaxBeams][64];
     __shared__ int source[kMaxBeams];
@@ -889,8 +891,8 @@ tbh_status tbh_paged_reorder_device(tbh_device *dev, const tbh_paged_layout *lay
         for (int i = 0; i < b.count / 2; ++i) b.arrays[2 * i] = k_caches[at + i], b.arrays[2 * i + 1] = v_caches[at + i];
         if (in_place || at > 0) b.table_out = nullptr;
         if (at > 0) b.reordered = nullptr;
-        // a row's blocks parted so that there are some thousands of thread blocks (1024, 2048, 8192
-        // or 32768 of them: the 64 rows above 103, 91, 64, 71 us, 64 rows of 100 positions 6.1,
+        // a row's blocks (here of 16) parted so that there are some thousands of thread blocks (1024, 2048,
+        // 8192 or 32768 of them: the 64 rows above 103, 91, 64, 71 us, 64 rows of 100 positions 6.1,
         // 7.4, 8.8, 8.6; how much there is to copy is known on the device alone)
         const int64_t ys = std::max(1, b.count);
         const int64_t steps = std::max<int64_t>(1, std::min<int64_t>(a.most, 8192 / std::min<int64_t>(8192, a.rows * ys)));

@@ -172,7 +172,7 @@ struct QuantizeArgs {
 };
 
 // A wave quantizes 16 rows x 128 and writes them in the layout of a weight.  Bound by
-// memory: 4096 x 4096 of bf16 9.5 us (33.5 MB read, 17 written: 5.3 TB/s, from the caches).
+// memory: 4096 x 4096 of bf16 10.5 us (33.5 MB read, 17 written: 4.8 TB/s).
 template <class XT, bool WIDE>
 __global__ __launch_bounds__(256) void fp8_quantize(QuantizeArgs a) {
     const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
@@ -214,8 +214,9 @@ struct TilesArgs {
 // from memory straight to registers: no barrier but that of the join.  For products that
 // do not fill the device with blocks of 128 x 256, bound by the latency of the loads and then by
 // the caches, which serve x to every block of outputs and the weight to every block of rows:
-// 21 rows by 4096 x 11008 10.4 us (4.3 TB/s of weight) behind the quantizing's 3.4, 333 of fp32
-// by 5632 x 2048 14 behind 4.
+// 21 rows by 4096 x 11008 10.3 us (4.4 TB/s of weight) behind the quantizing's 3.4, 333 of fp32
+// by 5632 x 2048 14.2 behind 5.4, in which waves ask the L2 caches for 207 MB (counted, 14.6 TB/s) of
+// operands that are 18 MB: two tiles by three take five loads for six products.
 template <class YT, int W, int RT, int KW, int CT>
 __global__ __launch_bounds__(64 * W) void fp8_few(TilesArgs a) {
     __shared__ f32x4 red[W][RT * CT][64];
@@ -285,9 +286,10 @@ constexpr uint32_t kPast = 0x7FFFFFF0u;   // past every buffer: reads as zeros
 // Two steps of 128 inputs in LDS: a step's one barrier says that its tiles have landed and
 // that every wave is done with the step before, whose place the loads issued then take, a few
 // behind each row of products (all at the step's start: 196 us and 364 of the 190 and 345 below).
-// 4096 rows by 4096 x 11008: 180 us of this kernel (2.05 PFLOP/s; loads alone 115, products
+// 4096 rows by 4096 x 11008: 182 to 203 us of this kernel by the card (medians of traces, 2.03 to 1.82
+// PFLOP/s; loads alone 115, products
 // alone 170), fp32 results 345 us with the quantizing.  Bound by the step: of its some 4100
-// cycles the matrix instructions are busy for 2050, LDS reads take 1536, loads 2800, and a
+// cycles (395000 a launch, three rounds of 32 steps) the matrix instructions are busy for 2050, LDS reads take 1536, loads 2800, and a
 // barrier joins them; 160 KiB of LDS hold no third step.  (Two halves of a block's
 // waves, one at LDS while the other multiplies: 210 us of then 203; cache lines touched two to
 // four steps ahead: 233; instructions of 32 x 32 results: 197 of 190.  Matrix instructions alone, out of registers and with these fp32 sums, run

@@ -10,9 +10,9 @@
 //   Three launches, as every chosen expert's h has to be whole before D_e, and the
 // choice before either.  Their times in us (route, up, down; floor: the chosen experts'
 // bytes at the 4.8 TB/s of a large copy):
-//   1 token, 2 of 8 experts of 2048 x 5632, fp32 rows      8.4  11.4  10.8   (14.5)
-//   13 tokens, 6 of 64 experts of 2048 x 1000, bf16       11.6  42.2  29.8   (59)
-//   64 tokens, 4 of 32 experts of 4096 x 2048, bf16       13.6   113  69.9   (168)
+//   1 token, 2 of 8 experts of 2048 x 5632, fp32 rows      8.5  11.8  10.0   (14.5)
+//   13 tokens, 6 of 64 experts of 2048 x 1000, bf16       11.4  41.2  29.5   (59)
+//   64 tokens, 4 of 32 experts of 4096 x 2048, bf16       13.2   111  69.8   (168)
 // What is above the floor is the latency of launches and of loads that depend on
 // one another (ids, lists, weights, the join), not the work.
 #include <algorithm>
@@ -436,8 +436,8 @@ __device__ __forceinline__ void up_tokens(const Args &a, int e, int tile, const 
 
 // Gate and up products of 16 inner columns of one expert and h = silu(gate) * up;
 // the waves part the inputs.  Gate's and up's tiles lie side by side, so that a wave
-// reads 4 KiB in a row a step.  Bound by memory: 32 experts of 4096 x 2048 (537 MB) in 105 us,
-// 5.1 TB/s, 2 of 2048 x 5632 (46 MB) in 9.6 behind the 1.0 of the search for the expert.  (Two
+// reads 4 KiB in a row a step.  Bound by memory: 32 experts of 4096 x 2048 (537 MB) in 111 us,
+// 4.8 TB/s, 2 of 2048 x 5632 (46 MB) in 11.8, of which 1.0 is the search for the expert.  (Two
 // or four steps' loads ahead of the products: no faster, the blocks of a CU hide each other's.)
 template <int P, int PH>
 __global__ __launch_bounds__(256) void moe_up(Args a) {
@@ -452,8 +452,9 @@ __global__ __launch_bounds__(256) void moe_up(Args a) {
         if (e >= 0 && (int)threadIdx.x < count) l[kListHead + threadIdx.x] = slots[threadIdx.x];
     }
     if (e < 0) return;
-    // two column tiles to a load of the weights while there are more than one's tokens (64 tokens, 2
-    // of 8 experts of 4096 x 4096: 120 us against 128 one at a time, of fp32 231 and 252)
+    // two column tiles to a load of the weights while there are more than one's tokens (a whole call of 64
+    // tokens, 2 of 8 experts of 4096 x 4096: 127 us against 136 one at a time, of fp32 224 and 248).  More
+    // tokens load them again, from the caches.
     int c0 = 0;
     for (; count - c0 > kTokens<P>; c0 += 2 * kTokens<P>) up_tokens<P, PH, 2>(a, e, blockIdx.x, slots, c0, count, red);
     if (c0 < count) up_tokens<P, PH, 1>(a, e, blockIdx.x, slots, c0, count, red);
@@ -466,7 +467,7 @@ __global__ __launch_bounds__(256) void moe_up(Args a) {
 // token needs twice as many loads of h as of weights, so that a wave takes two or four tiles a
 // load of h, see size_up.)  Bound by memory where there are many experts (268 MB in 70 us, 3.8 TB/s, which
 // with h in one piece of bf16 took 67), by the
-// latency of the join for one token: 4.6 of 10.8 us are products.  (kUnit 1, 2 or 4: a whole call on
+// latency of the join for one token: 4.6 of 10 us are products.  (kUnit 1, 2 or 4: a whole call on
 // 1 token 29.1, 28.9, 31.4 us, on 64, h in one piece, 177, 169, 169.)
 constexpr int kDownWaves = 8, kUnit = 2;
 
