@@ -610,8 +610,9 @@ tbh_status tbh_fp8_weight_destroy(tbh_fp8_weight *w);
  * summed in fp32, rounded once to y_type.  For TBH_BF16 q . w comes from the FP8
  * matrix instruction, which cuts its sums (about 2^-15 of their size, at most 2^-10
  * of a block's largest product; rounding to bf16 then does 2^-9); TBH_F32 results
- * have fp32 sums, on the bf16 instruction, to which q and w are widened exactly.  (Products of two scales outside
- * fp32's normal range lose precision or overflow.)  y does not overlap x.
+ * have fp32 sums, on the bf16 instruction, to which q and w are widened exactly.
+ * (Products of two scales outside fp32's normal range lose precision or overflow.)
+ * y does not overlap x.
  * Past 16 rows x is quantized into `workspace` (256-byte aligned,
  * tbh_fp8_matmul_workspace bytes for M rows), or, if that is NULL, into the
  * workspace of (device, stream), with tbh_matmul_device's rule for captured
